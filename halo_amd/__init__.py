@@ -13,13 +13,22 @@ from ._lib import (  # noqa: F401
     DType,
     ErrorCode,
     HaloError,
+    KvBatch,
+    KvCache,
+    KvState,
     Layout,
+    RopePairs,
+    RopeScaling,
     Variant,
     ARGMAX_RESULT_BYTES,
+    KV_LIST_MAX,
     SLAB_ROWS,
     STATUS_BAD_INDEX,
+    STATUS_KV_FULL,
     STATUS_SPLITK_TIMEOUT,
     argmax,
+    attention,
+    attention_workspace,
     block_bytes,
     block_elems,
     dequant_rows,
@@ -31,12 +40,21 @@ from ._lib import (  # noqa: F401
     gemv_group,
     gemv_noalloc,
     get_rows,
+    kv_compact,
+    kv_copy_pages,
+    kv_fork,
+    kv_page_bytes,
+    kv_read,
+    kv_resize,
+    kv_write,
     lib,
     lm_head,
     quantize,
     repack_slab,
     repack_slab_host,
     rms_norm,
+    rope,
+    rope_freqs,
     row_bytes,
     slab_bytes,
     stream_check,

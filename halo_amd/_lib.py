@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import enum
 import functools
+import typing
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -187,9 +188,68 @@ class _GetRowsParams(ctypes.Structure):
     ]
 
 
+class _RopeScaling(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_uint32), ("scale", ctypes.c_double), ("context", ctypes.c_double),
+                ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double)]
+
+
+class _RopePart(ctypes.Structure):
+    _fields_ = [("in_", ctypes.c_void_p), ("in_stride", ctypes.c_uint64), ("in_head_stride", ctypes.c_uint64),
+                ("out", ctypes.c_void_p), ("out_stride", ctypes.c_uint64), ("out_head_stride", ctypes.c_uint64),
+                ("n_heads", ctypes.c_uint32)]
+
+
+class _RopeParams(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_uint32), ("pairs", ctypes.c_uint32), ("parts", ctypes.POINTER(_RopePart)),
+                ("n_parts", ctypes.c_uint32), ("n_tokens", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("rot_dims", ctypes.c_uint32), ("positions", ctypes.c_void_p), ("freqs", ctypes.c_void_p),
+                ("factor", ctypes.c_float)]
+
+
+class _KvCache(ctypes.Structure):
+    _fields_ = [("pool", ctypes.c_void_p), ("n_pages", ctypes.c_uint32), ("n_layers", ctypes.c_uint32),
+                ("n_kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("block_tokens", ctypes.c_uint32)]
+
+
+class _KvBatch(ctypes.Structure):
+    _fields_ = [("tables", ctypes.c_void_p), ("table_stride", ctypes.c_uint64), ("table_width", ctypes.c_uint32),
+                ("kv_lens", ctypes.c_void_p), ("row_starts", ctypes.c_void_p), ("n_seqs", ctypes.c_uint32),
+                ("n_rows", ctypes.c_uint32), ("max_rows", ctypes.c_uint32), ("max_kv", ctypes.c_uint32)]
+
+
+class _KvWriteParams(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_uint32), ("cache", _KvCache), ("layer", ctypes.c_uint32), ("batch", _KvBatch),
+                ("k", ctypes.c_void_p), ("k_stride", ctypes.c_uint64), ("k_head_stride", ctypes.c_uint64),
+                ("v", ctypes.c_void_p), ("v_stride", ctypes.c_uint64), ("v_head_stride", ctypes.c_uint64),
+                ("status", ctypes.c_void_p), ("status_keep", ctypes.c_uint32)]
+
+
+class _KvReadParams(ctypes.Structure):
+    _fields_ = [("cache", _KvCache), ("layer", ctypes.c_uint32), ("batch", _KvBatch),
+                ("k_out", ctypes.c_void_p), ("k_stride", ctypes.c_uint64), ("k_head_stride", ctypes.c_uint64),
+                ("v_out", ctypes.c_void_p), ("v_stride", ctypes.c_uint64), ("v_head_stride", ctypes.c_uint64),
+                ("status", ctypes.c_void_p), ("status_keep", ctypes.c_uint32)]
+
+
+class _AttentionParams(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_uint32), ("cache", _KvCache), ("layer", ctypes.c_uint32), ("batch", _KvBatch),
+                ("q", ctypes.c_void_p), ("q_stride", ctypes.c_uint64), ("q_head_stride", ctypes.c_uint64),
+                ("out", ctypes.c_void_p), ("out_stride", ctypes.c_uint64), ("out_head_stride", ctypes.c_uint64),
+                ("n_heads", ctypes.c_uint32), ("scale", ctypes.c_float), ("window", ctypes.c_uint32),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+                ("status", ctypes.c_void_p), ("status_keep", ctypes.c_uint32)]
+
+
+class _KvState(ctypes.Structure):
+    _fields_ = [("refs", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("tables", ctypes.c_void_p),
+                ("table_stride", ctypes.c_uint64), ("table_width", ctypes.c_uint32), ("n_slots", ctypes.c_uint32)]
+
+
 ARGMAX_RESULT_BYTES = 12  # HALO_MI_ARGMAX_RESULT_BYTES: {index, value bits, poisoned} per vector
 STATUS_BAD_INDEX = 8  # HALO_MI_STATUS_BAD_INDEX: a GET_ROWS id outside the table
 STATUS_SPLITK_TIMEOUT = 0x100  # HALO_MI_STATUS_SPLITK_TIMEOUT: a split-K reduction gave up waiting
+STATUS_KV_FULL = 16  # HALO_MI_STATUS_KV_FULL: no free page, or no column in a sequence's table
+KV_LIST_MAX = 1024  # HALO_MI_KV_LIST_MAX: entries of one kv_resize or kv_fork call
 
 
 # Every symbol include/halo_mi355x.h declares, with its ctypes signature.
@@ -207,6 +267,17 @@ SIGNATURES = {
     "halo_mi_dequant_rows": (_INT, [_U32, _U32, _VP, _U64, _U32, _U32, _U32, _U32, _VP, _U64, _VP]),
     "halo_mi_get_rows": (_INT, [ctypes.POINTER(_GetRowsParams), _VP]),
     "halo_mi_rms_norm": (_INT, [_VP, _U64, _VP, _VP, _U64, _U32, _U32, ctypes.c_float, _VP]),
+    "halo_mi_rope_freqs": (_INT, [_U32, ctypes.c_double, ctypes.POINTER(_RopeScaling), _VP, ctypes.POINTER(ctypes.c_float)]),
+    "halo_mi_rope": (_INT, [ctypes.POINTER(_RopeParams), _VP]),
+    "halo_mi_kv_page_bytes": (_U64, [_U32, _U32, _U32, _U32]),
+    "halo_mi_kv_write": (_INT, [ctypes.POINTER(_KvWriteParams), _VP]),
+    "halo_mi_kv_read": (_INT, [ctypes.POINTER(_KvReadParams), _VP]),
+    "halo_mi_attention": (_INT, [ctypes.POINTER(_AttentionParams), _VP]),
+    "halo_mi_attention_workspace": (_U64, [ctypes.POINTER(_AttentionParams)]),
+    "halo_mi_kv_resize": (_INT, [ctypes.POINTER(_KvCache), ctypes.POINTER(_KvState), _VP, _VP, _U32, _VP, _U32, _VP]),
+    "halo_mi_kv_fork": (_INT, [ctypes.POINTER(_KvCache), ctypes.POINTER(_KvState), _VP, _VP, _U32, _VP, _U32, _VP]),
+    "halo_mi_kv_compact": (_INT, [ctypes.POINTER(_KvCache), ctypes.POINTER(_KvState), _VP, _VP]),
+    "halo_mi_kv_copy_pages": (_INT, [ctypes.POINTER(_KvCache), _VP, _VP, _U32, _VP, _U32, _VP]),
     "halo_mi_stream_read": (_INT, [_VP, _U64, _U32, _U32, _VP, _VP]),
     "halo_mi_stream_check": (_INT, [_VP]),
     "halo_mi_stream_release": (_INT, [_VP]),
@@ -427,6 +498,188 @@ def rms_norm(x, w, out, rows: int, cols: int, *, eps: float = 1e-6, x_stride: in
     """RMS_NORM (halo_mi_rms_norm), bitwise cpu::rms_norm."""
     _check(lib().halo_mi_rms_norm(_ptr(x), int(x_stride), _ptr(w), _ptr(out), int(out_stride), int(rows), int(cols),
                                   float(eps), _stream(stream)))
+
+
+# ---- attention over an 8-bit paged cache -------------------------------------------------
+
+
+class RopePairs(enum.IntEnum):
+    """The two elements that a rotation takes together."""
+
+    HALF = 0  # i and i + rot_dims / 2
+    INTERLEAVED = 1  # 2 i and 2 i + 1
+
+
+class RopeScaling(enum.IntEnum):
+    PLAIN = 0
+    LINEAR = 1
+    NTK = 2
+    YARN = 3
+
+
+class KvCache(typing.NamedTuple):
+    """The pool of an 8-bit paged cache (halo_mi_kv_cache): n_pages records of kv_page_bytes() bytes."""
+
+    pool: object
+    n_pages: int
+    n_layers: int
+    n_kv_heads: int
+    head_dim: int
+    block_tokens: int
+
+
+class KvBatch(typing.NamedTuple):
+    """The sequences of a call (halo_mi_kv_batch): rows row_starts[s] .. row_starts[s + 1] of the row operands are
+    the last tokens of sequence s, which holds kv_lens[s] tokens; tables, kv_lens and row_starts are int32
+    on the device."""
+
+    tables: object
+    table_width: int
+    kv_lens: object
+    row_starts: object
+    n_seqs: int
+    n_rows: int
+    max_rows: int = 0
+    max_kv: int = 0
+    table_stride: int = 0
+
+
+class KvState(typing.NamedTuple):
+    """Who holds which page (halo_mi_kv_state), int32 on the device: refs [n_pages], lens [n_slots], tables
+    [n_slots, table_width]."""
+
+    refs: object
+    lens: object
+    tables: object
+    n_slots: int
+    table_width: int
+    table_stride: int = 0
+
+
+def _dev(t) -> int:
+    """Device address of an operand; a tensor has to be on the current device."""
+    if t is None or isinstance(t, int):
+        return t or 0
+    import torch
+
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise HaloError(ErrorCode.Kernel, f"an operand is on {t.device}, not on the current GPU")
+    return t.data_ptr()
+
+
+def _cache(c: KvCache) -> _KvCache:
+    return _KvCache(_dev(c.pool), int(c.n_pages), int(c.n_layers), int(c.n_kv_heads), int(c.head_dim), int(c.block_tokens))
+
+
+def _batch(b: KvBatch) -> _KvBatch:
+    return _KvBatch(_dev(b.tables), int(b.table_stride), int(b.table_width), _dev(b.kv_lens), _dev(b.row_starts),
+                    int(b.n_seqs), int(b.n_rows), int(b.max_rows), int(b.max_kv))
+
+
+def _state(s: KvState) -> _KvState:
+    return _KvState(_dev(s.refs), _dev(s.lens), _dev(s.tables), int(s.table_stride), int(s.table_width), int(s.n_slots))
+
+
+def rope_freqs(rot_dims: int, theta: float = 10000.0, *, scaling: int = RopeScaling.PLAIN, scale: float = 1.0,
+               context: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0):
+    """The rot_dims / 2 frequencies in radians per position (float64 numpy array) and the factor on the rotated
+    values (halo_mi_rope_freqs)."""
+    import numpy as np
+
+    out = np.empty(max(int(rot_dims) // 2, 1), dtype=np.float64)
+    factor = ctypes.c_float(1.0)
+    sc = _RopeScaling(int(scaling), float(scale), float(context), float(beta_fast), float(beta_slow))
+    _check(lib().halo_mi_rope_freqs(int(rot_dims), float(theta), ctypes.byref(sc), out.ctypes.data, ctypes.byref(factor)))
+    return out, float(factor.value)
+
+
+def rope(t: int, positions, freqs, n_tokens: int, head_dim: int, rot_dims: int, q, q_out, n_heads: int, *, k=None,
+         k_out=None, n_kv_heads: int = 0, pairs: int = RopePairs.HALF, factor: float = 1.0, q_stride: int = 0,
+         q_head_stride: int = 0, q_out_stride: int = 0, q_out_head_stride: int = 0, k_stride: int = 0,
+         k_head_stride: int = 0, k_out_stride: int = 0, k_out_head_stride: int = 0, stream=None) -> None:
+    """PARTIAL_ROPE of q and, with k, of k in one launch (halo_mi_rope). q_out may be q, k_out may be k. positions:
+    int32, freqs: float64 radians per position (rope_freqs), both on the device; strides in elements."""
+    parts = (_RopePart * 2)(
+        _RopePart(_dev(q), int(q_stride), int(q_head_stride), _dev(q_out), int(q_out_stride), int(q_out_head_stride), int(n_heads)),
+        _RopePart(_dev(k), int(k_stride), int(k_head_stride), _dev(k_out), int(k_out_stride), int(k_out_head_stride), int(n_kv_heads)))
+    p = _RopeParams(int(t), int(pairs), parts, 1 if k is None else 2, int(n_tokens), int(head_dim), int(rot_dims), _dev(positions),
+                    _dev(freqs), float(factor))
+    _check(lib().halo_mi_rope(ctypes.byref(p), _stream(stream)))
+
+
+def kv_page_bytes(n_layers: int, n_kv_heads: int, head_dim: int, block_tokens: int) -> int:
+    """Bytes of a page of the 8-bit cache; 0 for a geometry that it does not have."""
+    return int(lib().halo_mi_kv_page_bytes(int(n_layers), int(n_kv_heads), int(head_dim), int(block_tokens)))
+
+
+def kv_write(t: int, cache: KvCache, layer: int, batch: KvBatch, k, v, *, k_stride: int = 0, k_head_stride: int = 0,
+             v_stride: int = 0, v_head_stride: int = 0, status=None, status_keep: bool = False, stream=None) -> None:
+    """KV_WRITE: the batch's rows of k and v into their sequences' pages (halo_mi_kv_write)."""
+    p = _KvWriteParams(int(t), _cache(cache), int(layer), _batch(batch), _dev(k), int(k_stride), int(k_head_stride), _dev(v),
+                       int(v_stride), int(v_head_stride), _dev(status), 1 if status_keep else 0)
+    _check(lib().halo_mi_kv_write(ctypes.byref(p), _stream(stream)))
+
+
+def kv_read(cache: KvCache, layer: int, batch: KvBatch, k_out=None, v_out=None, *, k_stride: int = 0, k_head_stride: int = 0,
+            v_stride: int = 0, v_head_stride: int = 0, status=None, status_keep: bool = False, stream=None) -> None:
+    """The values that the cache holds for the batch's rows, in fp32 (halo_mi_kv_read)."""
+    p = _KvReadParams(_cache(cache), int(layer), _batch(batch), _dev(k_out), int(k_stride), int(k_head_stride), _dev(v_out),
+                      int(v_stride), int(v_head_stride), _dev(status), 1 if status_keep else 0)
+    _check(lib().halo_mi_kv_read(ctypes.byref(p), _stream(stream)))
+
+
+def _attention_params(t, cache, layer, batch, q, out, n_heads, scale, window, q_stride, q_head_stride, out_stride, out_head_stride,
+                      workspace, workspace_bytes, status, status_keep):
+    if workspace is not None and not isinstance(workspace, int) and not workspace_bytes:
+        workspace_bytes = workspace.numel() * workspace.element_size()
+    return _AttentionParams(int(t), _cache(cache), int(layer), _batch(batch), _dev(q), int(q_stride), int(q_head_stride), _dev(out),
+                            int(out_stride), int(out_head_stride), int(n_heads), float(scale), int(window), _dev(workspace),
+                            int(workspace_bytes), _dev(status), 1 if status_keep else 0)
+
+
+def attention(t: int, cache: KvCache, layer: int, batch: KvBatch, q, out, n_heads: int, *, scale: float = 0.0, window: int = 0,
+              q_stride: int = 0, q_head_stride: int = 0, out_stride: int = 0, out_head_stride: int = 0, workspace=None,
+              workspace_bytes: int = 0, status=None, status_keep: bool = False, stream=None) -> None:
+    """ATTENTION of the batch's rows over their sequences' cached tokens, causal, over the last `window` tokens where it
+    is not 0 (halo_mi_attention). scale 0: 1 / sqrt(head_dim)."""
+    p = _attention_params(t, cache, layer, batch, q, out, n_heads, scale, window, q_stride, q_head_stride, out_stride, out_head_stride,
+                          workspace, workspace_bytes, status, status_keep)
+    _check(lib().halo_mi_attention(ctypes.byref(p), _stream(stream)))
+
+
+def attention_workspace(t: int, cache: KvCache, layer: int, batch: KvBatch, q, out, n_heads: int, *, window: int = 0,
+                        q_stride: int = 0, q_head_stride: int = 0, out_stride: int = 0, out_head_stride: int = 0) -> int:
+    """Workspace bytes that the same attention call makes use of (halo_mi_attention_workspace)."""
+    p = _attention_params(t, cache, layer, batch, q, out, n_heads, 0.0, window, q_stride, q_head_stride, out_stride, out_head_stride,
+                          None, 0, None, False)
+    return int(lib().halo_mi_attention_workspace(ctypes.byref(p)))
+
+
+def kv_resize(cache: KvCache, state: KvState, slots, new_lens, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
+    """Gives slots their new lengths, with pages taken and released (halo_mi_kv_resize); length 0 frees a slot."""
+    c, s = _cache(cache), _state(state)
+    _check(lib().halo_mi_kv_resize(ctypes.byref(c), ctypes.byref(s), _dev(slots), _dev(new_lens), int(n), _dev(status),
+                                   1 if status_keep else 0, _stream(stream)))
+
+
+def kv_fork(cache: KvCache, state: KvState, src, dst, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
+    """Empty slots dst become copies of src: whole pages shared, a last one that is not full copied (halo_mi_kv_fork)."""
+    c, s = _cache(cache), _state(state)
+    _check(lib().halo_mi_kv_fork(ctypes.byref(c), ctypes.byref(s), _dev(src), _dev(dst), int(n), _dev(status),
+                                 1 if status_keep else 0, _stream(stream)))
+
+
+def kv_compact(cache: KvCache, state: KvState, *, live=None, stream=None) -> None:
+    """Moves the live pages to the front of the pool (halo_mi_kv_compact); live (uint32 or int32) receives their number."""
+    c, s = _cache(cache), _state(state)
+    _check(lib().halo_mi_kv_compact(ctypes.byref(c), ctypes.byref(s), _dev(live), _stream(stream)))
+
+
+def kv_copy_pages(cache: KvCache, src, dst, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
+    """Copies whole pages (halo_mi_kv_copy_pages)."""
+    c = _cache(cache)
+    _check(lib().halo_mi_kv_copy_pages(ctypes.byref(c), _dev(src), _dev(dst), int(n), _dev(status), 1 if status_keep else 0,
+                                       _stream(stream)))
 
 
 def stream_read(p, nbytes: int, workgroups: int, unroll: int, sink, stream=None) -> None:

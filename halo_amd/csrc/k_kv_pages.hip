@@ -1,0 +1,341 @@
+// gfx950 kernels of the pages' owner: giving slots pages, releasing them, forking slots, packing the pool, and
+// copying pages. The state (reference counts, lengths, tables) lives on the device and is changed there, so a
+// serving loop needs no word from the host between steps and can be captured whole.
+//
+// Who gets which page is one order (the list's) over another (the free pages by number), so one workgroup of 1024
+// threads decides: prefix sums over the list and over the counts, 4096 counts a step. What costs time is the
+// pages' bytes (hundreds of KB each with all layers): a second kernel copies them with the whole GPU, from a
+// list that the first one leaves in scratch memory.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "kv.h"
+#include "kv_device.h"
+#include "launch.h"
+
+namespace halo_mi {
+namespace {
+
+using namespace dev;
+
+constexpr uint32_t kOwnerBlock = 1024;   // threads of the deciding workgroup; >= HALO_MI_KV_LIST_MAX
+constexpr uint32_t kOwnerWaves = kOwnerBlock / 64;
+constexpr uint32_t kCopyBlock = 256;
+constexpr uint32_t kCopyBytes = 16384;   // of a page per workgroup and step: 4 accesses of 16 bytes per thread
+constexpr uint32_t kCopyGrid = 2048;     // 8 workgroups per CU
+static_assert(kOwnerBlock >= HALO_MI_KV_LIST_MAX);
+
+// Exclusive prefix sum over the workgroup; total receives the sum. lds: kOwnerWaves words.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* lds, uint32_t& total) {
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    uint32_t sum = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t below = (uint32_t)__shfl_up((int)sum, off);
+        if (lane >= (uint32_t)off) sum += below;
+    }
+    __syncthreads();  // lds may still be read from the last scan
+    if (lane == 63) lds[wave] = sum;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kOwnerWaves; ++w) {
+        before += w < wave ? lds[w] : 0u;
+        total += lds[w];
+    }
+    return before + sum - v;
+}
+
+struct OwnerLds {
+    uint32_t scan[kOwnerWaves];
+    int32_t slots[kOwnerBlock];
+    uint32_t first[kOwnerBlock + 1];  // prefix sums of the entries' pages
+    uint32_t column[kOwnerBlock];     // where an entry's first new page goes in its table
+};
+
+// Whether entry i is the first that names `slot` (every thread calls it).
+__device__ __forceinline__ bool first_of_its_name(OwnerLds& l, int32_t slot, uint32_t i, uint32_t n) {
+    l.slots[i] = slot;
+    __syncthreads();
+    bool first = true;
+    for (uint32_t j = 0; j < min(i, n); ++j) first = first && l.slots[j] != slot;
+    return first;
+}
+
+// The lowest min(want, all) free pages, in order, to `list`; returns how many.
+__device__ uint32_t free_pages(const KvPagesArgs& a, uint32_t want, uint32_t* list, OwnerLds& l) {
+    uint32_t found = 0;
+    for (uint32_t p0 = 0; p0 < a.n_pages && found < want; p0 += 4 * kOwnerBlock) {
+        const uint32_t p = p0 + 4 * threadIdx.x;
+        bool is_free[4];
+        uint32_t mine = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            is_free[k] = p + k < a.n_pages && a.refs[p + k] <= 0;
+            mine += is_free[k];
+        }
+        uint32_t total, at = found + block_scan(mine, l.scan, total);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+            if (is_free[k] && at < want) list[at++] = p + k;
+        found += total;
+    }
+    __syncthreads();
+    return min(found, want);
+}
+
+// Entry i of a call (thread i): `need` pages from `column` of its slot's table on, of which the first becomes a
+// copy of page `copy` (-1: none). Returns whether the pages reach; they are then in the table, held once, and the
+// copies in `pairs` (count, then source and destination).
+__device__ bool take_pages(const KvPagesArgs& a, int32_t slot, uint32_t need, uint32_t column, int32_t copy, uint32_t* list,
+                           uint32_t* pairs, uint32_t* status, OwnerLds& l) {
+    const uint32_t i = threadIdx.x;
+    uint32_t total;
+    const uint32_t before = block_scan(need, l.scan, total);
+    l.first[i] = before;
+    l.column[i] = column;
+    l.slots[i] = slot;
+    if (i == 0) l.first[kOwnerBlock] = total;
+    const uint32_t found = free_pages(a, total, list, l);
+    const bool granted = need == 0 || before + need <= found;
+    if (!granted) set_status(status, kStatusKvFull);
+    for (uint32_t r = i; r < found; r += kOwnerBlock) {
+        uint32_t lo = 0, hi = kOwnerBlock;  // the entry that rank r belongs to: the last one with first <= r
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            (l.first[mid] <= r ? lo : hi) = mid;
+        }
+        if (l.first[lo + 1] > found) continue;  // not all of its pages are there
+        const uint32_t page = list[r];
+        a.tables[(uint64_t)l.slots[lo] * a.table_stride + l.column[lo] + (r - l.first[lo])] = (int32_t)page;
+        a.refs[page] = 1;
+    }
+    const bool copies = granted && need && copy >= 0;
+    const uint32_t at = block_scan(copies, l.scan, total);
+    if (copies) {
+        pairs[1 + 2 * at] = (uint32_t)copy;
+        pairs[2 + 2 * at] = list[before];
+    }
+    if (i == 0) pairs[0] = total;
+    return granted;
+}
+
+__device__ __forceinline__ uint32_t pages_of(int32_t len, uint32_t block) { return len > 0 ? ((uint32_t)len + block - 1) / block : 0; }
+
+// scratch: the copies (1 + 2 n words), then the free pages' list (n_pages words)
+__global__ __launch_bounds__(kOwnerBlock) void k_kv_resize(KvPagesArgs a, const int32_t* slots, const int32_t* new_lens, uint32_t n,
+                                                            uint32_t* scratch, uint32_t* status) {
+    __shared__ OwnerLds l;
+    __shared__ uint32_t cut[kOwnerBlock][2];  // columns that an entry releases
+    const uint32_t i = threadIdx.x;
+    const int32_t slot = i < n ? slots[i] : -1, want = i < n ? new_lens[i] : 0;
+    bool ok = first_of_its_name(l, slot, i, n) && i < n && (uint32_t)slot < a.n_slots && want >= 0;
+    if (i < n && !ok) set_status(status, kStatusKvBadIndex);
+    uint32_t have = 0, take = 0, column = 0;
+    int32_t len = 0, tail = -1;
+    const uint32_t goal = pages_of(want, a.block);
+    if (ok && goal > a.table_width) {
+        ok = false;
+        set_status(status, kStatusKvFull);
+    }
+    if (ok) {
+        len = max(a.lens[slot], 0);
+        have = min(pages_of(len, a.block), a.table_width);
+        column = have;
+        take = goal > have ? goal - have : 0;
+        if (want > len && len % a.block && have) {
+            // tokens go behind others in a page: if it is held twice, into a copy
+            const int32_t id = a.tables[(uint64_t)slot * a.table_stride + have - 1];
+            if ((uint32_t)id >= a.n_pages) set_status(status, kStatusKvBadIndex);
+            else if (a.refs[id] > 1) tail = id;
+            if (tail >= 0) {
+                ++take;
+                --column;
+            }
+        }
+    }
+    __syncthreads();  // every count, length and table entry has been read
+    const bool granted = take_pages(a, slot, take, column, tail, scratch + 1 + 2 * n, scratch, status, l);
+    ok = ok && granted;
+    if (ok && tail >= 0) atomicSub(a.refs + tail, 1);
+    if (ok) a.lens[slot] = want;
+    cut[i][0] = ok ? goal : 0;
+    cut[i][1] = ok ? have : 0;
+    __syncthreads();
+    for (uint32_t e = i / 64; e < n; e += kOwnerWaves)
+        for (uint32_t c = cut[e][0] + i % 64; c < cut[e][1]; c += 64) {
+            int32_t* entry = a.tables + (uint64_t)l.slots[e] * a.table_stride + c;
+            if ((uint32_t)*entry < a.n_pages) atomicSub(a.refs + *entry, 1);
+            else set_status(status, kStatusKvBadIndex);
+            *entry = -1;
+        }
+}
+
+__global__ __launch_bounds__(kOwnerBlock) void k_kv_fork(KvPagesArgs a, const int32_t* src, const int32_t* dst, uint32_t n,
+                                                          uint32_t* scratch, uint32_t* status) {
+    __shared__ OwnerLds l;
+    __shared__ uint32_t from[kOwnerBlock], shared_pages[kOwnerBlock];
+    const uint32_t i = threadIdx.x;
+    const int32_t s = i < n ? src[i] : -1, d = i < n ? dst[i] : -1;
+    bool ok = first_of_its_name(l, d, i, n) && i < n && (uint32_t)s < a.n_slots && (uint32_t)d < a.n_slots && s != d;
+    if (ok) ok = a.lens[d] == 0;
+    if (i < n && !ok) set_status(status, kStatusKvBadIndex);
+    int32_t len = 0, tail = -1;
+    uint32_t full = 0, part = 0;
+    if (ok) {
+        len = max(a.lens[s], 0);
+        full = (uint32_t)len / a.block;
+        part = (uint32_t)len % a.block != 0;
+        if (full + part > a.table_width) {
+            ok = false;
+            set_status(status, kStatusKvBadIndex);
+        } else if (part) {
+            tail = a.tables[(uint64_t)s * a.table_stride + full];
+            if ((uint32_t)tail >= a.n_pages) {
+                tail = -1;
+                set_status(status, kStatusKvBadIndex);
+            }
+        }
+    }
+    __syncthreads();
+    const bool granted = take_pages(a, d, ok ? part : 0, full, tail, scratch + 1 + 2 * n, scratch, status, l);
+    ok = ok && granted;
+    if (ok) a.lens[d] = len;
+    from[i] = (uint32_t)s;
+    shared_pages[i] = ok ? full : 0;
+    __syncthreads();
+    for (uint32_t e = i / 64; e < n; e += kOwnerWaves)
+        for (uint32_t c = i % 64; c < shared_pages[e]; c += 64) {
+            const int32_t id = a.tables[(uint64_t)from[e] * a.table_stride + c];
+            a.tables[(uint64_t)l.slots[e] * a.table_stride + c] = id;
+            if ((uint32_t)id < a.n_pages) atomicAdd(a.refs + id, 1);
+            else set_status(status, kStatusKvBadIndex);
+        }
+}
+
+// Bytes [at, at + kCopyBytes) of a page, or what there is of them (page_bytes is a multiple of 128).
+__device__ __forceinline__ void copy_part(const KvPagesArgs& a, uint32_t from, uint32_t to, uint64_t at) {
+    const uint4* s = reinterpret_cast<const uint4*>(a.pool + from * a.page_bytes + at);
+    uint4* d = reinterpret_cast<uint4*>(a.pool + to * a.page_bytes + at);
+    const uint32_t n = (uint32_t)(min(a.page_bytes - at, (uint64_t)kCopyBytes) / 16);
+    constexpr uint32_t U = kCopyBytes / 16 / kCopyBlock;
+    uint4 v[U];
+#pragma unroll
+    for (uint32_t k = 0; k < U; ++k)
+        if (threadIdx.x + k * kCopyBlock < n) v[k] = s[threadIdx.x + k * kCopyBlock];
+#pragma unroll
+    for (uint32_t k = 0; k < U; ++k)
+        if (threadIdx.x + k * kCopyBlock < n) d[threadIdx.x + k * kCopyBlock] = v[k];
+}
+
+// pairs: the count, then source and destination pages
+__global__ __launch_bounds__(kCopyBlock) void k_kv_copy_taken(KvPagesArgs a, const uint32_t* pairs) {
+    const uint32_t parts = (uint32_t)((a.page_bytes + kCopyBytes - 1) / kCopyBytes);
+    const uint64_t units = (uint64_t)pairs[0] * parts;
+    for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const uint32_t i = (uint32_t)(u / parts);
+        copy_part(a, pairs[1 + 2 * i], pairs[2 + 2 * i], u % parts * kCopyBytes);
+    }
+}
+
+__global__ __launch_bounds__(kCopyBlock) void k_kv_copy_listed(KvPagesArgs a, const int32_t* src, const int32_t* dst, uint32_t n,
+                                                                uint32_t* status) {
+    const uint32_t parts = (uint32_t)((a.page_bytes + kCopyBytes - 1) / kCopyBytes);
+    const uint64_t units = (uint64_t)n * parts;
+    for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int32_t s = src[u / parts], d = dst[u / parts];
+        if ((uint32_t)s < a.n_pages && (uint32_t)d < a.n_pages) copy_part(a, (uint32_t)s, (uint32_t)d, u % parts * kCopyBytes);
+        else if (threadIdx.x == 0) set_status(status, kStatusKvBadIndex);
+    }
+}
+
+// scratch: live pages, moves, then the moved pages, their new places, and every page's new place (n_pages words each)
+__global__ __launch_bounds__(kOwnerBlock) void k_kv_compact(KvPagesArgs a, uint32_t* scratch, uint32_t* live_out) {
+    __shared__ OwnerLds l;
+    uint32_t *moved = scratch + 2, *place = moved + a.n_pages, *where = place + a.n_pages;
+    uint32_t live = 0, total;
+    for (uint32_t p = threadIdx.x; p < a.n_pages; p += kOwnerBlock) live += a.refs[p] > 0;
+    block_scan(live, l.scan, total);
+    live = total;
+    uint32_t n_moved = 0, n_holes = 0;
+    for (uint32_t p0 = 0; p0 < a.n_pages; p0 += kOwnerBlock) {
+        const uint32_t p = p0 + threadIdx.x;
+        const bool in = p < a.n_pages, alive = in && a.refs[p] > 0, moves = alive && p >= live, hole = in && !alive && p < live;
+        if (in) where[p] = p;
+        // at most one of the two: one scan counts both (2 * 1024 fits 16 bits)
+        uint32_t both;
+        const uint32_t at = block_scan(moves | (uint32_t)hole << 16, l.scan, both);
+        if (moves) moved[n_moved + (at & 0xFFFFu)] = p;
+        if (hole) place[n_holes + (at >> 16)] = p;
+        n_moved += both & 0xFFFFu;
+        n_holes += both >> 16;
+    }
+    __threadfence_block();
+    __syncthreads();
+    for (uint32_t k = threadIdx.x; k < n_moved; k += kOwnerBlock) {
+        where[moved[k]] = place[k];
+        a.refs[place[k]] = a.refs[moved[k]];
+        a.refs[moved[k]] = 0;
+    }
+    if (threadIdx.x == 0) {
+        scratch[0] = live;
+        scratch[1] = n_moved;
+        if (live_out) *live_out = live;
+    }
+}
+
+__global__ __launch_bounds__(kCopyBlock) void k_kv_move(KvPagesArgs a, const uint32_t* scratch) {
+    const uint32_t live = scratch[0];
+    const uint32_t *moved = scratch + 2, *place = moved + a.n_pages, *where = place + a.n_pages;
+    const uint32_t parts = (uint32_t)((a.page_bytes + kCopyBytes - 1) / kCopyBytes);
+    const uint64_t units = (uint64_t)scratch[1] * parts;
+    for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const uint32_t i = (uint32_t)(u / parts);
+        copy_part(a, moved[i], place[i], u % parts * kCopyBytes);
+    }
+    for (uint64_t e = (uint64_t)blockIdx.x * kCopyBlock + threadIdx.x; e < (uint64_t)a.n_slots * a.table_width;
+         e += (uint64_t)gridDim.x * kCopyBlock) {
+        const uint32_t slot = (uint32_t)(e / a.table_width), c = (uint32_t)(e % a.table_width);
+        int32_t* entry = a.tables + slot * a.table_stride + c;
+        if (c >= pages_of(a.lens[slot], a.block)) continue;
+        const uint32_t id = (uint32_t)*entry;
+        if (id >= live && id < a.n_pages) *entry = (int32_t)where[id];
+    }
+}
+
+uint32_t copy_grid(const KvPagesArgs& a, uint64_t pages) {
+    const uint64_t units = pages * ((a.page_bytes + kCopyBytes - 1) / kCopyBytes);
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(units, kCopyGrid));
+}
+
+}  // namespace
+
+int launch_kv_resize(const KvPagesArgs& a, const int32_t* slots, const int32_t* new_lens, uint32_t n, uint32_t* scratch,
+                     uint32_t* status, hipStream_t st) {
+    hipLaunchKernelGGL(k_kv_resize, dim3(1), dim3(kOwnerBlock), 0, st, a, slots, new_lens, n, scratch, status);
+    hipLaunchKernelGGL(k_kv_copy_taken, dim3(copy_grid(a, n)), dim3(kCopyBlock), 0, st, a, scratch);
+    return hip_status(hipGetLastError(), "kv_resize");
+}
+
+int launch_kv_fork(const KvPagesArgs& a, const int32_t* src, const int32_t* dst, uint32_t n, uint32_t* scratch, uint32_t* status,
+                   hipStream_t st) {
+    hipLaunchKernelGGL(k_kv_fork, dim3(1), dim3(kOwnerBlock), 0, st, a, src, dst, n, scratch, status);
+    hipLaunchKernelGGL(k_kv_copy_taken, dim3(copy_grid(a, n)), dim3(kCopyBlock), 0, st, a, scratch);
+    return hip_status(hipGetLastError(), "kv_fork");
+}
+
+int launch_kv_compact(const KvPagesArgs& a, uint32_t* scratch, uint32_t* live, hipStream_t st) {
+    hipLaunchKernelGGL(k_kv_compact, dim3(1), dim3(kOwnerBlock), 0, st, a, scratch, live);
+    hipLaunchKernelGGL(k_kv_move, dim3(copy_grid(a, a.n_pages)), dim3(kCopyBlock), 0, st, a, scratch);
+    return hip_status(hipGetLastError(), "kv_compact");
+}
+
+int launch_kv_copy_pages(const KvPagesArgs& a, const int32_t* src, const int32_t* dst, uint32_t n, uint32_t* status, hipStream_t st) {
+    hipLaunchKernelGGL(k_kv_copy_listed, dim3(copy_grid(a, n)), dim3(kCopyBlock), 0, st, a, src, dst, n, status);
+    return hip_status(hipGetLastError(), "kv_copy_pages");
+}
+
+}  // namespace halo_mi

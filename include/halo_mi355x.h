@@ -395,6 +395,256 @@ int halo_mi_get_rows(const halo_mi_get_rows_params* p, void* stream);
 int halo_mi_rms_norm(const float* x, uint64_t x_stride, const float* w, float* out, uint64_t out_stride,
                      uint32_t rows, uint32_t cols, float eps, void* stream);
 
+/* ---- attention over an 8-bit paged cache ---------------------------------------------------- */
+/*
+ * What a layer runs between its q / k / v projections and its output projection, and what a server
+ * runs between steps: PARTIAL_ROPE (RopeArgs), KV_WRITE (KvWriteArgs) and ATTENTION (AttentionArgs)
+ * of the reference's interface (backend.h:369-418) over batches of sequences, with the cache held in
+ * 8 bits (KvType::Q8, backend.h:68-75) in a layout of this library's own.
+ *
+ * Element types (`type`) of q, k, v and out: HALO_MI_F32, HALO_MI_F16, HALO_MI_BF16. Strides count
+ * elements; a stride of 0 is the dense one.
+ *
+ * Device lists (positions, tables, lengths, row starts, slots) are read when the kernel runs, so a
+ * captured call follows their values at each replay. What they hold is checked on the device: an
+ * entry out of range is never followed; it sets a bit of the optional status word (as in
+ * halo_mi_get_rows: cleared by the call unless status_keep).
+ */
+#define HALO_MI_STATUS_KV_FULL 16u /* a sequence found no free page, or its table no column */
+
+/* The two elements that a rotation takes together, of the first rot_dims of a head. */
+enum {
+    HALO_MI_ROPE_HALF = 0,       /* i and i + rot_dims / 2 */
+    HALO_MI_ROPE_INTERLEAVED = 1 /* 2 i and 2 i + 1 */
+};
+
+enum {
+    HALO_MI_ROPE_PLAIN = 0,  /* f_i = theta^(-2 i / rot_dims) radians per position */
+    HALO_MI_ROPE_LINEAR = 1, /* f_i / scale */
+    HALO_MI_ROPE_NTK = 2,    /* theta times scale^(rot_dims / (rot_dims - 2)) */
+    HALO_MI_ROPE_YARN = 3    /* f_i / scale for pairs that turn less than beta_slow times over `context` positions, f_i for
+                                pairs that turn more than beta_fast times, a linear ramp between; factor 0.1 ln(scale) + 1 */
+};
+
+typedef struct halo_mi_rope_scaling {
+    uint32_t kind;
+    double scale;     /* >= 1 */
+    double context;   /* YARN: the positions that the model was trained on */
+    double beta_fast; /* YARN: 32 in the usual models */
+    double beta_slow; /* YARN: 1 */
+} halo_mi_rope_scaling;
+
+/*
+ * Host: the rot_dims / 2 frequencies in radians per position, in 64 bits, and the factor that the
+ * rotated values are multiplied by (1 but for YARN). A program computes them once per model and keeps
+ * the table on the device. scaling may be NULL (PLAIN).
+ */
+int halo_mi_rope_freqs(uint32_t rot_dims, double theta, const halo_mi_rope_scaling* scaling, double* freqs, float* factor);
+
+/*
+ * Rotary positions of q and, in the same launch, k: with a = positions[t] * freqs[i], the pair (x, y)
+ * becomes factor * (x cos a - y sin a, y cos a + x sin a); elements from rot_dims on are copied. The
+ * angle is reduced in 64 bits, so far positions keep their precision; products are in 32 bits.
+ *   parts[0..n_parts): in, out: n_tokens rows of n_heads heads of head_dim elements (n_heads may be 0); out may be in
+ *          (same strides), or must not overlap it or any other operand.
+ *   rot_dims: even, 2..min(head_dim, 512). freqs: rot_dims / 2 doubles on the device (8-byte aligned).
+ *   positions: n_tokens int32 on the device, any value.
+ */
+typedef struct halo_mi_rope_part {
+    const void* in;
+    uint64_t in_stride, in_head_stride;
+    void* out;
+    uint64_t out_stride, out_head_stride;
+    uint32_t n_heads;
+} halo_mi_rope_part;
+
+typedef struct halo_mi_rope_params {
+    uint32_t type;
+    uint32_t pairs;
+    const halo_mi_rope_part* parts;
+    uint32_t n_parts; /* 1 or 2 */
+    uint32_t n_tokens, head_dim, rot_dims;
+    const int32_t* positions;
+    const double* freqs;
+    float factor;
+} halo_mi_rope_params;
+
+int halo_mi_rope(const halo_mi_rope_params* p, void* stream);
+
+/*
+ * The cache: n_pages records of halo_mi_kv_page_bytes() bytes each (pool 16-byte aligned). A page holds
+ * block_tokens tokens of every layer:
+ *   int8 codes, for each layer: K [head][token][dim], then V [head][dim][token];
+ *   then fp32 scales, for each layer: K [head], then V [head]; then padding to a multiple of 128 bytes.
+ * A code c stands for c * scale. A scale is 0 (all codes 0) or at least 2^-80; NaN marks a block that
+ * was given a value that is not finite, and everything read from it is NaN.
+ * head_dim: 64, 96, 128, 192 or 256. block_tokens: 16, 32, 64 or 128.
+ */
+typedef struct halo_mi_kv_cache {
+    void* pool;
+    uint32_t n_pages, n_layers, n_kv_heads, head_dim, block_tokens;
+} halo_mi_kv_cache;
+
+/* Bytes of a page; 0 on error. */
+uint64_t halo_mi_kv_page_bytes(uint32_t n_layers, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_tokens);
+
+/*
+ * A batch of sequences. Rows [row_starts[s], row_starts[s + 1]) of the call's row operands are the LAST
+ * tokens of sequence s, which holds kv_lens[s] tokens with them: row i of n stands at position
+ * kv_lens[s] - n + i. Rows below row_starts[0] or from row_starts[n_seqs] on belong to no sequence:
+ * they are neither read nor written. Token t of s lives in page tables[s * table_stride + t / block_tokens].
+ *   tables: n_seqs rows of table_width int32, table_stride apart (0 = table_width).
+ *   kv_lens: n_seqs int32. row_starts: n_seqs + 1 int32, not decreasing, at most n_rows.
+ *   max_rows, max_kv: the most rows and tokens of a sequence, as the host knows them (0: n_rows, and
+ *     table_width * block_tokens). They shape the launch; larger values than these on the device are still
+ *     computed whole, only slower.
+ */
+typedef struct halo_mi_kv_batch {
+    const int32_t* tables;
+    uint64_t table_stride;
+    uint32_t table_width;
+    const int32_t* kv_lens;
+    const int32_t* row_starts;
+    uint32_t n_seqs, n_rows;
+    uint32_t max_rows, max_kv;
+} halo_mi_kv_batch;
+
+/*
+ * KV_WRITE: the batch's rows of k and v (n_rows rows of n_kv_heads heads of head_dim) into the sequences'
+ * pages of `layer`. Per (page, K or V, head), with amax over the rows that fall into the page:
+ *   scale' = max(scale, amax / 127), rounded to fp32; scale counts as 0 where the first row is the
+ *            page's first token; an amax / 127 below 2^-80 counts as 0;
+ *   code   = x / scale' rounded to the nearest integer, ties to even (0 where scale' is 0);
+ *   codes of the page's earlier tokens become code * scale / scale', rounded the same way, where the scale grew.
+ * A value that is not finite makes the scale NaN. Tokens of the page behind the last row keep their
+ * bytes. Every page that a call writes must belong to one sequence of the batch, in one place of its table.
+ * Rows at negative positions (more rows than kv_lens) are not written. A page id outside [0, n_pages), or a
+ * token past the table's columns, is not written and sets HALO_MI_STATUS_BAD_INDEX.
+ */
+typedef struct halo_mi_kv_write_params {
+    uint32_t type;
+    halo_mi_kv_cache cache;
+    uint32_t layer;
+    halo_mi_kv_batch batch;
+    const void* k;
+    uint64_t k_stride, k_head_stride;
+    const void* v;
+    uint64_t v_stride, v_head_stride;
+    uint32_t* status;
+    uint32_t status_keep;
+} halo_mi_kv_write_params;
+
+int halo_mi_kv_write(const halo_mi_kv_write_params* p, void* stream);
+
+/*
+ * The values that the cache holds for the batch's rows: code * scale in fp32, k_out and v_out n_rows
+ * rows of n_kv_heads heads of head_dim floats (either may be NULL). Rows at negative positions are zeros; rows in a
+ * page out of range are NaN and set HALO_MI_STATUS_BAD_INDEX.
+ */
+typedef struct halo_mi_kv_read_params {
+    halo_mi_kv_cache cache;
+    uint32_t layer;
+    halo_mi_kv_batch batch;
+    float* k_out;
+    uint64_t k_stride, k_head_stride;
+    float* v_out;
+    uint64_t v_stride, v_head_stride;
+    uint32_t* status;
+    uint32_t status_keep;
+} halo_mi_kv_read_params;
+
+int halo_mi_kv_read(const halo_mi_kv_read_params* p, void* stream);
+
+/*
+ * ATTENTION of the batch's rows over their sequences' cached tokens:
+ *   out[r][h] = sum_t p_t V_t / sum_t p_t, p_t = exp(scale * q[r][h] . K_t), K and V of head h / (n_heads / n_kv_heads),
+ * over the tokens t <= position (causal), and t > position - window where window is not 0. A row that sees
+ * no token (a negative position) is zeros. q and out are n_rows rows of n_heads heads of head_dim; n_heads is
+ * a multiple of n_kv_heads. A row of q that is not finite, and a row that sees a NaN block or a page out of
+ * range, is NaN; tokens that a row does not see never reach it, whatever their bytes are.
+ * Numerics: the codes are exact in the products; q and the softmax weights are rounded to 11 bits for 16-bit types (q
+ * exactly, but for elements under 2^-28 of their row's largest), and carried in two pieces, to within 2^-22,
+ * for fp32; sums and the softmax are in fp32.
+ *   scale: 0 = 1 / sqrt(head_dim).
+ *   workspace (optional, 16-byte aligned): workspace_bytes of device memory for the partial results of long
+ *     sequences, in place of the stream's own workspace. Graphs captured on one stream share that stream's
+ *     workspace: give each its own if their replays may overlap. halo_mi_attention_workspace() says what a
+ *     call makes use of; with less (or on a capturing stream that has none yet) sequences are split less.
+ * out may not overlap q, the pool, the batch's lists or the workspace.
+ */
+typedef struct halo_mi_attention_params {
+    uint32_t type;
+    halo_mi_kv_cache cache;
+    uint32_t layer;
+    halo_mi_kv_batch batch;
+    const void* q;
+    uint64_t q_stride, q_head_stride;
+    void* out;
+    uint64_t out_stride, out_head_stride;
+    uint32_t n_heads;
+    float scale;
+    uint32_t window;
+    void* workspace;
+    uint64_t workspace_bytes;
+    uint32_t* status;
+    uint32_t status_keep;
+} halo_mi_attention_params;
+
+int halo_mi_attention(const halo_mi_attention_params* p, void* stream);
+/* The workspace bytes that the call splits as it likes best with (0: none, or an argument out of range). */
+uint64_t halo_mi_attention_workspace(const halo_mi_attention_params* p);
+
+/*
+ * The pages' owner, kept on the device: how often each page is held (refs, n_pages int32), and each
+ * slot's tokens and pages (lens n_slots int32, tables n_slots rows of table_width int32, table_stride apart, 0 =
+ * table_width; entries past ceil(len / block_tokens) are not read). A slot is a sequence or is empty (length 0).
+ * The calls read and change this state in stream order, with no word from the host: a free page is one with refs
+ * 0, and the lowest free ones are given first, in the order of the call's list. A listed slot outside [0,
+ * n_slots), one that the list names before, and a page id out of range leave their entry's slot as it is and set
+ * HALO_MI_STATUS_BAD_INDEX. Where the pages run out, that entry and every later one that needs pages are left as they
+ * are and HALO_MI_STATUS_KV_FULL is set; so is an entry whose length does not fit the table's columns.
+ * At most HALO_MI_KV_LIST_MAX entries a call.
+ */
+#define HALO_MI_KV_LIST_MAX 1024u
+
+typedef struct halo_mi_kv_state {
+    int32_t* refs;
+    int32_t* lens;
+    int32_t* tables;
+    uint64_t table_stride;
+    uint32_t table_width, n_slots;
+} halo_mi_kv_state;
+
+/*
+ * Gives slots[i] the length new_lens[i], i < n: grown, it gets pages (their bytes are whatever they were);
+ * shrunk, the pages that it no longer needs are released (length 0 frees the slot); their table entries become -1. Where a slot
+ * grows behind tokens in a page that another slot holds too, it gets a copy of that page. Pages released by a
+ * call are free from the next call on. A negative length is out of range.
+ */
+int halo_mi_kv_resize(const halo_mi_kv_cache* cache, const halo_mi_kv_state* state, const int32_t* slots,
+                      const int32_t* new_lens, uint32_t n, uint32_t* status, uint32_t status_keep, void* stream);
+
+/*
+ * dst[i] becomes a copy of src[i], i < n: whole pages are shared (refs + 1), a last page that is not full is
+ * copied. dst[i] must be an empty slot (otherwise it is left as it is, HALO_MI_STATUS_BAD_INDEX); sources are
+ * read as they were before the call.
+ */
+int halo_mi_kv_fork(const halo_mi_kv_cache* cache, const halo_mi_kv_state* state, const int32_t* src, const int32_t* dst,
+                    uint32_t n, uint32_t* status, uint32_t status_keep, void* stream);
+
+/*
+ * Moves the live pages (refs > 0) to the front of the pool: with L of them, the k-th live page at or past L goes
+ * to the k-th free place below L, its table entries and its count with it. live (optional, one uint32 on the device) receives L.
+ */
+int halo_mi_kv_compact(const halo_mi_kv_cache* cache, const halo_mi_kv_state* state, uint32_t* live, void* stream);
+
+/*
+ * Copies page src[i] to page dst[i], i < n, all layers. No destination may be named twice or be a source.
+ * A pair with an id out of range is skipped and sets HALO_MI_STATUS_BAD_INDEX.
+ */
+int halo_mi_kv_copy_pages(const halo_mi_kv_cache* cache, const int32_t* src, const int32_t* dst, uint32_t n, uint32_t* status,
+                          uint32_t status_keep, void* stream);
+
 /* ---- stream state --------------------------------------------------------------------------- */
 /*
  * The kernels' own failures cannot be returned by the call that enqueued them. A split-K
