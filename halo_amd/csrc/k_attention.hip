@@ -28,250 +28,471 @@ namespace {
 using namespace dev;
 
 constexpr uint32_t kAttnWaves = 4;
-constexpr uint32_t kStep = 64;  // tokens a wave takes at a time
+constexpr uint32_t kStep = 64;                     // tokens a wave takes at a time
+constexpr uint32_t kChunk = kAttnWaves * kStep;    // tokens a workgroup takes at a time
+constexpr uint32_t kChunkLog2 = 8;
+static_assert(kChunk == 1u << kChunkLog2);
 // Weights are carried times 2^14, which leaves f16 all of its 11 bits for weights down to 2^-28.
 constexpr float kWeightShift = 14.0f;
-constexpr float kLog2Tiny = -80.0f;  // log2 of the scale that an all-zero block of V counts with
+constexpr uint32_t kFewGrid = 512;      // workgroups of a call with few rows at most: two per CU
+constexpr float kTinyScale = 0x1p-80f;  // the scale that an all-zero block of V counts with
 
-__device__ __forceinline__ float load_any(const void* p, uint32_t type, uint64_t i) {
-    if (type == HALO_MI_F16) return (float)static_cast<const _Float16*>(p)[i];
-    if (type == HALO_MI_BF16) return (float)static_cast<const __bf16*>(p)[i];
-    return static_cast<const float*>(p)[i];
+__device__ __forceinline__ float quiet_nan() { return __uint_as_float(0x7FC00000u); }
+
+// max over the lanes of a column: lane, lane ^ 16, lane ^ 32, lane ^ 48
+__device__ __forceinline__ float column_max(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    v = fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+}
+__device__ __forceinline__ float column_sum(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    v = __int_as_float(r[0]) + __int_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+
+// Eight consecutive elements as fp32. wide: p is 16-byte aligned.
+__device__ __forceinline__ void load8(const void* base, uint32_t type, uint64_t i, bool wide, float (&v)[8]) {
+    if (type == HALO_MI_F32) {
+        const float* p = static_cast<const float*>(base) + i;
+        if (wide) {
+            const float4v a = reinterpret_cast<const float4v*>(p)[0], b = reinterpret_cast<const float4v*>(p)[1];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = p[j];
+        }
+        return;
+    }
+    const uint16_t* p = static_cast<const uint16_t*>(base) + i;
+    uint16_t h[8];
+    if (wide) {
+        const Vec<uint16_t, 8> a = *reinterpret_cast<const Vec<uint16_t, 8>*>(p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = a.v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = p[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        v[j] = type == HALO_MI_F16 ? (float)__builtin_bit_cast(_Float16, h[j]) : __uint_as_float((uint32_t)h[j] << 16);
 }
 __device__ __forceinline__ void store_any(void* p, uint32_t type, uint64_t i, float v) {
     if (type == HALO_MI_F16) static_cast<_Float16*>(p)[i] = (_Float16)v;
     else if (type == HALO_MI_BF16) static_cast<__bf16*>(p)[i] = (__bf16)v;
     else static_cast<float*>(p)[i] = v;
 }
+// Whether rows can be read and written 16 bytes at a time (uniform).
+__device__ __forceinline__ bool wide_rows(const HeadRows& r, uint32_t type) {
+    const uint32_t mask = type == HALO_MI_F32 ? 3 : 7;
+    return reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && ((r.stride | r.head_stride) & mask) == 0;
+}
+// Four consecutive outputs, of any alignment.
+__device__ __forceinline__ void store4(const HeadRows& r, uint32_t type, uint64_t i, float4v v) {
+    void* p = const_cast<void*>(r.data);
+    if (wide_rows(r, type)) {
+        if (type == HALO_MI_F32) *reinterpret_cast<float4v*>(static_cast<float*>(p) + i) = v;
+        else if (type == HALO_MI_F16) *reinterpret_cast<Vec<_Float16, 4>*>(static_cast<_Float16*>(p) + i) = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+        else *reinterpret_cast<Vec<__bf16, 4>*>(static_cast<__bf16*>(p) + i) = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) store_any(p, type, i + j, v[j]);
+}
 
-// Partial results of (row, head) r and split s: D outputs (unnormalised), then the maximum and the sum.
-__device__ __forceinline__ float* part_of(const AttnArgs& a, uint64_t r, uint32_t s) {
-    return a.part + (r * a.splits + s) * (a.c.dim + 4);
+// A lane's row of a tile of 16: its tokens [lo, hi), q as f16 fragments scaled to the top of f16's range, and what
+// takes a score to the exponent's base 2: scale * log2(e) / (what q was scaled by), NaN where the row is not
+// finite. A negative scale turns q's sign, so that `c` is never negative.
+template <int D, int NP>
+struct QRow {
+    static constexpr int F = D / 32;  // fragments of 32 dims
+    half8v f[F][NP];
+    float c;
+    int32_t lo, hi;
+
+    // dim of element 0 of fragment i in lane group g: 16 bytes of codes hold two fragments' elements
+    static __device__ __forceinline__ uint32_t dim(int i, uint32_t g) {
+        return i / 2 * 2 + 1 < F ? i / 2 * 64 + 16 * g + i % 2 * 8 : i * 32 + 8 * g;
+    }
+
+    // packed row r of `packed`: token r / group, head r % group of kv head kvh. fetch only loads; finish converts.
+    __device__ __forceinline__ void fetch(const AttnArgs& a, const SeqRows& sr, uint32_t kvh, uint32_t r, uint32_t packed, uint32_t g,
+                                          int32_t cap, float (&v)[F][8]) {
+        const bool live = r < packed;
+        const uint32_t token = live ? r / a.group : 0, head = kvh * a.group + (live ? r % a.group : 0);
+        const uint64_t at = (uint64_t)(sr.row0 + token) * a.q.stride + head * a.q.head_stride;
+        const int32_t pos = sr.len - sr.rows + (int32_t)token;
+        hi = live ? max(pos + 1, 0) : 0;
+        lo = a.window ? min(max(pos - (int32_t)a.window + 1, 0), cap) : 0;
+        const bool wide = wide_rows(a.q, a.type);
+#pragma unroll
+        for (int i = 0; i < F; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < F; ++i) load8(a.q.data, a.type, at + dim(i, g), wide, v[i]);
+        }
+    }
+    __device__ __forceinline__ void finish(const AttnArgs& a, const float (&v)[F][8]) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < F; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[i][j]));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        const bool bad = top > kLargestFinite;
+        const int e = top == 0 || bad ? 0 : top < 0x00800000u ? (int)(31 - __builtin_clz(top)) - 149 : (int)(top >> 23) - 127;
+        c = bad ? quiet_nan() : ldexpf(fabsf(a.scale_log2), e - 14);
+        const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+        for (int i = 0; i < F; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = bad ? 0.0f : ldexpf(v[i][j] * sign, 14 - e);
+                f[i][0][j] = (_Float16)x;
+                if constexpr (NP == 2) f[i][1][j] = (_Float16)(x - (float)f[i][0][j]);
+            }
+    }
+};
+
+// What a lane group has of a step: K's and V's scales of its 16 tokens' block.
+struct Scales {
+    float k, lv, rv;  // K's; log2 of V's and its reciprocal
+};
+__device__ __forceinline__ Scales make_scales(float ks, float vs, bool page) {
+    vs = vs == 0.0f ? kTinyScale : vs;
+    return {page ? ks : quiet_nan(), __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
+}
+
+// The running maximum and sum of a row, and its outputs: O^T as DT tiles of 16 dims.
+template <int DT>
+struct Running {
+    float m, l;
+    float4v o[DT];
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] = float4v{0, 0, 0, 0};
+    }
+
+    // A step's scores become weights w = 2^(s k + lv - m + 14) as f16 fragments; m, l and o follow. tg: the
+    // position of this lane group's first token. all: every row sees every token (uniform).
+    template <int NP>
+    __device__ __forceinline__ void weigh(const float4v (&s)[4], const Scales& sc, float c, uint32_t tg, int32_t lo, int32_t hi, bool all,
+                                          half8v (&w)[2][NP]) {
+        const float k = sc.k * c;
+        float x[16];
+        float top = -INFINITY;
+        if (all) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                x[i] = fmaf(s[i / 4][i % 4], k, sc.lv);
+                top = fmaxf(top, x[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int32_t token = (int32_t)(tg + i);
+                x[i] = token >= lo && token < hi ? fmaf(s[i / 4][i % 4], k, sc.lv) : -INFINITY;
+                top = fmaxf(top, x[i]);
+            }
+        }
+        top = column_max(top);
+        if (__ballot(top > m)) {
+            const float m_new = fmaxf(m, top), f = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[t] *= f;
+            m = m_new;
+        }
+        const float shift = m == -INFINITY ? 0.0f : m - kWeightShift;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float v = __builtin_amdgcn_exp2f(x[i] - shift);
+            sum += v;
+            w[i / 8][0][i % 8] = (_Float16)v;
+            if constexpr (NP == 2) w[i / 8][1][i % 8] = (_Float16)(v - (float)w[i / 8][0][i % 8]);
+        }
+        l += sum == 0.0f ? 0.0f : sum * sc.rv;
+    }
+};
+
+__device__ __forceinline__ float4v mfma(half8v a, half8v b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// ---- few rows: the cache is streamed once ---------------------------------------------------------------------
+//
+// Work is cut into units: a unit is a.unit tokens (a multiple of kChunk) of one (sequence, kv head, row tile). All
+// units of the call, in that order, are dealt out evenly to the workgroups, each a run of `per`, so a batch
+// of ragged lengths loads every CU alike and no length is needed on the host. Where a run ends inside a
+// (sequence, kv head, tile), the parts meet in the workspace: slot 0 of a workgroup holds its first
+// segment, slot 1 its last. A segment that is whole writes out itself. Inside a unit a wave takes every fourth step.
+
+// A sequence in units.
+struct SeqUnits {
+    SeqRows r;
+    int32_t begin, end;  // tokens that its rows see: from a multiple of kStep
+    uint32_t chunks, tiles;
+    uint32_t units;
+};
+
+template <int ROWS>
+__device__ __forceinline__ SeqUnits seq_units(const AttnArgs& a, uint32_t seq) {
+    SeqUnits u;
+    u.r = seq_rows(a.b, seq);
+    const int32_t cap = (int32_t)(a.b.table_width * a.c.block);
+    u.begin = a.window ? min(max(u.r.len - u.r.rows - (int32_t)a.window + 1, 0), cap) / (int32_t)kStep * (int32_t)kStep : 0;
+    u.end = min(u.r.len, cap + 16);  // past the table: one group out of range, which makes its rows NaN
+    // without memory for parts a unit is all of its tokens
+    u.chunks = a.part && u.end > u.begin ? ((uint32_t)(u.end - u.begin) + a.unit - 1) >> a.unit_log2 : 1;
+    u.tiles = ((uint32_t)u.r.rows * a.group + ROWS - 1) / ROWS;
+    u.units = a.c.heads * u.tiles * u.chunks;
+    return u;
+}
+
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t below = (uint32_t)__shfl_up((int)v, off);
+        if (lane >= (uint32_t)off) v += below;
+    }
+    return v;
+}
+
+// The run of units of a workgroup (of `workgroups`), and the sequence that the run's first unit lies in, with the
+// units before that sequence. Every wave finds them for itself, 64 sequences at a time.
+struct Run {
+    uint32_t total, per;
+    uint32_t first, last;  // [first, last)
+    uint32_t seq, before;
+};
+template <int ROWS>
+__device__ __forceinline__ Run find_run(const AttnArgs& a, uint32_t lane, uint32_t workgroups, uint32_t id) {
+    Run r{};
+    const auto units = [&](uint32_t s) { return s < a.b.n_seqs ? seq_units<ROWS>(a, s).units : 0; };
+    uint32_t v = units(lane), sum = wave_scan(v, lane);
+    r.total = (uint32_t)__shfl((int)sum, 63);
+    for (uint32_t s0 = 64; s0 < a.b.n_seqs; s0 += 64) r.total += (uint32_t)__shfl((int)wave_scan(units(s0 + lane), lane), 63);
+    r.per = max(1u, (r.total + workgroups - 1) / workgroups);
+    r.first = min(id * r.per, r.total);
+    r.last = min(r.first + r.per, r.total);
+    for (uint32_t s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
+        if (s0) v = units(s0 + lane), sum = wave_scan(v, lane);
+        const uint64_t hit = __ballot(r.before + sum > r.first);
+        if (hit) {
+            const uint32_t l = (uint32_t)__ffsll((long long)hit) - 1;
+            r.before += (uint32_t)__shfl((int)(sum - v), l);
+            r.seq = s0 + l;
+            break;
+        }
+        r.before += (uint32_t)__shfl((int)sum, 63);
+    }
+    return r;
+}
+
+// Partial results of workgroup w's segment `slot`: ROWS rows of D outputs (unnormalised), the maximum and the sum.
+template <int ROWS>
+__device__ __forceinline__ float* part_of(const AttnArgs& a, uint64_t w, uint32_t slot, uint32_t row) {
+    return a.part + ((w * 2 + slot) * ROWS + row) * (a.c.dim + 4);
 }
 
 // D: head_dim. NP: f16 pieces of q and of the weights. NQ: row tiles of 16 that share K and V.
 template <int D, int NP, int NQ>
-__global__ __launch_bounds__(kAttnWaves * 64) void k_attention(AttnArgs a) {
+__global__ __launch_bounds__(kAttnWaves * 64, D <= 128 && NQ == 1 ? 2 : 1) void k_attention_few(AttnArgs a) {
     constexpr int C = D / 64, TAIL = D % 64 / 32;  // 64-dim chunks of a K row, and a last one of 32
     constexpr int DT = D / 16;                     // tiles of 16 dims
     constexpr int ROWS = 16 * NQ;
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, g = lane / 16;
-    uint32_t id = blockIdx.x;
-    const uint32_t split = id % a.splits;
-    id /= a.splits;
-    const uint32_t tile0 = id % a.tiles;
-    id /= a.tiles;
-    const uint32_t kvh = id % a.c.heads, seq = id / a.c.heads;
-    const SeqRows sr = seq_rows(a.b, seq);
-    const int32_t first = sr.len - sr.rows;  // position of the sequence's first row
-    const uint32_t packed = (uint32_t)sr.rows * a.group;
-    // tokens that the table has room for; what a length claims beyond is one group out of range (NaN)
-    const int32_t cap = (int32_t)(a.b.table_width * a.c.block);
-
-    __shared__ float lds_o[kAttnWaves][16][64 + 4];
+    constexpr int kWide = D < 128 ? D : 128;  // outputs that meet in LDS at a time
+    __shared__ __align__(16) float lds_o[kAttnWaves][16][kWide + 4];
     __shared__ float lds_m[kAttnWaves][ROWS], lds_l[kAttnWaves][ROWS];
 
-    for (uint32_t tile = tile0; tile * ROWS < packed; tile += a.tiles) {
-        // rows of this tile: packed row r is token r / group, head r % group of the kv head's
-        half8v qf[NQ][2 * C + TAIL][NP];
-        float c_log2[NQ];      // scale * log2(e) * 2^-(what q was scaled by)
-        int32_t lo[NQ], hi[NQ];  // tokens that this lane's row sees: [lo, hi)
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            const uint32_t r = tile * ROWS + 16 * n + col;
-            const bool live = r < packed;
-            const uint32_t token = live ? r / a.group : 0, head = kvh * a.group + (live ? r % a.group : 0);
-            const uint64_t at = (uint64_t)(sr.row0 + token) * a.q.stride + head * a.q.head_stride;
-            const int32_t pos = first + (int32_t)token;
-            hi[n] = live ? max(pos + 1, 0) : 0;
-            lo[n] = a.window ? min(max(pos - (int32_t)a.window + 1, 0), cap) : 0;
-            uint32_t top = 0;
-#pragma unroll
-            for (int f = 0; f < 2 * C + TAIL; ++f)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t d = f < 2 * C ? f / 2 * 64 + 16 * g + f % 2 * 8 + j : C * 64 + 8 * g + j;
-                    top = max(top, live ? abs_bits(load_any(a.q.data, a.type, at + d)) : 0u);
-                }
-            top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-            top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-            const int e = top ? ilogbf(__uint_as_float(min(top, kLargestFinite))) : 0;
-            const bool bad = top > kLargestFinite;
-            c_log2[n] = bad ? __uint_as_float(0x7FC00000u) : ldexpf(a.scale_log2, e - 14);
-#pragma unroll
-            for (int f = 0; f < 2 * C + TAIL; ++f)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t d = f < 2 * C ? f / 2 * 64 + 16 * g + f % 2 * 8 + j : C * 64 + 8 * g + j;
-                    const float v = live && !bad ? ldexpf(load_any(a.q.data, a.type, at + d), 14 - e) : 0.0f;
-                    qf[n][f][0][j] = (_Float16)v;
-                    if constexpr (NP == 2) qf[n][f][1][j] = (_Float16)(v - (float)(_Float16)v);
-                }
-        }
-        // the tile's tokens, and this workgroup's share of them
-        const int32_t pos_min = first + (int32_t)(tile * ROWS / a.group);
-        const int32_t pos_max = first + (int32_t)((min(tile * ROWS + ROWS, packed) - 1) / a.group);
-        const int32_t begin = a.window ? min(max(pos_min - (int32_t)a.window + 1, 0), cap) / (int32_t)kStep * (int32_t)kStep : 0;
-        const int32_t end = min(max(pos_max + 1, 0), cap + 16);
-        const int64_t from = begin + (int64_t)split * a.chunk;
-        const int64_t to = split + 1 == a.splits ? end : min((int64_t)end, from + a.chunk);
+    const Run mine = find_run<ROWS>(a, lane, gridDim.x, blockIdx.x);
+    uint32_t u = mine.first, before = mine.before, seq = mine.seq;
+    if (u >= mine.last) return;
+    SeqUnits su = seq_units<ROWS>(a, seq);
+    const int32_t cap = (int32_t)(a.b.table_width * a.c.block);
 
-        float4v o[NQ][DT];
-        float m[NQ], l[NQ];
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            m[n] = -INFINITY;
-            l[n] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < DT; ++t) o[n][t] = float4v{0, 0, 0, 0};
+    for (bool first = true; u < mine.last; first = false) {
+        while (u >= before + su.units) {
+            before += su.units;
+            su = seq_units<ROWS>(a, ++seq);
         }
-        for (int64_t t64 = from + wave * kStep; t64 < to; t64 += kAttnWaves * kStep) {
-            const uint32_t t0 = (uint32_t)t64;
-            // the page of group g; a page out of range reads page 0 and counts as NaN
+        // the segment: chunks [chunk, chunk + n) of (seq, kvh, tile)
+        const uint32_t in_seq = (u - before) / su.chunks, chunk = (u - before) - in_seq * su.chunks;
+        const uint32_t kvh = in_seq / su.tiles, tile = in_seq % su.tiles;
+        const uint32_t n_chunks = min(su.chunks - chunk, mine.last - u);
+        const bool whole = n_chunks == su.chunks;
+        u += n_chunks;
+        const uint32_t packed = (uint32_t)su.r.rows * a.group;
+
+        // tokens that every row of the tile sees
+        const int32_t pos0 = su.r.len - su.r.rows + (int32_t)(tile * ROWS / a.group);
+        const int32_t pos1 = su.r.len - su.r.rows + (int32_t)((min(tile * ROWS + ROWS, packed) - 1) / a.group);
+        const uint32_t all_hi = (uint32_t)max(pos0 + 1, 0), all_lo = a.window ? (uint32_t)max(pos1 - (int32_t)a.window + 1, 0) : 0;
+        const uint32_t end = (uint32_t)max(min(pos1 + 1, su.end), 0);
+        const uint32_t t_first = (uint32_t)su.begin + (chunk << a.unit_log2) + wave * kStep;
+        const uint32_t t_end = whole ? end : min((uint32_t)su.begin + ((chunk + n_chunks) << a.unit_log2), end);
+
+        const int32_t* table = a.b.tables + (uint64_t)seq * a.b.table_stride;
+        const uint32_t head_codes = a.c.codes + kvh * a.c.plane;
+        // the table entry of this lane group's 16 tokens of the step at t
+        const auto entry = [&](uint32_t t) { return table[min((t + 16 * g) >> a.c.block_log2, a.b.table_width - 1)]; };
+        // ... and what it says: the page, or page 0 and `ok` false
+        const auto page_of = [&](uint32_t t, int32_t id, bool& ok) {
+            const uint32_t tg = t + 16 * g;
+            ok = (uint32_t)id < a.c.n_pages && (tg >> a.c.block_log2) < a.b.table_width;
+            return page_ptr(a.c, ok ? id : 0);
+        };
+        uint4 kb[4][C > 0 ? C : 1];
+        uint2 kt[4];
+        float ks = 0.0f, vs = 0.0f;
+        bool ok = true;
+        const uint8_t* page = a.c.pool;
+        // K of the step at t: the K row of tile i in this lane is token 4 i + col % 4 of group col / 4
+        const auto load_k = [&](uint32_t t, int32_t id) {
+            page = page_of(t, id, ok);
+            const uint32_t row = (t + 16 * (col / 4)) % a.c.block + col % 4;
+            const uint8_t* k = reinterpret_cast<const uint8_t*>(__shfl((long long)page, 16 * (col / 4))) + head_codes + row * D;
+            const float* sc = reinterpret_cast<const float*>(page + a.c.scales) + kvh;
+            ks = sc[0];
+            vs = sc[a.c.heads];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int c = 0; c < C; ++c) kb[i][c] = *reinterpret_cast<const uint4*>(k + 4 * i * D + c * 64 + 16 * g);
+                if constexpr (TAIL) kt[i] = *reinterpret_cast<const uint2*>(k + 4 * i * D + C * 64 + 8 * g);
+            }
+        };
+        int32_t id_next = 0;
+        QRow<D, NP> q[NQ];
+        Running<DT> run[NQ];
+        {
+            const int32_t id = t_first < t_end ? entry(t_first) : 0;
+            float raw[NQ][QRow<D, NP>::F][8];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) q[n].fetch(a, su.r, kvh, tile * ROWS + 16 * n + col, packed, g, cap, raw[n]);
+            if (t_first < t_end) {
+                load_k(t_first, id);
+                id_next = entry(t_first + kChunk);
+            }
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                q[n].finish(a, raw[n]);
+                run[n].clear();
+            }
+        }
+        for (uint32_t t0 = t_first; t0 < t_end; t0 += kChunk) {
             const uint32_t tg = t0 + 16 * g;
-            int32_t page = 0;
-            bool no_page = false;
-            if (tg < (uint32_t)end) {
-                page = page_at(a.b, a.c, seq, tg >> a.c.block_log2);
-                no_page = page < 0;
-                page = max(page, 0);
+            // V of this step: 16 tokens of dim 16 i + col of group g
+            uint4 vb[DT];
+            {
+                const uint8_t* v = page + head_codes + a.c.heads * a.c.plane + col * a.c.block + (tg & (a.c.block - 1));
+#pragma unroll
+                for (int i = 0; i < DT; ++i) vb[i] = *reinterpret_cast<const uint4*>(v + i * 16 * a.c.block);
             }
-            const uint8_t* base = page_ptr(a.c, page) + a.c.codes + kvh * a.c.plane;
-            const float* scales = reinterpret_cast<const float*>(page_ptr(a.c, page) + a.c.scales) + kvh;
-            float ks = scales[0], vs = scales[a.c.heads];
-            if (no_page) {
-                ks = __uint_as_float(0x7FC00000u);
-                set_status(a.status, kStatusKvBadIndex);
-            }
-            const float lv = vs == 0.0f ? kLog2Tiny : log2f(vs);
-            const float rv = vs == 0.0f ? 0x1p80f : 1.0f / vs;
-            // S^T: the K row of tile a in this lane is token 4 a + col % 4 of group col / 4
-            const uint32_t row_off = (t0 + 16 * (col / 4)) % a.c.block + col % 4;
-            const uint8_t* krow = reinterpret_cast<const uint8_t*>(__shfl((long long)base, 16 * (col / 4))) + row_off * D;
+            __builtin_amdgcn_sched_barrier(0);
+            const Scales sc = make_scales(ks, vs, ok || tg >= end);
+            if (!ok && tg < end) set_status(a.status, kStatusKvBadIndex);
             float4v s[NQ][4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const uint8_t* k = krow + 4 * t * D;
+            for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) s[n][t] = float4v{0, 0, 0, 0};
+                for (int n = 0; n < NQ; ++n) s[n][i] = float4v{0, 0, 0, 0};
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(k + c * 64 + 16 * g);
-                    const half8v k0 = codes_f16(w.x, w.y), k1 = codes_f16(w.z, w.w);
+                    const half8v k0 = codes_f16(kb[i][c].x, kb[i][c].y), k1 = codes_f16(kb[i][c].z, kb[i][c].w);
 #pragma unroll
                     for (int n = 0; n < NQ; ++n)
 #pragma unroll
                         for (int p = 0; p < NP; ++p) {
-                            s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf[n][2 * c][p], s[n][t], 0, 0, 0);
-                            s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qf[n][2 * c + 1][p], s[n][t], 0, 0, 0);
+                            s[n][i] = mfma(k0, q[n].f[2 * c][p], s[n][i]);
+                            s[n][i] = mfma(k1, q[n].f[2 * c + 1][p], s[n][i]);
                         }
                 }
                 if constexpr (TAIL) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(k + C * 64 + 8 * g);
-                    const half8v k0 = codes_f16(w.x, w.y);
+                    const half8v k0 = codes_f16(kt[i].x, kt[i].y);
 #pragma unroll
                     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                        for (int p = 0; p < NP; ++p)
-                            s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf[n][2 * C][p], s[n][t], 0, 0, 0);
+                        for (int p = 0; p < NP; ++p) s[n][i] = mfma(k0, q[n].f[2 * C][p], s[n][i]);
                 }
             }
-            half8v wf[NQ][2][NP];
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                const float k = ks * c_log2[n];
-                float x[16], top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int32_t token = (int32_t)(tg + i);
-                    const bool seen = token >= lo[n] && token < hi[n];
-                    x[i] = seen ? fmaf(s[n][i / 4][i % 4], k, lv) : -INFINITY;
-                    top = fmaxf(top, x[i]);
-                }
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float m_new = fmaxf(m[n], top);
-                if (__ballot(m_new > m[n])) {
-                    const float f = m_new == m[n] ? 1.0f : exp2f(m[n] - m_new);
-                    l[n] *= f;
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) o[n][t] *= f;
-                }
-                m[n] = m_new;
-                const float shift = m_new == -INFINITY ? 0.0f : m_new - kWeightShift;
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float w = exp2f(x[i] - shift);
-                    sum += w;
-                    wf[n][i / 8][0][i % 8] = (_Float16)w;
-                    if constexpr (NP == 2) wf[n][i / 8][1][i % 8] = (_Float16)(w - (float)(_Float16)w);
-                }
-                l[n] += sum == 0.0f ? 0.0f : sum * rv;
+            __builtin_amdgcn_sched_barrier(0);
+            if (t0 + kChunk < t_end) {
+                load_k(t0 + kChunk, id_next);
+                id_next = entry(t0 + 2 * kChunk);
             }
-            // O^T: 16 tokens of dim 16 t + col of group g
-            const uint8_t* vrow = base + a.c.heads * a.c.plane + col * a.c.block + (tg & (a.c.block - 1));
+            __builtin_amdgcn_sched_barrier(0);
+            const bool all = t0 >= all_lo && t0 + kStep <= all_hi;
+            half8v w[NQ][2][NP];
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const uint4 w = *reinterpret_cast<const uint4*>(vrow + t * 16 * a.c.block);
-                const half8v v0 = codes_f16(w.x, w.y), v1 = codes_f16(w.z, w.w);
+            for (int n = 0; n < NQ; ++n) run[n].template weigh<NP>(s[n], sc, q[n].c, tg, q[n].lo, q[n].hi, all, w[n]);
+#pragma unroll
+            for (int i = 0; i < DT; ++i) {
+                const half8v v0 = codes_f16(vb[i].x, vb[i].y), v1 = codes_f16(vb[i].z, vb[i].w);
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
 #pragma unroll
                     for (int p = 0; p < NP; ++p) {
-                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, wf[n][0][p], o[n][t], 0, 0, 0);
-                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, wf[n][1][p], o[n][t], 0, 0, 0);
+                        run[n].o[i] = mfma(v0, w[n][0][p], run[n].o[i]);
+                        run[n].o[i] = mfma(v1, w[n][1][p], run[n].o[i]);
                     }
             }
         }
-        // the waves' results: l over the groups, then the waves in order
+        // the waves' results, added in wave order
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            l[n] += __shfl_xor(l[n], 16);
-            l[n] += __shfl_xor(l[n], 32);
+            const float l = column_sum(run[n].l);
             if (g == 0) {
-                lds_m[wave][16 * n + col] = m[n];
-                lds_l[wave][16 * n + col] = l[n];
+                lds_m[wave][16 * n + col] = run[n].m;
+                lds_l[wave][16 * n + col] = l;
             }
         }
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            float top = -INFINITY;
+            float m[kAttnWaves], peak = -INFINITY, sum = 0.0f;
 #pragma unroll
-            for (uint32_t w = 0; w < kAttnWaves; ++w) top = fmaxf(top, lds_m[w][16 * n + col]);
-            const float mine = m[n] == -INFINITY ? (l[n] == 0.0f ? 0.0f : 1.0f) : exp2f(m[n] - top);
+            for (uint32_t w = 0; w < kAttnWaves; ++w) peak = fmaxf(peak, m[w] = lds_m[w][16 * n + col]);
 #pragma unroll
-            for (int d0 = 0; d0 < D; d0 += 64) {
+            for (uint32_t w = 0; w < kAttnWaves; ++w) {
+                // a wave without a maximum has no weights, or only NaN
+                const float l = lds_l[w][16 * n + col];
+                sum += m[w] == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m[w] - peak);
+            }
+            const float part_f = run[n].m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run[n].m - peak);
+            const float f = !whole ? part_f : sum == 0.0f ? 0.0f : part_f / sum;
+            if (!whole && wave == 0 && g == 0) {
+                float* part = part_of<ROWS>(a, blockIdx.x, first ? 0 : 1, 16 * n + col);
+                part[D] = peak;
+                part[D + 1] = sum;
+            }
 #pragma unroll
-                for (int t = 0; t < 4 && d0 / 16 + t < DT; ++t)
+            for (int d0 = 0; d0 < D; d0 += kWide) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) lds_o[wave][col][16 * t + 4 * g + i] = o[n][d0 / 16 + t][i] * mine;
+                for (int t = 0; t < kWide / 16 && d0 / 16 + t < DT; ++t)
+                    *reinterpret_cast<float4v*>(&lds_o[wave][col][16 * t + 4 * g]) = run[n].o[d0 / 16 + t] * f;
                 __syncthreads();
-                constexpr int WIDE = D < 64 ? D : 64;
-                for (uint32_t i = threadIdx.x; i < 16 * WIDE; i += kAttnWaves * 64) {
-                    const uint32_t q = i / WIDE, d = d0 + i % WIDE, r = tile * ROWS + 16 * n + q;
+#pragma unroll
+                for (uint32_t i = threadIdx.x; i < 16 * kWide / 4; i += kAttnWaves * 64) {
+                    const uint32_t row = i / (kWide / 4), d = d0 + i % (kWide / 4) * 4, r = tile * ROWS + 16 * n + row;
                     if (r >= packed || d >= D) continue;
-                    float peak = -INFINITY, sum = 0.0f, acc = 0.0f;
+                    float4v acc = {0, 0, 0, 0};
 #pragma unroll
-                    for (uint32_t w = 0; w < kAttnWaves; ++w) peak = fmaxf(peak, lds_m[w][16 * n + q]);
-#pragma unroll
-                    for (uint32_t w = 0; w < kAttnWaves; ++w) {
-                        const float mw = lds_m[w][16 * n + q], lw = lds_l[w][16 * n + q];
-                        sum += lw == 0.0f ? 0.0f : lw * (mw == -INFINITY ? 1.0f : exp2f(mw - peak));
-                        acc += lds_o[w][q][i % WIDE];
-                    }
-                    const uint32_t token = r / a.group, head = kvh * a.group + r % a.group;
-                    if (a.splits > 1) {
-                        float* part = part_of(a, (uint64_t)(sr.row0 + token) * a.heads + head, split);
-                        part[d] = acc;
-                        if (d == 0) {
-                            part[D] = peak;
-                            part[D + 1] = sum;
-                        }
+                    for (uint32_t w = 0; w < kAttnWaves; ++w) acc += *reinterpret_cast<const float4v*>(&lds_o[w][row][d - d0]);
+                    if (!whole) {
+                        *reinterpret_cast<float4v*>(part_of<ROWS>(a, blockIdx.x, first ? 0 : 1, 16 * n + row) + d) = acc;
                     } else {
-                        store_any(const_cast<void*>(a.out.data), a.type,
-                                  (uint64_t)(sr.row0 + token) * a.out.stride + head * a.out.head_stride + d, sum == 0.0f ? 0.0f : acc / sum);
+                        const uint32_t token = r / a.group, head = kvh * a.group + r % a.group;
+                        store4(a.out, a.type, (uint64_t)(su.r.row0 + token) * a.out.stride + head * a.out.head_stride + d, acc);
                     }
                 }
                 __syncthreads();
@@ -280,73 +501,120 @@ __global__ __launch_bounds__(kAttnWaves * 64) void k_attention(AttnArgs a) {
     }
 }
 
-// One wave per (row, head): the splits' results, in order.
-__global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
-    const uint32_t lane = threadIdx.x % 64, D = a.c.dim;
-    const uint64_t r = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    if (r >= (uint64_t)a.b.n_rows * a.heads) return;
-    const uint32_t row = (uint32_t)(r / a.heads), head = (uint32_t)(r % a.heads);
-    const int32_t r0 = max(a.b.row_starts[0], 0), r1 = a.b.row_starts[a.b.n_seqs];
-    if ((int32_t)row < r0 || (int32_t)row >= r1) return;  // of no sequence
-    float peak = -INFINITY;
-    for (uint32_t s = 0; s < a.splits; ++s) peak = fmaxf(peak, part_of(a, r, s)[D]);
-    float sum = 0.0f, acc[4] = {};
-    for (uint32_t s = 0; s < a.splits; ++s) {
-        const float* p = part_of(a, r, s);
-        if (p[D + 1] == 0.0f) continue;
-        const float f = p[D] == -INFINITY ? 1.0f : exp2f(p[D] - peak);
-        sum += p[D + 1] * f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 64 * i < D) acc[i] += p[lane + 64 * i] * f;
+// Joins the parts of the (sequence, kv head, tile)s that several workgroups of k_attention_few had, in unit order: a
+// workgroup has one row. Its threads take the parts' maxima and sums side by side, then, as 256 / (D / 4) groups,
+// every so many-th part's outputs, and the groups are added in order.
+template <int ROWS>
+__global__ __launch_bounds__(256) void k_attention_few_join(AttnArgs a, uint32_t workgroups) {
+    __shared__ float factor[kFewGrid], red[4];
+    __shared__ float4v acc_of[256];
+    const uint32_t tid = threadIdx.x, lane = tid % 64, D = a.c.dim, quads = D / 4;
+    const Run run = find_run<ROWS>(a, lane, workgroups, 0);
+    // blockIdx.x counts (sequence, kv head, tile) by their sequences' most tiles
+    const uint32_t seq = blockIdx.x / (a.c.heads * a.tiles), kvh = blockIdx.x / a.tiles % a.c.heads;
+    const SeqUnits su = seq_units<ROWS>(a, seq);
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < seq; s0 += 64) {
+        const uint32_t v = s0 + lane < seq ? seq_units<ROWS>(a, s0 + lane).units : 0;
+        before += (uint32_t)__shfl((int)wave_scan(v, lane), 63);
     }
+    const uint32_t packed = (uint32_t)su.r.rows * a.group;
+    // of its rows, gridDim.y at a time
+    for (uint32_t tile = blockIdx.x % a.tiles, row = blockIdx.y; tile < su.tiles; row += gridDim.y) {
+        const uint32_t u0 = before + (kvh * su.tiles + tile) * su.chunks, r = tile * ROWS + row;
+        const uint32_t w0 = u0 / run.per, w1 = (u0 + su.chunks - 1) / run.per, n = w1 - w0 + 1;
+        if (n == 1 || row >= ROWS || r >= packed) {
+            tile += a.tiles;
+            row = blockIdx.y - gridDim.y;
+            continue;
+        }
+        // a workgroup that began before u0 has this as its last segment
+        const auto part = [&](uint32_t i) { return part_of<ROWS>(a, w0 + i, (w0 + i) * run.per < u0 ? 1 : 0, row); };
+        float top = -INFINITY;
+        for (uint32_t i = tid; i < n; i += 256) top = fmaxf(top, factor[i] = part(i)[D]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < D)
-            store_any(const_cast<void*>(a.out.data), a.type, row * a.out.stride + head * a.out.head_stride + lane + 64 * i,
-                      sum == 0.0f ? 0.0f : acc[i] / sum);
+        for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+        if (lane == 0) red[tid / 64] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        float sum = 0.0f;
+        for (uint32_t i = tid; i < n; i += 256) {
+            const float l = part(i)[D + 1], f = factor[i] == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(factor[i] - top);
+            factor[i] = f;
+            sum += l * f;
+        }
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
+        __syncthreads();
+        if (lane == 0) red[tid / 64] = sum;
+        __syncthreads();
+        sum = (red[0] + red[1]) + (red[2] + red[3]);
+        const uint32_t groups = 256 / quads, group = tid / quads, d = tid % quads * 4;
+        float4v acc = {0, 0, 0, 0};
+        if (group < groups) {
+#pragma unroll 16
+            for (uint32_t i = group; i < n; i += groups) acc += *reinterpret_cast<const float4v*>(part(i) + d) * factor[i];
+        }
+        acc_of[tid] = acc;
+        __syncthreads();
+        if (group == 0) {
+            for (uint32_t k = 1; k < groups; ++k) acc += acc_of[k * quads + tid];
+            const uint32_t token = r / a.group, head = kvh * a.group + r % a.group;
+            store4(a.out, a.type, (uint64_t)(su.r.row0 + token) * a.out.stride + head * a.out.head_stride + d, sum == 0.0f ? float4v{0, 0, 0, 0} : acc / sum);
+        }
+        __syncthreads();
+    }
 }
 
-uint32_t rows_per_tile(const AttnArgs& a) { return (uint64_t)a.b.max_rows * a.group <= 16 ? 16 : 32; }
+// Rows of a tile: a wider one reads K and V once for twice the rows, where the registers hold its outputs.
+uint32_t few_rows(const AttnArgs& a) { return (uint64_t)a.b.max_rows * a.group <= 16 || a.c.dim > 128 ? 16 : 32; }
 
-template <int D>
-void run_attention(const AttnArgs& a, uint32_t grid, hipStream_t st) {
-    const bool two = a.type == HALO_MI_F32, small = rows_per_tile(a) == 16;
-    auto* k = two ? (small ? k_attention<D, 2, 1> : k_attention<D, 2, 2>) : (small ? k_attention<D, 1, 1> : k_attention<D, 1, 2>);
-    hipLaunchKernelGGL(k, dim3(grid), dim3(kAttnWaves * 64), 0, st, a);
+template <int D, int NP>
+void run_few(const AttnArgs& a, hipStream_t st) {
+    const uint32_t rows = few_rows(a);
+    const dim3 join(a.b.n_seqs * a.c.heads * a.tiles, std::min<uint32_t>(rows, std::max<uint64_t>(1, (uint64_t)a.b.max_rows * a.group)));
+    if constexpr (D <= 128) {
+        if (rows == 32) {
+            hipLaunchKernelGGL((k_attention_few<D, NP, 2>), dim3(a.splits), dim3(kAttnWaves * 64), 0, st, a);
+            if (a.part) hipLaunchKernelGGL(k_attention_few_join<32>, join, dim3(256), 0, st, a, a.splits);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((k_attention_few<D, NP, 1>), dim3(a.splits), dim3(kAttnWaves * 64), 0, st, a);
+    if (a.part) hipLaunchKernelGGL(k_attention_few_join<16>, join, dim3(256), 0, st, a, a.splits);
 }
 
 }  // namespace
 
+// As many workgroups as the registers let run at once, one or two per CU, or fewer where there are not as many units. With memory for fewer parts than there are
+// (sequence, kv head, tile)s, each of these is one unit.
 uint64_t plan_attention(AttnArgs& a, uint64_t part_bytes) {
-    const uint64_t rows = rows_per_tile(a);
-    a.tiles = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(((uint64_t)a.b.max_rows * a.group + rows - 1) / rows, 1u << 16));
-    const uint64_t groups = (uint64_t)a.tiles * a.c.heads * a.b.n_seqs;
-    uint64_t span = a.b.max_kv;
-    if (a.window) span = std::min<uint64_t>(span, (uint64_t)a.window + a.b.max_rows + kStep);
-    // two workgroups per CU, of at least one step per wave
-    const uint64_t most = std::max<uint64_t>(1, (span + kAttnWaves * kStep - 1) / (kAttnWaves * kStep));
-    uint64_t splits = std::max<uint64_t>(1, std::min(most, 1024 / groups));
-    const uint64_t each = (uint64_t)a.b.n_rows * a.heads * (a.c.dim + 4) * sizeof(float);
-    splits = std::max<uint64_t>(1, std::min(splits, part_bytes / each));
-    const uint64_t steps = (span + kStep - 1) / kStep;
-    a.chunk = (uint32_t)((steps + splits - 1) / splits * kStep);
-    a.splits = (uint32_t)std::max<uint64_t>(1, (span + a.chunk - 1) / std::max(a.chunk, 1u));
-    if (a.chunk == 0) a.chunk = kStep;
-    return a.splits > 1 ? each * a.splits : 0;
+    const uint32_t rows = few_rows(a);
+    a.tiles = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(((uint64_t)a.b.max_rows * a.group + rows - 1) / rows, 1u << 10));
+    // units of a call at most: sequences' tiles, by the table's tokens; a unit grows until they fit 31 bits
+    const uint64_t cap = (uint64_t)a.b.table_width * a.c.block + 16, pairs = (uint64_t)a.b.n_seqs * a.c.heads * a.tiles;
+    const uint64_t most = ((uint64_t)a.b.n_rows * a.group / rows + a.b.n_seqs) * a.c.heads;
+    a.unit_log2 = kChunkLog2;
+    while (a.unit_log2 < 31 && most * ((cap >> a.unit_log2) + 2) > 0x7FFFFFFFull) ++a.unit_log2;
+    a.unit = 1u << a.unit_log2;
+    const uint64_t per_wg = 2ull * rows * (a.c.dim + 4) * sizeof(float);
+    const uint64_t chunks = std::max<uint64_t>(1, ((uint64_t)a.b.max_kv + a.unit - 1) / a.unit);
+    a.splits = (uint32_t)std::min<uint64_t>(a.c.dim <= 128 && rows == 16 ? kFewGrid : kFewGrid / 2, pairs * chunks);
+    const uint64_t fit = part_bytes / per_wg;
+    const bool split = chunks > 1 && fit >= std::min<uint64_t>(a.splits, pairs);
+    if (split) a.splits = (uint32_t)std::min<uint64_t>(a.splits, fit);
+    return split ? a.splits * per_wg : 0;
 }
 
 int launch_attention(const AttnArgs& a, hipStream_t st) {
-    const uint32_t grid = a.splits * a.tiles * a.c.heads * a.b.n_seqs;
+    const bool two = a.type == HALO_MI_F32;
     switch (a.c.dim) {
-        case 64: run_attention<64>(a, grid, st); break;
-        case 96: run_attention<96>(a, grid, st); break;
-        case 128: run_attention<128>(a, grid, st); break;
-        case 192: run_attention<192>(a, grid, st); break;
-        default: run_attention<256>(a, grid, st); break;
+        case 64: two ? run_few<64, 2>(a, st) : run_few<64, 1>(a, st); break;
+        case 96: two ? run_few<96, 2>(a, st) : run_few<96, 1>(a, st); break;
+        case 128: two ? run_few<128, 2>(a, st) : run_few<128, 1>(a, st); break;
+        case 192: two ? run_few<192, 2>(a, st) : run_few<192, 1>(a, st); break;
+        default: two ? run_few<256, 2>(a, st) : run_few<256, 1>(a, st); break;
     }
-    if (a.splits > 1)
-        hipLaunchKernelGGL(k_attention_join, dim3((uint32_t)(((uint64_t)a.b.n_rows * a.heads + 3) / 4)), dim3(256), 0, st, a);
     return hip_status(hipGetLastError(), "ATTENTION");
 }
 

@@ -76,9 +76,9 @@ struct AttnArgs {
     uint32_t type, heads, group;  // group: q heads per kv head
     uint32_t window;
     float scale_log2;  // scale * log2(e)
-    // The split of the sequences' tokens: each of `splits` workgroups of a (sequence, kv head, row tile) takes
-    // `chunk` tokens, the last one the rest; their results meet in `part` when there are several.
-    uint32_t splits, chunk, tiles;
+    // How the work is dealt out (plan_attention): workgroups, row tiles of the longest sequence, tokens of a unit;
+    // the parts of what several workgroups have meet in `part` (null: nothing is split).
+    uint32_t splits, tiles, unit, unit_log2;
     float* part;
     uint32_t* status;
 };

@@ -380,15 +380,14 @@ int halo_mi_attention(const halo_mi_attention_params* p, void* stream) {
     auto st = static_cast<hipStream_t>(stream);
     if ((rc = take_status(op, p->status, p->status_keep, st, {q, out, pool, ws, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
     if (a.b.n_seqs == 0 || a.b.n_rows == 0) return HALO_MI_OK;
-    if (plan_attention(a, ws.bytes ? ws.bytes : kPartialFloats * sizeof(float)) != 0) {
-        a.part = static_cast<float*>(p->workspace);
-        if (!ws.bytes) {
-            Workspace* w = nullptr;
-            if ((rc = workspace_for(st, &w))) return rc;
-            if (w) a.part = w->partials;
-            else plan_attention(a, 0);  // a capturing stream that has none yet: unsplit
-        }
+    float* part = static_cast<float*>(p->workspace);
+    uint64_t bytes = ws.bytes;
+    if (!part) {
+        Workspace* w = nullptr;
+        if ((rc = workspace_for(st, &w))) return rc;
+        if (w) part = w->partials, bytes = kPartialFloats * sizeof(float);
     }
+    if (plan_attention(a, bytes)) a.part = part;
     return launch_attention(a, st);
 }
 
