@@ -104,6 +104,11 @@ __device__ __forceinline__ void store4(const HeadRows& r, uint32_t type, uint64_
     for (int j = 0; j < 4; ++j) store_any(p, type, i + j, v[j]);
 }
 
+// The first token that a row at `pos` sees. Past the table's room every row sees the group there, which is out of range.
+__device__ __forceinline__ int32_t first_seen(const AttnArgs& a, int32_t pos, int32_t cap) {
+    return a.window && pos >= (int32_t)a.window ? min(pos - (int32_t)a.window + 1, cap) : 0;
+}
+
 // A lane's row of a tile of 16: its tokens [lo, hi), q as f16 fragments scaled to the top of f16's range, and what
 // takes a score to the exponent's base 2: scale * log2(e) / (what q was scaled by), NaN where the row is not
 // finite. A negative scale turns q's sign, so that `c` is never negative.
@@ -127,7 +132,7 @@ struct QRow {
         const uint64_t at = (uint64_t)(sr.row0 + token) * a.q.stride + head * a.q.head_stride;
         const int32_t pos = sr.len - sr.rows + (int32_t)token;
         hi = live ? max(pos + 1, 0) : 0;
-        lo = a.window ? min(max(pos - (int32_t)a.window + 1, 0), cap) : 0;
+        lo = first_seen(a, pos, cap);
         const bool wide = wide_rows(a.q, a.type);
 #pragma unroll
         for (int i = 0; i < F; ++i)
@@ -248,7 +253,7 @@ __device__ __forceinline__ SeqUnits seq_units(const AttnArgs& a, uint32_t seq) {
     SeqUnits u;
     u.r = seq_rows(a.b, seq);
     const int32_t cap = (int32_t)(a.b.table_width * a.c.block);
-    u.begin = a.window ? min(max(u.r.len - u.r.rows - (int32_t)a.window + 1, 0), cap) / (int32_t)kStep * (int32_t)kStep : 0;
+    u.begin = first_seen(a, u.r.len - u.r.rows, cap) / (int32_t)kStep * (int32_t)kStep;
     u.end = min(u.r.len, cap + 16);  // past the table: one group out of range, which makes its rows NaN
     // without memory for parts a unit is all of its tokens
     u.chunks = a.part && u.end > u.begin ? ((uint32_t)(u.end - u.begin) + a.unit - 1) >> a.unit_log2 : 1;
@@ -303,6 +308,9 @@ __device__ __forceinline__ float* part_of(const AttnArgs& a, uint64_t w, uint32_
     return a.part + ((w * 2 + slot) * ROWS + row) * (a.c.dim + 4);
 }
 
+// The same of (row, head) r and split s of a call with many rows.
+__device__ __forceinline__ float* many_part(const AttnArgs& a, uint64_t r, uint32_t s) { return a.part + (r * a.splits + s) * (a.c.dim + 4); }
+
 // D: head_dim. NP: f16 pieces of q and of the weights. NQ: row tiles of 16 that share K and V.
 template <int D, int NP, int NQ>
 __global__ __launch_bounds__(kAttnWaves * 64, D <= 128 && NQ == 1 ? 2 : 1) void k_attention_few(AttnArgs a) {
@@ -336,7 +344,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, D <= 128 && NQ == 1 ? 2 : 1) void 
         // tokens that every row of the tile sees
         const int32_t pos0 = su.r.len - su.r.rows + (int32_t)(tile * ROWS / a.group);
         const int32_t pos1 = su.r.len - su.r.rows + (int32_t)((min(tile * ROWS + ROWS, packed) - 1) / a.group);
-        const uint32_t all_hi = (uint32_t)max(pos0 + 1, 0), all_lo = a.window ? (uint32_t)max(pos1 - (int32_t)a.window + 1, 0) : 0;
+        const uint32_t all_hi = (uint32_t)max(pos0 + 1, 0), all_lo = (uint32_t)first_seen(a, pos1, cap);
         const uint32_t end = (uint32_t)max(min(pos1 + 1, su.end), 0);
         const uint32_t t_first = (uint32_t)su.begin + (chunk << a.unit_log2) + wave * kStep;
         const uint32_t t_end = whole ? end : min((uint32_t)su.begin + ((chunk + n_chunks) << a.unit_log2), end);
@@ -584,30 +592,293 @@ void run_few(const AttnArgs& a, hipStream_t st) {
     if (a.part) hipLaunchKernelGGL(k_attention_few_join<16>, join, dim3(256), 0, st, a, a.splits);
 }
 
+// ---- many rows: prompts and chunks ----------------------------------------------------------------------------
+//
+// A workgroup has a tile of WAVES * 16 * NQ rows (tokens x the heads of a kv head) and goes over the tokens they see, 64 at a
+// time. The codes of a step are widened to f16 once for all its waves and laid in LDS as the MFMA's A fragments, lane by
+// lane, so that every write and read of LDS is 16 bytes per lane without a bank conflict; two buffers, so that the next step's
+// codes are loaded, widened and stored while this one's are used: one barrier per step. The tiles of the latest rows,
+// which see most, start first. With fewer tiles than CUs the tokens of each are split, and k_attention_many_join adds the parts.
+
+template <int D>
+struct StepLds {
+    half8v k[4][D / 32][64];  // [tile of 16 tokens][fragment][lane]
+    half8v v[D / 16][2][64];  // [tile of 16 dims][half of a group's tokens][lane]
+    Scales scale[4];
+};
+
+template <int D, int NP, int NQ, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) void k_attention_many(AttnArgs a) {
+    constexpr int F = D / 32, C = D / 64, TAIL = D % 64 / 32, DT = D / 16;
+    constexpr int ROWS = 16 * NQ * WAVES;
+    constexpr int KU = 4 * (C + TAIL), KW = (KU + WAVES - 1) / WAVES, VW = (DT + WAVES - 1) / WAVES;  // loads of a step, and per wave
+    extern __shared__ __align__(16) uint8_t lds_raw[];
+    StepLds<D>* lds = reinterpret_cast<StepLds<D>*>(lds_raw);
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, g = lane / 16;
+    const uint32_t pairs = a.b.n_seqs * a.c.heads;
+    uint32_t id = blockIdx.x;
+    const uint32_t kvh = id % a.c.heads, seq = id % pairs / a.c.heads;
+    id /= pairs;
+    const uint32_t split = id % a.splits;
+    const SeqRows sr = seq_rows(a.b, seq);
+    const uint32_t packed = (uint32_t)sr.rows * a.group, tiles = (packed + ROWS - 1) / ROWS;
+    const int32_t cap = (int32_t)(a.b.table_width * a.c.block), first = sr.len - sr.rows;
+    const int32_t* table = a.b.tables + (uint64_t)seq * a.b.table_stride;
+    const uint32_t head_codes = a.c.codes + kvh * a.c.plane;
+
+    for (uint32_t back = id / a.splits; back < tiles; back += a.tiles) {
+        const uint32_t row0 = (tiles - 1 - back) * ROWS, row_n = min(row0 + ROWS, packed);
+        const uint32_t my0 = row0 + wave * 16 * NQ, my_n = min(my0 + 16 * NQ, row_n);  // this wave's rows: [my0, my_n)
+        // tokens that the tile sees, and this split's share of them
+        const int32_t tile_lo = first + (int32_t)(row0 / a.group), tile_hi = first + (int32_t)((row_n - 1) / a.group);
+        const uint32_t begin = (uint32_t)first_seen(a, tile_lo, cap) / kStep * kStep;
+        const uint32_t end = (uint32_t)max(min(tile_hi + 1, cap + 16), 0);
+        const uint32_t steps = end > begin ? (end - begin + kStep - 1) / kStep : 0, share = (steps + a.splits - 1) / a.splits;
+        const uint32_t t_first = begin + min(split * share, steps) * kStep, t_end = min(begin + min((split + 1) * share, steps) * kStep, end);
+        // tokens that some row of this wave sees, and that all of them see
+        const int32_t my_lo = first + (int32_t)(my0 / a.group), my_hi = my0 < my_n ? first + (int32_t)((my_n - 1) / a.group) : -1;
+        const uint32_t any_hi = (uint32_t)max(my_hi + 1, 0), all_hi = (uint32_t)max(my_lo + 1, 0);
+        const uint32_t any_lo = (uint32_t)first_seen(a, my_lo, cap), all_lo = (uint32_t)first_seen(a, my_hi, cap);
+
+        QRow<D, NP> q[NQ];
+        Running<DT> run[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float raw[F][8];
+            q[n].fetch(a, sr, kvh, my0 + 16 * n + col, packed, g, cap, raw);
+            q[n].finish(a, raw);
+            run[n].clear();
+        }
+
+        // the codes of a step on their way from the cache to LDS
+        uint4 kb[KW], vb[VW];
+        float ks = 0.0f, vs = 0.0f;
+        bool ok = true;
+        const auto entry = [&](uint32_t t) { return table[min((t + 16 * g) >> a.c.block_log2, a.b.table_width - 1)]; };
+        const auto load = [&](uint32_t t, int32_t page_id) {
+            const uint32_t tg = t + 16 * g;
+            ok = (uint32_t)page_id < a.c.n_pages && (tg >> a.c.block_log2) < a.b.table_width;
+            const uint8_t* page = page_ptr(a.c, ok ? page_id : 0);
+            ok = ok || tg >= end;
+            const uint32_t row = (t + 16 * (col / 4)) % a.c.block + col % 4;
+            const uint8_t* k = reinterpret_cast<const uint8_t*>(__shfl((long long)page, 16 * (col / 4))) + head_codes + row * D;
+            const uint8_t* v = page + head_codes + a.c.heads * a.c.plane + col * a.c.block + (tg & (a.c.block - 1));
+#pragma unroll
+            for (int j = 0; j < KW; ++j) {
+                const uint32_t u = wave * KW + j, i = u / (C + TAIL), c = u % (C + TAIL);
+                if (KU % WAVES && u >= KU) break;
+                if (TAIL && c == C) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(k + 4 * i * D + C * 64 + 8 * g);
+                    kb[j] = {w.x, w.y, 0, 0};
+                } else {
+                    kb[j] = *reinterpret_cast<const uint4*>(k + 4 * i * D + c * 64 + 16 * g);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                const uint32_t t16 = wave * VW + j;
+                if (DT % WAVES && t16 >= DT) break;
+                vb[j] = *reinterpret_cast<const uint4*>(v + t16 * 16 * a.c.block);
+            }
+            if (wave == 0) {
+                const float* sc = reinterpret_cast<const float*>(page + a.c.scales) + kvh;
+                ks = sc[0];
+                vs = sc[a.c.heads];
+            }
+        };
+        const auto store = [&](StepLds<D>& to) {
+#pragma unroll
+            for (int j = 0; j < KW; ++j) {
+                const uint32_t u = wave * KW + j, i = u / (C + TAIL), c = u % (C + TAIL);
+                if (KU % WAVES && u >= KU) break;
+                to.k[i][2 * c][lane] = codes_f16(kb[j].x, kb[j].y);
+                if (!TAIL || c < C) to.k[i][2 * c + 1][lane] = codes_f16(kb[j].z, kb[j].w);
+            }
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                const uint32_t t16 = wave * VW + j;
+                if (DT % WAVES && t16 >= DT) break;
+                to.v[t16][0][lane] = codes_f16(vb[j].x, vb[j].y);
+                to.v[t16][1][lane] = codes_f16(vb[j].z, vb[j].w);
+            }
+            if (wave == 0) {
+                if (!ok) set_status(a.status, kStatusKvBadIndex);
+                if (col == 0) to.scale[g] = make_scales(ks, vs, ok);
+            }
+        };
+
+        int32_t id_next = 0;
+        if (t_first < t_end) {
+            load(t_first, entry(t_first));
+            id_next = entry(t_first + kStep);
+            store(lds[0]);
+        }
+        __syncthreads();
+        uint32_t buf = 0;
+        for (uint32_t t0 = t_first; t0 < t_end; t0 += kStep, buf ^= 1) {
+            const bool more = t0 + kStep < t_end;
+            if (more) {
+                load(t0 + kStep, id_next);
+                id_next = entry(t0 + 2 * kStep);
+            }
+            if (t0 < any_hi && t0 + kStep > any_lo) {
+                const StepLds<D>& from = lds[buf];
+                const Scales sc = from.scale[g];
+                float4v s[NQ][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) s[n][i] = float4v{0, 0, 0, 0};
+#pragma unroll
+                    for (int f = 0; f < F; ++f) {
+                        const half8v k = from.k[i][f][lane];
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                            for (int p = 0; p < NP; ++p) s[n][i] = mfma(k, q[n].f[f][p], s[n][i]);
+                    }
+                }
+                const bool all = t0 >= all_lo && t0 + kStep <= all_hi;
+                half8v w[NQ][2][NP];
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) run[n].template weigh<NP>(s[n], sc, q[n].c, t0 + 16 * g, q[n].lo, q[n].hi, all, w[n]);
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const half8v v = from.v[t][h][lane];
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                            for (int p = 0; p < NP; ++p) run[n].o[t] = mfma(v, w[n][h][p], run[n].o[t]);
+                    }
+            }
+            if (more) store(lds[buf ^ 1]);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            const uint32_t r = my0 + 16 * n + col;
+            const float l = column_sum(run[n].l), f = l == 0.0f ? 0.0f : 1.0f / l;
+            if (r >= packed) continue;
+            const uint32_t token = sr.row0 + r / a.group, head = kvh * a.group + r % a.group;
+            if (a.splits > 1) {
+                float* part = many_part(a, (uint64_t)token * a.heads + head, split);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) *reinterpret_cast<float4v*>(part + 16 * t + 4 * g) = run[n].o[t];
+                if (g == 0) {
+                    part[D] = run[n].m;
+                    part[D + 1] = l;
+                }
+            } else {
+                const uint64_t at = (uint64_t)token * a.out.stride + head * a.out.head_stride;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) store4(a.out, a.type, at + 16 * t + 4 * g, run[n].o[t] * f);
+            }
+        }
+    }
+}
+
+// Joins the splits of each (row, head), in order: D / 4 lanes a row.
+__global__ __launch_bounds__(256) void k_attention_many_join(AttnArgs a) {
+    const uint32_t D = a.c.dim, quads = D / 4, at_once = 256 / quads, d = threadIdx.x % quads * 4;
+    const uint64_t r = (uint64_t)blockIdx.x * at_once + threadIdx.x / quads;
+    if (threadIdx.x / quads >= at_once || r >= (uint64_t)a.b.n_rows * a.heads) return;
+    const uint32_t row = (uint32_t)(r / a.heads), head = (uint32_t)(r % a.heads);
+    if ((int32_t)row < max(a.b.row_starts[0], 0) || (int32_t)row >= a.b.row_starts[a.b.n_seqs]) return;  // of no sequence
+    float top = -INFINITY;
+    for (uint32_t s = 0; s < a.splits; ++s) top = fmaxf(top, many_part(a, r, s)[D]);
+    float sum = 0.0f;
+    float4v acc = {0, 0, 0, 0};
+    for (uint32_t s = 0; s < a.splits; ++s) {
+        const float* p = many_part(a, r, s);
+        const float m = p[D], l = p[D + 1], f = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m - top);
+        sum += l * f;
+        acc += *reinterpret_cast<const float4v*>(p + d) * f;
+    }
+    store4(a.out, a.type, row * a.out.stride + head * a.out.head_stride + d, sum == 0.0f ? float4v{0, 0, 0, 0} : acc / sum);
+}
+
+template <int D>
+constexpr int many_waves() {
+    return 4;
+}
+
+template <int D, int NP>
+int run_many(const AttnArgs& a, hipStream_t st) {
+    constexpr int W = many_waves<D>();
+    auto* k = k_attention_many<D, NP, 2, W>;
+    const size_t lds = 2 * sizeof(StepLds<D>);
+    // more than 64 KiB of LDS has to be asked for, once per device and kernel; cheap enough to ask every time
+    if (lds > 65536)
+        if (int rc = hip_status(hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "ATTENTION")) return rc;
+    hipLaunchKernelGGL(k, dim3(a.splits * a.tiles * a.c.heads * a.b.n_seqs), dim3(W * 64), lds, st, a);
+    if (a.splits > 1) {
+        const uint64_t at_once = 256 / (a.c.dim / 4), rows = (uint64_t)a.b.n_rows * a.heads;
+        hipLaunchKernelGGL(k_attention_many_join, dim3((uint32_t)((rows + at_once - 1) / at_once)), dim3(256), 0, st, a);
+    }
+    return HALO_MI_OK;
+}
+
+constexpr uint64_t kMaxGrid = 1u << 22;  // workgroups of a launch (256 threads each; n_seqs * kv heads is at most this)
+constexpr uint32_t many_rows(uint32_t) { return 128; }
+
+}  // namespace
+
+namespace {
+
+// Tiles of a call with many rows, and the splits that bring two workgroups (one at a head_dim over 128) to every CU.
+uint64_t plan_many(AttnArgs& a, uint64_t part_bytes) {
+    const uint32_t rows = many_rows(a.c.dim);
+    const uint64_t pairs = (uint64_t)a.c.heads * a.b.n_seqs;
+    a.tiles = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(((uint64_t)a.b.max_rows * a.group + rows - 1) / rows, kMaxGrid / pairs));
+    const uint64_t groups = a.tiles * pairs, want = a.c.dim <= 128 ? 512 : 256;
+    uint64_t span = a.b.max_kv;
+    if (a.window) span = std::min<uint64_t>(span, (uint64_t)a.window + rows / a.group + kStep);
+    const uint64_t each = (uint64_t)a.b.n_rows * a.heads * (a.c.dim + 4) * sizeof(float);
+    a.splits = (uint32_t)std::max<uint64_t>(1, std::min({want / groups, (span + 4 * kStep - 1) / (4 * kStep), part_bytes / each}));
+    return a.splits > 1 ? a.splits * each : 0;
+}
+
 }  // namespace
 
 // As many workgroups as the registers let run at once, one or two per CU, or fewer where there are not as many units. With memory for fewer parts than there are
 // (sequence, kv head, tile)s, each of these is one unit.
 uint64_t plan_attention(AttnArgs& a, uint64_t part_bytes) {
+    // Few rows per kv head: what counts is the cache's stream. More: the products, on tiles that share K and V.
+    a.few = (uint64_t)a.b.max_rows * a.group <= 32;
+    if (!a.few) return plan_many(a, part_bytes);
     const uint32_t rows = few_rows(a);
-    a.tiles = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(((uint64_t)a.b.max_rows * a.group + rows - 1) / rows, 1u << 10));
+    const uint64_t pairs = (uint64_t)a.b.n_seqs * a.c.heads;
+    a.tiles = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(((uint64_t)a.b.max_rows * a.group + rows - 1) / rows, kMaxGrid / pairs));
     // units of a call at most: sequences' tiles, by the table's tokens; a unit grows until they fit 31 bits
-    const uint64_t cap = (uint64_t)a.b.table_width * a.c.block + 16, pairs = (uint64_t)a.b.n_seqs * a.c.heads * a.tiles;
+    const uint64_t cap = (uint64_t)a.b.table_width * a.c.block + 16;
     const uint64_t most = ((uint64_t)a.b.n_rows * a.group / rows + a.b.n_seqs) * a.c.heads;
     a.unit_log2 = kChunkLog2;
     while (a.unit_log2 < 31 && most * ((cap >> a.unit_log2) + 2) > 0x7FFFFFFFull) ++a.unit_log2;
     a.unit = 1u << a.unit_log2;
     const uint64_t per_wg = 2ull * rows * (a.c.dim + 4) * sizeof(float);
     const uint64_t chunks = std::max<uint64_t>(1, ((uint64_t)a.b.max_kv + a.unit - 1) / a.unit);
-    a.splits = (uint32_t)std::min<uint64_t>(a.c.dim <= 128 && rows == 16 ? kFewGrid : kFewGrid / 2, pairs * chunks);
+    a.splits = (uint32_t)std::min<uint64_t>(a.c.dim <= 128 && rows == 16 ? kFewGrid : kFewGrid / 2, pairs * a.tiles * chunks);
     const uint64_t fit = part_bytes / per_wg;
-    const bool split = chunks > 1 && fit >= std::min<uint64_t>(a.splits, pairs);
+    const bool split = chunks > 1 && fit >= std::min<uint64_t>(a.splits, pairs * a.tiles);
     if (split) a.splits = (uint32_t)std::min<uint64_t>(a.splits, fit);
     return split ? a.splits * per_wg : 0;
 }
 
 int launch_attention(const AttnArgs& a, hipStream_t st) {
     const bool two = a.type == HALO_MI_F32;
+    if (!a.few) {
+        int rc;
+        switch (a.c.dim) {
+            case 64: rc = two ? run_many<64, 2>(a, st) : run_many<64, 1>(a, st); break;
+            case 96: rc = two ? run_many<96, 2>(a, st) : run_many<96, 1>(a, st); break;
+            case 128: rc = two ? run_many<128, 2>(a, st) : run_many<128, 1>(a, st); break;
+            case 192: rc = two ? run_many<192, 2>(a, st) : run_many<192, 1>(a, st); break;
+            default: rc = two ? run_many<256, 2>(a, st) : run_many<256, 1>(a, st); break;
+        }
+        return rc ? rc : hip_status(hipGetLastError(), "ATTENTION");
+    }
     switch (a.c.dim) {
         case 64: two ? run_few<64, 2>(a, st) : run_few<64, 1>(a, st); break;
         case 96: two ? run_few<96, 2>(a, st) : run_few<96, 1>(a, st); break;

@@ -78,6 +78,7 @@ struct AttnArgs {
     float scale_log2;  // scale * log2(e)
     // How the work is dealt out (plan_attention): workgroups, row tiles of the longest sequence, tokens of a unit;
     // the parts of what several workgroups have meet in `part` (null: nothing is split).
+    bool few;
     uint32_t splits, tiles, unit, unit_log2;
     float* part;
     uint32_t* status;

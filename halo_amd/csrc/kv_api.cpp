@@ -159,7 +159,9 @@ int check_attention(const halo_mi_attention_params* p, AttnArgs* a, std::initial
     a->type = p->type;
     a->heads = p->n_heads;
     a->group = p->n_heads / p->cache.n_kv_heads;
-    a->window = std::min(p->window, 0x7FFFFFFFu);
+    if ((uint64_t)p->batch.n_seqs * p->cache.n_kv_heads > 1u << 22)
+        return set_error(HALO_MI_E_UNSUPPORTED, "%s: %u sequences of %u kv heads in one call", op, p->batch.n_seqs, p->cache.n_kv_heads);
+    a->window = p->window < 0x7FFFFFFFu ? p->window : 0;  // more than any table holds
     const float scale = p->scale == 0.0f ? 1.0f / std::sqrt((float)p->cache.head_dim) : p->scale;
     a->scale_log2 = (float)(scale * 1.4426950408889634);
     a->part = nullptr;
