@@ -188,26 +188,26 @@ struct Running {
     }
 
     // A step's scores become weights w = 2^(s k + lv - m + 14) as f16 fragments; m, l and o follow. tg: the
-    // position of this lane group's first token. all: every row sees every token (uniform).
+    // position of this lane group's first token. all: every row sees every token (uniform). The maximum is taken over
+    // the scores (k is not negative), so a score costs half a max3, one multiply-add, one exp2, one add and half a
+    // conversion.
     template <int NP>
     __device__ __forceinline__ void weigh(const float4v (&s)[4], const Scales& sc, float c, uint32_t tg, int32_t lo, int32_t hi, bool all,
                                           half8v (&w)[2][NP]) {
         const float k = sc.k * c;
-        float x[16];
+        uint32_t seen = 0xFFFFu;  // of the group's 16 tokens
         float top = -INFINITY;
         if (all) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[i] = fmaf(s[i / 4][i % 4], k, sc.lv);
-                top = fmaxf(top, x[i]);
-            }
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i / 4][i % 4]);
+            top = fmaf(top, k, sc.lv);
         } else {
+            __asm__ volatile("");  // a branch: most steps see everything
+            const int32_t from = min(max(lo - (int32_t)tg, 0), 16), to = min(max(hi - (int32_t)tg, 0), 16);
+            seen = ((1u << to) - 1u) & ~((1u << from) - 1u);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int32_t token = (int32_t)(tg + i);
-                x[i] = token >= lo && token < hi ? fmaf(s[i / 4][i % 4], k, sc.lv) : -INFINITY;
-                top = fmaxf(top, x[i]);
-            }
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, seen >> i & 1 ? s[i / 4][i % 4] : -INFINITY);
+            if (seen) top = fmaf(top, k, sc.lv);
         }
         top = column_max(top);
         if (__ballot(top > m)) {
@@ -217,13 +217,22 @@ struct Running {
             for (int t = 0; t < DT; ++t) o[t] *= f;
             m = m_new;
         }
-        const float shift = m == -INFINITY ? 0.0f : m - kWeightShift;
+        const float shift = sc.lv - (m == -INFINITY ? 0.0f : m - kWeightShift);
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = fmaf(s[i / 4][i % 4], k, shift);
+        if (!all) {
+            __asm__ volatile("");
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = seen >> i & 1 ? x[i] : -INFINITY;
+        }
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float v = __builtin_amdgcn_exp2f(x[i] - shift);
-            sum += v;
+            const float v = __builtin_amdgcn_exp2f(x[i]);
             w[i / 8][0][i % 8] = (_Float16)v;
+            // in fp32: where V's scale is far below the others', f16 would lose weights that 1 / vs makes count
+            sum += v;
             if constexpr (NP == 2) w[i / 8][1][i % 8] = (_Float16)(v - (float)w[i / 8][0][i % 8]);
         }
         l += sum == 0.0f ? 0.0f : sum * sc.rv;
