@@ -175,6 +175,12 @@ __device__ __forceinline__ Scales make_scales(float ks, float vs, bool page) {
     return {page ? ks : quiet_nan(), __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
 }
 
+// Bit i: token tg + i is in [lo, hi), i < 16.
+__device__ __forceinline__ uint32_t seen_tokens(uint32_t tg, int32_t lo, int32_t hi) {
+    const int32_t from = min(max(lo - (int32_t)tg, 0), 16), to = min(max(hi - (int32_t)tg, 0), 16);
+    return ((1u << to) - 1u) & ~((1u << from) - 1u);
+}
+
 // The running maximum and sum of a row, and its outputs: O^T as DT tiles of 16 dims.
 template <int DT>
 struct Running {
@@ -187,28 +193,25 @@ struct Running {
         for (int t = 0; t < DT; ++t) o[t] = float4v{0, 0, 0, 0};
     }
 
-    // A step's scores become weights w = 2^(s k + lv - m + 14) as f16 fragments; m, l and o follow. tg: the
-    // position of this lane group's first token. all: every row sees every token (uniform). The maximum is taken over
-    // the scores (k is not negative), so a score costs half a max3, one multiply-add, one exp2, one add and half a
-    // conversion.
-    template <int NP>
-    __device__ __forceinline__ void weigh(const float4v (&s)[4], const Scales& sc, float c, uint32_t tg, int32_t lo, int32_t hi, bool all,
-                                          half8v (&w)[2][NP]) {
-        const float k = sc.k * c;
-        uint32_t seen = 0xFFFFu;  // of the group's 16 tokens
+    // A step's scores become weights w = 2^(s k + lv - m + 14) as f16 fragments; m, l and o follow. The maximum is
+    // taken over the scores (k is not negative), so a score costs half a max3, one multiply-add, one exp2, one add and
+    // half a conversion. Four parts, so that a caller can put products between them; in all: weigh().
+
+    // The largest exponent of the lane's scores, of all 16 tokens of its group or of those that are `seen`.
+    __device__ __forceinline__ static float peak(const float4v (&s)[4], const Scales& sc, float c) {
         float top = -INFINITY;
-        if (all) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i / 4][i % 4]);
-            top = fmaf(top, k, sc.lv);
-        } else {
-            __asm__ volatile("");  // a branch: most steps see everything
-            const int32_t from = min(max(lo - (int32_t)tg, 0), 16), to = min(max(hi - (int32_t)tg, 0), 16);
-            seen = ((1u << to) - 1u) & ~((1u << from) - 1u);
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i / 4][i % 4]);
+        return fmaf(top, sc.k * c, sc.lv);
+    }
+    __device__ __forceinline__ static float peak_seen(const float4v (&s)[4], const Scales& sc, float c, uint32_t seen) {
+        float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, seen >> i & 1 ? s[i / 4][i % 4] : -INFINITY);
-            if (seen) top = fmaf(top, k, sc.lv);
-        }
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, seen >> i & 1 ? s[i / 4][i % 4] : -INFINITY);
+        return seen ? fmaf(top, sc.k * c, sc.lv) : -INFINITY;
+    }
+    // `top`, over the column's lanes, joins the maximum.
+    __device__ __forceinline__ void raise(float top) {
         top = column_max(top);
         if (__ballot(top > m)) {
             const float m_new = fmaxf(m, top), f = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
@@ -217,15 +220,20 @@ struct Running {
             for (int t = 0; t < DT; ++t) o[t] *= f;
             m = m_new;
         }
-        const float shift = sc.lv - (m == -INFINITY ? 0.0f : m - kWeightShift);
-        float x[16];
+    }
+    // The exponents; with `seen`, -inf for the others.
+    __device__ __forceinline__ void exponents(const float4v (&s)[4], const Scales& sc, float c, bool all, uint32_t seen, float (&x)[16]) const {
+        const float k = sc.k * c, shift = sc.lv - (m == -INFINITY ? 0.0f : m - kWeightShift);
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = fmaf(s[i / 4][i % 4], k, shift);
         if (!all) {
-            __asm__ volatile("");
+            __asm__ volatile("");  // a branch: most steps see everything
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = seen >> i & 1 ? x[i] : -INFINITY;
         }
+    }
+    template <int NP>
+    __device__ __forceinline__ void weights(const float (&x)[16], const Scales& sc, half8v (&w)[2][NP]) {
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -236,6 +244,21 @@ struct Running {
             if constexpr (NP == 2) w[i / 8][1][i % 8] = (_Float16)(v - (float)w[i / 8][0][i % 8]);
         }
         l += sum == 0.0f ? 0.0f : sum * sc.rv;
+    }
+    template <int NP>
+    __device__ __forceinline__ void weigh(const float4v (&s)[4], const Scales& sc, float c, uint32_t tg, int32_t lo, int32_t hi, bool all,
+                                          half8v (&w)[2][NP]) {
+        uint32_t seen = 0xFFFFu;
+        if (all) {
+            raise(peak(s, sc, c));
+        } else {
+            __asm__ volatile("");
+            seen = seen_tokens(tg, lo, hi);
+            raise(peak_seen(s, sc, c, seen));
+        }
+        float x[16];
+        exponents(s, sc, c, all, seen, x);
+        weights<NP>(x, sc, w);
     }
 };
 
@@ -376,8 +399,9 @@ __global__ __launch_bounds__(kAttnWaves * 64, D <= 128 && NQ == 1 ? 2 : 1) void 
         // K of the step at t: the K row of tile i in this lane is token 4 i + col % 4 of group col / 4
         const auto load_k = [&](uint32_t t, int32_t id) {
             page = page_of(t, id, ok);
+            // a page's number crosses the lanes, not its address: loads stay global ones (flat ones would hold up LDS)
             const uint32_t row = (t + 16 * (col / 4)) % a.c.block + col % 4;
-            const uint8_t* k = reinterpret_cast<const uint8_t*>(__shfl((long long)page, 16 * (col / 4))) + head_codes + row * D;
+            const uint8_t* k = page_ptr(a.c, __shfl(ok ? id : 0, 16 * (col / 4))) + head_codes + row * D;
             const float* sc = reinterpret_cast<const float*>(page + a.c.scales) + kvh;
             ks = sc[0];
             vs = sc[a.c.heads];
@@ -620,6 +644,7 @@ template <int D, int NP, int NQ, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) void k_attention_many(AttnArgs a) {
     constexpr int F = D / 32, C = D / 64, TAIL = D % 64 / 32, DT = D / 16;
     constexpr int ROWS = 16 * NQ * WAVES;
+    constexpr int kAhead = 4;  // V fragments read ahead
     constexpr int KU = 4 * (C + TAIL), KW = (KU + WAVES - 1) / WAVES, VW = (DT + WAVES - 1) / WAVES;  // loads of a step, and per wave
     extern __shared__ __align__(16) uint8_t lds_raw[];
     StepLds<D>* lds = reinterpret_cast<StepLds<D>*>(lds_raw);
@@ -667,10 +692,12 @@ __global__ __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) void k_attention_many
         const auto load = [&](uint32_t t, int32_t page_id) {
             const uint32_t tg = t + 16 * g;
             ok = (uint32_t)page_id < a.c.n_pages && (tg >> a.c.block_log2) < a.b.table_width;
-            const uint8_t* page = page_ptr(a.c, ok ? page_id : 0);
+            const int32_t number = ok ? page_id : 0;
+            const uint8_t* page = page_ptr(a.c, number);
             ok = ok || tg >= end;
+            // a page's number crosses the lanes, not its address: loads stay global ones (flat ones would hold up LDS)
             const uint32_t row = (t + 16 * (col / 4)) % a.c.block + col % 4;
-            const uint8_t* k = reinterpret_cast<const uint8_t*>(__shfl((long long)page, 16 * (col / 4))) + head_codes + row * D;
+            const uint8_t* k = page_ptr(a.c, __shfl(number, 16 * (col / 4))) + head_codes + row * D;
             const uint8_t* v = page + head_codes + a.c.heads * a.c.plane + col * a.c.block + (tg & (a.c.block - 1));
 #pragma unroll
             for (int j = 0; j < KW; ++j) {
@@ -733,34 +760,52 @@ __global__ __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) void k_attention_many
             if (t0 < any_hi && t0 + kStep > any_lo) {
                 const StepLds<D>& from = lds[buf];
                 const Scales sc = from.scale[g];
+                // fragments are read a tile ahead of the products that take them
+                half8v kf[2][F], vf[kAhead][2];
                 float4v s[NQ][4];
 #pragma unroll
+                for (int f = 0; f < F; ++f) kf[0][f] = from.k[0][f][lane];
+#pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    if (i < 3) {
+#pragma unroll
+                        for (int f = 0; f < F; ++f) kf[(i + 1) & 1][f] = from.k[i + 1][f][lane];
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < kAhead; ++t)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) vf[t][h] = from.v[t][h][lane];
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) s[n][i] = float4v{0, 0, 0, 0};
 #pragma unroll
-                    for (int f = 0; f < F; ++f) {
-                        const half8v k = from.k[i][f][lane];
+                    for (int f = 0; f < F; ++f)
 #pragma unroll
                         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                            for (int p = 0; p < NP; ++p) s[n][i] = mfma(k, q[n].f[f][p], s[n][i]);
-                    }
+                            for (int p = 0; p < NP; ++p) s[n][i] = mfma(kf[i & 1][f], q[n].f[f][p], s[n][i]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 const bool all = t0 >= all_lo && t0 + kStep <= all_hi;
                 half8v w[NQ][2][NP];
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) run[n].template weigh<NP>(s[n], sc, q[n].c, t0 + 16 * g, q[n].lo, q[n].hi, all, w[n]);
 #pragma unroll
-                for (int t = 0; t < DT; ++t)
+                for (int t = 0; t < DT; ++t) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const half8v v = from.v[t][h][lane];
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                            for (int p = 0; p < NP; ++p) run[n].o[t] = mfma(v, w[n][h][p], run[n].o[t]);
+                            for (int p = 0; p < NP; ++p) run[n].o[t] = mfma(vf[t % kAhead][h], w[n][h][p], run[n].o[t]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (t + kAhead < DT) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) vf[t % kAhead][h] = from.v[t + kAhead][h][lane];
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
             if (more) store(lds[buf ^ 1]);
             __syncthreads();
