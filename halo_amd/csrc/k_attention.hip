@@ -112,16 +112,17 @@ __device__ __forceinline__ int32_t first_seen(const AttnArgs& a, int32_t pos, in
 // A lane's row of a tile of 16: its tokens [lo, hi), q as f16 fragments scaled to the top of f16's range, and what
 // takes a score to the exponent's base 2: scale * log2(e) / (what q was scaled by), NaN where the row is not
 // finite. A negative scale turns q's sign, so that `c` is never negative.
-template <int D, int NP>
+// GROUPS lane groups share a row: 4 (16 x 16 tiles) or 2 (32 x 32).
+template <int D, int NP, int GROUPS = 4>
 struct QRow {
-    static constexpr int F = D / 32;  // fragments of 32 dims
+    static constexpr int F = D / (8 * GROUPS);  // fragments of 8 elements a lane
     half8v f[F][NP];
     float c;
     int32_t lo, hi;
 
     // dim of element 0 of fragment i in lane group g: 16 bytes of codes hold two fragments' elements
     static __device__ __forceinline__ uint32_t dim(int i, uint32_t g) {
-        return i / 2 * 2 + 1 < F ? i / 2 * 64 + 16 * g + i % 2 * 8 : i * 32 + 8 * g;
+        return i / 2 * 2 + 1 < F ? i / 2 * 16 * GROUPS + 16 * g + i % 2 * 8 : i * 8 * GROUPS + 8 * g;
     }
 
     // packed row r of `packed`: token r / group, head r % group of kv head kvh. fetch only loads; finish converts.
@@ -149,7 +150,7 @@ struct QRow {
         for (int i = 0; i < F; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[i][j]));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+        if constexpr (GROUPS == 4) top = max(top, (uint32_t)__shfl_xor((int)top, 16));
         top = max(top, (uint32_t)__shfl_xor((int)top, 32));
         const bool bad = top > kLargestFinite;
         const int e = top == 0 || bad ? 0 : top < 0x00800000u ? (int)(31 - __builtin_clz(top)) - 149 : (int)(top >> 23) - 127;
@@ -627,28 +628,114 @@ void run_few(const AttnArgs& a, hipStream_t st) {
 
 // ---- many rows: prompts and chunks ----------------------------------------------------------------------------
 //
-// A workgroup has a tile of WAVES * 16 * NQ rows (tokens x the heads of a kv head) and goes over the tokens they see, 64 at a
+// A workgroup has a tile of WAVES * 32 rows (tokens x the heads of a kv head) and goes over the tokens they see, 64 at a
 // time. The codes of a step are widened to f16 once for all its waves and laid in LDS as the MFMA's A fragments, lane by
 // lane, so that every write and read of LDS is 16 bytes per lane without a bank conflict; two buffers, so that the next step's
-// codes are loaded, widened and stored while this one's are used: one barrier per step. The tiles of the latest rows,
-// which see most, start first. With fewer tiles than CUs the tokens of each are split, and k_attention_many_join adds the parts.
+// codes are loaded, widened and stored while this one's are used: one barrier per step. A wave reads kAhead fragments
+// ahead of the products that take them, V's first ones before the softmax.
+//
+// v_mfma_f32_32x32x16_f16: half the instructions of the 16 x 16 form for the same work, and the vector unit runs beside it
+// (16 cycles of either form side by side with a v_exp_f32 stream: 1.01 against 1.13 times the stream alone). A
+// step is two tiles u of 32 tokens; lane (r, h) = (lane % 32, lane / 32) has the scores of row r with the 16 tokens of
+// group 2 u + h, as K's row r of tile u is token 4 (r / 8) + r % 4 of group 2 u + r / 4 % 2.
+//
+// The tiles of the latest rows, which see most, start first. With fewer tiles than CUs the tokens of each are split, and
+// k_attention_many_join adds the parts.
+
+typedef float float16v __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ float16v mfma32(half8v a, half8v b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 template <int D>
 struct StepLds {
-    half8v k[4][D / 32][64];  // [tile of 16 tokens][fragment][lane]
-    half8v v[D / 16][2][64];  // [tile of 16 dims][half of a group's tokens][lane]
+    half8v k[2][D / 16][64];  // [tile of 32 tokens][16 dims][lane]
+    half8v v[4][D / 32][64];  // [2 u + half of a group's tokens][tile of 32 dims][lane]
     Scales scale[4];
 };
 
-template <int D, int NP, int NQ, int WAVES>
+// The maximum and sum of a lane's row, and its outputs: O^T as tiles of 32 dims.
+template <int D>
+struct Running32 {
+    float m, l;
+    float16v o[D / 32];
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    }
+    // As Running::weigh, over both tiles of a step. tg: the position of this lane's first token of tile 0.
+    template <int NP>
+    __device__ __forceinline__ void weigh(const float16v (&s)[2], const Scales (&sc)[2], float c, uint32_t tg, int32_t lo, int32_t hi, bool all,
+                                          half8v (&w)[2][2][NP]) {
+        const float k[2] = {sc[0].k * c, sc[1].k * c};
+        uint32_t seen[2] = {0xFFFFu, 0xFFFFu};
+        float top[2] = {-INFINITY, -INFINITY};
+        if (all) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top[u] = fmaxf(top[u], s[u][i]);
+                top[u] = fmaf(top[u], k[u], sc[u].lv);
+            }
+        } else {
+            __asm__ volatile("");  // a branch: most steps see everything
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                seen[u] = seen_tokens(tg + 32 * u, lo, hi);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top[u] = fmaxf(top[u], seen[u] >> i & 1 ? s[u][i] : -INFINITY);
+                top[u] = seen[u] ? fmaf(top[u], k[u], sc[u].lv) : -INFINITY;
+            }
+        }
+        float peak = fmaxf(top[0], top[1]);
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(peak), __float_as_int(peak), false, false);
+        peak = fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+        if (__ballot(peak > m)) {
+            const float m_new = fmaxf(m, peak), f = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t) o[t] *= f;
+            m = m_new;
+        }
+        const float base = m == -INFINITY ? 0.0f : m - kWeightShift;
+        float x[2][16];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[u][i] = fmaf(s[u][i], k[u], sc[u].lv - base);
+        if (!all) {
+            __asm__ volatile("");
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[u][i] = seen[u] >> i & 1 ? x[u][i] : -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float v = __builtin_amdgcn_exp2f(x[u][i]);
+                sum += v;
+                w[u][i / 8][0][i % 8] = (_Float16)v;
+                if constexpr (NP == 2) w[u][i / 8][1][i % 8] = (_Float16)(v - (float)w[u][i / 8][0][i % 8]);
+            }
+            l += sum == 0.0f ? 0.0f : sum * sc[u].rv;
+        }
+    }
+};
+
+template <int D, int NP, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) void k_attention_many(AttnArgs a) {
-    constexpr int F = D / 32, C = D / 64, TAIL = D % 64 / 32, DT = D / 16;
-    constexpr int ROWS = 16 * NQ * WAVES;
-    constexpr int kAhead = 4;  // V fragments read ahead
-    constexpr int KU = 4 * (C + TAIL), KW = (KU + WAVES - 1) / WAVES, VW = (DT + WAVES - 1) / WAVES;  // loads of a step, and per wave
+    constexpr int F = D / 16, C = D / 32, ROWS = 32 * WAVES;
+    constexpr int UW = (C + WAVES / 2 - 1) / (WAVES / 2);  // 16-byte loads of K, and of V, per wave and step
+    constexpr int kAhead = 8;                              // fragments read ahead
     extern __shared__ __align__(16) uint8_t lds_raw[];
     StepLds<D>* lds = reinterpret_cast<StepLds<D>*>(lds_raw);
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, g = lane / 16;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, row = lane % 32, h = lane / 32;
     const uint32_t pairs = a.b.n_seqs * a.c.heads;
     uint32_t id = blockIdx.x;
     const uint32_t kvh = id % a.c.heads, seq = id % pairs / a.c.heads;
@@ -662,7 +749,7 @@ __global__ __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) void k_attention_many
 
     for (uint32_t back = id / a.splits; back < tiles; back += a.tiles) {
         const uint32_t row0 = (tiles - 1 - back) * ROWS, row_n = min(row0 + ROWS, packed);
-        const uint32_t my0 = row0 + wave * 16 * NQ, my_n = min(my0 + 16 * NQ, row_n);  // this wave's rows: [my0, my_n)
+        const uint32_t my0 = row0 + wave * 32, my_n = min(my0 + 32, row_n);  // this wave's rows: [my0, my_n)
         // tokens that the tile sees, and this split's share of them
         const int32_t tile_lo = first + (int32_t)(row0 / a.group), tile_hi = first + (int32_t)((row_n - 1) / a.group);
         const uint32_t begin = (uint32_t)first_seen(a, tile_lo, cap) / kStep * kStep;
@@ -674,72 +761,57 @@ __global__ __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) void k_attention_many
         const uint32_t any_hi = (uint32_t)max(my_hi + 1, 0), all_hi = (uint32_t)max(my_lo + 1, 0);
         const uint32_t any_lo = (uint32_t)first_seen(a, my_lo, cap), all_lo = (uint32_t)first_seen(a, my_hi, cap);
 
-        QRow<D, NP> q[NQ];
-        Running<DT> run[NQ];
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
+        QRow<D, NP, 2> q;
+        Running32<D> run;
+        {
             float raw[F][8];
-            q[n].fetch(a, sr, kvh, my0 + 16 * n + col, packed, g, cap, raw);
-            q[n].finish(a, raw);
-            run[n].clear();
+            q.fetch(a, sr, kvh, my0 + row, packed, h, cap, raw);
+            q.finish(a, raw);
+            run.clear();
         }
 
-        // the codes of a step on their way from the cache to LDS
-        uint4 kb[KW], vb[VW];
+        // The codes of a step on their way from the cache to LDS: this wave's are of tile wave % 2. A lane has the
+        // table entry of group lane % 4; numbers of pages cross the lanes, not addresses: loads stay global ones (flat ones
+        // would hold up LDS).
+        uint4 kb[UW], vb[UW];
         float ks = 0.0f, vs = 0.0f;
         bool ok = true;
-        const auto entry = [&](uint32_t t) { return table[min((t + 16 * g) >> a.c.block_log2, a.b.table_width - 1)]; };
+        const uint32_t u0 = wave % 2, c0 = wave / 2;
+        const auto entry = [&](uint32_t t) { return table[min((t + 16 * (lane % 4)) >> a.c.block_log2, a.b.table_width - 1)]; };
         const auto load = [&](uint32_t t, int32_t page_id) {
-            const uint32_t tg = t + 16 * g;
+            const uint32_t tg = t + 16 * (lane % 4);
             ok = (uint32_t)page_id < a.c.n_pages && (tg >> a.c.block_log2) < a.b.table_width;
             const int32_t number = ok ? page_id : 0;
-            const uint8_t* page = page_ptr(a.c, number);
             ok = ok || tg >= end;
-            // a page's number crosses the lanes, not its address: loads stay global ones (flat ones would hold up LDS)
-            const uint32_t row = (t + 16 * (col / 4)) % a.c.block + col % 4;
-            const uint8_t* k = page_ptr(a.c, __shfl(number, 16 * (col / 4))) + head_codes + row * D;
-            const uint8_t* v = page + head_codes + a.c.heads * a.c.plane + col * a.c.block + (tg & (a.c.block - 1));
+            const uint32_t kg = 2 * u0 + row / 4 % 2, vg = 2 * u0 + h;
+            const uint8_t* k = page_ptr(a.c, __shfl(number, kg)) + head_codes + ((t + 16 * kg) % a.c.block + 4 * (row / 8) + row % 4) * D + 16 * h;
+            const uint8_t* v = page_ptr(a.c, __shfl(number, vg)) + head_codes + a.c.heads * a.c.plane + row * a.c.block + (t + 16 * vg) % a.c.block;
 #pragma unroll
-            for (int j = 0; j < KW; ++j) {
-                const uint32_t u = wave * KW + j, i = u / (C + TAIL), c = u % (C + TAIL);
-                if (KU % WAVES && u >= KU) break;
-                if (TAIL && c == C) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(k + 4 * i * D + C * 64 + 8 * g);
-                    kb[j] = {w.x, w.y, 0, 0};
-                } else {
-                    kb[j] = *reinterpret_cast<const uint4*>(k + 4 * i * D + c * 64 + 16 * g);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < VW; ++j) {
-                const uint32_t t16 = wave * VW + j;
-                if (DT % WAVES && t16 >= DT) break;
-                vb[j] = *reinterpret_cast<const uint4*>(v + t16 * 16 * a.c.block);
+            for (int j = 0; j < UW; ++j) {
+                const uint32_t c = c0 + j * (WAVES / 2);
+                if (C % (WAVES / 2) && c >= C) break;
+                kb[j] = *reinterpret_cast<const uint4*>(k + c * 32);
+                vb[j] = *reinterpret_cast<const uint4*>(v + c * 32 * a.c.block);
             }
             if (wave == 0) {
-                const float* sc = reinterpret_cast<const float*>(page + a.c.scales) + kvh;
+                const float* sc = reinterpret_cast<const float*>(page_ptr(a.c, number) + a.c.scales) + kvh;
                 ks = sc[0];
                 vs = sc[a.c.heads];
             }
         };
         const auto store = [&](StepLds<D>& to) {
 #pragma unroll
-            for (int j = 0; j < KW; ++j) {
-                const uint32_t u = wave * KW + j, i = u / (C + TAIL), c = u % (C + TAIL);
-                if (KU % WAVES && u >= KU) break;
-                to.k[i][2 * c][lane] = codes_f16(kb[j].x, kb[j].y);
-                if (!TAIL || c < C) to.k[i][2 * c + 1][lane] = codes_f16(kb[j].z, kb[j].w);
-            }
-#pragma unroll
-            for (int j = 0; j < VW; ++j) {
-                const uint32_t t16 = wave * VW + j;
-                if (DT % WAVES && t16 >= DT) break;
-                to.v[t16][0][lane] = codes_f16(vb[j].x, vb[j].y);
-                to.v[t16][1][lane] = codes_f16(vb[j].z, vb[j].w);
+            for (int j = 0; j < UW; ++j) {
+                const uint32_t c = c0 + j * (WAVES / 2);
+                if (C % (WAVES / 2) && c >= C) break;
+                to.k[u0][2 * c][lane] = codes_f16(kb[j].x, kb[j].y);
+                to.k[u0][2 * c + 1][lane] = codes_f16(kb[j].z, kb[j].w);
+                to.v[2 * u0][c][lane] = codes_f16(vb[j].x, vb[j].y);
+                to.v[2 * u0 + 1][c][lane] = codes_f16(vb[j].z, vb[j].w);
             }
             if (wave == 0) {
                 if (!ok) set_status(a.status, kStatusKvBadIndex);
-                if (col == 0) to.scale[g] = make_scales(ks, vs, ok);
+                if (lane < 4) to.scale[lane] = make_scales(ks, vs, ok);
             }
         };
 
@@ -759,76 +831,70 @@ __global__ __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) void k_attention_many
             }
             if (t0 < any_hi && t0 + kStep > any_lo) {
                 const StepLds<D>& from = lds[buf];
-                const Scales sc = from.scale[g];
-                // fragments are read a tile ahead of the products that take them
-                half8v kf[2][F], vf[kAhead][2];
-                float4v s[NQ][4];
+                // the fragments in the order of their use: K's of both tiles, dims by dims, then V's
+                const auto fragment = [&](int i) { return i < 2 * F ? from.k[i % 2][i / 2][lane] : from.v[(i - 2 * F) / C][(i - 2 * F) % C][lane]; };
+                half8v ring[kAhead];
 #pragma unroll
-                for (int f = 0; f < F; ++f) kf[0][f] = from.k[0][f][lane];
+                for (int i = 0; i < kAhead; ++i) ring[i] = fragment(i);
+                const Scales sc[2] = {from.scale[h], from.scale[2 + h]};
+                float16v s[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (i < 3) {
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int f = 0; f < F; ++f) kf[(i + 1) & 1][f] = from.k[i + 1][f][lane];
-                    } else {
+                    for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
 #pragma unroll
-                        for (int t = 0; t < kAhead; ++t)
+                for (int i = 0; i < 2 * F; i += 4) {
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) vf[t][h] = from.v[t][h][lane];
-                    }
+                    for (int j = i; j < i + 4; ++j)
+#pragma unroll
+                        for (int p = 0; p < NP; ++p) s[j % 2] = mfma32(ring[j % kAhead], q.f[j / 2][p], s[j % 2]);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int n = 0; n < NQ; ++n) s[n][i] = float4v{0, 0, 0, 0};
-#pragma unroll
-                    for (int f = 0; f < F; ++f)
-#pragma unroll
-                        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                            for (int p = 0; p < NP; ++p) s[n][i] = mfma(kf[i & 1][f], q[n].f[f][p], s[n][i]);
+                    for (int j = i; j < i + 4; ++j) ring[j % kAhead] = fragment(j + kAhead);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 const bool all = t0 >= all_lo && t0 + kStep <= all_hi;
-                half8v w[NQ][2][NP];
+                half8v w[2][2][NP];
+                run.template weigh<NP>(s, sc, q.c, t0 + 16 * h, q.lo, q.hi, all, w);
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) run[n].template weigh<NP>(s[n], sc, q[n].c, t0 + 16 * g, q[n].lo, q[n].hi, all, w[n]);
+                for (int i = 0; i < 4 * C; i += 4) {
 #pragma unroll
-                for (int t = 0; t < DT; ++t) {
+                    for (int j = i; j < i + 4; ++j)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                            for (int p = 0; p < NP; ++p) run[n].o[t] = mfma(vf[t % kAhead][h], w[n][h][p], run[n].o[t]);
+                        for (int p = 0; p < NP; ++p)
+                            run.o[j % C] = mfma32(ring[(2 * F + j) % kAhead], w[j / C / 2][j / C % 2][p], run.o[j % C]);
                     __builtin_amdgcn_sched_barrier(0);
-                    if (t + kAhead < DT) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) vf[t % kAhead][h] = from.v[t + kAhead][h][lane];
-                    }
+                    for (int j = i; j < i + 4; ++j)
+                        if (j + kAhead < 4 * C) ring[(2 * F + j) % kAhead] = fragment(2 * F + j + kAhead);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if (more) store(lds[buf ^ 1]);
             __syncthreads();
         }
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(run.l), __float_as_int(run.l), false, false);
+        const float l = __int_as_float(r[0]) + __int_as_float(r[1]), f = l == 0.0f ? 0.0f : 1.0f / l;
+        if (my0 + row >= packed) continue;
+        const uint32_t token = sr.row0 + (my0 + row) / a.group, head = kvh * a.group + (my0 + row) % a.group;
+        if (a.splits > 1) {
+            float* part = many_part(a, (uint64_t)token * a.heads + head, split);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            const uint32_t r = my0 + 16 * n + col;
-            const float l = column_sum(run[n].l), f = l == 0.0f ? 0.0f : 1.0f / l;
-            if (r >= packed) continue;
-            const uint32_t token = sr.row0 + r / a.group, head = kvh * a.group + r % a.group;
-            if (a.splits > 1) {
-                float* part = many_part(a, (uint64_t)token * a.heads + head, split);
+            for (int t = 0; t < C; ++t)
 #pragma unroll
-                for (int t = 0; t < DT; ++t) *reinterpret_cast<float4v*>(part + 16 * t + 4 * g) = run[n].o[t];
-                if (g == 0) {
-                    part[D] = run[n].m;
-                    part[D + 1] = l;
-                }
-            } else {
-                const uint64_t at = (uint64_t)token * a.out.stride + head * a.out.head_stride;
-#pragma unroll
-                for (int t = 0; t < DT; ++t) store4(a.out, a.type, at + 16 * t + 4 * g, run[n].o[t] * f);
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<float4v*>(part + 32 * t + 8 * i + 4 * h) = float4v{run.o[t][4 * i], run.o[t][4 * i + 1], run.o[t][4 * i + 2], run.o[t][4 * i + 3]};
+            if (h == 0) {
+                part[D] = run.m;
+                part[D + 1] = l;
             }
+        } else {
+            const uint64_t at = (uint64_t)token * a.out.stride + head * a.out.head_stride;
+#pragma unroll
+            for (int t = 0; t < C; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    store4(a.out, a.type, at + 32 * t + 8 * i + 4 * h, float4v{run.o[t][4 * i], run.o[t][4 * i + 1], run.o[t][4 * i + 2], run.o[t][4 * i + 3]} * f);
         }
     }
 }
@@ -861,7 +927,7 @@ constexpr int many_waves() {
 template <int D, int NP>
 int run_many(const AttnArgs& a, hipStream_t st) {
     constexpr int W = many_waves<D>();
-    auto* k = k_attention_many<D, NP, 2, W>;
+    auto* k = k_attention_many<D, NP, W>;
     const size_t lds = 2 * sizeof(StepLds<D>);
     // more than 64 KiB of LDS has to be asked for, once per device and kernel; cheap enough to ask every time
     if (lds > 65536)
