@@ -32,8 +32,13 @@ constexpr uint32_t kStep = 64;                     // tokens a wave takes at a t
 constexpr uint32_t kChunk = kAttnWaves * kStep;    // tokens a workgroup takes at a time
 constexpr uint32_t kChunkLog2 = 8;
 static_assert(kChunk == 1u << kChunkLog2);
-// Weights are carried times 2^14, which leaves f16 all of its 11 bits for weights down to 2^-28.
-constexpr float kWeightShift = 14.0f;
+// Weights are carried times 2^kShift, and the reference that they are taken against follows the maximum only where it would
+// take them past 2^15.5 (largest f16: 65504), so that most steps leave the outputs as they are. One piece: 2^8, which
+// leaves f16 all of its 11 bits for weights down to 2^-22 of the largest and an absolute 2^-33; two pieces: 2^14, 2^-39.
+template <int NP>
+constexpr float kShift = NP == 1 ? 8.0f : 14.0f;
+template <int NP>
+constexpr float kSlack = NP == 1 ? 7.5f : 1.5f;
 constexpr uint32_t kFewGrid = 512;      // workgroups of a call with few rows at most: two per CU
 constexpr float kTinyScale = 0x1p-80f;  // the scale that an all-zero block of V counts with
 
@@ -194,7 +199,7 @@ struct Running {
         for (int t = 0; t < DT; ++t) o[t] = float4v{0, 0, 0, 0};
     }
 
-    // A step's scores become weights w = 2^(s k + lv - m + 14) as f16 fragments; m, l and o follow. The maximum is
+    // A step's scores become weights w = 2^(s k + lv - m + kShift) as f16 fragments; m, l and o follow. The maximum is
     // taken over the scores (k is not negative), so a score costs half a max3, one multiply-add, one exp2, one add and
     // half a conversion. Four parts, so that a caller can put products between them; in all: weigh().
 
@@ -212,9 +217,10 @@ struct Running {
         return seen ? fmaf(top, sc.k * c, sc.lv) : -INFINITY;
     }
     // `top`, over the column's lanes, joins the maximum.
+    template <int NP>
     __device__ __forceinline__ void raise(float top) {
         top = column_max(top);
-        if (__ballot(top > m)) {
+        if (__ballot(top > m + kSlack<NP>)) {
             const float m_new = fmaxf(m, top), f = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
             l *= f;
 #pragma unroll
@@ -223,8 +229,9 @@ struct Running {
         }
     }
     // The exponents; with `seen`, -inf for the others.
+    template <int NP>
     __device__ __forceinline__ void exponents(const float4v (&s)[4], const Scales& sc, float c, bool all, uint32_t seen, float (&x)[16]) const {
-        const float k = sc.k * c, shift = sc.lv - (m == -INFINITY ? 0.0f : m - kWeightShift);
+        const float k = sc.k * c, shift = sc.lv - (m == -INFINITY ? 0.0f : m - kShift<NP>);
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = fmaf(s[i / 4][i % 4], k, shift);
         if (!all) {
@@ -251,14 +258,14 @@ struct Running {
                                           half8v (&w)[2][NP]) {
         uint32_t seen = 0xFFFFu;
         if (all) {
-            raise(peak(s, sc, c));
+            raise<NP>(peak(s, sc, c));
         } else {
             __asm__ volatile("");
             seen = seen_tokens(tg, lo, hi);
-            raise(peak_seen(s, sc, c, seen));
+            raise<NP>(peak_seen(s, sc, c, seen));
         }
         float x[16];
-        exponents(s, sc, c, all, seen, x);
+        exponents<NP>(s, sc, c, all, seen, x);
         weights<NP>(x, sc, w);
     }
 };
@@ -693,14 +700,14 @@ struct Running32 {
         float peak = fmaxf(top[0], top[1]);
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(peak), __float_as_int(peak), false, false);
         peak = fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
-        if (__ballot(peak > m)) {
+        if (__ballot(peak > m + kSlack<NP>)) {
             const float m_new = fmaxf(m, peak), f = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
             l *= f;
 #pragma unroll
             for (int t = 0; t < D / 32; ++t) o[t] *= f;
             m = m_new;
         }
-        const float base = m == -INFINITY ? 0.0f : m - kWeightShift;
+        const float base = m == -INFINITY ? 0.0f : m - kShift<NP>;
         float x[2][16];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -729,10 +736,10 @@ struct Running32 {
 };
 
 template <int D, int NP, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) void k_attention_many(AttnArgs a) {
+__global__ __launch_bounds__(WAVES * 64, 2) void k_attention_many(AttnArgs a) {
     constexpr int F = D / 16, C = D / 32, ROWS = 32 * WAVES;
     constexpr int UW = (C + WAVES / 2 - 1) / (WAVES / 2);  // 16-byte loads of K, and of V, per wave and step
-    constexpr int kAhead = 8;                              // fragments read ahead
+    constexpr int kAhead = NP == 2 ? 4 : 8;                // fragments read ahead (8 spill at two pieces)
     extern __shared__ __align__(16) uint8_t lds_raw[];
     StepLds<D>* lds = reinterpret_cast<StepLds<D>*>(lds_raw);
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, row = lane % 32, h = lane / 32;
@@ -899,6 +906,174 @@ __global__ __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) void k_attention_many
     }
 }
 
+// The same on v_mfma_f32_16x16x32_f16, 16 rows a wave, for the head_dims whose outputs would not leave 32-row tiles two
+// waves per SIMD. Each wave reads all of K and V from LDS for half the rows, so LDS bounds it beside the
+// products; one wave per SIMD with 32 rows was slower all the same (fp32, 24 heads of 256, 256 rows over 16300 tokens: 338 us).
+template <int D>
+struct StepLds16 {
+    half8v k[4][D / 32][64];  // [tile of 16 tokens][32 dims][lane]
+    half8v v[2][D / 16][64];  // [half of a group's tokens][tile of 16 dims][lane]
+    Scales scale[4];
+};
+
+template <int D, int NP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void k_attention_many16(AttnArgs a) {
+    static_assert(D % 64 == 0 && WAVES == 8);
+    constexpr int F = D / 32, C = D / 64, DT = D / 16, ROWS = 16 * WAVES;
+    constexpr int KW = (C + 1) / 2, VW = (DT + WAVES - 1) / WAVES;  // 16-byte loads of K and V per wave and step
+    constexpr int kAhead = 4;                                       // fragments read ahead (8 spill: 195 against 188 us)
+    extern __shared__ __align__(16) uint8_t lds_raw[];
+    StepLds16<D>* lds = reinterpret_cast<StepLds16<D>*>(lds_raw);
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, g = lane / 16;
+    const uint32_t pairs = a.b.n_seqs * a.c.heads;
+    uint32_t id = blockIdx.x;
+    const uint32_t kvh = id % a.c.heads, seq = id % pairs / a.c.heads;
+    id /= pairs;
+    const uint32_t split = id % a.splits;
+    const SeqRows sr = seq_rows(a.b, seq);
+    const uint32_t packed = (uint32_t)sr.rows * a.group, tiles = (packed + ROWS - 1) / ROWS;
+    const int32_t cap = (int32_t)(a.b.table_width * a.c.block), first = sr.len - sr.rows;
+    const int32_t* table = a.b.tables + (uint64_t)seq * a.b.table_stride;
+    const uint32_t head_codes = a.c.codes + kvh * a.c.plane;
+
+    for (uint32_t back = id / a.splits; back < tiles; back += a.tiles) {
+        const uint32_t row0 = (tiles - 1 - back) * ROWS, row_n = min(row0 + ROWS, packed);
+        const uint32_t my0 = row0 + wave * 16, my_n = min(my0 + 16, row_n);
+        const int32_t tile_lo = first + (int32_t)(row0 / a.group), tile_hi = first + (int32_t)((row_n - 1) / a.group);
+        const uint32_t begin = (uint32_t)first_seen(a, tile_lo, cap) / kStep * kStep;
+        const uint32_t end = (uint32_t)max(min(tile_hi + 1, cap + 16), 0);
+        const uint32_t steps = end > begin ? (end - begin + kStep - 1) / kStep : 0, share = (steps + a.splits - 1) / a.splits;
+        const uint32_t t_first = begin + min(split * share, steps) * kStep, t_end = min(begin + min((split + 1) * share, steps) * kStep, end);
+        const int32_t my_lo = first + (int32_t)(my0 / a.group), my_hi = my0 < my_n ? first + (int32_t)((my_n - 1) / a.group) : -1;
+        const uint32_t any_hi = (uint32_t)max(my_hi + 1, 0), all_hi = (uint32_t)max(my_lo + 1, 0);
+        const uint32_t any_lo = (uint32_t)first_seen(a, my_lo, cap), all_lo = (uint32_t)first_seen(a, my_hi, cap);
+
+        QRow<D, NP> q;
+        Running<DT> run;
+        {
+            float raw[F][8];
+            q.fetch(a, sr, kvh, my0 + col, packed, g, cap, raw);
+            q.finish(a, raw);
+            run.clear();
+        }
+
+        uint4 kb[KW], vb[VW];
+        float ks = 0.0f, vs = 0.0f;
+        bool ok = true;
+        const uint32_t tile = wave % 4, c0 = wave / 4;  // this wave's loads of K: of one tile of 16 tokens
+        const auto entry = [&](uint32_t t) { return table[min((t + 16 * (lane % 4)) >> a.c.block_log2, a.b.table_width - 1)]; };
+        const auto load = [&](uint32_t t, int32_t page_id) {
+            const uint32_t tg = t + 16 * (lane % 4);
+            ok = (uint32_t)page_id < a.c.n_pages && (tg >> a.c.block_log2) < a.b.table_width;
+            const int32_t number = ok ? page_id : 0;
+            ok = ok || tg >= end;
+            const uint32_t kg = col / 4;
+            const uint8_t* k = page_ptr(a.c, __shfl(number, kg)) + head_codes + ((t + 16 * kg) % a.c.block + 4 * tile + col % 4) * D + 16 * g;
+            const uint8_t* v = page_ptr(a.c, __shfl(number, g)) + head_codes + a.c.heads * a.c.plane + col * a.c.block + (t + 16 * g) % a.c.block;
+#pragma unroll
+            for (int j = 0; j < KW; ++j)
+                if (C % 2 == 0 || c0 + 2 * j < C) kb[j] = *reinterpret_cast<const uint4*>(k + (c0 + 2 * j) * 64);
+#pragma unroll
+            for (int j = 0; j < VW; ++j)
+                if (DT % WAVES == 0 || wave + WAVES * j < DT) vb[j] = *reinterpret_cast<const uint4*>(v + (wave + WAVES * j) * 16 * a.c.block);
+            if (wave == 0) {
+                const float* sc = reinterpret_cast<const float*>(page_ptr(a.c, number) + a.c.scales) + kvh;
+                ks = sc[0];
+                vs = sc[a.c.heads];
+            }
+        };
+        const auto store = [&](StepLds16<D>& to) {
+#pragma unroll
+            for (int j = 0; j < KW; ++j)
+                if (C % 2 == 0 || c0 + 2 * j < C) {
+                    to.k[tile][2 * (c0 + 2 * j)][lane] = codes_f16(kb[j].x, kb[j].y);
+                    to.k[tile][2 * (c0 + 2 * j) + 1][lane] = codes_f16(kb[j].z, kb[j].w);
+                }
+#pragma unroll
+            for (int j = 0; j < VW; ++j)
+                if (DT % WAVES == 0 || wave + WAVES * j < DT) {
+                    to.v[0][wave + WAVES * j][lane] = codes_f16(vb[j].x, vb[j].y);
+                    to.v[1][wave + WAVES * j][lane] = codes_f16(vb[j].z, vb[j].w);
+                }
+            if (wave == 0) {
+                if (!ok) set_status(a.status, kStatusKvBadIndex);
+                if (lane < 4) to.scale[lane] = make_scales(ks, vs, ok);
+            }
+        };
+
+        int32_t id_next = 0;
+        if (t_first < t_end) {
+            load(t_first, entry(t_first));
+            id_next = entry(t_first + kStep);
+            store(lds[0]);
+        }
+        __syncthreads();
+        uint32_t buf = 0;
+        for (uint32_t t0 = t_first; t0 < t_end; t0 += kStep, buf ^= 1) {
+            const bool more = t0 + kStep < t_end;
+            if (more) {
+                load(t0 + kStep, id_next);
+                id_next = entry(t0 + 2 * kStep);
+            }
+            if (t0 < any_hi && t0 + kStep > any_lo) {
+                const StepLds16<D>& from = lds[buf];
+                const auto fragment = [&](int i) { return i < 4 * F ? from.k[i % 4][i / 4][lane] : from.v[(i - 4 * F) / DT][(i - 4 * F) % DT][lane]; };
+                half8v ring[kAhead];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) ring[i] = fragment(i);
+                const Scales sc = from.scale[g];
+                float4v s[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] = float4v{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 4 * F; i += 4) {
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+#pragma unroll
+                        for (int j = i; j < i + 4; ++j) s[j % 4] = mfma(ring[j % kAhead], q.f[j / 4][p], s[j % 4]);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int j = i; j < i + 4; ++j) ring[j % kAhead] = fragment(j + kAhead);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const bool all = t0 >= all_lo && t0 + kStep <= all_hi;
+                half8v w[2][NP];
+                run.template weigh<NP>(s, sc, q.c, t0 + 16 * g, q.lo, q.hi, all, w);
+#pragma unroll
+                for (int i = 0; i < 2 * DT; i += 4) {
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+#pragma unroll
+                        for (int j = i; j < i + 4; ++j) run.o[j % DT] = mfma(ring[(4 * F + j) % kAhead], w[j / DT][p], run.o[j % DT]);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int j = i; j < i + 4; ++j)
+                        if (j + kAhead < 2 * DT) ring[(4 * F + j) % kAhead] = fragment(4 * F + j + kAhead);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (more) store(lds[buf ^ 1]);
+            __syncthreads();
+        }
+        const float l = column_sum(run.l), f = l == 0.0f ? 0.0f : 1.0f / l;
+        if (my0 + col >= packed) continue;
+        const uint32_t token = sr.row0 + (my0 + col) / a.group, head = kvh * a.group + (my0 + col) % a.group;
+        if (a.splits > 1) {
+            float* part = many_part(a, (uint64_t)token * a.heads + head, split);
+#pragma unroll
+            for (int t = 0; t < DT; ++t) *reinterpret_cast<float4v*>(part + 16 * t + 4 * g) = run.o[t];
+            if (g == 0) {
+                part[D] = run.m;
+                part[D + 1] = l;
+            }
+        } else {
+            const uint64_t at = (uint64_t)token * a.out.stride + head * a.out.head_stride;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) store4(a.out, a.type, at + 16 * t + 4 * g, run.o[t] * f);
+        }
+    }
+}
+
 // Joins the splits of each (row, head), in order: D / 4 lanes a row.
 __global__ __launch_bounds__(256) void k_attention_many_join(AttnArgs a) {
     const uint32_t D = a.c.dim, quads = D / 4, at_once = 256 / quads, d = threadIdx.x % quads * 4;
@@ -919,16 +1094,24 @@ __global__ __launch_bounds__(256) void k_attention_many_join(AttnArgs a) {
     store4(a.out, a.type, row * a.out.stride + head * a.out.head_stride + d, sum == 0.0f ? float4v{0, 0, 0, 0} : acc / sum);
 }
 
+// Waves of a workgroup: of 32 rows each, or of 16 where the outputs of 32 would leave one wave per SIMD.
 template <int D>
-constexpr int many_waves() {
-    return 4;
-}
+constexpr int kManyWaves = 8;
+template <int D>
+constexpr bool kHalfTiles = D > 128;
 
 template <int D, int NP>
 int run_many(const AttnArgs& a, hipStream_t st) {
-    constexpr int W = many_waves<D>();
-    auto* k = k_attention_many<D, NP, W>;
-    const size_t lds = 2 * sizeof(StepLds<D>);
+    constexpr int W = kManyWaves<D>;
+    void (*k)(AttnArgs);
+    size_t lds;
+    if constexpr (kHalfTiles<D>) {
+        k = k_attention_many16<D, NP, W>;
+        lds = 2 * sizeof(StepLds16<D>);
+    } else {
+        k = k_attention_many<D, NP, W>;
+        lds = 2 * sizeof(StepLds<D>);
+    }
     // more than 64 KiB of LDS has to be asked for, once per device and kernel; cheap enough to ask every time
     if (lds > 65536)
         if (int rc = hip_status(hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "ATTENTION")) return rc;
@@ -940,19 +1123,19 @@ int run_many(const AttnArgs& a, hipStream_t st) {
     return HALO_MI_OK;
 }
 
-constexpr uint64_t kMaxGrid = 1u << 22;  // workgroups of a launch (256 threads each; n_seqs * kv heads is at most this)
-constexpr uint32_t many_rows(uint32_t) { return 128; }
+constexpr uint64_t kMaxGrid = 1u << 22;  // workgroups of a launch (up to 512 threads each; n_seqs * kv heads is at most this)
+constexpr uint32_t many_rows(uint32_t dim) { return dim > 128 ? 128 : 256; }
 
 }  // namespace
 
 namespace {
 
-// Tiles of a call with many rows, and the splits that bring two workgroups (one at a head_dim over 128) to every CU.
+// Tiles of a call with many rows, and the splits that bring a workgroup to every CU.
 uint64_t plan_many(AttnArgs& a, uint64_t part_bytes) {
     const uint32_t rows = many_rows(a.c.dim);
     const uint64_t pairs = (uint64_t)a.c.heads * a.b.n_seqs;
     a.tiles = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(((uint64_t)a.b.max_rows * a.group + rows - 1) / rows, kMaxGrid / pairs));
-    const uint64_t groups = a.tiles * pairs, want = a.c.dim <= 128 ? 512 : 256;
+    const uint64_t groups = a.tiles * pairs, want = 256;
     uint64_t span = a.b.max_kv;
     if (a.window) span = std::min<uint64_t>(span, (uint64_t)a.window + rows / a.group + kStep);
     const uint64_t each = (uint64_t)a.b.n_rows * a.heads * (a.c.dim + 4) * sizeof(float);

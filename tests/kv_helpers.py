@@ -165,14 +165,15 @@ def attention_bound(t, dim, tokens, out, weight, reach, vmax):
     Scores: dim products summed in fp32 (dim U), q within 2^-22 for fp32 and exact for 16 bits, the two
     multiplications by scales and the logarithm's rounding (4 U) on values up to the score plus |log2 vs| < 32 and the
     shift by the maximum: (dim + 8) U + 2^-22 of reach, and 64 U at the level of the exponent.
-    Weights: exp2 within 2 U, then 11 bits (2^-12 kept relative) or two pieces (2^-22); weights under 2^-28 of the
-    row's largest keep 2^-39 of it. Both sums have up to `tokens` terms: tokens U each. A relative error e of
+    Weights: exp2 within 2 U, then 11 bits (2^-12 kept relative) or two pieces (2^-22). They are carried times 2^8 (two
+    pieces: 2^14) of a reference that is at most the row's largest, and f16's smallest step is 2^-24: what is lost
+    under its normal numbers is up to 2^-25 / 2^8 (2^-25 / 2^14) of the largest weight, for each token. Both sums have up to `tokens` terms: tokens U each. A relative error e of
     every weight moves the quotient by at most 2 e sum p |v|.
     """
     pieces = 2.0 ** -22 if t == F32 else 2.0 ** -12
     e = ((dim + 8) * U + (2.0 ** -22 if t == F32 else 0)) * reach[..., None] + 64 * U + pieces
     sums = 2 * (tokens + 16) * U
-    return weight * (2 * e + sums) + tokens * 2.0 ** -38 * vmax + HALF_STEP[t] * np.abs(out) * 1.01 + HALF_LEAST[t] + 1e-30
+    return weight * (2 * e + sums) + tokens * (2.0 ** -38 if t == F32 else 2.0 ** -32) * vmax + HALF_STEP[t] * np.abs(out) * 1.01 + HALF_LEAST[t] + 1e-30
 
 
 def batch(rows):
