@@ -199,6 +199,9 @@ class _RopePart(ctypes.Structure):
                 ("n_heads", ctypes.c_uint32)]
 
 
+_RopeParts = _RopePart * 2
+
+
 class _RopeParams(ctypes.Structure):
     _fields_ = [("type", ctypes.c_uint32), ("pairs", ctypes.c_uint32), ("parts", ctypes.POINTER(_RopePart)),
                 ("n_parts", ctypes.c_uint32), ("n_tokens", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
@@ -556,28 +559,52 @@ class KvState(typing.NamedTuple):
     table_stride: int = 0
 
 
-def _dev(t) -> int:
-    """Device address of an operand; a tensor has to be on the current device."""
-    if t is None or isinstance(t, int):
-        return t or 0
+def _current_device() -> int:
+    """The current GPU, or -2 where nothing runs on one yet (no tensor is there then: a CPU tensor's is -1)."""
     import torch
 
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+
+
+def _raw_stream(stream, dev: int) -> int:
+    """The given stream, or torch's current one on device dev."""
+    if stream is not None:
+        return int(stream)
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(dev) if dev >= 0 else _stream(None)
+
+
+def _dev(t, dev: int) -> int:
+    """Device address of an operand; a tensor has to be on the current device."""
+    if t is None:
+        return 0
+    if t.__class__ is int:
+        return t
+    if t.get_device() != dev:
         raise HaloError(ErrorCode.Kernel, f"an operand is on {t.device}, not on the current GPU")
     return t.data_ptr()
 
 
-def _cache(c: KvCache) -> _KvCache:
-    return _KvCache(_dev(c.pool), int(c.n_pages), int(c.n_layers), int(c.n_kv_heads), int(c.head_dim), int(c.block_tokens))
+def _block(cls, *values):
+    """A parameter block. Integers of other kinds (numpy's) are converted where there are any."""
+    try:
+        return cls(*values)
+    except TypeError:
+        return cls(*(int(v) if hasattr(v, "__index__") else v for v in values))
 
 
-def _batch(b: KvBatch) -> _KvBatch:
-    return _KvBatch(_dev(b.tables), int(b.table_stride), int(b.table_width), _dev(b.kv_lens), _dev(b.row_starts),
-                    int(b.n_seqs), int(b.n_rows), int(b.max_rows), int(b.max_kv))
+def _cache(c: KvCache, dev: int) -> _KvCache:
+    return _block(_KvCache, _dev(c.pool, dev), c.n_pages, c.n_layers, c.n_kv_heads, c.head_dim, c.block_tokens)
 
 
-def _state(s: KvState) -> _KvState:
-    return _KvState(_dev(s.refs), _dev(s.lens), _dev(s.tables), int(s.table_stride), int(s.table_width), int(s.n_slots))
+def _batch(b: KvBatch, dev: int) -> _KvBatch:
+    return _block(_KvBatch, _dev(b.tables, dev), b.table_stride, b.table_width, _dev(b.kv_lens, dev), _dev(b.row_starts, dev), b.n_seqs, b.n_rows,
+                    b.max_rows, b.max_kv)
+
+
+def _state(s: KvState, dev: int) -> _KvState:
+    return _block(_KvState, _dev(s.refs, dev), _dev(s.lens, dev), _dev(s.tables, dev), s.table_stride, s.table_width, s.n_slots)
 
 
 def rope_freqs(rot_dims: int, theta: float = 10000.0, *, scaling: int = RopeScaling.PLAIN, scale: float = 1.0,
@@ -599,42 +626,45 @@ def rope(t: int, positions, freqs, n_tokens: int, head_dim: int, rot_dims: int, 
          k_head_stride: int = 0, k_out_stride: int = 0, k_out_head_stride: int = 0, stream=None) -> None:
     """PARTIAL_ROPE of q and, with k, of k in one launch (halo_mi_rope). q_out may be q, k_out may be k. positions:
     int32, freqs: float64 radians per position (rope_freqs), both on the device; strides in elements."""
-    parts = (_RopePart * 2)(
-        _RopePart(_dev(q), int(q_stride), int(q_head_stride), _dev(q_out), int(q_out_stride), int(q_out_head_stride), int(n_heads)),
-        _RopePart(_dev(k), int(k_stride), int(k_head_stride), _dev(k_out), int(k_out_stride), int(k_out_head_stride), int(n_kv_heads)))
-    p = _RopeParams(int(t), int(pairs), parts, 1 if k is None else 2, int(n_tokens), int(head_dim), int(rot_dims), _dev(positions),
-                    _dev(freqs), float(factor))
-    _check(lib().halo_mi_rope(ctypes.byref(p), _stream(stream)))
+    dev = _current_device()
+    parts = _RopeParts(
+        _block(_RopePart, _dev(q, dev), q_stride, q_head_stride, _dev(q_out, dev), q_out_stride, q_out_head_stride, n_heads),
+        _block(_RopePart, _dev(k, dev), k_stride, k_head_stride, _dev(k_out, dev), k_out_stride, k_out_head_stride, n_kv_heads))
+    p = _block(_RopeParams, t, pairs, parts, 1 if k is None else 2, n_tokens, head_dim, rot_dims, _dev(positions, dev),
+                    _dev(freqs, dev), factor)
+    _check(lib().halo_mi_rope(ctypes.byref(p), _raw_stream(stream, dev)))
 
 
 def kv_page_bytes(n_layers: int, n_kv_heads: int, head_dim: int, block_tokens: int) -> int:
     """Bytes of a page of the 8-bit cache; 0 for a geometry that it does not have."""
-    return int(lib().halo_mi_kv_page_bytes(int(n_layers), int(n_kv_heads), int(head_dim), int(block_tokens)))
+    return int(lib().halo_mi_kv_page_bytes(n_layers, n_kv_heads, head_dim, block_tokens))
 
 
 def kv_write(t: int, cache: KvCache, layer: int, batch: KvBatch, k, v, *, k_stride: int = 0, k_head_stride: int = 0,
              v_stride: int = 0, v_head_stride: int = 0, status=None, status_keep: bool = False, stream=None) -> None:
     """KV_WRITE: the batch's rows of k and v into their sequences' pages (halo_mi_kv_write)."""
-    p = _KvWriteParams(int(t), _cache(cache), int(layer), _batch(batch), _dev(k), int(k_stride), int(k_head_stride), _dev(v),
-                       int(v_stride), int(v_head_stride), _dev(status), 1 if status_keep else 0)
-    _check(lib().halo_mi_kv_write(ctypes.byref(p), _stream(stream)))
+    dev = _current_device()
+    p = _block(_KvWriteParams, t, _cache(cache, dev), layer, _batch(batch, dev), _dev(k, dev), k_stride, k_head_stride, _dev(v, dev),
+                       v_stride, v_head_stride, _dev(status, dev), 1 if status_keep else 0)
+    _check(lib().halo_mi_kv_write(ctypes.byref(p), _raw_stream(stream, dev)))
 
 
 def kv_read(cache: KvCache, layer: int, batch: KvBatch, k_out=None, v_out=None, *, k_stride: int = 0, k_head_stride: int = 0,
             v_stride: int = 0, v_head_stride: int = 0, status=None, status_keep: bool = False, stream=None) -> None:
     """The values that the cache holds for the batch's rows, in fp32 (halo_mi_kv_read)."""
-    p = _KvReadParams(_cache(cache), int(layer), _batch(batch), _dev(k_out), int(k_stride), int(k_head_stride), _dev(v_out),
-                      int(v_stride), int(v_head_stride), _dev(status), 1 if status_keep else 0)
-    _check(lib().halo_mi_kv_read(ctypes.byref(p), _stream(stream)))
+    dev = _current_device()
+    p = _block(_KvReadParams, _cache(cache, dev), layer, _batch(batch, dev), _dev(k_out, dev), k_stride, k_head_stride, _dev(v_out, dev),
+                      v_stride, v_head_stride, _dev(status, dev), 1 if status_keep else 0)
+    _check(lib().halo_mi_kv_read(ctypes.byref(p), _raw_stream(stream, dev)))
 
 
 def _attention_params(t, cache, layer, batch, q, out, n_heads, scale, window, q_stride, q_head_stride, out_stride, out_head_stride,
-                      workspace, workspace_bytes, status, status_keep):
+                      workspace, workspace_bytes, status, status_keep, dev):
     if workspace is not None and not isinstance(workspace, int) and not workspace_bytes:
         workspace_bytes = workspace.numel() * workspace.element_size()
-    return _AttentionParams(int(t), _cache(cache), int(layer), _batch(batch), _dev(q), int(q_stride), int(q_head_stride), _dev(out),
-                            int(out_stride), int(out_head_stride), int(n_heads), float(scale), int(window), _dev(workspace),
-                            int(workspace_bytes), _dev(status), 1 if status_keep else 0)
+    return _block(_AttentionParams, t, _cache(cache, dev), layer, _batch(batch, dev), _dev(q, dev), q_stride, q_head_stride, _dev(out, dev),
+                            out_stride, out_head_stride, n_heads, scale, window, _dev(workspace, dev),
+                            workspace_bytes, _dev(status, dev), 1 if status_keep else 0)
 
 
 def attention(t: int, cache: KvCache, layer: int, batch: KvBatch, q, out, n_heads: int, *, scale: float = 0.0, window: int = 0,
@@ -642,44 +672,50 @@ def attention(t: int, cache: KvCache, layer: int, batch: KvBatch, q, out, n_head
               workspace_bytes: int = 0, status=None, status_keep: bool = False, stream=None) -> None:
     """ATTENTION of the batch's rows over their sequences' cached tokens, causal, over the last `window` tokens where it
     is not 0 (halo_mi_attention). scale 0: 1 / sqrt(head_dim)."""
+    dev = _current_device()
     p = _attention_params(t, cache, layer, batch, q, out, n_heads, scale, window, q_stride, q_head_stride, out_stride, out_head_stride,
-                          workspace, workspace_bytes, status, status_keep)
-    _check(lib().halo_mi_attention(ctypes.byref(p), _stream(stream)))
+                          workspace, workspace_bytes, status, status_keep, dev)
+    _check(lib().halo_mi_attention(ctypes.byref(p), _raw_stream(stream, dev)))
 
 
 def attention_workspace(t: int, cache: KvCache, layer: int, batch: KvBatch, q, out, n_heads: int, *, window: int = 0,
                         q_stride: int = 0, q_head_stride: int = 0, out_stride: int = 0, out_head_stride: int = 0) -> int:
     """Workspace bytes that the same attention call makes use of (halo_mi_attention_workspace)."""
+    dev = _current_device()
     p = _attention_params(t, cache, layer, batch, q, out, n_heads, 0.0, window, q_stride, q_head_stride, out_stride, out_head_stride,
-                          None, 0, None, False)
+                          None, 0, None, False, dev)
     return int(lib().halo_mi_attention_workspace(ctypes.byref(p)))
 
 
 def kv_resize(cache: KvCache, state: KvState, slots, new_lens, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
     """Gives slots their new lengths, with pages taken and released (halo_mi_kv_resize); length 0 frees a slot."""
-    c, s = _cache(cache), _state(state)
-    _check(lib().halo_mi_kv_resize(ctypes.byref(c), ctypes.byref(s), _dev(slots), _dev(new_lens), int(n), _dev(status),
-                                   1 if status_keep else 0, _stream(stream)))
+    dev = _current_device()
+    c, s = _cache(cache, dev), _state(state, dev)
+    _check(lib().halo_mi_kv_resize(ctypes.byref(c), ctypes.byref(s), _dev(slots, dev), _dev(new_lens, dev), n, _dev(status, dev),
+                                   1 if status_keep else 0, _raw_stream(stream, dev)))
 
 
 def kv_fork(cache: KvCache, state: KvState, src, dst, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
     """Empty slots dst become copies of src: whole pages shared, a last one that is not full copied (halo_mi_kv_fork)."""
-    c, s = _cache(cache), _state(state)
-    _check(lib().halo_mi_kv_fork(ctypes.byref(c), ctypes.byref(s), _dev(src), _dev(dst), int(n), _dev(status),
-                                 1 if status_keep else 0, _stream(stream)))
+    dev = _current_device()
+    c, s = _cache(cache, dev), _state(state, dev)
+    _check(lib().halo_mi_kv_fork(ctypes.byref(c), ctypes.byref(s), _dev(src, dev), _dev(dst, dev), n, _dev(status, dev),
+                                 1 if status_keep else 0, _raw_stream(stream, dev)))
 
 
 def kv_compact(cache: KvCache, state: KvState, *, live=None, stream=None) -> None:
     """Moves the live pages to the front of the pool (halo_mi_kv_compact); live (uint32 or int32) receives their number."""
-    c, s = _cache(cache), _state(state)
-    _check(lib().halo_mi_kv_compact(ctypes.byref(c), ctypes.byref(s), _dev(live), _stream(stream)))
+    dev = _current_device()
+    c, s = _cache(cache, dev), _state(state, dev)
+    _check(lib().halo_mi_kv_compact(ctypes.byref(c), ctypes.byref(s), _dev(live, dev), _raw_stream(stream, dev)))
 
 
 def kv_copy_pages(cache: KvCache, src, dst, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
     """Copies whole pages (halo_mi_kv_copy_pages)."""
-    c = _cache(cache)
-    _check(lib().halo_mi_kv_copy_pages(ctypes.byref(c), _dev(src), _dev(dst), int(n), _dev(status), 1 if status_keep else 0,
-                                       _stream(stream)))
+    dev = _current_device()
+    c = _cache(cache, dev)
+    _check(lib().halo_mi_kv_copy_pages(ctypes.byref(c), _dev(src, dev), _dev(dst, dev), n, _dev(status, dev), 1 if status_keep else 0,
+                                       _raw_stream(stream, dev)))
 
 
 def stream_read(p, nbytes: int, workgroups: int, unroll: int, sink, stream=None) -> None:
