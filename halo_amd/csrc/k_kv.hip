@@ -3,16 +3,16 @@
 //
 // A page holds block tokens of a layer as int8 codes with one scale for K and one for V per head. Rows that
 // fall into a page widen its scale to max(scale, amax / 127); where it grew, the codes of the tokens that the
-// page holds already move to the new scale. Codes are the nearest integers to x / scale exactly (ties to even):
-// the fp32 product with the reciprocal is within 2^-22 of the quotient, and only a value that close to a border
-// between two codes is decided in 64 bits, where both sides of the comparison are exact.
+// page holds already move to the new scale. Codes are the nearest integers to x / scale exactly (ties to even).
 //
-// One workgroup owns one (page, K or V, head): nobody else touches its codes and scale. K rows are [token][dim];
-// V is [dim][token], so a thread takes 16 tokens of one dim and stores them as 16 bytes.
+// One workgroup owns one (page, K or V, head): nobody else touches its codes and scale. K rows are [token][dim], V
+// [dim][token]: a thread takes patches of 4 tokens by 16 bytes of a row, which are whole words of V's codes, and keeps
+// them in registers from the maximum to the codes, so that x is read once.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "kv.h"
 #include "kv_device.h"
@@ -25,18 +25,20 @@ using namespace dev;
 
 constexpr uint32_t kKvBlock = 256;
 
-// The integer nearest to x / s (ties to even) for |x| <= 127.5 s, s > 0; inv = 1 / s rounded.
-__device__ __forceinline__ int32_t nearest(float x, float s, float inv) {
-    const float q = x * inv;
-    int32_t r = (int32_t)rintf(q);
-    const float from_border = 0.5f - fabsf(q - (float)r);
-    if (from_border < 0x1p-14f) {  // 2^-22 * 127 at most is lost in q
-        // 2 x against (2 r + 1) s and (2 r - 1) s: 24 + 9 bits, exact in 64
-        const double x2 = 2.0 * x, up = (double)(2 * r + 1) * s, down = (double)(2 * r - 1) * s;
-        if (x2 > up || (x2 == up && (r & 1))) ++r;
-        else if (x2 < down || (x2 == down && (r & 1))) --r;
+// The integer nearest to x / s (ties to even), exactly, for |x| <= 127 s (1 + 2^-23), s normal; inv = 1 / s rounded. Without
+// EXACT it is that or its neighbour, the latter only where `unsure` is set. r is one of the two, and e = x - r s decides:
+// for r even and not 0, x >= 1.5 s is a multiple of s's last bit and e fits 24 bits; for r = 0 e is x; for r = +-1 e is
+// exact from x = s / 2 on, and below, where it may round to s / 2, the tie moves an odd r the same way.
+template <bool EXACT>
+__device__ __forceinline__ int32_t nearest(float x, float s, float inv, bool& unsure) {
+    float r = rintf(x * inv);
+    const float e = fmaf(-r, s, x), half = 0.5f * s;
+    if constexpr (EXACT) {
+        if (fabsf(e) > half || (fabsf(e) == half && ((int32_t)r & 1))) r += copysignf(1.0f, e);
+    } else {
+        unsure = unsure || fabsf(e) >= half;
     }
-    return min(max(r, -127), 127);
+    return (int32_t)r;
 }
 
 // The code c of a block of scale s0 in scale s1 > s0: the integer nearest to c * s0 / s1, exactly.
@@ -77,81 +79,165 @@ __device__ __forceinline__ bool page_part(const KvBatch& b, const KvLayer& c, ui
     return true;
 }
 
-// V: elements per load of a K or V row.
+// A thread's patch: 4 tokens that share a word of V's codes, V consecutive dims of each.
 template <typename T, int V>
+struct Patch {
+    Vec<T, V> row[4];
+};
+
+// The largest |element| of a patch as a word that orders like it (abs_bits, or the type's own 16 bits twice).
+template <typename T, int V>
+__device__ __forceinline__ uint32_t patch_peak(const Patch<T, V>& q, uint32_t top) {
+    if constexpr (sizeof(T) == 2 && V > 1) {
+        typedef uint16_t ushort2v __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int j = 0; j < V; j += 2) {
+                const uint32_t w = (uint32_t)__builtin_bit_cast(uint16_t, q.row[k].v[j]) | (uint32_t)__builtin_bit_cast(uint16_t, q.row[k].v[j + 1]) << 16;
+                top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, top), __builtin_bit_cast(ushort2v, w & 0x7FFF7FFFu)));
+            }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) top = max(top, abs_bits(to_f32(q.row[k].v[j])));
+    }
+    return top;
+}
+// ... and what it stands for, as abs_bits.
+template <typename T, int V>
+__device__ __forceinline__ uint32_t peak_bits(uint32_t top) {
+    if constexpr (sizeof(T) == 2 && V > 1) {
+        const uint16_t h = (uint16_t)max(top & 0xFFFFu, top >> 16);
+        return abs_bits(to_f32(__builtin_bit_cast(T, h)));
+    } else {
+        return top;
+    }
+}
+
+// V: elements per load of a K or V row. KEEP: patches per thread that stay in registers between the maximum and the
+// codes; a part with more is read again.
+template <typename T, int V, int KEEP>
 __device__ void write_part(const KvWriteArgs& a, const PagePart& p, uint32_t which, uint32_t head, uint32_t* lds) {
     const KvLayer& c = a.c;
-    const uint32_t tid = threadIdx.x, dim = c.dim;
-    uint8_t* page = c.pool + (uint64_t)(uint32_t)p.page * c.page_bytes;
-    uint8_t* codes = page + c.codes + (which * c.heads + head) * c.plane;
-    float* scale = reinterpret_cast<float*>(page + c.scales) + which * c.heads + head;
+    const uint32_t tid = threadIdx.x, dim = c.dim, vecs = dim / V;
     const T* x = static_cast<const T*>(a.x[which].data) + (uint64_t)p.row * a.x[which].stride + head * a.x[which].head_stride;
     const uint64_t stride = a.x[which].stride;
-    const float s0 = p.off ? *scale : 0.0f;
-
-    uint32_t top = 0;
-    const uint32_t vecs = dim / V;
-    for (uint32_t i = tid; i < p.n * vecs; i += kKvBlock) {
-        const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + (i / vecs) * stride + i % vecs * V);
+    // groups of 4 tokens, aligned in the page, that the part touches
+    const uint32_t g0 = p.off / 4, patches = ((p.off + p.n + 3) / 4 - g0) * vecs;
+    const bool kept = patches <= KEEP * kKvBlock;
+    const auto load = [&](uint32_t i, Patch<T, V>& q) {
+        const uint32_t t0 = (g0 + i / vecs) * 4, d = i % vecs * V;
 #pragma unroll
-        for (int k = 0; k < V; ++k) top = max(top, abs_bits(to_f32(v.v[k])));
+        for (uint32_t k = 0; k < 4; ++k)
+            if (t0 + k >= p.off && t0 + k < p.off + p.n) q.row[k] = *reinterpret_cast<const Vec<T, V>*>(x + (t0 + k - p.off) * stride + d);
+            else q.row[k] = {};
+    };
+    uint32_t top = 0;
+    Patch<T, V> mine[KEEP];
+    if (kept) {
+#pragma unroll
+        for (int j = 0; j < KEEP; ++j) load(min(tid + j * kKvBlock, patches - 1), mine[j]);  // past the end: not used
     }
+    uint8_t* page = c.pool + (uint64_t)(uint32_t)p.page * c.page_bytes;
+    uint8_t* codes = page + c.codes + (which * c.heads + head) * c.plane;
+    uint32_t* words = reinterpret_cast<uint32_t*>(codes);
+    float* scale = reinterpret_cast<float*>(page + c.scales) + which * c.heads + head;
+    const float s0 = p.off ? *scale : 0.0f;
+    if (kept) {
+#pragma unroll
+        for (int j = 0; j < KEEP; ++j) top = patch_peak(mine[j], top);
+    } else {
+        for (uint32_t i = tid; i < patches; i += kKvBlock) {
+            load(i, mine[0]);
+            top = patch_peak(mine[0], top);
+        }
+    }
+    top = peak_bits<T, V>(top);
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
     if (tid % 64 == 0) lds[tid / 64] = top;
-    __syncthreads();
+    __syncthreads();  // every thread has s0, too
     top = max(max(lds[0], lds[1]), max(lds[2], lds[3]));
     const float fit = __uint_as_float(top) / 127.0f;
     float s1 = fit < kKvMinScale ? s0 : fmaxf(s0, fit);
     if (top > kLargestFinite || s0 != s0) s1 = __uint_as_float(0x7FC00000u);
-    __syncthreads();  // every thread has s0 and the partial maxima
     if (tid == 0) *scale = s1;
     if (s1 != s1) return;  // the codes of a NaN block mean nothing
-    const bool grew = p.off && s1 > s0 && s0 > 0.0f;
-    const float inv = s1 > 0.0f ? 1.0f / s1 : 0.0f;
-    auto code = [&](float v) { return s1 > 0.0f ? (uint32_t)(uint8_t)nearest(v, s1, inv) : 0u; };
 
-    if (which == 0) {
-        uint32_t* rows = reinterpret_cast<uint32_t*>(codes);
-        if (grew)
-            for (uint32_t i = tid; i < p.off * dim / 4; i += kKvBlock) rows[i] = rescaled4(rows[i], s0, s1);
-        constexpr int W = V < 4 ? 4 : V;  // codes per store
-        for (uint32_t i = tid; i < p.n * (dim / W); i += kKvBlock) {
-            const uint32_t t = i / (dim / W), d = i % (dim / W) * W;
-            uint32_t word[W / 4] = {};
-#pragma unroll
-            for (int k = 0; k < W; k += V) {
-                const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + t * stride + d + k);
-#pragma unroll
-                for (int j = 0; j < V; ++j) word[(k + j) / 4] |= code(to_f32(v.v[j])) << (8 * ((k + j) % 4));
+    if (p.off && s1 > s0 && s0 > 0.0f) {  // the scale grew: the earlier tokens' codes follow
+        if (which == 0) {
+            for (uint32_t i = tid; i < p.off * dim / 4; i += kKvBlock) words[i] = rescaled4(words[i], s0, s1);
+        } else {
+            const uint32_t per = (p.off + 3) / 4;  // words of a dim
+            for (uint32_t i = tid; i < per * dim; i += kKvBlock) {
+                uint32_t* w = words + i / per * (c.block / 4) + i % per;
+                const uint32_t keep = i % per * 4 + 4 <= p.off ? 0u : 0xFFFFFFFFu << 8 * (p.off % 4), old = *w;
+                *w = (old & keep) | (rescaled4(old, s0, s1) & ~keep);
             }
-#pragma unroll
-            for (int k = 0; k < W / 4; ++k) rows[((p.off + t) * dim + d) / 4 + k] = word[k];
         }
-        return;
+        __syncthreads();
     }
-    // V: 16 tokens of one dim at a time; from the page's first one where the earlier codes change
-    const uint32_t g0 = grew ? 0 : p.off / 16, g1 = (p.off + p.n + 15) / 16;
-    for (uint32_t i = tid; i < (g1 - g0) * dim; i += kKvBlock) {
-        const uint32_t d = i % dim, t0 = (g0 + i / dim) * 16;
-        uint4* at = reinterpret_cast<uint4*>(codes + d * c.block + t0);
-        uint4 old = {};
-        if (t0 < p.off || t0 + 16 > p.off + p.n) old = *at;
-        uint32_t word[4] = {old.x, old.y, old.z, old.w};
+    const float inv = s1 > 0.0f ? 1.0f / s1 : 0.0f;
+    const bool some = s1 > 0.0f;
+    // The patch's codes, four tokens of a dim to a word; exactly where an element is too near a border to be sure.
+    const auto codes_of = [&](const Patch<T, V>& q, uint32_t (&word)[V]) {
+        const auto all = [&](auto exact, float by, float inv) {
+            bool unsure = false;
 #pragma unroll
-        for (uint32_t k = 0; k < 16; ++k) {
-            const uint32_t t = t0 + k, shift = 8 * (k % 4), have = word[k / 4];
-            uint32_t v;
-            if (t >= p.off && t < p.off + p.n) v = code(to_f32(x[(t - p.off) * stride + d]));
-            else if (t < p.off && grew) v = (uint8_t)rescaled((int8_t)(have >> shift), s0, s1);
-            else continue;
-            word[k / 4] = (have & ~(0xFFu << shift)) | v << shift;
+            for (int j = 0; j < V; ++j) {
+                word[j] = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    word[j] |= (uint32_t)(uint8_t)nearest<decltype(exact)::value>(to_f32(q.row[k].v[j]), by, inv, unsure) << 8 * k;
+            }
+            return unsure;
+        };
+        if (all(std::false_type{}, s1, inv)) {
+            float by = s1, again = inv;
+            __asm__ volatile("" : "+v"(by), "+v"(again));  // nothing of the first pass is kept in registers for this one
+            all(std::true_type{}, by, again);
         }
-        *at = {word[0], word[1], word[2], word[3]};
+    };
+    const auto store = [&](uint32_t i, const Patch<T, V>& q) {
+        const uint32_t t0 = (g0 + i / vecs) * 4, d = i % vecs * V;
+        uint32_t cover = 0;  // the bytes of a word of V's that are this part's
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+            if (t0 + k >= p.off && t0 + k < p.off + p.n) cover |= 0xFFu << 8 * k;
+        uint32_t word[V] = {};
+        if (some) codes_of(q, word);
+        if (which == 0) {
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                if (!(cover >> 8 * k & 1)) continue;
+                Vec<uint8_t, V> out;
+#pragma unroll
+                for (int j = 0; j < V; ++j) out.v[j] = (uint8_t)(word[j] >> 8 * k);
+                *reinterpret_cast<Vec<uint8_t, V>*>(codes + (t0 + k) * dim + d) = out;
+            }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            uint32_t* w = words + ((d + j) * c.block + t0) / 4;
+            *w = cover == 0xFFFFFFFFu ? word[j] : (*w & ~cover) | (word[j] & cover);
+        }
+    };
+    if (kept) {
+#pragma unroll
+        for (int j = 0; j < KEEP; ++j)
+            if (tid + j * kKvBlock < patches) store(tid + j * kKvBlock, mine[j]);
+    } else {
+        for (uint32_t i = tid; i < patches; i += kKvBlock) {
+            load(i, mine[0]);
+            store(i, mine[0]);
+        }
     }
 }
 
-template <typename T, int V>
+template <typename T, int V, int KEEP>
 __global__ __launch_bounds__(kKvBlock) void k_kv_write(KvWriteArgs a) {
     __shared__ uint32_t lds[kKvBlock / 64];
     const uint32_t s = blockIdx.z, head = blockIdx.y >> 1, which = blockIdx.y & 1;
@@ -162,7 +248,7 @@ __global__ __launch_bounds__(kKvBlock) void k_kv_write(KvWriteArgs a) {
             if (threadIdx.x == 0) set_status(a.status, kStatusKvBadIndex);
             continue;
         }
-        write_part<T, V>(a, p, which, head, lds);
+        write_part<T, V, KEEP>(a, p, which, head, lds);
         __syncthreads();
     }
 }
@@ -221,7 +307,10 @@ int launch_write_typed(const KvWriteArgs& a, hipStream_t st) {
     bool wide = true;
     for (const HeadRows& r : a.x)
         wide = wide && reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && r.stride % V == 0 && r.head_stride % V == 0;
-    hipLaunchKernelGGL((wide ? k_kv_write<T, V> : k_kv_write<T, 1>), page_grid(a.c, a.b), dim3(kKvBlock), 0, st, a);
+    // patches of a page per thread
+    const uint32_t each = (a.c.block / 4 * (a.c.dim / V) + kKvBlock - 1) / kKvBlock;
+    auto* k = !wide ? k_kv_write<T, 1, 4> : each <= 1 ? k_kv_write<T, V, 1> : each <= 2 ? k_kv_write<T, V, 2> : k_kv_write<T, V, 4>;
+    hipLaunchKernelGGL(k, page_grid(a.c, a.b), dim3(kKvBlock), 0, st, a);
     return hip_status(hipGetLastError(), "KV_WRITE");
 }
 

@@ -4,8 +4,8 @@
 //
 // Who gets which page is one order (the list's) over another (the free pages by number), so one workgroup of 1024
 // threads decides: prefix sums over the list and over the counts, 4096 counts a step. What costs time is the
-// pages' bytes (hundreds of KB each with all layers): a second kernel copies them with the whole GPU, from a
-// list that the first one leaves in scratch memory.
+// pages' bytes (hundreds of KB each with all layers) and long tables: a second kernel copies them with the whole GPU,
+// from lists that the first one leaves in scratch memory.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -25,6 +25,10 @@ constexpr uint32_t kOwnerWaves = kOwnerBlock / 64;
 constexpr uint32_t kCopyBlock = 256;
 constexpr uint32_t kCopyBytes = 16384;   // of a page per workgroup and step: 4 accesses of 16 bytes per thread
 constexpr uint32_t kCopyGrid = 2048;     // 8 workgroups per CU
+// Words of scratch before the free pages' list: the copies (their number, then source and destination), then
+// what the second kernel does to each entry's table.
+constexpr uint32_t entry_words(uint32_t n) { return 1 + 2 * n; }
+constexpr uint32_t list_words(uint32_t n) { return entry_words(n) + 3 * n; }
 static_assert(kOwnerBlock >= HALO_MI_KV_LIST_MAX);
 
 // Exclusive prefix sum over the workgroup; total receives the sum. lds: kOwnerWaves words.
@@ -125,11 +129,9 @@ __device__ bool take_pages(const KvPagesArgs& a, int32_t slot, uint32_t need, ui
 
 __device__ __forceinline__ uint32_t pages_of(int32_t len, uint32_t block) { return len > 0 ? ((uint32_t)len + block - 1) / block : 0; }
 
-// scratch: the copies (1 + 2 n words), then the free pages' list (n_pages words)
 __global__ __launch_bounds__(kOwnerBlock) void k_kv_resize(KvPagesArgs a, const int32_t* slots, const int32_t* new_lens, uint32_t n,
                                                             uint32_t* scratch, uint32_t* status) {
     __shared__ OwnerLds l;
-    __shared__ uint32_t cut[kOwnerBlock][2];  // columns that an entry releases
     const uint32_t i = threadIdx.x;
     const int32_t slot = i < n ? slots[i] : -1, want = i < n ? new_lens[i] : 0;
     bool ok = first_of_its_name(l, slot, i, n) && i < n && (uint32_t)slot < a.n_slots && want >= 0;
@@ -158,26 +160,21 @@ __global__ __launch_bounds__(kOwnerBlock) void k_kv_resize(KvPagesArgs a, const 
         }
     }
     __syncthreads();  // every count, length and table entry has been read
-    const bool granted = take_pages(a, slot, take, column, tail, scratch + 1 + 2 * n, scratch, status, l);
+    const bool granted = take_pages(a, slot, take, column, tail, scratch + list_words(n), scratch, status, l);
     ok = ok && granted;
     if (ok && tail >= 0) atomicSub(a.refs + tail, 1);
     if (ok) a.lens[slot] = want;
-    cut[i][0] = ok ? goal : 0;
-    cut[i][1] = ok ? have : 0;
-    __syncthreads();
-    for (uint32_t e = i / 64; e < n; e += kOwnerWaves)
-        for (uint32_t c = cut[e][0] + i % 64; c < cut[e][1]; c += 64) {
-            int32_t* entry = a.tables + (uint64_t)l.slots[e] * a.table_stride + c;
-            if ((uint32_t)*entry < a.n_pages) atomicSub(a.refs + *entry, 1);
-            else set_status(status, kStatusKvBadIndex);
-            *entry = -1;
-        }
+    if (i < n) {  // the columns that the slot gives back
+        uint32_t* e = scratch + entry_words(n) + 3 * i;
+        e[0] = (uint32_t)slot;
+        e[1] = ok ? goal : 0;
+        e[2] = ok ? have : 0;
+    }
 }
 
 __global__ __launch_bounds__(kOwnerBlock) void k_kv_fork(KvPagesArgs a, const int32_t* src, const int32_t* dst, uint32_t n,
                                                           uint32_t* scratch, uint32_t* status) {
     __shared__ OwnerLds l;
-    __shared__ uint32_t from[kOwnerBlock], shared_pages[kOwnerBlock];
     const uint32_t i = threadIdx.x;
     const int32_t s = i < n ? src[i] : -1, d = i < n ? dst[i] : -1;
     bool ok = first_of_its_name(l, d, i, n) && i < n && (uint32_t)s < a.n_slots && (uint32_t)d < a.n_slots && s != d;
@@ -201,43 +198,56 @@ __global__ __launch_bounds__(kOwnerBlock) void k_kv_fork(KvPagesArgs a, const in
         }
     }
     __syncthreads();
-    const bool granted = take_pages(a, d, ok ? part : 0, full, tail, scratch + 1 + 2 * n, scratch, status, l);
+    const bool granted = take_pages(a, d, ok ? part : 0, full, tail, scratch + list_words(n), scratch, status, l);
     ok = ok && granted;
     if (ok) a.lens[d] = len;
-    from[i] = (uint32_t)s;
-    shared_pages[i] = ok ? full : 0;
-    __syncthreads();
-    for (uint32_t e = i / 64; e < n; e += kOwnerWaves)
-        for (uint32_t c = i % 64; c < shared_pages[e]; c += 64) {
-            const int32_t id = a.tables[(uint64_t)from[e] * a.table_stride + c];
-            a.tables[(uint64_t)l.slots[e] * a.table_stride + c] = id;
-            if ((uint32_t)id < a.n_pages) atomicAdd(a.refs + id, 1);
-            else set_status(status, kStatusKvBadIndex);
-        }
+    if (i < n) {  // the columns that the two slots share
+        uint32_t* e = scratch + entry_words(n) + 3 * i;
+        e[0] = (uint32_t)s;
+        e[1] = (uint32_t)d;
+        e[2] = ok ? full : 0;
+    }
 }
 
 // Bytes [at, at + kCopyBytes) of a page, or what there is of them (page_bytes is a multiple of 128).
 __device__ __forceinline__ void copy_part(const KvPagesArgs& a, uint32_t from, uint32_t to, uint64_t at) {
-    const uint4* s = reinterpret_cast<const uint4*>(a.pool + from * a.page_bytes + at);
-    uint4* d = reinterpret_cast<uint4*>(a.pool + to * a.page_bytes + at);
+    typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+    const uint4v* s = reinterpret_cast<const uint4v*>(a.pool + from * a.page_bytes + at);
+    uint4v* d = reinterpret_cast<uint4v*>(a.pool + to * a.page_bytes + at);
     const uint32_t n = (uint32_t)(min(a.page_bytes - at, (uint64_t)kCopyBytes) / 16);
+    if (n < kCopyBytes / 16) {  // a page's end
+        for (uint32_t k = threadIdx.x; k < n; k += kCopyBlock) d[k] = s[k];
+        return;
+    }
     constexpr uint32_t U = kCopyBytes / 16 / kCopyBlock;
-    uint4 v[U];
+    uint4v v[U];
 #pragma unroll
-    for (uint32_t k = 0; k < U; ++k)
-        if (threadIdx.x + k * kCopyBlock < n) v[k] = s[threadIdx.x + k * kCopyBlock];
+    for (uint32_t k = 0; k < U; ++k) v[k] = s[threadIdx.x + k * kCopyBlock];
 #pragma unroll
-    for (uint32_t k = 0; k < U; ++k)
-        if (threadIdx.x + k * kCopyBlock < n) d[threadIdx.x + k * kCopyBlock] = v[k];
+    for (uint32_t k = 0; k < U; ++k) d[threadIdx.x + k * kCopyBlock] = v[k];
 }
 
-// pairs: the count, then source and destination pages
-__global__ __launch_bounds__(kCopyBlock) void k_kv_copy_taken(KvPagesArgs a, const uint32_t* pairs) {
+// The pages' bytes and the whole tables' entries, after the deciding kernel. FORK: entries share columns [0, full) of the
+// source's table; otherwise they give back columns [goal, have).
+template <bool FORK>
+__global__ __launch_bounds__(kCopyBlock) void k_kv_apply(KvPagesArgs a, const uint32_t* scratch, uint32_t n, uint32_t* status) {
     const uint32_t parts = (uint32_t)((a.page_bytes + kCopyBytes - 1) / kCopyBytes);
-    const uint64_t units = (uint64_t)pairs[0] * parts;
+    const uint64_t units = (uint64_t)scratch[0] * parts;
+    for (uint32_t e = blockIdx.x; e < n; e += gridDim.x) {
+        const uint32_t* w = scratch + entry_words(n) + 3 * e;
+        const uint32_t s = w[0], from = FORK ? 0 : w[1], to = w[2];
+        for (uint32_t c = from + threadIdx.x; c < to; c += kCopyBlock) {
+            int32_t* entry = a.tables + (uint64_t)s * a.table_stride + c;
+            const int32_t id = *entry;
+            if ((uint32_t)id < a.n_pages) atomicAdd(a.refs + id, FORK ? 1 : -1);
+            else set_status(status, kStatusKvBadIndex);
+            if (FORK) a.tables[(uint64_t)w[1] * a.table_stride + c] = id;
+            else *entry = -1;
+        }
+    }
     for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
         const uint32_t i = (uint32_t)(u / parts);
-        copy_part(a, pairs[1 + 2 * i], pairs[2 + 2 * i], u % parts * kCopyBytes);
+        copy_part(a, scratch[1 + 2 * i], scratch[2 + 2 * i], u % parts * kCopyBytes);
     }
 }
 
@@ -316,14 +326,14 @@ uint32_t copy_grid(const KvPagesArgs& a, uint64_t pages) {
 int launch_kv_resize(const KvPagesArgs& a, const int32_t* slots, const int32_t* new_lens, uint32_t n, uint32_t* scratch,
                      uint32_t* status, hipStream_t st) {
     hipLaunchKernelGGL(k_kv_resize, dim3(1), dim3(kOwnerBlock), 0, st, a, slots, new_lens, n, scratch, status);
-    hipLaunchKernelGGL(k_kv_copy_taken, dim3(copy_grid(a, n)), dim3(kCopyBlock), 0, st, a, scratch);
+    hipLaunchKernelGGL(k_kv_apply<false>, dim3(copy_grid(a, n)), dim3(kCopyBlock), 0, st, a, scratch, n, status);
     return hip_status(hipGetLastError(), "kv_resize");
 }
 
 int launch_kv_fork(const KvPagesArgs& a, const int32_t* src, const int32_t* dst, uint32_t n, uint32_t* scratch, uint32_t* status,
                    hipStream_t st) {
     hipLaunchKernelGGL(k_kv_fork, dim3(1), dim3(kOwnerBlock), 0, st, a, src, dst, n, scratch, status);
-    hipLaunchKernelGGL(k_kv_copy_taken, dim3(copy_grid(a, n)), dim3(kCopyBlock), 0, st, a, scratch);
+    hipLaunchKernelGGL(k_kv_apply<true>, dim3(copy_grid(a, n)), dim3(kCopyBlock), 0, st, a, scratch, n, status);
     return hip_status(hipGetLastError(), "kv_fork");
 }
 

@@ -101,7 +101,7 @@ int launch_kv_read(const KvReadArgs& a, hipStream_t st);
 // The split that fits part_bytes of partial results (0: unsplit); sets a.splits, a.chunk and a.tiles.
 uint64_t plan_attention(AttnArgs& a, uint64_t part_bytes);
 int launch_attention(const AttnArgs& a, hipStream_t st);
-// scratch: 2 * n + 1 words (resize, fork); 3 * n_pages + 2 words (compact)
+// scratch: 1 + 5 n + n_pages words (resize, fork); 2 + 3 n_pages words (compact)
 int launch_kv_resize(const KvPagesArgs& a, const int32_t* slots, const int32_t* new_lens, uint32_t n, uint32_t* scratch,
                      uint32_t* status, hipStream_t st);
 int launch_kv_fork(const KvPagesArgs& a, const int32_t* src, const int32_t* dst, uint32_t n, uint32_t* scratch, uint32_t* status,

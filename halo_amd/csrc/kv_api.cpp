@@ -410,7 +410,7 @@ int halo_mi_kv_resize(const halo_mi_kv_cache* cache, const halo_mi_kv_state* sta
     uint32_t* scratch = nullptr;
     auto st = static_cast<hipStream_t>(stream);
     if ((rc = check_state(op, cache, state, &a)) || (rc = check_lists(op, a, slots, new_lens, n))) return rc;
-    if ((rc = scratch_for(op, st, 1 + 2ull * n + a.n_pages, &scratch))) return rc;
+    if ((rc = scratch_for(op, st, 1 + 5ull * n + a.n_pages, &scratch))) return rc;
     if ((rc = take_status(op, status, status_keep, st, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, {slots, 4ull * n, "slots"}, {new_lens, 4ull * n, "new_lens"}, {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
     return n ? launch_kv_resize(a, slots, new_lens, n, scratch, status, st) : HALO_MI_OK;
 }
@@ -424,7 +424,7 @@ int halo_mi_kv_fork(const halo_mi_kv_cache* cache, const halo_mi_kv_state* state
     uint32_t* scratch = nullptr;
     auto st = static_cast<hipStream_t>(stream);
     if ((rc = check_state(op, cache, state, &a)) || (rc = check_lists(op, a, src, dst, n))) return rc;
-    if ((rc = scratch_for(op, st, 1 + 2ull * n + a.n_pages, &scratch))) return rc;
+    if ((rc = scratch_for(op, st, 1 + 5ull * n + a.n_pages, &scratch))) return rc;
     if ((rc = take_status(op, status, status_keep, st, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, {src, 4ull * n, "src"}, {dst, 4ull * n, "dst"}, {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
     return n ? launch_kv_fork(a, src, dst, n, scratch, status, st) : HALO_MI_OK;
 }
