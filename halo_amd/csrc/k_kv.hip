@@ -25,20 +25,27 @@ using namespace dev;
 
 constexpr uint32_t kKvBlock = 256;
 
-// The integer nearest to x / s (ties to even), exactly, for |x| <= 127 s (1 + 2^-23), s normal; inv = 1 / s rounded. Without
-// EXACT it is that or its neighbour, the latter only where `unsure` is set. r is one of the two, and e = x - r s decides:
-// for r even and not 0, x >= 1.5 s is a multiple of s's last bit and e fits 24 bits; for r = 0 e is x; for r = +-1 e is
-// exact from x = s / 2 on, and below, where it may round to s / 2, the tie moves an odd r the same way.
+// The integer nearest to x / s (ties to even) as the low byte of the result's bits, for |x| <= 127 s (1 + 2^-23), s normal; inv =
+// 1 / s rounded. The multiply-add rounds x inv to an integer r, the quotient's or its neighbour (1.5 2^23 is where
+// fp32 has steps of 1), and e = x - r s decides: for r even and not 0, x >= 1.5 s is a multiple of s's last bit and e
+// fits 24 bits; for r = 0 e is x; for r = +-1 e is exact from x = s / 2 on, and below, where it may round to s / 2,
+// the tie moves an odd r the same way. Without EXACT only `unsure` is set where r may have to move.
 template <bool EXACT>
-__device__ __forceinline__ int32_t nearest(float x, float s, float inv, bool& unsure) {
-    float r = rintf(x * inv);
+__device__ __forceinline__ uint32_t nearest(float x, float s, float inv, bool& unsure) {
+    constexpr float kStepsOfOne = 12582912.0f;
+    const float t = fmaf(x, inv, kStepsOfOne), r = t - kStepsOfOne;
     const float e = fmaf(-r, s, x), half = 0.5f * s;
     if constexpr (EXACT) {
-        if (fabsf(e) > half || (fabsf(e) == half && ((int32_t)r & 1))) r += copysignf(1.0f, e);
+        const bool move = fabsf(e) > half || (fabsf(e) == half && (__float_as_uint(t) & 1));
+        return __float_as_uint(move ? t + copysignf(1.0f, e) : t);
     } else {
         unsure = unsure || fabsf(e) >= half;
+        return __float_as_uint(t);
     }
-    return (int32_t)r;
+}
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0400u), __builtin_amdgcn_perm(b, a, 0x0C0C0400u), 0x05040100u);
 }
 
 // The code c of a block of scale s0 in scale s1 > s0: the integer nearest to c * s0 / s1, exactly.
@@ -49,13 +56,6 @@ __device__ __forceinline__ int32_t rescaled(int32_t c, float s0, float s1) {
     if (x2 > up || (x2 == up && (r & 1))) ++r;
     else if (x2 < down || (x2 == down && (r & 1))) --r;
     return r;
-}
-
-__device__ __forceinline__ uint32_t rescaled4(uint32_t codes, float s0, float s1) {
-    uint32_t out = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out |= (uint32_t)(uint8_t)rescaled((int8_t)(codes >> (8 * i)), s0, s1) << (8 * i);
-    return out;
 }
 
 // What one workgroup of a write or read has: tokens [lo, hi) of a sequence, in one page.
@@ -116,29 +116,36 @@ __device__ __forceinline__ uint32_t peak_bits(uint32_t top) {
     }
 }
 
-// V: elements per load of a K or V row. KEEP: patches per thread that stay in registers between the maximum and the
-// codes; a part with more is read again.
+// V: elements per load of a K or V row, 4 or 1. KEEP: patches per thread that stay in registers between the maximum and
+// the codes; a part with more is read again. A thread has one place of `vecs` in a row and every `at_once`-th group of
+// 4 tokens.
 template <typename T, int V, int KEEP>
 __device__ void write_part(const KvWriteArgs& a, const PagePart& p, uint32_t which, uint32_t head, uint32_t* lds) {
+    typedef std::conditional_t<V == 1, uint64_t, uint32_t> Offset;  // wide rows are at most 2^22 elements apart
     const KvLayer& c = a.c;
-    const uint32_t tid = threadIdx.x, dim = c.dim, vecs = dim / V;
+    const uint32_t tid = threadIdx.x, dim = c.dim, vecs = dim / V, at_once = kKvBlock / vecs;
+    const uint32_t d = tid % vecs * V, mine_first = tid / vecs;
     const T* x = static_cast<const T*>(a.x[which].data) + (uint64_t)p.row * a.x[which].stride + head * a.x[which].head_stride;
-    const uint64_t stride = a.x[which].stride;
+    const Offset stride = (Offset)a.x[which].stride;
     // groups of 4 tokens, aligned in the page, that the part touches
-    const uint32_t g0 = p.off / 4, patches = ((p.off + p.n + 3) / 4 - g0) * vecs;
-    const bool kept = patches <= KEEP * kKvBlock;
-    const auto load = [&](uint32_t i, Patch<T, V>& q) {
-        const uint32_t t0 = (g0 + i / vecs) * 4, d = i % vecs * V;
+    const uint32_t g0 = p.off / 4, groups = (p.off + p.n + 3) / 4 - g0, my_groups = mine_first < at_once ? groups : 0;
+    const bool kept = groups <= KEEP * at_once;
+    const auto load = [&](uint32_t g, Patch<T, V>& q) {
+        const uint32_t t0 = (g0 + g) * 4;
+        // tokens outside the part repeat its nearest row: no branch, the same maximum; their codes are not stored
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k)
-            if (t0 + k >= p.off && t0 + k < p.off + p.n) q.row[k] = *reinterpret_cast<const Vec<T, V>*>(x + (t0 + k - p.off) * stride + d);
-            else q.row[k] = {};
+            q.row[k] = *reinterpret_cast<const Vec<T, V>*>(x + ((Offset)(min(max(t0 + k, p.off), p.off + p.n - 1) - p.off) * stride + d));
     };
     uint32_t top = 0;
     Patch<T, V> mine[KEEP];
     if (kept) {
 #pragma unroll
-        for (int j = 0; j < KEEP; ++j) load(min(tid + j * kKvBlock, patches - 1), mine[j]);  // past the end: not used
+        for (int j = 0; j < KEEP; ++j) load(min(mine_first + j * at_once, groups - 1), mine[j]);  // past the end: not used
+    }
+    if (p.page < 0) {  // the rows are on their way while the table's entry is
+        if (tid == 0) set_status(a.status, kStatusKvBadIndex);
+        return;
     }
     uint8_t* page = c.pool + (uint64_t)(uint32_t)p.page * c.page_bytes;
     uint8_t* codes = page + c.codes + (which * c.heads + head) * c.plane;
@@ -149,8 +156,8 @@ __device__ void write_part(const KvWriteArgs& a, const PagePart& p, uint32_t whi
 #pragma unroll
         for (int j = 0; j < KEEP; ++j) top = patch_peak(mine[j], top);
     } else {
-        for (uint32_t i = tid; i < patches; i += kKvBlock) {
-            load(i, mine[0]);
+        for (uint32_t g = mine_first; g < my_groups; g += at_once) {
+            load(g, mine[0]);
             top = patch_peak(mine[0], top);
         }
     }
@@ -167,31 +174,27 @@ __device__ void write_part(const KvWriteArgs& a, const PagePart& p, uint32_t whi
     if (s1 != s1) return;  // the codes of a NaN block mean nothing
 
     if (p.off && s1 > s0 && s0 > 0.0f) {  // the scale grew: the earlier tokens' codes follow
-        if (which == 0) {
-            for (uint32_t i = tid; i < p.off * dim / 4; i += kKvBlock) words[i] = rescaled4(words[i], s0, s1);
-        } else {
-            const uint32_t per = (p.off + 3) / 4;  // words of a dim
-            for (uint32_t i = tid; i < per * dim; i += kKvBlock) {
-                uint32_t* w = words + i / per * (c.block / 4) + i % per;
-                const uint32_t keep = i % per * 4 + 4 <= p.off ? 0u : 0xFFFFFFFFu << 8 * (p.off % 4), old = *w;
-                *w = (old & keep) | (rescaled4(old, s0, s1) & ~keep);
-            }
+        const uint32_t per = which ? (p.off + 3) / 4 : p.off * dim / 4;  // words of a dim of V; of K
+        const uint32_t rows = which ? dim : 1;
+        for (uint32_t i = tid; i < per * rows; i += kKvBlock) {
+            uint32_t* w = words + i / per * (c.block / 4) + i % per;
+            const uint32_t keep = !which || i % per * 4 + 4 <= p.off ? 0u : 0xFFFFFFFFu << 8 * (p.off % 4);
+            uint32_t word = *w & keep;
+            for (uint32_t k = 0; k < 32; k += 8)
+                if (!(keep >> k & 1)) word |= (uint32_t)(uint8_t)rescaled((int8_t)(*w >> k), s0, s1) << k;
+            *w = word;
         }
         __syncthreads();
     }
     const float inv = s1 > 0.0f ? 1.0f / s1 : 0.0f;
-    const bool some = s1 > 0.0f;
-    // The patch's codes, four tokens of a dim to a word; exactly where an element is too near a border to be sure.
-    const auto codes_of = [&](const Patch<T, V>& q, uint32_t (&word)[V]) {
-        const auto all = [&](auto exact, float by, float inv) {
+    // The patch's codes; exactly where an element is too near a border to be sure. code[k][j]: token k, dim j.
+    const auto codes_of = [&](const Patch<T, V>& q, uint32_t (&code)[4][V]) {
+        const auto all = [&](auto exact, float by, float times) {
             bool unsure = false;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                word[j] = 0;
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    word[j] |= (uint32_t)(uint8_t)nearest<decltype(exact)::value>(to_f32(q.row[k].v[j]), by, inv, unsure) << 8 * k;
-            }
+                for (int j = 0; j < V; ++j) code[k][j] = nearest<decltype(exact)::value>(to_f32(q.row[k].v[j]), by, times, unsure);
             return unsure;
         };
         if (all(std::false_type{}, s1, inv)) {
@@ -200,39 +203,42 @@ __device__ void write_part(const KvWriteArgs& a, const PagePart& p, uint32_t whi
             all(std::true_type{}, by, again);
         }
     };
-    const auto store = [&](uint32_t i, const Patch<T, V>& q) {
-        const uint32_t t0 = (g0 + i / vecs) * 4, d = i % vecs * V;
-        uint32_t cover = 0;  // the bytes of a word of V's that are this part's
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k)
-            if (t0 + k >= p.off && t0 + k < p.off + p.n) cover |= 0xFFu << 8 * k;
-        uint32_t word[V] = {};
-        if (some) codes_of(q, word);
+    const auto store = [&](uint32_t g, const Patch<T, V>& q) {
+        const uint32_t t0 = (g0 + g) * 4;
+        uint32_t code[4][V] = {};
+        if (s1 > 0.0f) codes_of(q, code);
+        const bool whole = t0 >= p.off && t0 + 4 <= p.off + p.n;
+        const auto mine_too = [&](uint32_t k) { return whole || (t0 + k >= p.off && t0 + k < p.off + p.n); };
         if (which == 0) {
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
-                if (!(cover >> 8 * k & 1)) continue;
-                Vec<uint8_t, V> out;
-#pragma unroll
-                for (int j = 0; j < V; ++j) out.v[j] = (uint8_t)(word[j] >> 8 * k);
-                *reinterpret_cast<Vec<uint8_t, V>*>(codes + (t0 + k) * dim + d) = out;
+                if (!mine_too(k)) continue;
+                if constexpr (V == 4) words[((t0 + k) * dim + d) / 4] = low_bytes(code[k][0], code[k][1], code[k][2], code[k][3]);
+                else codes[(t0 + k) * dim + d] = (uint8_t)code[k][0];
             }
             return;
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             uint32_t* w = words + ((d + j) * c.block + t0) / 4;
-            *w = cover == 0xFFFFFFFFu ? word[j] : (*w & ~cover) | (word[j] & cover);
+            uint32_t word = low_bytes(code[0][j], code[1][j], code[2][j], code[3][j]);
+            if (!whole) {  // the word's other tokens keep their bytes
+                uint32_t cover = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) cover |= mine_too(k) ? 0xFFu << 8 * k : 0u;
+                word = (*w & ~cover) | (word & cover);
+            }
+            *w = word;
         }
     };
     if (kept) {
 #pragma unroll
         for (int j = 0; j < KEEP; ++j)
-            if (tid + j * kKvBlock < patches) store(tid + j * kKvBlock, mine[j]);
+            if (mine_first + j * at_once < my_groups) store(mine_first + j * at_once, mine[j]);
     } else {
-        for (uint32_t i = tid; i < patches; i += kKvBlock) {
-            load(i, mine[0]);
-            store(i, mine[0]);
+        for (uint32_t g = mine_first; g < my_groups; g += at_once) {
+            load(g, mine[0]);
+            store(g, mine[0]);
         }
     }
 }
@@ -244,10 +250,6 @@ __global__ __launch_bounds__(kKvBlock) void k_kv_write(KvWriteArgs a) {
     const SeqRows r = seq_rows(a.b, s);
     PagePart p;
     for (uint32_t j = blockIdx.x; page_part(a.b, a.c, s, r, j, p); j += gridDim.x) {
-        if (p.page < 0) {
-            if (threadIdx.x == 0) set_status(a.status, kStatusKvBadIndex);
-            continue;
-        }
         write_part<T, V, KEEP>(a, p, which, head, lds);
         __syncthreads();
     }
@@ -303,13 +305,13 @@ dim3 page_grid(const KvLayer& c, const KvBatch& b) {
 
 template <typename T>
 int launch_write_typed(const KvWriteArgs& a, hipStream_t st) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 4;
     bool wide = true;
     for (const HeadRows& r : a.x)
-        wide = wide && reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && r.stride % V == 0 && r.head_stride % V == 0;
-    // patches of a page per thread
-    const uint32_t each = (a.c.block / 4 * (a.c.dim / V) + kKvBlock - 1) / kKvBlock;
-    auto* k = !wide ? k_kv_write<T, 1, 4> : each <= 1 ? k_kv_write<T, V, 1> : each <= 2 ? k_kv_write<T, V, 2> : k_kv_write<T, V, 4>;
+        wide = wide && reinterpret_cast<uintptr_t>(r.data) % (V * sizeof(T)) == 0 && r.stride % V == 0 && r.head_stride % V == 0 && r.stride <= 1u << 22;
+    // groups of 4 tokens of a page per thread
+    const uint32_t at_once = kKvBlock / (a.c.dim / V), each = (a.c.block / 4 + at_once - 1) / at_once;
+    auto* k = !wide ? k_kv_write<T, 1, 4> : each <= 1 ? k_kv_write<T, V, 1> : each <= 2 ? k_kv_write<T, V, 2> : each <= 4 ? k_kv_write<T, V, 4> : k_kv_write<T, V, 8>;
     hipLaunchKernelGGL(k, page_grid(a.c, a.b), dim3(kKvBlock), 0, st, a);
     return hip_status(hipGetLastError(), "KV_WRITE");
 }
