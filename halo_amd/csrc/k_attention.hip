@@ -39,7 +39,7 @@ template <int NP>
 constexpr float kShift = NP == 1 ? 8.0f : 14.0f;
 template <int NP>
 constexpr float kSlack = NP == 1 ? 7.5f : 1.5f;
-constexpr uint32_t kFewGrid = 512;      // workgroups of a call with few rows at most: two per CU
+constexpr uint32_t kFewGrid = 768;      // workgroups of a call with few rows at most: three per CU
 constexpr float kTinyScale = 0x1p-80f;  // the scale that an all-zero block of V counts with
 
 __device__ __forceinline__ float quiet_nan() { return __uint_as_float(0x7FC00000u); }
@@ -351,9 +351,26 @@ __device__ __forceinline__ float* part_of(const AttnArgs& a, uint64_t w, uint32_
 // The same of (row, head) r and split s of a call with many rows.
 __device__ __forceinline__ float* many_part(const AttnArgs& a, uint64_t r, uint32_t s) { return a.part + (r * a.splits + s) * (a.c.dim + 4); }
 
+// 16 bytes of the cache. ONCE: nothing else reads them soon (48 ragged sequences of bf16, 405 MB: 97 us against 104; one
+// sequence of 131000 tokens 59 against 63; 33 MB that two row tiles read 30 against 27).
+template <bool ONCE>
+__device__ __forceinline__ uint4 stream16(const uint8_t* p) {
+    typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+    if constexpr (ONCE) {
+        const uint4v v = __builtin_nontemporal_load(reinterpret_cast<const uint4v*>(p));
+        return {v[0], v[1], v[2], v[3]};
+    } else {
+        return *reinterpret_cast<const uint4*>(p);
+    }
+}
+
+// Workgroups of k_attention_few that a CU's registers hold (4 waves each, one per SIMD).
+template <int D, int NQ>
+constexpr int kFewPerCu = D == 64 && NQ == 1 ? 3 : D <= 128 && NQ == 1 ? 2 : 1;
+
 // D: head_dim. NP: f16 pieces of q and of the weights. NQ: row tiles of 16 that share K and V.
-template <int D, int NP, int NQ>
-__global__ __launch_bounds__(kAttnWaves * 64, D <= 128 && NQ == 1 ? 2 : 1) void k_attention_few(AttnArgs a) {
+template <int D, int NP, int NQ, bool ONCE>
+__global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attention_few(AttnArgs a) {
     constexpr int C = D / 64, TAIL = D % 64 / 32;  // 64-dim chunks of a K row, and a last one of 32
     constexpr int DT = D / 16;                     // tiles of 16 dims
     constexpr int ROWS = 16 * NQ;
@@ -416,7 +433,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, D <= 128 && NQ == 1 ? 2 : 1) void 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int c = 0; c < C; ++c) kb[i][c] = *reinterpret_cast<const uint4*>(k + 4 * i * D + c * 64 + 16 * g);
+                for (int c = 0; c < C; ++c) kb[i][c] = stream16<ONCE>(k + 4 * i * D + c * 64 + 16 * g);
                 if constexpr (TAIL) kt[i] = *reinterpret_cast<const uint2*>(k + 4 * i * D + C * 64 + 8 * g);
             }
         };
@@ -445,7 +462,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, D <= 128 && NQ == 1 ? 2 : 1) void 
             {
                 const uint8_t* v = page + head_codes + a.c.heads * a.c.plane + col * a.c.block + (tg & (a.c.block - 1));
 #pragma unroll
-                for (int i = 0; i < DT; ++i) vb[i] = *reinterpret_cast<const uint4*>(v + i * 16 * a.c.block);
+                for (int i = 0; i < DT; ++i) vb[i] = stream16<ONCE>(v + i * 16 * a.c.block);
             }
             __builtin_amdgcn_sched_barrier(0);
             const Scales sc = make_scales(ks, vs, ok || tg >= end);
@@ -622,14 +639,17 @@ template <int D, int NP>
 void run_few(const AttnArgs& a, hipStream_t st) {
     const uint32_t rows = few_rows(a);
     const dim3 join(a.b.n_seqs * a.c.heads * a.tiles, std::min<uint32_t>(rows, std::max<uint64_t>(1, (uint64_t)a.b.max_rows * a.group)));
+    // one row tile, and more bytes than the L2 caches hold: read once
+    const bool once = a.tiles == 1 && 2ull * a.b.n_seqs * a.b.max_kv * a.c.heads * D > 32ull << 20;
     if constexpr (D <= 128) {
         if (rows == 32) {
-            hipLaunchKernelGGL((k_attention_few<D, NP, 2>), dim3(a.splits), dim3(kAttnWaves * 64), 0, st, a);
+            hipLaunchKernelGGL((k_attention_few<D, NP, 2, false>), dim3(a.splits), dim3(kAttnWaves * 64), 0, st, a);
             if (a.part) hipLaunchKernelGGL(k_attention_few_join<32>, join, dim3(256), 0, st, a, a.splits);
             return;
         }
     }
-    hipLaunchKernelGGL((k_attention_few<D, NP, 1>), dim3(a.splits), dim3(kAttnWaves * 64), 0, st, a);
+    auto* k = once ? k_attention_few<D, NP, 1, true> : k_attention_few<D, NP, 1, false>;
+    hipLaunchKernelGGL(k, dim3(a.splits), dim3(kAttnWaves * 64), 0, st, a);
     if (a.part) hipLaunchKernelGGL(k_attention_few_join<16>, join, dim3(256), 0, st, a, a.splits);
 }
 
@@ -1145,11 +1165,15 @@ uint64_t plan_many(AttnArgs& a, uint64_t part_bytes) {
 
 }  // namespace
 
-// As many workgroups as the registers let run at once, one or two per CU, or fewer where there are not as many units. With memory for fewer parts than there are
+// As many workgroups as the registers let run at once, one to three per CU, or fewer where there are not as many units. With memory for fewer parts than there are
 // (sequence, kv head, tile)s, each of these is one unit.
 uint64_t plan_attention(AttnArgs& a, uint64_t part_bytes) {
-    // Few rows per kv head: what counts is the cache's stream. More: the products, on tiles that share K and V.
-    a.few = (uint64_t)a.b.max_rows * a.group <= 32;
+    // Few rows per kv head: what counts is the cache's stream. More: the products, on tiles that share K and V. A second tile
+    // of few rows streams the cache again, which pays while the streams are too few to fill the GPU: 64 rows over 4000 tokens
+    // (bf16, head_dim 128), 4 sequences of 4 kv heads: 23.5 us against 29.1 with many, 10 sequences of fp32 47 against 40; 24
+    // rows (head_dim 256, two tiles) 2 sequences 21 against 27, 32 sequences 95 against 73.
+    const uint64_t all = (uint64_t)a.b.max_rows * a.group, tile = few_rows(a);
+    a.few = all <= tile || (all <= 2 * tile && (uint64_t)a.b.n_seqs * a.c.heads <= 32);
     if (!a.few) return plan_many(a, part_bytes);
     const uint32_t rows = few_rows(a);
     const uint64_t pairs = (uint64_t)a.b.n_seqs * a.c.heads;
@@ -1162,7 +1186,8 @@ uint64_t plan_attention(AttnArgs& a, uint64_t part_bytes) {
     a.unit = 1u << a.unit_log2;
     const uint64_t per_wg = 2ull * rows * (a.c.dim + 4) * sizeof(float);
     const uint64_t chunks = std::max<uint64_t>(1, ((uint64_t)a.b.max_kv + a.unit - 1) / a.unit);
-    a.splits = (uint32_t)std::min<uint64_t>(a.c.dim <= 128 && rows == 16 ? kFewGrid : kFewGrid / 2, pairs * a.tiles * chunks);
+    const uint32_t per_cu = rows == 32 ? kFewPerCu<128, 2> : a.c.dim == 64 ? kFewPerCu<64, 1> : a.c.dim <= 128 ? kFewPerCu<128, 1> : kFewPerCu<256, 1>;
+    a.splits = (uint32_t)std::min<uint64_t>(256 * per_cu, pairs * a.tiles * chunks);
     const uint64_t fit = part_bytes / per_wg;
     const bool split = chunks > 1 && fit >= std::min<uint64_t>(a.splits, pairs * a.tiles);
     if (split) a.splits = (uint32_t)std::min<uint64_t>(a.splits, fit);
