@@ -58,34 +58,6 @@ __device__ __forceinline__ float column_sum(float v) {
     return __int_as_float(r[0]) + __int_as_float(r[1]);
 }
 
-// Eight consecutive elements as fp32. wide: p is 16-byte aligned.
-__device__ __forceinline__ void load8(const void* base, uint32_t type, uint64_t i, bool wide, float (&v)[8]) {
-    if (type == HALO_MI_F32) {
-        const float* p = static_cast<const float*>(base) + i;
-        if (wide) {
-            const float4v a = reinterpret_cast<const float4v*>(p)[0], b = reinterpret_cast<const float4v*>(p)[1];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = p[j];
-        }
-        return;
-    }
-    const uint16_t* p = static_cast<const uint16_t*>(base) + i;
-    uint16_t h[8];
-    if (wide) {
-        const Vec<uint16_t, 8> a = *reinterpret_cast<const Vec<uint16_t, 8>*>(p);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = a.v[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = p[j];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        v[j] = type == HALO_MI_F16 ? (float)__builtin_bit_cast(_Float16, h[j]) : __uint_as_float((uint32_t)h[j] << 16);
-}
 __device__ __forceinline__ void store_any(void* p, uint32_t type, uint64_t i, float v) {
     if (type == HALO_MI_F16) static_cast<_Float16*>(p)[i] = (_Float16)v;
     else if (type == HALO_MI_BF16) static_cast<__bf16*>(p)[i] = (__bf16)v;
@@ -130,42 +102,75 @@ struct QRow {
         return i / 2 * 2 + 1 < F ? i / 2 * 16 * GROUPS + 16 * g + i % 2 * 8 : i * 8 * GROUPS + 8 * g;
     }
 
-    // packed row r of `packed`: token r / group, head r % group of kv head kvh. fetch only loads; finish converts.
+    // Packed row r of `packed`: token r / group, head r % group of kv head kvh. fetch only loads, every word before the
+    // first is used, one round trip (a tile of 16 rows of a verify step: 26.1 us against 27.6); finish converts. Rows past
+    // the last are not read: lanes that all ask for one row wait for each other (one row of 6 heads at 256 dims: 17.0 us
+    // against 20.1 with row 0 read in their place). Two pieces: fp32, a word an element; one: 16 bits, two a word.
+    static constexpr int W = NP == 2 ? 8 : 4;
     __device__ __forceinline__ void fetch(const AttnArgs& a, const SeqRows& sr, uint32_t kvh, uint32_t r, uint32_t packed, uint32_t g,
-                                          int32_t cap, float (&v)[F][8]) {
+                                          int32_t cap, uint32_t (&raw)[F][W]) {
         const bool live = r < packed;
         const uint32_t token = live ? r / a.group : 0, head = kvh * a.group + (live ? r % a.group : 0);
         const uint64_t at = (uint64_t)(sr.row0 + token) * a.q.stride + head * a.q.head_stride;
         const int32_t pos = sr.len - sr.rows + (int32_t)token;
         hi = live ? max(pos + 1, 0) : 0;
         lo = first_seen(a, pos, cap);
-        const bool wide = wide_rows(a.q, a.type);
 #pragma unroll
         for (int i = 0; i < F; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-        if (live) {
+            for (int j = 0; j < W; ++j) raw[i][j] = 0;
+        if (!live) return;
+        if (wide_rows(a.q, a.type)) {
 #pragma unroll
-            for (int i = 0; i < F; ++i) load8(a.q.data, a.type, at + dim(i, g), wide, v[i]);
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int h = 0; h < W; h += 4) {
+                    const Vec<uint32_t, 4> x = *reinterpret_cast<const Vec<uint32_t, 4>*>(
+                        static_cast<const uint8_t*>(a.q.data) + (at + dim(i, g)) * (NP == 2 ? 4 : 2) + h * 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) raw[i][h + j] = x.v[j];
+                }
+        } else if constexpr (NP == 2) {
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) raw[i][j] = (static_cast<const uint32_t*>(a.q.data) + at)[dim(i, g) + j];
+        } else {
+            const uint16_t* p = static_cast<const uint16_t*>(a.q.data) + at;
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) raw[i][j] = (uint32_t)p[dim(i, g) + 2 * j] | (uint32_t)p[dim(i, g) + 2 * j + 1] << 16;
         }
     }
-    __device__ __forceinline__ void finish(const AttnArgs& a, const float (&v)[F][8]) {
+    __device__ __forceinline__ void finish(const AttnArgs& a, const uint32_t (&raw)[F][W]) {
+        const bool half = a.type == HALO_MI_F16;
+        const auto element = [&](int i, int j) {
+            if constexpr (NP == 2) {
+                return __uint_as_float(raw[i][j]);
+            } else {
+                const uint32_t w = raw[i][j / 2];
+                const float b = __uint_as_float(j % 2 ? w & 0xFFFF0000u : w << 16);
+                return half ? (float)__builtin_bit_cast(half2v, w)[j % 2] : b;
+            }
+        };
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < F; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[i][j]));
+            for (int j = 0; j < 8; ++j) top = max(top, abs_bits(element(i, j)));
         if constexpr (GROUPS == 4) top = max(top, (uint32_t)__shfl_xor((int)top, 16));
         top = max(top, (uint32_t)__shfl_xor((int)top, 32));
         const bool bad = top > kLargestFinite;
-        const int e = top == 0 || bad ? 0 : top < 0x00800000u ? (int)(31 - __builtin_clz(top)) - 149 : (int)(top >> 23) - 127;
-        c = bad ? quiet_nan() : ldexpf(fabsf(a.scale_log2), e - 14);
-        const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
+        // 2^up takes the row's largest to [2^14, 2^15); rows under 2^-112, whose scores are nothing, go up by 2^126
+        const int32_t e = (int32_t)(top >> 23) - 127, up = min(14 - e, 126);
+        c = bad ? quiet_nan() : ldexpf(fabsf(a.scale_log2), -up);
+        const float times = __uint_as_float((uint32_t)(up + 127) << 23) * (a.scale_log2 < 0.0f ? -1.0f : 1.0f);
 #pragma unroll
         for (int i = 0; i < F; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float x = bad ? 0.0f : ldexpf(v[i][j] * sign, 14 - e);
+                const float x = bad ? 0.0f : element(i, j) * times;
                 f[i][0][j] = (_Float16)x;
                 if constexpr (NP == 2) f[i][1][j] = (_Float16)(x - (float)f[i][0][j]);
             }
@@ -288,10 +293,15 @@ struct SeqUnits {
     uint32_t units;
 };
 
+// A value that the whole wave shares, as the scalar that the compiler cannot see it is; lane l's, l itself shared. Loop
+// bounds, pages' places and the mask's limits then stay out of the vector registers (36 bytes of scratch a lane, then none).
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ uint32_t of_lane(uint32_t v, uint32_t l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)l); }
+
 template <int ROWS>
-__device__ __forceinline__ SeqUnits seq_units(const AttnArgs& a, uint32_t seq) {
+__device__ __forceinline__ SeqUnits seq_units(const AttnArgs& a, const SeqRows& rows) {
     SeqUnits u;
-    u.r = seq_rows(a.b, seq);
+    u.r = rows;
     const int32_t cap = (int32_t)(a.b.table_width * a.c.block);
     u.begin = first_seen(a, u.r.len - u.r.rows, cap) / (int32_t)kStep * (int32_t)kStep;
     u.end = min(u.r.len, cap + 16);  // past the table: one group out of range, which makes its rows NaN
@@ -302,11 +312,16 @@ __device__ __forceinline__ SeqUnits seq_units(const AttnArgs& a, uint32_t seq) {
     return u;
 }
 
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
+template <int ROWS>
+__device__ __forceinline__ SeqUnits seq_units(const AttnArgs& a, uint32_t seq) {
+    return seq_units<ROWS>(a, seq_rows(a.b, seq));
+}
+
+// Sums of lanes 0..lane, right for the lanes under n.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane, uint32_t n) {
+    for (uint32_t off = 1; off < min(n, 64u); off <<= 1) {
         const uint32_t below = (uint32_t)__shfl_up((int)v, off);
-        if (lane >= (uint32_t)off) v += below;
+        if (lane >= off) v += below;
     }
     return v;
 }
@@ -322,22 +337,23 @@ template <int ROWS>
 __device__ __forceinline__ Run find_run(const AttnArgs& a, uint32_t lane, uint32_t workgroups, uint32_t id) {
     Run r{};
     const auto units = [&](uint32_t s) { return s < a.b.n_seqs ? seq_units<ROWS>(a, s).units : 0; };
-    uint32_t v = units(lane), sum = wave_scan(v, lane);
-    r.total = (uint32_t)__shfl((int)sum, 63);
-    for (uint32_t s0 = 64; s0 < a.b.n_seqs; s0 += 64) r.total += (uint32_t)__shfl((int)wave_scan(units(s0 + lane), lane), 63);
+    const auto batch = [&](uint32_t s0) { return min(a.b.n_seqs - s0, 64u); };
+    uint32_t v = units(lane), sum = wave_scan(v, lane, batch(0));
+    r.total = of_lane(sum, batch(0) - 1);
+    for (uint32_t s0 = 64; s0 < a.b.n_seqs; s0 += 64) r.total += of_lane(wave_scan(units(s0 + lane), lane, batch(s0)), batch(s0) - 1);
     r.per = max(1u, (r.total + workgroups - 1) / workgroups);
     r.first = min(id * r.per, r.total);
     r.last = min(r.first + r.per, r.total);
     for (uint32_t s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
-        if (s0) v = units(s0 + lane), sum = wave_scan(v, lane);
-        const uint64_t hit = __ballot(r.before + sum > r.first);
+        if (a.b.n_seqs > 64) v = units(s0 + lane), sum = wave_scan(v, lane, batch(s0));
+        const uint64_t hit = __ballot(lane < batch(s0) && r.before + sum > r.first);
         if (hit) {
             const uint32_t l = (uint32_t)__ffsll((long long)hit) - 1;
-            r.before += (uint32_t)__shfl((int)(sum - v), l);
+            r.before += of_lane(sum - v, l);
             r.seq = s0 + l;
             break;
         }
-        r.before += (uint32_t)__shfl((int)sum, 63);
+        r.before += of_lane(sum, batch(s0) - 1);
     }
     return r;
 }
@@ -374,7 +390,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attenti
     constexpr int C = D / 64, TAIL = D % 64 / 32;  // 64-dim chunks of a K row, and a last one of 32
     constexpr int DT = D / 16;                     // tiles of 16 dims
     constexpr int ROWS = 16 * NQ;
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, g = lane / 16;
+    const uint32_t lane = threadIdx.x % 64, wave = uniform(threadIdx.x / 64), col = lane % 16, g = lane / 16;
     constexpr int kWide = D < 128 ? D : 128;  // outputs that meet in LDS at a time
     __shared__ __align__(16) float lds_o[kAttnWaves][16][kWide + 4];
     __shared__ float lds_m[kAttnWaves][ROWS], lds_l[kAttnWaves][ROWS];
@@ -442,7 +458,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attenti
         Running<DT> run[NQ];
         {
             const int32_t id = t_first < t_end ? entry(t_first) : 0;
-            float raw[NQ][QRow<D, NP>::F][8];
+            uint32_t raw[NQ][QRow<D, NP>::F][QRow<D, NP>::W];
 #pragma unroll
             for (int n = 0; n < NQ; ++n) q[n].fetch(a, su.r, kvh, tile * ROWS + 16 * n + col, packed, g, cap, raw[n]);
             if (t_first < t_end) {
@@ -467,28 +483,34 @@ __global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attenti
             __builtin_amdgcn_sched_barrier(0);
             const Scales sc = make_scales(ks, vs, ok || tg >= end);
             if (!ok && tg < end) set_status(a.status, kStatusKvBadIndex);
+            // dims outside, tiles inside: consecutive products have accumulators of their own
             float4v s[NQ][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) s[n][i] = float4v{0, 0, 0, 0};
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const half8v k0 = codes_f16(kb[i][c].x, kb[i][c].y), k1 = codes_f16(kb[i][c].z, kb[i][c].w);
+            for (int c = 0; c < C; ++c) {
+                half8v k[2][4];
 #pragma unroll
-                    for (int n = 0; n < NQ; ++n)
+                for (int i = 0; i < 4; ++i) k[0][i] = codes_f16(kb[i][c].x, kb[i][c].y), k[1][i] = codes_f16(kb[i][c].z, kb[i][c].w);
 #pragma unroll
-                        for (int p = 0; p < NP; ++p) {
-                            s[n][i] = mfma(k0, q[n].f[2 * c][p], s[n][i]);
-                            s[n][i] = mfma(k1, q[n].f[2 * c + 1][p], s[n][i]);
-                        }
-                }
-                if constexpr (TAIL) {
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[n][i] = mfma(k[h][i], q[n].f[2 * c + h][p], s[n][i]);
+            }
+            if constexpr (TAIL) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
                     const half8v k0 = codes_f16(kt[i].x, kt[i].y);
 #pragma unroll
-                    for (int n = 0; n < NQ; ++n)
+                    for (int p = 0; p < NP; ++p)
 #pragma unroll
-                        for (int p = 0; p < NP; ++p) s[n][i] = mfma(k0, q[n].f[2 * C][p], s[n][i]);
+                        for (int n = 0; n < NQ; ++n) s[n][i] = mfma(k0, q[n].f[2 * C][p], s[n][i]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -581,8 +603,8 @@ __global__ __launch_bounds__(256) void k_attention_few_join(AttnArgs a, uint32_t
     const SeqUnits su = seq_units<ROWS>(a, seq);
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < seq; s0 += 64) {
-        const uint32_t v = s0 + lane < seq ? seq_units<ROWS>(a, s0 + lane).units : 0;
-        before += (uint32_t)__shfl((int)wave_scan(v, lane), 63);
+        const uint32_t v = s0 + lane < seq ? seq_units<ROWS>(a, s0 + lane).units : 0, n = min(seq - s0, 64u);
+        before += of_lane(wave_scan(v, lane, n), n - 1);
     }
     const uint32_t packed = (uint32_t)su.r.rows * a.group;
     // of its rows, gridDim.y at a time
@@ -762,7 +784,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attention_many(AttnArgs a) {
     constexpr int kAhead = NP == 2 ? 4 : 8;                // fragments read ahead (8 spill at two pieces)
     extern __shared__ __align__(16) uint8_t lds_raw[];
     StepLds<D>* lds = reinterpret_cast<StepLds<D>*>(lds_raw);
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, row = lane % 32, h = lane / 32;
+    const uint32_t lane = threadIdx.x % 64, wave = uniform(threadIdx.x / 64), row = lane % 32, h = lane / 32;
     const uint32_t pairs = a.b.n_seqs * a.c.heads;
     uint32_t id = blockIdx.x;
     const uint32_t kvh = id % a.c.heads, seq = id % pairs / a.c.heads;
@@ -791,7 +813,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attention_many(AttnArgs a) {
         QRow<D, NP, 2> q;
         Running32<D> run;
         {
-            float raw[F][8];
+            uint32_t raw[F][QRow<D, NP, 2>::W];
             q.fetch(a, sr, kvh, my0 + row, packed, h, cap, raw);
             q.finish(a, raw);
             run.clear();
@@ -944,7 +966,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attention_many16(AttnArgs a) 
     constexpr int kAhead = 4;                                       // fragments read ahead (8 spill: 195 against 188 us)
     extern __shared__ __align__(16) uint8_t lds_raw[];
     StepLds16<D>* lds = reinterpret_cast<StepLds16<D>*>(lds_raw);
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, g = lane / 16;
+    const uint32_t lane = threadIdx.x % 64, wave = uniform(threadIdx.x / 64), col = lane % 16, g = lane / 16;
     const uint32_t pairs = a.b.n_seqs * a.c.heads;
     uint32_t id = blockIdx.x;
     const uint32_t kvh = id % a.c.heads, seq = id % pairs / a.c.heads;
@@ -971,7 +993,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attention_many16(AttnArgs a) 
         QRow<D, NP> q;
         Running<DT> run;
         {
-            float raw[F][8];
+            uint32_t raw[F][QRow<D, NP>::W];
             q.fetch(a, sr, kvh, my0 + col, packed, g, cap, raw);
             q.finish(a, raw);
             run.clear();
