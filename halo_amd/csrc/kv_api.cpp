@@ -42,7 +42,7 @@ int check_rows(const char* op, const char* name, HeadRows& r, uint64_t rows, uin
     *bytes = 0;
     if (rows == 0 || heads == 0) return HALO_MI_OK;
     if (!r.data) return set_error(HALO_MI_E_KERNEL, "%s: operand %s is empty", op, name);
-    if (r.head_stride > 1ull << 40 || r.stride > 1ull << 40) return set_error(HALO_MI_E_KERNEL, "%s: a stride of %s is out of range", op, name);
+    if (r.head_stride > 1ull << 40 || r.stride > 1ull << 40 || (rows > 1 && r.stride > (1ull << 58) / rows)) return set_error(HALO_MI_E_KERNEL, "%s: a stride of %s is out of range", op, name);
     if (heads > 1 && r.head_stride < dim) return set_error(HALO_MI_E_KERNEL, "%s: %s head stride < %u elements", op, name, dim);
     // rows may lie inside the heads' stride (a layout [head][row][dim]) or around them
     if (rows > 1 && r.stride < row && !(r.stride >= dim && (heads == 1 || r.head_stride >= (rows - 1) * r.stride + dim)))
@@ -178,7 +178,7 @@ int check_state(const char* op, const halo_mi_kv_cache* cache, const halo_mi_kv_
     if ((rc = check_cache(op, *cache, &a->page_bytes))) return rc;
     const uint64_t stride = s->table_stride ? s->table_stride : s->table_width;
     if (s->n_slots == 0 || s->n_slots > 0x7FFFFFFFu) return set_error(HALO_MI_E_KERNEL, "%s: n_slots %u is out of range", op, s->n_slots);
-    if (s->table_width == 0 || (uint64_t)s->table_width * cache->block_tokens > 0x7FFFFF00u || stride > 1ull << 40 ||
+    if (s->table_width == 0 || (uint64_t)s->table_width * cache->block_tokens > 0x7FFFFF00u || stride > (1ull << 58) / s->n_slots ||
         (s->n_slots > 1 && stride < s->table_width))
         return set_error(HALO_MI_E_KERNEL, "%s: table width %u or its stride is out of range", op, s->table_width);
     if ((rc = check_aligned(op, "refs", s->refs, 4)) || (rc = check_aligned(op, "lens", s->lens, 4)) ||
@@ -200,6 +200,10 @@ int check_state(const char* op, const halo_mi_kv_cache* cache, const halo_mi_kv_
     return check_apart(op, tables, {pool});
 }
 
+Range tables_range(const KvPagesArgs& a) {
+    return {a.tables, extent(a.n_slots, a.table_stride * 4, (uint64_t)a.table_width * 4), "tables"};
+}
+
 // A listed call's lists: n int32 each, apart from what the call changes.
 int check_lists(const char* op, const KvPagesArgs& a, const int32_t* x, const int32_t* y, uint32_t n) {
     int rc;
@@ -211,7 +215,7 @@ int check_lists(const char* op, const KvPagesArgs& a, const int32_t* x, const in
                               {{a.pool, a.n_pages * a.page_bytes, "the pool"},
                                {a.refs, 4ull * a.n_pages, "refs"},
                                {a.lens, 4ull * a.n_slots, "lens"},
-                               {a.tables, extent(a.n_slots, a.table_stride * 4, (uint64_t)a.table_width * 4), "tables"}})))
+                               tables_range(a)})))
             return rc;
     return HALO_MI_OK;
 }
@@ -410,8 +414,8 @@ int halo_mi_kv_resize(const halo_mi_kv_cache* cache, const halo_mi_kv_state* sta
     uint32_t* scratch = nullptr;
     auto st = static_cast<hipStream_t>(stream);
     if ((rc = check_state(op, cache, state, &a)) || (rc = check_lists(op, a, slots, new_lens, n))) return rc;
+    if ((rc = take_status(op, status, status_keep, st, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, tables_range(a), {slots, 4ull * n, "slots"}, {new_lens, 4ull * n, "new_lens"}, {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
     if ((rc = scratch_for(op, st, 1 + 5ull * n + a.n_pages, &scratch))) return rc;
-    if ((rc = take_status(op, status, status_keep, st, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, {slots, 4ull * n, "slots"}, {new_lens, 4ull * n, "new_lens"}, {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
     return n ? launch_kv_resize(a, slots, new_lens, n, scratch, status, st) : HALO_MI_OK;
 }
 
@@ -424,8 +428,8 @@ int halo_mi_kv_fork(const halo_mi_kv_cache* cache, const halo_mi_kv_state* state
     uint32_t* scratch = nullptr;
     auto st = static_cast<hipStream_t>(stream);
     if ((rc = check_state(op, cache, state, &a)) || (rc = check_lists(op, a, src, dst, n))) return rc;
+    if ((rc = take_status(op, status, status_keep, st, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, tables_range(a), {src, 4ull * n, "src"}, {dst, 4ull * n, "dst"}, {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
     if ((rc = scratch_for(op, st, 1 + 5ull * n + a.n_pages, &scratch))) return rc;
-    if ((rc = take_status(op, status, status_keep, st, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, {src, 4ull * n, "src"}, {dst, 4ull * n, "dst"}, {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
     return n ? launch_kv_fork(a, src, dst, n, scratch, status, st) : HALO_MI_OK;
 }
 
@@ -439,7 +443,7 @@ int halo_mi_kv_compact(const halo_mi_kv_cache* cache, const halo_mi_kv_state* st
     if ((rc = check_state(op, cache, state, &a))) return rc;
     if (live) {
         if ((rc = check_aligned(op, "live", live, 4))) return rc;
-        if ((rc = check_apart(op, {live, 4, "live"}, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
+        if ((rc = check_apart(op, {live, 4, "live"}, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, tables_range(a), {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
     }
     if ((rc = scratch_for(op, st, 2 + 3ull * a.n_pages, &scratch))) return rc;
     return launch_kv_compact(a, scratch, live, st);

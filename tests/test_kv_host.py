@@ -191,8 +191,12 @@ def test_page_refusals(hl):
         refused(hl, K, f, _cache(hl), st(), x=0)
         refused(hl, K, f, _cache(hl), st(), y=E + 2)
         refused(hl, K, f, _cache(hl), st(), x=B + 0x1004)
+        for word in (B + 8, B + 0x1004, B + 0x2010, A + 4096, D + 4, E + 8, F + 2):  # on refs, lens, tables, the pool, a list
+            refused(hl, K, f, _cache(hl), st(), status=word)
+        refused(hl, K, f, _cache(hl), st(slots=1 << 30, table_stride=1 << 40))
     refused(hl, U, compact, _cache(hl, pages=1 << 24, layers=1, heads=1, dim=64), st(refs=1 << 44, lens=1 << 45, tables=1 << 46))
-    refused(hl, K, compact, _cache(hl), st(), live=B)
+    for word in (B, B + 0x1004, B + 0x2010, A + 4096, F + 1):
+        refused(hl, K, compact, _cache(hl), st(), live=word)
     copy = lambda c, x=D, y=E, n=3, **kw: hl.kv_copy_pages(c, x, y, n, stream=0, **kw)  # noqa: E731
     refused(hl, U, copy, _cache(hl, block=24))
     refused(hl, K, copy, _cache(hl), x=0)
