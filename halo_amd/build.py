@@ -80,17 +80,17 @@ def build_oracle() -> Path:
     return ROOT / "oracle" / "liboracle.so"
 
 
-CPP_TEST_SRC = ROOT / "tests" / "cpp" / "backend_pair.cpp"
-CPP_TEST_BIN = ROOT / "tests" / "cpp" / "backend_pair"
+CPP_TESTS = [ROOT / "tests" / "cpp" / name for name in ("backend_pair", "backend_kv")]
 
 
-def build_cpp_tests() -> Path:
-    """The C++ test of the Backend adapter (host code only: g++, linked against the library
+def build_cpp_tests() -> list[Path]:
+    """The C++ tests of the Backend adapter (host code only: g++, linked against the library
     and the oracle, found through $ORIGIN-relative run paths)."""
-    _run(["g++", "-std=c++20", "-O1", "-Wall", "-o", str(CPP_TEST_BIN), str(CPP_TEST_SRC),
-          "-L" + str(PKG), "-lhalo_mi355x", "-L" + str(ROOT / "oracle"), "-loracle",
-          "-Wl,-rpath,$ORIGIN/../../halo_amd:$ORIGIN/../../oracle"])
-    return CPP_TEST_BIN
+    for test in CPP_TESTS:
+        _run(["g++", "-std=c++20", "-O1", "-Wall", "-o", str(test), str(test.with_suffix(".cpp")),
+              "-L" + str(PKG), "-lhalo_mi355x", "-L" + str(ROOT / "oracle"), "-loracle",
+              "-Wl,-rpath,$ORIGIN/../../halo_amd:$ORIGIN/../../oracle"])
+    return CPP_TESTS
 
 
 def build_all() -> None:

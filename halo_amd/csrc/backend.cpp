@@ -117,8 +117,8 @@ private:
 
 class Mi355xBackend;
 
-// A stream owns its hipStream_t and one device word for the GET_ROWS status bits of the ops
-// enqueued since the last wait(); the library's per-stream workspace is released with it.
+// A stream owns its hipStream_t and two device words for the status bits of the ops enqueued since the last
+// wait(), GET_ROWS's and the paged cache's; the library's per-stream workspace is released with it.
 class HipStream final : public MiStream {
 public:
     HipStream(Mi355xBackend* owner, hipStream_t s, std::uint32_t* status) : owner_(owner), s_(s), status_(status) {}
@@ -137,6 +137,11 @@ public:
     std::uint32_t* get_rows_status() noexcept {
         status_used_ = true;
         return status_;
+    }
+    // ... and the paged cache's
+    std::uint32_t* kv_status() noexcept {
+        status_used_ = true;
+        return status_ + 1;
     }
 
 private:
@@ -237,7 +242,7 @@ private:
 
 // ---- variant registry (explicit, append-only ids; grouped by op) ----------------------------
 
-constexpr std::array<VariantInfo, 21> kVariants{{
+constexpr std::array<VariantInfo, 26> kVariants{{
     {kDequantRows, "dequant_rows_exact", OpId::GetRows, {}},
     {kRmsNorm, "rms_norm_cpu_order", OpId::RmsNorm, {}},
     {kGemvGgufRef, "gemv_gguf_ref_b256", OpId::Gemv, {}},
@@ -259,6 +264,11 @@ constexpr std::array<VariantInfo, 21> kVariants{{
     {kGateUpGemmSmallM, "gate_up_gemm_bf16_mfma_small_m", OpId::GateUpSwiglu, {}},
     {kGateUpExactSmallM, "gate_up_gemm_exact_small_m", OpId::GateUpSwiglu, {}},
     {kGateUpExactInvariant, "gate_up_gemm_exact_invariant", OpId::GateUpSwiglu, {}},
+    {kRopeTable, "rope_table", OpId::Rope, {}},
+    {kKv8Write, "kv8_write", OpId::Kv8Write, {}},
+    {kKv8Read, "kv8_read", OpId::Kv8Read, {}},
+    {kKv8Attention, "kv8_attention_mfma", OpId::Kv8Attention, {}},
+    {kKv8Pages, "kv8_pages", OpId::Kv8Pages, {}},
 }};
 
 bool has_variant(OpId op, std::uint32_t id) {
@@ -392,7 +402,7 @@ public:
             (void)hipStreamDestroy(s);
             fail(ErrorCode::Memory, "mi355x backend: cannot allocate a stream's status word");
         }
-        if (hipMemsetAsync(status, 0, 4, s) != hipSuccess || hipStreamSynchronize(s) != hipSuccess) {
+        if (hipMemsetAsync(status, 0, 8, s) != hipSuccess || hipStreamSynchronize(s) != hipSuccess) {
             (void)hipFree(status);
             (void)hipStreamDestroy(s);
             fail(ErrorCode::Device, "mi355x backend: cannot clear a stream's status word");
@@ -676,6 +686,99 @@ public:
               ErrorCode::Device, "COPY: hipMemcpyAsync failed");
     }
 
+    // ---- attention over an 8-bit paged cache: ownership, ranges and writability are checked here, everything
+    // else (types, geometry, strides, overlap) by the C ABI before it enqueues
+
+    void rope(Stream& s, const RopeTableArgs& a) override {
+        HipStream& st = stream(s, "ROPE");
+        check_choice(a.kernel, OpId::Rope);
+        CHECK(a.n_parts == 1 || a.n_parts == 2, ErrorCode::Unsupported, "ROPE: %u parts (1 or 2)", a.n_parts);
+        const Resolver r(this, "ROPE");
+        const std::uint32_t size = value_bytes(a.type, r.op());
+        halo_mi_rope_part parts[2] = {};
+        for (std::uint32_t i = 0; i < a.n_parts; ++i) {
+            const RopePart& p = a.parts[i];
+            const Operand in = heads_of(r, p.in, a.n_tokens, p.n_heads, a.head_dim, p.in_head_stride, size, Access::Read, "in");
+            const Operand out = heads_of(r, p.out, a.n_tokens, p.n_heads, a.head_dim, p.out_head_stride, size, Access::Write, "out");
+            parts[i] = {in.base, in.stride / size, p.in_head_stride, out.base, out.stride / size, p.out_head_stride, p.n_heads};
+        }
+        const Operand pos = r.get(a.positions, 1, mul_u64(a.n_tokens, 4, r.op(), "positions"), 4, Access::Read, "positions");
+        const Operand freqs = r.get(a.freqs, 1, a.rot_dims / 2 * 8ull, 8, Access::Read, "freqs");
+        const halo_mi_rope_params p{static_cast<std::uint32_t>(a.type),
+                                    a.interleaved ? HALO_MI_ROPE_INTERLEAVED : HALO_MI_ROPE_HALF,
+                                    parts, a.n_parts, a.n_tokens, a.head_dim, a.rot_dims,
+                                    reinterpret_cast<const std::int32_t*>(pos.base), reinterpret_cast<const double*>(freqs.base), a.factor};
+        check_abi(halo_mi_rope(&p, st.native()));
+    }
+
+    void kv8_write(Stream& s, const Kv8WriteArgs& a) override {
+        HipStream& st = stream(s, "KV8_WRITE");
+        check_choice(a.kernel, OpId::Kv8Write);
+        const Resolver r(this, "KV8_WRITE");
+        const std::uint32_t size = value_bytes(a.type, r.op());
+        halo_mi_kv_write_params p{static_cast<std::uint32_t>(a.type), cache_of(r, a.cache, Access::Write), a.layer, batch_of(r, a.batch)};
+        const Operand k = heads_of(r, a.k, a.batch.n_rows, a.cache.n_kv_heads, a.cache.head_dim, a.k_head_stride, size, Access::Read, "k");
+        const Operand v = heads_of(r, a.v, a.batch.n_rows, a.cache.n_kv_heads, a.cache.head_dim, a.v_head_stride, size, Access::Read, "v");
+        p.k = k.base, p.k_stride = k.stride / size, p.k_head_stride = a.k_head_stride;
+        p.v = v.base, p.v_stride = v.stride / size, p.v_head_stride = a.v_head_stride;
+        p.status = status_of(r, a.status, st, &p.status_keep);
+        check_abi(halo_mi_kv_write(&p, st.native()));
+    }
+
+    void kv8_read(Stream& s, const Kv8ReadArgs& a) override {
+        HipStream& st = stream(s, "KV8_READ");
+        check_choice(a.kernel, OpId::Kv8Read);
+        const Resolver r(this, "KV8_READ");
+        halo_mi_kv_read_params p{cache_of(r, a.cache, Access::Read), a.layer, batch_of(r, a.batch)};
+        const auto rows = [&](const TensorRef& t, std::uint64_t head_stride, const char* name) {
+            return t.empty() ? Operand{}
+                             : heads_of(r, t, a.batch.n_rows, a.cache.n_kv_heads, a.cache.head_dim, head_stride, kF32, Access::Write, name);
+        };
+        const Operand k = rows(a.k, a.k_head_stride, "k"), v = rows(a.v, a.v_head_stride, "v");
+        p.k_out = reinterpret_cast<float*>(k.base), p.k_stride = k.stride / kF32, p.k_head_stride = a.k_head_stride;
+        p.v_out = reinterpret_cast<float*>(v.base), p.v_stride = v.stride / kF32, p.v_head_stride = a.v_head_stride;
+        p.status = status_of(r, a.status, st, &p.status_keep);
+        check_abi(halo_mi_kv_read(&p, st.native()));
+    }
+
+    void kv8_attention(Stream& s, const Kv8AttentionArgs& a) override {
+        HipStream& st = stream(s, "KV8_ATTENTION");
+        check_choice(a.kernel, OpId::Kv8Attention);
+        const Resolver r(this, "KV8_ATTENTION");
+        const std::uint32_t size = value_bytes(a.type, r.op());
+        halo_mi_attention_params p{static_cast<std::uint32_t>(a.type), cache_of(r, a.cache, Access::Read), a.layer, batch_of(r, a.batch)};
+        const Operand q = heads_of(r, a.q, a.batch.n_rows, a.n_heads, a.cache.head_dim, a.q_head_stride, size, Access::Read, "q");
+        const Operand out = heads_of(r, a.out, a.batch.n_rows, a.n_heads, a.cache.head_dim, a.out_head_stride, size, Access::Write, "out");
+        p.q = q.base, p.q_stride = q.stride / size, p.q_head_stride = a.q_head_stride;
+        p.out = out.base, p.out_stride = out.stride / size, p.out_head_stride = a.out_head_stride;
+        p.n_heads = a.n_heads, p.scale = a.scale, p.window = a.window;
+        if (!a.workspace.empty()) {
+            const Operand w = r.get(a.workspace, 1, a.workspace.view_bytes() / 16 * 16, 16, Access::Write, "workspace");
+            p.workspace = w.base, p.workspace_bytes = w.extent;
+        }
+        p.status = status_of(r, a.status, st, &p.status_keep);
+        check_abi(halo_mi_attention(&p, st.native()));
+    }
+
+    void kv8_resize(Stream& s, const Kv8PagesArgs& a) override { listed(s, a, true, halo_mi_kv_resize); }
+    void kv8_fork(Stream& s, const Kv8PagesArgs& a) override { listed(s, a, true, halo_mi_kv_fork); }
+    void kv8_copy_pages(Stream& s, const Kv8PagesArgs& a) override {
+        listed(s, a, false, [](const halo_mi_kv_cache* c, const halo_mi_kv_state*, const std::int32_t* x, const std::int32_t* y,
+                               std::uint32_t n, std::uint32_t* status, std::uint32_t keep, void* st) {
+            return halo_mi_kv_copy_pages(c, x, y, n, status, keep, st);
+        });
+    }
+
+    void kv8_compact(Stream& s, const Kv8CompactArgs& a) override {
+        HipStream& st = stream(s, "KV8_PAGES");
+        check_choice(a.kernel, OpId::Kv8Pages);
+        const Resolver r(this, "KV8_PAGES");
+        const halo_mi_kv_cache c = cache_of(r, a.cache, Access::Write);
+        const halo_mi_kv_state state = state_of(r, a.state, a.cache);
+        const Operand live = a.live.empty() ? Operand{} : r.get(a.live, 1, 4, 4, Access::Write, "live");
+        check_abi(halo_mi_kv_compact(&c, &state, reinterpret_cast<std::uint32_t*>(live.base), st.native()));
+    }
+
     // The ops of the reference interface outside this path.
     void add_rms_norm(Stream&, const AddRmsNormArgs&) override { unsupported(OpId::AddRmsNorm); }
     void gdn_gates(Stream&, const GdnGateArgs&) override { unsupported(OpId::GdnGates); }
@@ -693,6 +796,72 @@ private:
     [[noreturn]] static void unsupported(OpId op) {
         fail(ErrorCode::Unsupported, "%.*s is not implemented by the mi355x backend (quantized matmul path only)",
              (int)op_name(op).size(), op_name(op).data());
+    }
+
+    static void check_choice(const KernelChoice& k, OpId op) {
+        CHECK(has_variant(op, k.variant_id), ErrorCode::Config, "%.*s: unknown kernel variant id %u", (int)op_name(op).size(),
+              op_name(op).data(), k.variant_id);
+    }
+
+    static std::uint32_t value_bytes(DType t, const char* op) {
+        CHECK(t == DType::F32 || t == DType::F16 || t == DType::BF16, ErrorCode::Unsupported, "%s: element type %s is not F32, F16 or BF16",
+              op, type_name(t));
+        return t == DType::F32 ? 4 : 2;
+    }
+
+    // rows x heads x dim elements of `size` bytes, heads `head_stride` elements apart (0 = dim) inside a row.
+    static Operand heads_of(const Resolver& r, const TensorRef& t, std::uint64_t rows, std::uint32_t heads, std::uint32_t dim,
+                            std::uint64_t head_stride, std::uint32_t size, Access access, const char* name) {
+        CHECK(head_stride <= 1ull << 40, ErrorCode::Kernel, "%s: the head stride of %s is out of range", r.op(), name);
+        const std::uint64_t row = heads == 0 ? 0 : (heads - 1) * (head_stride ? head_stride : dim) + dim;
+        return r.get(t, rows, mul_u64(row, size, r.op(), name), size, access, name);
+    }
+
+    static halo_mi_kv_cache cache_of(const Resolver& r, const Kv8Cache& c, Access access) {
+        const std::uint64_t page = halo_mi_kv_page_bytes(c.n_layers, c.n_kv_heads, c.head_dim, c.block_tokens);
+        CHECK(page != 0, ErrorCode::Unsupported, "%s: no cache of %u layers, %u heads of %u, %u tokens a page", r.op(), c.n_layers,
+              c.n_kv_heads, c.head_dim, c.block_tokens);
+        CHECK(c.pool.row_stride == 0 || c.pool.row_stride == page, ErrorCode::Kernel, "%s: pages are dense", r.op());
+        const Operand pool = r.get(c.pool, c.n_pages, page, 16, access, "pool");
+        return {pool.base, c.n_pages, c.n_layers, c.n_kv_heads, c.head_dim, c.block_tokens};
+    }
+
+    static halo_mi_kv_batch batch_of(const Resolver& r, const Kv8Batch& b) {
+        const Operand tables = r.get(b.tables, b.n_seqs, 4ull * b.table_width, 4, Access::Read, "tables");
+        const Operand lens = r.get(b.kv_lens, 1, 4ull * b.n_seqs, 4, Access::Read, "kv_lens");
+        const Operand starts = r.get(b.row_starts, 1, b.n_seqs ? 4ull * b.n_seqs + 4 : 0, 4, Access::Read, "row_starts");
+        return {reinterpret_cast<const std::int32_t*>(tables.base), tables.stride / 4, b.table_width,
+                reinterpret_cast<const std::int32_t*>(lens.base), reinterpret_cast<const std::int32_t*>(starts.base),
+                b.n_seqs, b.n_rows, b.max_rows, b.max_kv};
+    }
+
+    static halo_mi_kv_state state_of(const Resolver& r, const Kv8State& s, const Kv8Cache& c) {
+        const Operand refs = r.get(s.refs, 1, 4ull * c.n_pages, 4, Access::Write, "refs");
+        const Operand lens = r.get(s.lens, 1, 4ull * s.n_slots, 4, Access::Write, "lens");
+        const Operand tables = r.get(s.tables, s.n_slots, 4ull * s.table_width, 4, Access::Write, "tables");
+        return {reinterpret_cast<std::int32_t*>(refs.base), reinterpret_cast<std::int32_t*>(lens.base),
+                reinterpret_cast<std::int32_t*>(tables.base), tables.stride / 4, s.table_width, s.n_slots};
+    }
+
+    // The caller's status word, cleared by the op, or the stream's, which collects until wait().
+    static std::uint32_t* status_of(const Resolver& r, const TensorRef& t, HipStream& st, std::uint32_t* keep) {
+        *keep = t.empty();
+        if (t.empty()) return st.kv_status();
+        return reinterpret_cast<std::uint32_t*>(r.get(t, 1, 4, 4, Access::Write, "status").base);
+    }
+
+    template <class Call>
+    void listed(Stream& s, const Kv8PagesArgs& a, bool with_state, const Call& call) {
+        HipStream& st = stream(s, "KV8_PAGES");
+        check_choice(a.kernel, OpId::Kv8Pages);
+        const Resolver r(this, "KV8_PAGES");
+        const halo_mi_kv_cache c = cache_of(r, a.cache, Access::Write);
+        const halo_mi_kv_state state = with_state ? state_of(r, a.state, a.cache) : halo_mi_kv_state{};
+        const Operand x = r.get(a.a, 1, 4ull * a.n, 4, Access::Read, "a"), y = r.get(a.b, 1, 4ull * a.n, 4, Access::Read, "b");
+        std::uint32_t keep = 0;
+        std::uint32_t* status = status_of(r, a.status, st, &keep);
+        check_abi(call(&c, &state, reinterpret_cast<const std::int32_t*>(x.base), reinterpret_cast<const std::int32_t*>(y.base), a.n, status,
+                       keep, st.native()));
     }
 
     static bool is_slab(const TensorRef& t) {
@@ -754,13 +923,15 @@ void HipStream::wait() {
     }
     if (!status_used_) return;
     status_used_ = false;
-    std::uint32_t word = 0;
-    if (hipMemcpy(&word, status_, 4, hipMemcpyDeviceToHost) != hipSuccess ||
-        (word != 0 && hipMemsetAsync(status_, 0, 4, s_) != hipSuccess) || hipStreamSynchronize(s_) != hipSuccess) {
+    std::uint32_t words[2] = {};
+    if (hipMemcpy(words, status_, 8, hipMemcpyDeviceToHost) != hipSuccess ||
+        ((words[0] | words[1]) != 0 && hipMemsetAsync(status_, 0, 8, s_) != hipSuccess) || hipStreamSynchronize(s_) != hipSuccess) {
         owner_->poison(false);
         throw Error(ErrorCode::Device, "stream wait: cannot read the status word");
     }
-    CHECK(!(word & kStatusBadIndex), ErrorCode::Kernel, "GET_ROWS: an id lies outside the table (status 0x%x)", word);
+    CHECK(!(words[0] & kStatusBadIndex), ErrorCode::Kernel, "GET_ROWS: an id lies outside the table (status 0x%x)", words[0]);
+    CHECK(!(words[1] & kStatusBadIndex), ErrorCode::Kernel, "paged cache: a page, slot or length is out of range (status 0x%x)", words[1]);
+    CHECK(!(words[1] & kStatusKvFull), ErrorCode::Memory, "paged cache: no free page, or no column in a table (status 0x%x)", words[1]);
 }
 
 }  // namespace
@@ -816,6 +987,11 @@ std::string_view op_name(OpId op) noexcept {
         case OpId::TopK: return "TOP_K";
         case OpId::Copy: return "COPY";
         case OpId::GateUpSwiglu: return "GATE_UP_SWIGLU";
+        case OpId::Rope: return "ROPE";
+        case OpId::Kv8Write: return "KV8_WRITE";
+        case OpId::Kv8Read: return "KV8_READ";
+        case OpId::Kv8Attention: return "KV8_ATTENTION";
+        case OpId::Kv8Pages: return "KV8_PAGES";
     }
     return "UNKNOWN";
 }
@@ -860,7 +1036,8 @@ void Backend::run_op(Stream& s, const OpInvocation& inv) {
         case OpId::Argmax: return argmax(s, args_of<ArgmaxArgs>(inv));
         case OpId::TopK: return top_k(s, args_of<TopKArgs>(inv));
         case OpId::Copy: return copy(s, args_of<CopyArgs>(inv));
-        case OpId::GateUpSwiglu: break;  // an addition with no args type in OpInvocation
+        case OpId::GateUpSwiglu: case OpId::Rope: case OpId::Kv8Write: case OpId::Kv8Read: case OpId::Kv8Attention:
+        case OpId::Kv8Pages: break;  // additions with no args type in OpInvocation
     }
     fail(ErrorCode::Api, "run_op: unknown op id %u", static_cast<unsigned>(inv.op));
 }

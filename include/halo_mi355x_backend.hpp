@@ -25,8 +25,9 @@
 // MiBackend, never in the reference's classes: weights imported straight into the SLAB device
 // layout (MiBackend::import_weights), GET_ROWS over a contiguous row range
 // (MiBackend::dequant_rows), the FFN's gate/up/SwiGLU composition (src/models/qwen35.cpp:789-805)
-// as one op (MiBackend::gate_up_swiglu), device addresses and layouts of buffers, and the
-// hipStream_t of a stream.
+// as one op (MiBackend::gate_up_swiglu), rotary positions and attention over a batch of sequences with
+// an 8-bit paged cache (MiBackend::rope, kv8_*), device addresses and layouts of buffers, and the hipStream_t
+// of a stream.
 #pragma once
 
 #include <cstddef>
@@ -143,6 +144,8 @@ enum class OpId : std::uint16_t {
     GatedRmsNorm = 7, PartialRope = 8, KvWrite = 9, Attention = 10, Swiglu = 11, MulSigmoid = 12, Add = 13,
     LmHead = 14, Argmax = 15, TopK = 16, Copy = 17,
     GateUpSwiglu = 18,  // addition: gemv(gate) + gemv(up) + swiglu in one launch (MiBackend::gate_up_swiglu)
+    // additions: MiBackend's rotary positions from a table of frequencies and its 8-bit paged cache
+    Rope = 19, Kv8Write = 20, Kv8Read = 21, Kv8Attention = 22, Kv8Pages = 23,
 };
 inline constexpr std::size_t kOpCount = 18;  // the reference's ops
 
@@ -467,6 +470,105 @@ struct GateUpArgs {
     float norm_eps = 1e-6f;
 };
 
+// ---- attention over an 8-bit paged cache (halo_mi355x.h says what each op computes) --------
+//
+// `type` is F32, F16 or BF16. Rows are TensorRef rows (row_stride in bytes, 0 = dense); a head stride
+// counts elements, 0 = head_dim. Lists are int32 on the device, read when the op runs. What an op finds wrong in
+// them is reported by the stream's next wait(): Error(Kernel) for an entry out of range, Error(Memory) where the
+// pages or a table's columns ran out; with `status` set (4 bytes, cleared by the op), the bits are left there instead
+// (kStatusBadIndex, kStatusKvFull) and wait() does not throw for them.
+
+inline constexpr std::uint32_t kStatusKvFull = 16u;
+
+struct RopePart {
+    TensorRef in{}, out{};  ///< n_tokens rows of n_heads heads; out may be in
+    std::uint32_t n_heads = 0;
+    std::uint64_t in_head_stride = 0, out_head_stride = 0;
+};
+
+/// Rotary positions of q and, in the same launch, k (n_parts 1 or 2).
+struct RopeTableArgs {
+    DType type = DType::F32;
+    bool interleaved = false;
+    RopePart parts[2]{};
+    std::uint32_t n_parts = 1, n_tokens = 0, head_dim = 0, rot_dims = 0;
+    TensorRef positions{}, freqs{};  ///< n_tokens int32; rot_dims / 2 doubles (halo_mi_rope_freqs)
+    float factor = 1.0f;
+    KernelChoice kernel{};
+};
+
+struct Kv8Cache {
+    TensorRef pool{};  ///< n_pages records of halo_mi_kv_page_bytes()
+    std::uint32_t n_pages = 0, n_layers = 1, n_kv_heads = 0, head_dim = 0, block_tokens = 16;
+};
+
+/// Rows [row_starts[s], row_starts[s + 1]) are the last tokens of sequence s, which holds kv_lens[s] tokens.
+struct Kv8Batch {
+    TensorRef tables{}, kv_lens{}, row_starts{};  ///< n_seqs rows of table_width; n_seqs; n_seqs + 1
+    std::uint32_t n_seqs = 0, n_rows = 0, table_width = 0;
+    std::uint32_t max_rows = 0, max_kv = 0;  ///< as the host knows them, 0 = unknown
+};
+
+struct Kv8WriteArgs {
+    DType type = DType::F32;
+    Kv8Cache cache{};
+    std::uint32_t layer = 0;
+    Kv8Batch batch{};
+    TensorRef k{}, v{};
+    std::uint64_t k_head_stride = 0, v_head_stride = 0;
+    TensorRef status{};
+    KernelChoice kernel{};
+};
+
+/// The cached values of the batch's rows in fp32; k or v may be empty.
+struct Kv8ReadArgs {
+    Kv8Cache cache{};
+    std::uint32_t layer = 0;
+    Kv8Batch batch{};
+    TensorRef k{}, v{};
+    std::uint64_t k_head_stride = 0, v_head_stride = 0;
+    TensorRef status{};
+    KernelChoice kernel{};
+};
+
+struct Kv8AttentionArgs {
+    DType type = DType::F32;
+    Kv8Cache cache{};
+    std::uint32_t layer = 0;
+    Kv8Batch batch{};
+    TensorRef q{}, out{};
+    std::uint64_t q_head_stride = 0, out_head_stride = 0;
+    std::uint32_t n_heads = 0, window = 0;
+    float scale = 0.0f;     ///< 0 = 1 / sqrt(head_dim)
+    TensorRef workspace{};  ///< empty = the stream's own
+    TensorRef status{};
+    KernelChoice kernel{};
+};
+
+/// The pages' owner: refs n_pages, lens n_slots, tables n_slots rows of table_width.
+struct Kv8State {
+    TensorRef refs{}, lens{}, tables{};
+    std::uint32_t n_slots = 0, table_width = 0;
+};
+
+/// kv8_resize: a = slots, b = their new lengths; kv8_fork: a = sources, b = destinations; kv8_copy_pages: a =
+/// source pages, b = destination pages (state unused).
+struct Kv8PagesArgs {
+    Kv8Cache cache{};
+    Kv8State state{};
+    TensorRef a{}, b{};
+    std::uint32_t n = 0;
+    TensorRef status{};
+    KernelChoice kernel{};
+};
+
+struct Kv8CompactArgs {
+    Kv8Cache cache{};
+    Kv8State state{};
+    TensorRef live{};  ///< one u32, or empty
+    KernelChoice kernel{};
+};
+
 /// The MI355X backend's own interface on top of the reference's.
 class MiBackend : public Backend {
 public:
@@ -477,6 +579,14 @@ public:
                                                                  std::uint64_t row_stride = 0) = 0;
     virtual void dequant_rows(Stream&, const DequantRowsArgs&) = 0;
     virtual void gate_up_swiglu(Stream&, const GateUpArgs&) = 0;
+    virtual void rope(Stream&, const RopeTableArgs&) = 0;
+    virtual void kv8_write(Stream&, const Kv8WriteArgs&) = 0;
+    virtual void kv8_read(Stream&, const Kv8ReadArgs&) = 0;
+    virtual void kv8_attention(Stream&, const Kv8AttentionArgs&) = 0;
+    virtual void kv8_resize(Stream&, const Kv8PagesArgs&) = 0;
+    virtual void kv8_fork(Stream&, const Kv8PagesArgs&) = 0;
+    virtual void kv8_compact(Stream&, const Kv8CompactArgs&) = 0;
+    virtual void kv8_copy_pages(Stream&, const Kv8PagesArgs&) = 0;
 };
 
 /// The kernel family a MATMUL or GATE_UP_SWIGLU call with `allow_gemm == false` and kernel
@@ -520,5 +630,10 @@ inline constexpr std::uint32_t kGemmSlabExactSmallM = 47;  // HALO_MI_GEMM_SLAB_
 inline constexpr std::uint32_t kGateUpExactSmallM = 48;    // GATE_UP_SWIGLU on the exact small-M GEMM
 inline constexpr std::uint32_t kGemmSlabExactInvariant = 49;  // HALO_MI_GEMM_SLAB_EXACT_INVARIANT
 inline constexpr std::uint32_t kGateUpExactInvariant = 50;    // GATE_UP_SWIGLU on it
+inline constexpr std::uint32_t kRopeTable = 51;         // rope
+inline constexpr std::uint32_t kKv8Write = 52;          // kv8_write
+inline constexpr std::uint32_t kKv8Read = 53;           // kv8_read
+inline constexpr std::uint32_t kKv8Attention = 54;      // kv8_attention (the library picks the kernel by the rows)
+inline constexpr std::uint32_t kKv8Pages = 55;          // kv8_resize, kv8_fork, kv8_compact, kv8_copy_pages
 
 }  // namespace halo_mi::backend
