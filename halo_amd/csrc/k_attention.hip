@@ -1182,6 +1182,7 @@ uint64_t plan_many(AttnArgs& a, uint64_t part_bytes) {
     if (a.window) span = std::min<uint64_t>(span, (uint64_t)a.window + rows / a.group + kStep);
     const uint64_t each = (uint64_t)a.b.n_rows * a.heads * (a.c.dim + 4) * sizeof(float);
     a.splits = (uint32_t)std::max<uint64_t>(1, std::min({want / groups, (span + 4 * kStep - 1) / (4 * kStep), part_bytes / each}));
+    if ((uint64_t)a.b.n_rows * a.heads > 4 * kMaxGrid) a.splits = 1;  // the join's grid (rows behind the last sequence count)
     return a.splits > 1 ? a.splits * each : 0;
 }
 

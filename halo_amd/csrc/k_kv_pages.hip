@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kOwnerBlock) void k_kv_resize(KvPagesArgs a, const 
         len = max(a.lens[slot], 0);
         have = min(pages_of(len, a.block), a.table_width);
         column = have;
-        take = goal > have ? goal - have : 0;
+        take = goal > have ? min(goal - have, a.n_pages + 1) : 0;  // more than all pages is as much as any: sums stay in 32 bits
         if (want > len && len % a.block && have) {
             // tokens go behind others in a page: if it is held twice, into a copy
             const int32_t id = a.tables[(uint64_t)slot * a.table_stride + have - 1];

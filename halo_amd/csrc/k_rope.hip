@@ -21,6 +21,7 @@ namespace {
 using namespace dev;
 
 constexpr uint32_t kRopeBlock = 256;
+constexpr uint32_t kRopeTokens = 1u << 23;  // of a launch: a grid has fewer than 2^32 threads along x
 constexpr uint32_t kRopePairs = HALO_MI_ROPE_INTERLEAVED;
 
 // cos and sin of `angle` radians: the nearest quarter turn comes off in 64 bits.
@@ -104,11 +105,18 @@ int launch_typed(uint32_t pairs, const RopeArgs& a, hipStream_t st) {
     const uint32_t at_once = std::max(1u, kRopeBlock / items);
     // few tokens: their heads over several workgroups, one pass each
     const uint32_t passes = std::max<uint64_t>(1, std::min<uint64_t>(a.heads, (uint64_t)a.n_tokens * ((a.heads + at_once - 1) / at_once) / 2048));
-    const uint32_t heads_per = std::min(a.heads, passes * at_once);
-    const dim3 grid(a.n_tokens, (a.heads + heads_per - 1) / heads_per);
+    // at most 2^15 workgroups along y
+    const uint32_t heads_per = std::min(a.heads, std::max(passes * at_once, a.heads / 32768 + 1));
     const bool inter = pairs == kRopePairs;
     auto* k = wide ? (inter ? k_rope<T, V, true> : k_rope<T, V, false>) : (inter ? k_rope<T, 1, true> : k_rope<T, 1, false>);
-    hipLaunchKernelGGL(k, grid, dim3(kRopeBlock), 0, st, a, heads_per);
+    for (uint32_t t = 0; t < a.n_tokens; t += kRopeTokens) {
+        RopeArgs some = a;
+        some.n_tokens = std::min(a.n_tokens - t, kRopeTokens);
+        some.positions += t;
+        for (RopePart& p : some.part)
+            for (HeadRows* r : {&p.in, &p.out}) r->data = static_cast<const T*>(r->data) + t * r->stride;
+        hipLaunchKernelGGL(k, dim3(some.n_tokens, (a.heads + heads_per - 1) / heads_per), dim3(kRopeBlock), 0, st, some, heads_per);
+    }
     return hip_status(hipGetLastError(), "PARTIAL_ROPE");
 }
 

@@ -208,6 +208,9 @@ Range tables_range(const KvPagesArgs& a) {
 int check_lists(const char* op, const KvPagesArgs& a, const int32_t* x, const int32_t* y, uint32_t n) {
     int rc;
     if (n > HALO_MI_KV_LIST_MAX) return set_error(HALO_MI_E_UNSUPPORTED, "%s: %u entries in one call (%u at most)", op, n, HALO_MI_KV_LIST_MAX);
+    // what the entries ask for together is summed in 32 bits
+    if ((uint64_t)n * (std::min(a.table_width, a.n_pages) + 2ull) > 0xFFFFFFFFull)
+        return set_error(HALO_MI_E_UNSUPPORTED, "%s: %u entries of %u columns in one call", op, n, a.table_width);
     if (n == 0) return HALO_MI_OK;
     if ((rc = check_aligned(op, "a list", x, 4)) || (rc = check_aligned(op, "a list", y, 4))) return rc;
     for (const int32_t* l : {x, y})

@@ -603,7 +603,9 @@ uint64_t halo_mi_attention_workspace(const halo_mi_attention_params* p);
  * n_slots), one that the list names before, and a page id out of range leave their entry's slot as it is and set
  * HALO_MI_STATUS_BAD_INDEX. Where the pages run out, that entry and every later one that needs pages are left as they
  * are and HALO_MI_STATUS_KV_FULL is set; so is an entry whose length does not fit the table's columns.
- * At most HALO_MI_KV_LIST_MAX entries a call.
+ * At most HALO_MI_KV_LIST_MAX entries a call, and fewer than 2^32 columns of the entries' tables (or pages of the pool,
+ * if it has fewer) together. The calls work in the stream's workspace: replays of graphs captured on one stream must not
+ * overlap, and a capturing stream needs its workspace already (E_MEMORY; any earlier call that takes one makes it).
  */
 #define HALO_MI_KV_LIST_MAX 1024u
 

@@ -105,3 +105,26 @@ def test_rope_nothing(hl, dev):
     """No tokens, or no heads: nothing is read or written."""
     hl.rope(F32, 0, 0, 0, 128, 128, 0, 0, 4)
     hl.rope(F32, 0, 0, 5, 128, 128, 0, 0, 0)
+
+
+@pytest.mark.parametrize("tokens,heads,kv", [((1 << 24) + 3, 1, 0), (2, 65535, 65535)])
+def test_rope_sizes_past_a_grid(hl, dev, tokens, heads, kv):
+    """More tokens than a launch's grid has threads for, more heads than it has rows."""
+    import torch
+
+    print("[case] rope past a grid", tokens, heads, kv, flush=True)
+    g = torch.Generator(device=dev).manual_seed(5)
+    q = torch.randn(tokens, heads, 2, device=dev, generator=g).half()
+    k = torch.randn(tokens, kv, 2, device=dev, generator=g).half()
+    pos = torch.randint(0, 1 << 16, (tokens,), device=dev, generator=g, dtype=torch.int32)
+    freqs = torch.tensor([0.37], dtype=torch.float64, device=dev)
+    qo, ko = torch.full_like(q, 7), torch.full_like(k, 7)
+    hl.rope(F16, pos, freqs, tokens, 2, 2, q, qo, heads, k=k if kv else None, k_out=ko if kv else None, n_kv_heads=kv)
+    angle = (pos.double() * 0.37)[:, None]
+    for x, y in ((q, qo), (k, ko)):
+        a, b = x[..., 0].double(), x[..., 1].double()
+        c, s = angle.cos(), angle.sin()
+        # as check() has it: the angle in 64 bits, sine and cosine and the products in 32, the result in 16
+        reach = (a.abs() + b.abs()) * (8 * 2.0 ** -24 + 2.0 ** 16 * 0.37 * 2.0 ** -51) + HALF_LEAST[F16]
+        for got, want in ((y[..., 0], a * c - b * s), (y[..., 1], b * c + a * s)):
+            assert bool(((got.double() - want).abs() <= reach + want.abs() * HALF_STEP[F16] * 1.01).all())

@@ -188,6 +188,7 @@ def test_page_refusals(hl):
         refused(hl, K, f, _cache(hl), st(tables=A + 256))  # in the pool
     for f in (resize, fork):
         refused(hl, U, f, _cache(hl), st(), n=hl.KV_LIST_MAX + 1)
+        refused(hl, U, f, _cache(hl, pages=1 << 23, layers=1, heads=1, dim=64), st(refs=1 << 44, lens=1 << 45, tables=1 << 46, width=1 << 23), n=1024)
         refused(hl, K, f, _cache(hl), st(), x=0)
         refused(hl, K, f, _cache(hl), st(), y=E + 2)
         refused(hl, K, f, _cache(hl), st(), x=B + 0x1004)
