@@ -329,31 +329,38 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane, uint32_
 // The run of units of a workgroup (of `workgroups`), and the sequence that the run's first unit lies in, with the
 // units before that sequence. Every wave finds them for itself, 64 sequences at a time.
 struct Run {
-    uint32_t total, per;
     uint32_t first, last;  // [first, last)
     uint32_t seq, before;
+    SeqRows rows;  // of seq
 };
 template <int ROWS>
 __device__ __forceinline__ Run find_run(const AttnArgs& a, uint32_t lane, uint32_t workgroups, uint32_t id) {
     Run r{};
-    const auto units = [&](uint32_t s) { return s < a.b.n_seqs ? seq_units<ROWS>(a, s).units : 0; };
-    const auto batch = [&](uint32_t s0) { return min(a.b.n_seqs - s0, 64u); };
-    uint32_t v = units(lane), sum = wave_scan(v, lane, batch(0));
-    r.total = of_lane(sum, batch(0) - 1);
-    for (uint32_t s0 = 64; s0 < a.b.n_seqs; s0 += 64) r.total += of_lane(wave_scan(units(s0 + lane), lane, batch(s0)), batch(s0) - 1);
-    r.per = max(1u, (r.total + workgroups - 1) / workgroups);
-    r.first = min(id * r.per, r.total);
-    r.last = min(r.first + r.per, r.total);
-    for (uint32_t s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
-        if (a.b.n_seqs > 64) v = units(s0 + lane), sum = wave_scan(v, lane, batch(s0));
-        const uint64_t hit = __ballot(lane < batch(s0) && r.before + sum > r.first);
+    const uint32_t n = a.b.n_seqs;
+    SeqRows rows = seq_rows(a.b, min(lane, n - 1));
+    uint32_t v = lane < n ? seq_units<ROWS>(a, rows).units : 0, sum = wave_scan(v, lane, n), total = of_lane(sum, min(n, 64u) - 1);
+    for (uint32_t s0 = 64; s0 < n; s0 += 64) {
+        const uint32_t w = s0 + lane < n ? seq_units<ROWS>(a, s0 + lane).units : 0;
+        total += of_lane(wave_scan(w, lane, n - s0), min(n - s0, 64u) - 1);
+    }
+    const uint32_t per = max(1u, (total + workgroups - 1) / workgroups);
+    r.first = min(id * per, total);
+    r.last = min(r.first + per, total);
+    for (uint32_t s0 = 0; s0 < n; s0 += 64) {
+        if (s0) {
+            rows = seq_rows(a.b, min(s0 + lane, n - 1));
+            v = s0 + lane < n ? seq_units<ROWS>(a, rows).units : 0;
+            sum = wave_scan(v, lane, n - s0);
+        }
+        const uint64_t hit = __ballot(s0 + lane < n && r.before + sum > r.first);
         if (hit) {
             const uint32_t l = (uint32_t)__ffsll((long long)hit) - 1;
             r.before += of_lane(sum - v, l);
             r.seq = s0 + l;
+            r.rows = {of_lane(rows.row0, l), (int32_t)of_lane((uint32_t)rows.rows, l), (int32_t)of_lane((uint32_t)rows.len, l)};
             break;
         }
-        r.before += of_lane(sum, batch(s0) - 1);
+        r.before += of_lane(sum, min(n - s0, 64u) - 1);
     }
     return r;
 }
@@ -398,7 +405,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attenti
     const Run mine = find_run<ROWS>(a, lane, gridDim.x, blockIdx.x);
     uint32_t u = mine.first, before = mine.before, seq = mine.seq;
     if (u >= mine.last) return;
-    SeqUnits su = seq_units<ROWS>(a, seq);
+    SeqUnits su = seq_units<ROWS>(a, mine.rows);
     const int32_t cap = (int32_t)(a.b.table_width * a.c.block);
 
     for (bool first = true; u < mine.last; first = false) {
@@ -591,57 +598,75 @@ __global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attenti
 
 // Joins the parts of the (sequence, kv head, tile)s that several workgroups of k_attention_few had, in unit order: a
 // workgroup has one row. Its threads take the parts' maxima and sums side by side, then, as 256 / (D / 4) groups,
-// every so many-th part's outputs, and the groups are added in order.
+// every so many-th part's outputs, and the groups are added in order. What it waits for is memory, so the first outputs are
+// asked for together with the maxima.
 template <int ROWS>
 __global__ __launch_bounds__(256) void k_attention_few_join(AttnArgs a, uint32_t workgroups) {
-    __shared__ float factor[kFewGrid], red[4];
+    constexpr int kEach = kFewGrid / 256, kEarly = 4;
+    __shared__ float factor[kFewGrid], red[2][4];
     __shared__ float4v acc_of[256];
     const uint32_t tid = threadIdx.x, lane = tid % 64, D = a.c.dim, quads = D / 4;
-    const Run run = find_run<ROWS>(a, lane, workgroups, 0);
+    const uint32_t groups = 256 / quads, group = tid / quads, d = tid % quads * 4;
     // blockIdx.x counts (sequence, kv head, tile) by their sequences' most tiles
     const uint32_t seq = blockIdx.x / (a.c.heads * a.tiles), kvh = blockIdx.x / a.tiles % a.c.heads;
     const SeqUnits su = seq_units<ROWS>(a, seq);
-    uint32_t before = 0;
-    for (uint32_t s0 = 0; s0 < seq; s0 += 64) {
-        const uint32_t v = s0 + lane < seq ? seq_units<ROWS>(a, s0 + lane).units : 0, n = min(seq - s0, 64u);
-        before += of_lane(wave_scan(v, lane, n), n - 1);
+    uint32_t total = 0, before = 0;
+    for (uint32_t s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
+        const uint32_t n = min(a.b.n_seqs - s0, 64u), v = lane < n ? seq_units<ROWS>(a, s0 + lane).units : 0, sum = wave_scan(v, lane, n);
+        if (seq - s0 < 64) before = total + of_lane(sum - v, seq - s0);
+        total += of_lane(sum, n - 1);
     }
+    const uint32_t per = max(1u, (total + workgroups - 1) / workgroups);
     const uint32_t packed = (uint32_t)su.r.rows * a.group;
     // of its rows, gridDim.y at a time
     for (uint32_t tile = blockIdx.x % a.tiles, row = blockIdx.y; tile < su.tiles; row += gridDim.y) {
         const uint32_t u0 = before + (kvh * su.tiles + tile) * su.chunks, r = tile * ROWS + row;
-        const uint32_t w0 = u0 / run.per, w1 = (u0 + su.chunks - 1) / run.per, n = w1 - w0 + 1;
+        const uint32_t w0 = u0 / per, w1 = (u0 + su.chunks - 1) / per, n = w1 - w0 + 1;
         if (n == 1 || row >= ROWS || r >= packed) {
             tile += a.tiles;
             row = blockIdx.y - gridDim.y;
             continue;
         }
         // a workgroup that began before u0 has this as its last segment
-        const auto part = [&](uint32_t i) { return part_of<ROWS>(a, w0 + i, (w0 + i) * run.per < u0 ? 1 : 0, row); };
-        float top = -INFINITY;
-        for (uint32_t i = tid; i < n; i += 256) top = fmaxf(top, factor[i] = part(i)[D]);
+        const auto part = [&](uint32_t i) { return part_of<ROWS>(a, w0 + i, (w0 + i) * per < u0 ? 1 : 0, row); };
+        float m[kEach], l[kEach];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const uint32_t i = tid + k * 256;
+            m[k] = -INFINITY, l[k] = 0.0f;
+            if (i < n) m[k] = part(i)[D], l[k] = part(i)[D + 1];
+        }
+        float4v early[kEarly];
+#pragma unroll
+        for (int k = 0; k < kEarly; ++k) early[k] = *reinterpret_cast<const float4v*>(part(min(group + k * groups, n - 1)) + d);
+        float top = m[0];
+#pragma unroll
+        for (int k = 1; k < kEach; ++k) top = fmaxf(top, m[k]);
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
-        if (lane == 0) red[tid / 64] = top;
+        if (lane == 0) red[0][tid / 64] = top;
         __syncthreads();
-        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
         float sum = 0.0f;
-        for (uint32_t i = tid; i < n; i += 256) {
-            const float l = part(i)[D + 1], f = factor[i] == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(factor[i] - top);
-            factor[i] = f;
-            sum += l * f;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const uint32_t i = tid + k * 256;
+            const float f = m[k] == -INFINITY ? (l[k] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m[k] - top);
+            if (i < n) factor[i] = f;
+            sum += l[k] * f;
         }
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
+        if (lane == 0) red[1][tid / 64] = sum;
         __syncthreads();
-        if (lane == 0) red[tid / 64] = sum;
-        __syncthreads();
-        sum = (red[0] + red[1]) + (red[2] + red[3]);
-        const uint32_t groups = 256 / quads, group = tid / quads, d = tid % quads * 4;
+        sum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
         float4v acc = {0, 0, 0, 0};
         if (group < groups) {
+#pragma unroll
+            for (int k = 0; k < kEarly; ++k)
+                if (group + k * groups < n) acc += early[k] * factor[group + k * groups];
 #pragma unroll 16
-            for (uint32_t i = group; i < n; i += groups) acc += *reinterpret_cast<const float4v*>(part(i) + d) * factor[i];
+            for (uint32_t i = group + kEarly * groups; i < n; i += groups) acc += *reinterpret_cast<const float4v*>(part(i) + d) * factor[i];
         }
         acc_of[tid] = acc;
         __syncthreads();
