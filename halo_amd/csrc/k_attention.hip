@@ -602,21 +602,26 @@ __global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attenti
 // asked for together with the maxima.
 template <int ROWS>
 __global__ __launch_bounds__(256) void k_attention_few_join(AttnArgs a, uint32_t workgroups) {
-    constexpr int kEach = kFewGrid / 256, kEarly = 4;
+    constexpr int kEach = kFewGrid / 256, kEarly = 4, kBatch = 8;
     __shared__ float factor[kFewGrid], red[2][4];
+    __shared__ uint32_t found[2];
     __shared__ float4v acc_of[256];
     const uint32_t tid = threadIdx.x, lane = tid % 64, D = a.c.dim, quads = D / 4;
     const uint32_t groups = 256 / quads, group = tid / quads, d = tid % quads * 4;
     // blockIdx.x counts (sequence, kv head, tile) by their sequences' most tiles
     const uint32_t seq = blockIdx.x / (a.c.heads * a.tiles), kvh = blockIdx.x / a.tiles % a.c.heads;
     const SeqUnits su = seq_units<ROWS>(a, seq);
-    uint32_t total = 0, before = 0;
-    for (uint32_t s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
-        const uint32_t n = min(a.b.n_seqs - s0, 64u), v = lane < n ? seq_units<ROWS>(a, s0 + lane).units : 0, sum = wave_scan(v, lane, n);
-        if (seq - s0 < 64) before = total + of_lane(sum - v, seq - s0);
-        total += of_lane(sum, n - 1);
+    if (tid < 64) {  // one wave looks the sequences up: every workgroup of the call reads the same lines
+        uint32_t total = 0, before = 0;
+        for (uint32_t s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
+            const uint32_t n = min(a.b.n_seqs - s0, 64u), v = lane < n ? seq_units<ROWS>(a, s0 + lane).units : 0, sum = wave_scan(v, lane, n);
+            if (seq - s0 < 64) before = total + of_lane(sum - v, seq - s0);
+            total += of_lane(sum, n - 1);
+        }
+        if (lane == 0) found[0] = max(1u, (total + workgroups - 1) / workgroups), found[1] = before;
     }
-    const uint32_t per = max(1u, (total + workgroups - 1) / workgroups);
+    __syncthreads();
+    const uint32_t per = uniform(found[0]), before = uniform(found[1]);
     const uint32_t packed = (uint32_t)su.r.rows * a.group;
     // of its rows, gridDim.y at a time
     for (uint32_t tile = blockIdx.x % a.tiles, row = blockIdx.y; tile < su.tiles; row += gridDim.y) {
@@ -665,8 +670,15 @@ __global__ __launch_bounds__(256) void k_attention_few_join(AttnArgs a, uint32_t
 #pragma unroll
             for (int k = 0; k < kEarly; ++k)
                 if (group + k * groups < n) acc += early[k] * factor[group + k * groups];
-#pragma unroll 16
-            for (uint32_t i = group + kEarly * groups; i < n; i += groups) acc += *reinterpret_cast<const float4v*>(part(i) + d) * factor[i];
+            // whole batches, the last one's too: a loop's remainder would wait for one part after another
+            for (uint32_t i = group + kEarly * groups; i < n; i += kBatch * groups) {
+                float4v v[kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) v[k] = *reinterpret_cast<const float4v*>(part(min(i + k * groups, n - 1)) + d);
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k)
+                    if (i + k * groups < n) acc += v[k] * factor[i + k * groups];
+            }
         }
         acc_of[tid] = acc;
         __syncthreads();
