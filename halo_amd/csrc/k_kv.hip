@@ -124,7 +124,9 @@ __device__ void write_part(const KvWriteArgs& a, const PagePart& p, uint32_t whi
     typedef std::conditional_t<V == 1, uint64_t, uint32_t> Offset;  // wide rows are at most 2^22 elements apart
     const KvLayer& c = a.c;
     const uint32_t tid = threadIdx.x, dim = c.dim, vecs = dim / V, at_once = kKvBlock / vecs;
-    const uint32_t d = tid % vecs * V, mine_first = tid / vecs;
+    // V's words of 4 tokens lie side by side along the tokens: 8 lanes along a row, then up to 8 groups of tokens
+    const uint32_t beside = which ? min(at_once & -at_once, 8u) : 1, rest = tid / 8 / beside;
+    const uint32_t d = (rest % (vecs / 8) * 8 + tid % 8) * V, mine_first = rest / (vecs / 8) * beside + tid / 8 % beside;
     const T* x = static_cast<const T*>(a.x[which].data) + (uint64_t)p.row * a.x[which].stride + head * a.x[which].head_stride;
     const Offset stride = (Offset)a.x[which].stride;
     // groups of 4 tokens, aligned in the page, that the part touches
