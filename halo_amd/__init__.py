@@ -4,8 +4,9 @@ IQ4_XS).
 The compute path is hand-written HIP for gfx950 in ``libhalo_mi355x.so``, reached through the
 C ABI declared in ``include/halo_mi355x.h``. This package loads that library with ctypes and
 mirrors the reference's operator interface for the path (``Backend::gemv`` over
-``GemvArgs``; include/halo/backend/backend.h:283-314, :562). There is no CPU fallback: if the
-library is missing every entry point raises.
+``GemvArgs``; include/halo/backend/backend.h:283-314, :562). Beside it stand rotary positions, an
+8-bit paged cache and the attention over it (``rope``, ``kv_*``, ``attention``). There is no CPU
+fallback: if the library is missing every entry point raises.
 """
 from __future__ import annotations
 

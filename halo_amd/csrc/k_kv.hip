@@ -6,8 +6,13 @@
 // page holds already move to the new scale. Codes are the nearest integers to x / scale exactly (ties to even).
 //
 // One workgroup owns one (page, K or V, head): nobody else touches its codes and scale. K rows are [token][dim], V
-// [dim][token]: a thread takes patches of 4 tokens by 16 bytes of a row, which are whole words of V's codes, and keeps
-// them in registers from the maximum to the codes, so that x is read once.
+// [dim][token]: a thread takes patches of 4 tokens by 4 elements of a row, which are whole words of V's codes, and keeps
+// them in registers from the maximum to the codes, so that x is read once. V's threads lie along the tokens, so that
+// their words join into whole lines (17.6 us against 18.7 with threads along the dims).
+//
+// Bound by memory: 7 bf16 prompts of 201 to 2100 rows, 8 heads of 128, written in 17.6 us (56 MB, 3.2 TB/s: the chain of
+// lengths, rows, maximum and codes of a workgroup shows, as 2300 workgroups are not much more than fit at once) and read
+// back in 18.2 (94 MB, 5.2 TB/s); 61 sequences' single tokens 5.4 and 5.8 us, one launch each.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

