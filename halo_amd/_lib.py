@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import enum
 import functools
+import struct
 import typing
 from pathlib import Path
 
@@ -193,59 +194,37 @@ class _RopeScaling(ctypes.Structure):
                 ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double)]
 
 
-class _RopePart(ctypes.Structure):
-    _fields_ = [("in_", ctypes.c_void_p), ("in_stride", ctypes.c_uint64), ("in_head_stride", ctypes.c_uint64),
-                ("out", ctypes.c_void_p), ("out_stride", ctypes.c_uint64), ("out_head_stride", ctypes.c_uint64),
-                ("n_heads", ctypes.c_uint32)]
+class _Layout:
+    """A parameter block of the C ABI as one struct.pack: these calls are made hundreds of times a step, and a decode step's
+    kernels take less time than filling a ctypes.Structure field by field (a rope call of one token: 7.0 us, packed 5.6)."""
+
+    def __init__(self, *parts: str):
+        packer = struct.Struct("@" + "".join(parts))
+        self.pack_into, self.buffer = packer.pack_into, ctypes.c_char * packer.size
+
+    def __call__(self, *values):
+        out = self.buffer()
+        try:
+            self.pack_into(out, 0, *values)
+        except (struct.error, OverflowError) as e:
+            raise HaloError(ErrorCode.Kernel, f"an argument is out of range or of the wrong kind: {e}") from None
+        return out
 
 
-_RopeParts = _RopePart * 2
-
-
-class _RopeParams(ctypes.Structure):
-    _fields_ = [("type", ctypes.c_uint32), ("pairs", ctypes.c_uint32), ("parts", ctypes.POINTER(_RopePart)),
-                ("n_parts", ctypes.c_uint32), ("n_tokens", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
-                ("rot_dims", ctypes.c_uint32), ("positions", ctypes.c_void_p), ("freqs", ctypes.c_void_p),
-                ("factor", ctypes.c_float)]
-
-
-class _KvCache(ctypes.Structure):
-    _fields_ = [("pool", ctypes.c_void_p), ("n_pages", ctypes.c_uint32), ("n_layers", ctypes.c_uint32),
-                ("n_kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("block_tokens", ctypes.c_uint32)]
-
-
-class _KvBatch(ctypes.Structure):
-    _fields_ = [("tables", ctypes.c_void_p), ("table_stride", ctypes.c_uint64), ("table_width", ctypes.c_uint32),
-                ("kv_lens", ctypes.c_void_p), ("row_starts", ctypes.c_void_p), ("n_seqs", ctypes.c_uint32),
-                ("n_rows", ctypes.c_uint32), ("max_rows", ctypes.c_uint32), ("max_kv", ctypes.c_uint32)]
-
-
-class _KvWriteParams(ctypes.Structure):
-    _fields_ = [("type", ctypes.c_uint32), ("cache", _KvCache), ("layer", ctypes.c_uint32), ("batch", _KvBatch),
-                ("k", ctypes.c_void_p), ("k_stride", ctypes.c_uint64), ("k_head_stride", ctypes.c_uint64),
-                ("v", ctypes.c_void_p), ("v_stride", ctypes.c_uint64), ("v_head_stride", ctypes.c_uint64),
-                ("status", ctypes.c_void_p), ("status_keep", ctypes.c_uint32)]
-
-
-class _KvReadParams(ctypes.Structure):
-    _fields_ = [("cache", _KvCache), ("layer", ctypes.c_uint32), ("batch", _KvBatch),
-                ("k_out", ctypes.c_void_p), ("k_stride", ctypes.c_uint64), ("k_head_stride", ctypes.c_uint64),
-                ("v_out", ctypes.c_void_p), ("v_stride", ctypes.c_uint64), ("v_head_stride", ctypes.c_uint64),
-                ("status", ctypes.c_void_p), ("status_keep", ctypes.c_uint32)]
-
-
-class _AttentionParams(ctypes.Structure):
-    _fields_ = [("type", ctypes.c_uint32), ("cache", _KvCache), ("layer", ctypes.c_uint32), ("batch", _KvBatch),
-                ("q", ctypes.c_void_p), ("q_stride", ctypes.c_uint64), ("q_head_stride", ctypes.c_uint64),
-                ("out", ctypes.c_void_p), ("out_stride", ctypes.c_uint64), ("out_head_stride", ctypes.c_uint64),
-                ("n_heads", ctypes.c_uint32), ("scale", ctypes.c_float), ("window", ctypes.c_uint32),
-                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
-                ("status", ctypes.c_void_p), ("status_keep", ctypes.c_uint32)]
-
-
-class _KvState(ctypes.Structure):
-    _fields_ = [("refs", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("tables", ctypes.c_void_p),
-                ("table_stride", ctypes.c_uint64), ("table_width", ctypes.c_uint32), ("n_slots", ctypes.c_uint32)]
+# Members in the order of halo_mi355x.h, padded as C pads them (P: pointer, Q: uint64, I: uint32, f: float).
+_ROWS = "PQQ"  # data, stride, head stride
+_CACHE = "P5I4x"  # pool, n_pages, n_layers, n_kv_heads, head_dim, block_tokens
+_BATCH = "PQI4xPP4I"  # tables, stride, width, kv_lens, row_starts, n_seqs, n_rows, max_rows, max_kv
+_STATUS = "PI4x"  # status, status_keep
+_ROPE_PART = _ROWS + _ROWS + "I4x"  # in, out, n_heads
+_rope_params = _Layout(_ROPE_PART, _ROPE_PART, "IIPIIIIPPf4x")  # the two parts, then halo_mi_rope_params
+_POINTER = struct.Struct("@P")
+_ROPE_PARAMS_AT = 2 * struct.calcsize("@" + _ROPE_PART)
+_kv_write_params = _Layout("I4x", _CACHE, "I4x", _BATCH, _ROWS, _ROWS, _STATUS)
+_kv_read_params = _Layout(_CACHE, "I4x", _BATCH, _ROWS, _ROWS, _STATUS)
+_attention_block = _Layout("I4x", _CACHE, "I4x", _BATCH, _ROWS, _ROWS, "IfI4xPQ", _STATUS)
+_cache_block = _Layout(_CACHE)
+_state_block = _Layout("PPPQII")
 
 
 ARGMAX_RESULT_BYTES = 12  # HALO_MI_ARGMAX_RESULT_BYTES: {index, value bits, poisoned} per vector
@@ -271,16 +250,16 @@ SIGNATURES = {
     "halo_mi_get_rows": (_INT, [ctypes.POINTER(_GetRowsParams), _VP]),
     "halo_mi_rms_norm": (_INT, [_VP, _U64, _VP, _VP, _U64, _U32, _U32, ctypes.c_float, _VP]),
     "halo_mi_rope_freqs": (_INT, [_U32, ctypes.c_double, ctypes.POINTER(_RopeScaling), _VP, ctypes.POINTER(ctypes.c_float)]),
-    "halo_mi_rope": (_INT, [ctypes.POINTER(_RopeParams), _VP]),
+    "halo_mi_rope": (_INT, [_VP, _VP]),
     "halo_mi_kv_page_bytes": (_U64, [_U32, _U32, _U32, _U32]),
-    "halo_mi_kv_write": (_INT, [ctypes.POINTER(_KvWriteParams), _VP]),
-    "halo_mi_kv_read": (_INT, [ctypes.POINTER(_KvReadParams), _VP]),
-    "halo_mi_attention": (_INT, [ctypes.POINTER(_AttentionParams), _VP]),
-    "halo_mi_attention_workspace": (_U64, [ctypes.POINTER(_AttentionParams)]),
-    "halo_mi_kv_resize": (_INT, [ctypes.POINTER(_KvCache), ctypes.POINTER(_KvState), _VP, _VP, _U32, _VP, _U32, _VP]),
-    "halo_mi_kv_fork": (_INT, [ctypes.POINTER(_KvCache), ctypes.POINTER(_KvState), _VP, _VP, _U32, _VP, _U32, _VP]),
-    "halo_mi_kv_compact": (_INT, [ctypes.POINTER(_KvCache), ctypes.POINTER(_KvState), _VP, _VP]),
-    "halo_mi_kv_copy_pages": (_INT, [ctypes.POINTER(_KvCache), _VP, _VP, _U32, _VP, _U32, _VP]),
+    "halo_mi_kv_write": (_INT, [_VP, _VP]),
+    "halo_mi_kv_read": (_INT, [_VP, _VP]),
+    "halo_mi_attention": (_INT, [_VP, _VP]),
+    "halo_mi_attention_workspace": (_U64, [_VP]),
+    "halo_mi_kv_resize": (_INT, [_VP, _VP, _VP, _VP, _U32, _VP, _U32, _VP]),
+    "halo_mi_kv_fork": (_INT, [_VP, _VP, _VP, _VP, _U32, _VP, _U32, _VP]),
+    "halo_mi_kv_compact": (_INT, [_VP, _VP, _VP, _VP]),
+    "halo_mi_kv_copy_pages": (_INT, [_VP, _VP, _VP, _U32, _VP, _U32, _VP]),
     "halo_mi_stream_read": (_INT, [_VP, _U64, _U32, _U32, _VP, _VP]),
     "halo_mi_stream_check": (_INT, [_VP]),
     "halo_mi_stream_release": (_INT, [_VP]),
@@ -586,25 +565,18 @@ def _dev(t, dev: int) -> int:
     return t.data_ptr()
 
 
-def _block(cls, *values):
-    """A parameter block. Integers of other kinds (numpy's) are converted where there are any."""
-    try:
-        return cls(*values)
-    except TypeError:
-        return cls(*(int(v) if hasattr(v, "__index__") else v for v in values))
+def _cache(c: KvCache, dev: int) -> tuple:
+    return (_dev(c[0], dev), *c[1:])
 
 
-def _cache(c: KvCache, dev: int) -> _KvCache:
-    return _block(_KvCache, _dev(c.pool, dev), c.n_pages, c.n_layers, c.n_kv_heads, c.head_dim, c.block_tokens)
+def _batch(b: KvBatch, dev: int) -> tuple:
+    tables, width, kv_lens, row_starts, n_seqs, n_rows, max_rows, max_kv, stride = b
+    return _dev(tables, dev), stride, width, _dev(kv_lens, dev), _dev(row_starts, dev), n_seqs, n_rows, max_rows, max_kv
 
 
-def _batch(b: KvBatch, dev: int) -> _KvBatch:
-    return _block(_KvBatch, _dev(b.tables, dev), b.table_stride, b.table_width, _dev(b.kv_lens, dev), _dev(b.row_starts, dev), b.n_seqs, b.n_rows,
-                    b.max_rows, b.max_kv)
-
-
-def _state(s: KvState, dev: int) -> _KvState:
-    return _block(_KvState, _dev(s.refs, dev), _dev(s.lens, dev), _dev(s.tables, dev), s.table_stride, s.table_width, s.n_slots)
+def _state(s: KvState, dev: int):
+    refs, lens, tables, n_slots, width, stride = s
+    return _state_block(_dev(refs, dev), _dev(lens, dev), _dev(tables, dev), stride, width, n_slots)
 
 
 def rope_freqs(rot_dims: int, theta: float = 10000.0, *, scaling: int = RopeScaling.PLAIN, scale: float = 1.0,
@@ -627,12 +599,12 @@ def rope(t: int, positions, freqs, n_tokens: int, head_dim: int, rot_dims: int, 
     """PARTIAL_ROPE of q and, with k, of k in one launch (halo_mi_rope). q_out may be q, k_out may be k. positions:
     int32, freqs: float64 radians per position (rope_freqs), both on the device; strides in elements."""
     dev = _current_device()
-    parts = _RopeParts(
-        _block(_RopePart, _dev(q, dev), q_stride, q_head_stride, _dev(q_out, dev), q_out_stride, q_out_head_stride, n_heads),
-        _block(_RopePart, _dev(k, dev), k_stride, k_head_stride, _dev(k_out, dev), k_out_stride, k_out_head_stride, n_kv_heads))
-    p = _block(_RopeParams, t, pairs, parts, 1 if k is None else 2, n_tokens, head_dim, rot_dims, _dev(positions, dev),
-                    _dev(freqs, dev), factor)
-    _check(lib().halo_mi_rope(ctypes.byref(p), _raw_stream(stream, dev)))
+    p = _rope_params(_dev(q, dev), q_stride, q_head_stride, _dev(q_out, dev), q_out_stride, q_out_head_stride, n_heads,
+                     _dev(k, dev), k_stride, k_head_stride, _dev(k_out, dev), k_out_stride, k_out_head_stride, n_kv_heads,
+                     t, pairs, 0, 1 if k is None else 2, n_tokens, head_dim, rot_dims, _dev(positions, dev), _dev(freqs, dev), factor)
+    at = ctypes.addressof(p)
+    _POINTER.pack_into(p, _ROPE_PARAMS_AT + 8, at)  # halo_mi_rope_params.parts
+    _check(lib().halo_mi_rope(at + _ROPE_PARAMS_AT, _raw_stream(stream, dev)))
 
 
 def kv_page_bytes(n_layers: int, n_kv_heads: int, head_dim: int, block_tokens: int) -> int:
@@ -644,27 +616,27 @@ def kv_write(t: int, cache: KvCache, layer: int, batch: KvBatch, k, v, *, k_stri
              v_stride: int = 0, v_head_stride: int = 0, status=None, status_keep: bool = False, stream=None) -> None:
     """KV_WRITE: the batch's rows of k and v into their sequences' pages (halo_mi_kv_write)."""
     dev = _current_device()
-    p = _block(_KvWriteParams, t, _cache(cache, dev), layer, _batch(batch, dev), _dev(k, dev), k_stride, k_head_stride, _dev(v, dev),
-                       v_stride, v_head_stride, _dev(status, dev), 1 if status_keep else 0)
-    _check(lib().halo_mi_kv_write(ctypes.byref(p), _raw_stream(stream, dev)))
+    p = _kv_write_params(t, *_cache(cache, dev), layer, *_batch(batch, dev), _dev(k, dev), k_stride, k_head_stride, _dev(v, dev),
+                         v_stride, v_head_stride, _dev(status, dev), 1 if status_keep else 0)
+    _check(lib().halo_mi_kv_write(p, _raw_stream(stream, dev)))
 
 
 def kv_read(cache: KvCache, layer: int, batch: KvBatch, k_out=None, v_out=None, *, k_stride: int = 0, k_head_stride: int = 0,
             v_stride: int = 0, v_head_stride: int = 0, status=None, status_keep: bool = False, stream=None) -> None:
     """The values that the cache holds for the batch's rows, in fp32 (halo_mi_kv_read)."""
     dev = _current_device()
-    p = _block(_KvReadParams, _cache(cache, dev), layer, _batch(batch, dev), _dev(k_out, dev), k_stride, k_head_stride, _dev(v_out, dev),
-                      v_stride, v_head_stride, _dev(status, dev), 1 if status_keep else 0)
-    _check(lib().halo_mi_kv_read(ctypes.byref(p), _raw_stream(stream, dev)))
+    p = _kv_read_params(*_cache(cache, dev), layer, *_batch(batch, dev), _dev(k_out, dev), k_stride, k_head_stride, _dev(v_out, dev),
+                        v_stride, v_head_stride, _dev(status, dev), 1 if status_keep else 0)
+    _check(lib().halo_mi_kv_read(p, _raw_stream(stream, dev)))
 
 
 def _attention_params(t, cache, layer, batch, q, out, n_heads, scale, window, q_stride, q_head_stride, out_stride, out_head_stride,
                       workspace, workspace_bytes, status, status_keep, dev):
     if workspace is not None and not isinstance(workspace, int) and not workspace_bytes:
         workspace_bytes = workspace.numel() * workspace.element_size()
-    return _block(_AttentionParams, t, _cache(cache, dev), layer, _batch(batch, dev), _dev(q, dev), q_stride, q_head_stride, _dev(out, dev),
-                            out_stride, out_head_stride, n_heads, scale, window, _dev(workspace, dev),
-                            workspace_bytes, _dev(status, dev), 1 if status_keep else 0)
+    return _attention_block(t, *_cache(cache, dev), layer, *_batch(batch, dev), _dev(q, dev), q_stride, q_head_stride, _dev(out, dev),
+                            out_stride, out_head_stride, n_heads, scale, window, _dev(workspace, dev), workspace_bytes,
+                            _dev(status, dev), 1 if status_keep else 0)
 
 
 def attention(t: int, cache: KvCache, layer: int, batch: KvBatch, q, out, n_heads: int, *, scale: float = 0.0, window: int = 0,
@@ -675,7 +647,7 @@ def attention(t: int, cache: KvCache, layer: int, batch: KvBatch, q, out, n_head
     dev = _current_device()
     p = _attention_params(t, cache, layer, batch, q, out, n_heads, scale, window, q_stride, q_head_stride, out_stride, out_head_stride,
                           workspace, workspace_bytes, status, status_keep, dev)
-    _check(lib().halo_mi_attention(ctypes.byref(p), _raw_stream(stream, dev)))
+    _check(lib().halo_mi_attention(p, _raw_stream(stream, dev)))
 
 
 def attention_workspace(t: int, cache: KvCache, layer: int, batch: KvBatch, q, out, n_heads: int, *, window: int = 0,
@@ -684,37 +656,37 @@ def attention_workspace(t: int, cache: KvCache, layer: int, batch: KvBatch, q, o
     dev = _current_device()
     p = _attention_params(t, cache, layer, batch, q, out, n_heads, 0.0, window, q_stride, q_head_stride, out_stride, out_head_stride,
                           None, 0, None, False, dev)
-    return int(lib().halo_mi_attention_workspace(ctypes.byref(p)))
+    return int(lib().halo_mi_attention_workspace(p))
 
 
 def kv_resize(cache: KvCache, state: KvState, slots, new_lens, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
     """Gives slots their new lengths, with pages taken and released (halo_mi_kv_resize); length 0 frees a slot."""
     dev = _current_device()
-    c, s = _cache(cache, dev), _state(state, dev)
-    _check(lib().halo_mi_kv_resize(ctypes.byref(c), ctypes.byref(s), _dev(slots, dev), _dev(new_lens, dev), n, _dev(status, dev),
+    c, s = _cache_block(*_cache(cache, dev)), _state(state, dev)
+    _check(lib().halo_mi_kv_resize(c, s, _dev(slots, dev), _dev(new_lens, dev), n, _dev(status, dev),
                                    1 if status_keep else 0, _raw_stream(stream, dev)))
 
 
 def kv_fork(cache: KvCache, state: KvState, src, dst, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
     """Empty slots dst become copies of src: whole pages shared, a last one that is not full copied (halo_mi_kv_fork)."""
     dev = _current_device()
-    c, s = _cache(cache, dev), _state(state, dev)
-    _check(lib().halo_mi_kv_fork(ctypes.byref(c), ctypes.byref(s), _dev(src, dev), _dev(dst, dev), n, _dev(status, dev),
+    c, s = _cache_block(*_cache(cache, dev)), _state(state, dev)
+    _check(lib().halo_mi_kv_fork(c, s, _dev(src, dev), _dev(dst, dev), n, _dev(status, dev),
                                  1 if status_keep else 0, _raw_stream(stream, dev)))
 
 
 def kv_compact(cache: KvCache, state: KvState, *, live=None, stream=None) -> None:
     """Moves the live pages to the front of the pool (halo_mi_kv_compact); live (uint32 or int32) receives their number."""
     dev = _current_device()
-    c, s = _cache(cache, dev), _state(state, dev)
-    _check(lib().halo_mi_kv_compact(ctypes.byref(c), ctypes.byref(s), _dev(live, dev), _raw_stream(stream, dev)))
+    c, s = _cache_block(*_cache(cache, dev)), _state(state, dev)
+    _check(lib().halo_mi_kv_compact(c, s, _dev(live, dev), _raw_stream(stream, dev)))
 
 
 def kv_copy_pages(cache: KvCache, src, dst, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
     """Copies whole pages (halo_mi_kv_copy_pages)."""
     dev = _current_device()
-    c = _cache(cache, dev)
-    _check(lib().halo_mi_kv_copy_pages(ctypes.byref(c), _dev(src, dev), _dev(dst, dev), n, _dev(status, dev), 1 if status_keep else 0,
+    c = _cache_block(*_cache(cache, dev))
+    _check(lib().halo_mi_kv_copy_pages(c, _dev(src, dev), _dev(dst, dev), n, _dev(status, dev), 1 if status_keep else 0,
                                        _raw_stream(stream, dev)))
 
 

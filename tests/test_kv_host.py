@@ -213,3 +213,24 @@ def test_null_params(hl):
     assert lib.halo_mi_kv_compact(None, None, None, None) == hl.ErrorCode.Kernel
     assert lib.halo_mi_kv_copy_pages(None, None, None, 0, None, 0, None) == hl.ErrorCode.Kernel
     assert lib.halo_mi_rope_freqs(64, ctypes.c_double(1e4), None, None, None) == hl.ErrorCode.Kernel
+
+
+def test_kinds_of_numbers(hl):
+    """Any integer kind serves; one that does not fit its member, or is none, is refused and not wrapped."""
+    import numpy as np
+
+    K = hl.ErrorCode.Kernel
+    call = lambda n=0, dim=128, **kw: hl.rope(F32, A, B, n, dim, 64, C_, D, 4, stream=0, **kw)  # noqa: E731
+    call(np.int64(0), np.uint8(128), q_stride=np.int32(512), factor=np.float64(1.5))
+    for bad in (-1, 1 << 32, 1.5, "3", None):
+        refused(hl, K, call, n=bad)
+    refused(hl, K, call, q_stride=-512)
+    refused(hl, K, call, q_stride=1 << 64)
+    refused(hl, K, call, factor=1e39)
+    empty = _batch(hl, seqs=np.int64(0), rows=np.int32(0))
+    for name, f in _batched_calls(hl).items():
+        f(_cache(hl, pages=np.int64(10)), np.int16(1), empty)
+        refused(hl, K, f, _cache(hl, pages=-1), 0, empty)
+        refused(hl, K, f, _cache(hl), -1, empty)
+        refused(hl, K, f, _cache(hl), 0, _batch(hl, rows=-3))
+        refused(hl, K, f, _cache(hl), 0, _batch(hl, table_stride=-1))
