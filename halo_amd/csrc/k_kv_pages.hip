@@ -58,18 +58,25 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* lds, uint32
 
 struct OwnerLds {
     uint32_t scan[kOwnerWaves];
-    int32_t slots[kOwnerBlock];
+    __align__(16) int32_t slots[kOwnerBlock];
     uint32_t first[kOwnerBlock + 1];  // prefix sums of the entries' pages
     uint32_t column[kOwnerBlock];     // where an entry's first new page goes in its table
 };
 
-// Whether entry i is the first that names `slot` (every thread calls it).
+// Whether entry i is the first that names `slot` (every thread calls it). Four names a read and no way out of the loop, so
+// that the reads follow each other without a wait.
 __device__ __forceinline__ bool first_of_its_name(OwnerLds& l, int32_t slot, uint32_t i, uint32_t n) {
+    typedef int32_t int4v __attribute__((ext_vector_type(4)));
     l.slots[i] = slot;
     __syncthreads();
-    bool first = true;
-    for (uint32_t j = 0; j < min(i, n); ++j) first = first && l.slots[j] != slot;
-    return first;
+    bool seen = false;
+#pragma unroll 4
+    for (uint32_t j = 0; j < n; j += 4) {
+        const int4v name = *reinterpret_cast<const int4v*>(&l.slots[j]);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) seen |= (name[k] == slot) & (j + k < i);
+    }
+    return !seen;
 }
 
 // The lowest min(want, all) free pages, in order, to `list`; returns how many.
