@@ -122,13 +122,14 @@ __device__ __forceinline__ uint32_t peak_bits(uint32_t top) {
 }
 
 // V: elements per load of a K or V row, 4 or 1. KEEP: patches per thread that stay in registers between the maximum and
-// the codes; a part with more is read again. A thread has one place of `vecs` in a row and every `at_once`-th group of
-// 4 tokens.
-template <typename T, int V, int KEEP>
+// the codes; a part with more is read again. THREADS: of the workgroup, as few as have a whole page's patches between them,
+// so that more pages of 16 tokens are under way at once. A thread has one place of `vecs` in a row and every `at_once`-th
+// group of 4 tokens.
+template <typename T, int V, int KEEP, uint32_t THREADS>
 __device__ void write_part(const KvWriteArgs& a, const PagePart& p, uint32_t which, uint32_t head, uint32_t* lds) {
     typedef std::conditional_t<V == 1, uint64_t, uint32_t> Offset;  // wide rows are at most 2^22 elements apart
     const KvLayer& c = a.c;
-    const uint32_t tid = threadIdx.x, dim = c.dim, vecs = dim / V, at_once = kKvBlock / vecs;
+    const uint32_t tid = threadIdx.x, dim = c.dim, vecs = dim / V, at_once = min(THREADS / vecs, c.block / 4);
     // V's words of 4 tokens lie side by side along the tokens: 8 lanes along a row, then up to 8 groups of tokens
     const uint32_t beside = which ? min(at_once & -at_once, 8u) : 1, rest = tid / 8 / beside;
     const uint32_t d = (rest % (vecs / 8) * 8 + tid % 8) * V, mine_first = rest / (vecs / 8) * beside + tid / 8 % beside;
@@ -173,7 +174,9 @@ __device__ void write_part(const KvWriteArgs& a, const PagePart& p, uint32_t whi
     for (int off = 1; off < 64; off <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
     if (tid % 64 == 0) lds[tid / 64] = top;
     __syncthreads();  // every thread has s0, too
-    top = max(max(lds[0], lds[1]), max(lds[2], lds[3]));
+    top = lds[0];
+#pragma unroll
+    for (uint32_t w = 1; w < THREADS / 64; ++w) top = max(top, lds[w]);
     const float fit = __uint_as_float(top) / 127.0f;
     float s1 = fit < kKvMinScale ? s0 : fmaxf(s0, fit);
     if (top > kLargestFinite || s0 != s0) s1 = __uint_as_float(0x7FC00000u);
@@ -183,7 +186,7 @@ __device__ void write_part(const KvWriteArgs& a, const PagePart& p, uint32_t whi
     if (p.off && s1 > s0 && s0 > 0.0f) {  // the scale grew: the earlier tokens' codes follow
         const uint32_t per = which ? (p.off + 3) / 4 : p.off * dim / 4;  // words of a dim of V; of K
         const uint32_t rows = which ? dim : 1;
-        for (uint32_t i = tid; i < per * rows; i += kKvBlock) {
+        for (uint32_t i = tid; i < per * rows; i += THREADS) {
             uint32_t* w = words + i / per * (c.block / 4) + i % per;
             const uint32_t keep = !which || i % per * 4 + 4 <= p.off ? 0u : 0xFFFFFFFFu << 8 * (p.off % 4);
             uint32_t word = *w & keep;
@@ -250,40 +253,41 @@ __device__ void write_part(const KvWriteArgs& a, const PagePart& p, uint32_t whi
     }
 }
 
-template <typename T, int V, int KEEP>
-__global__ __launch_bounds__(kKvBlock) void k_kv_write(KvWriteArgs a) {
-    __shared__ uint32_t lds[kKvBlock / 64];
+template <typename T, int V, int KEEP, uint32_t THREADS>
+__global__ __launch_bounds__(THREADS) void k_kv_write(KvWriteArgs a) {
+    __shared__ uint32_t lds[THREADS / 64];
     const uint32_t s = blockIdx.z, head = blockIdx.y >> 1, which = blockIdx.y & 1;
     const SeqRows r = seq_rows(a.b, s);
     PagePart p;
     for (uint32_t j = blockIdx.x; page_part(a.b, a.c, s, r, j, p); j += gridDim.x) {
-        write_part<T, V, KEEP>(a, p, which, head, lds);
+        write_part<T, V, KEEP, THREADS>(a, p, which, head, lds);
         __syncthreads();
     }
 }
 
 __global__ __launch_bounds__(kKvBlock) void k_kv_read(KvReadArgs a) {
+    const uint32_t threads = blockDim.x;  // a page's 16 tokens of a dim each, up to kKvBlock
     const uint32_t s = blockIdx.z, head = blockIdx.y >> 1, which = blockIdx.y & 1, dim = a.c.dim;
     if (!a.out[which].data) return;
     const SeqRows r = seq_rows(a.b, s);
     float* out = const_cast<float*>(static_cast<const float*>(a.out[which].data)) + head * a.out[which].head_stride;
     const uint64_t stride = a.out[which].stride;
     if (r.len < r.rows)  // rows before position 0
-        for (uint64_t i = blockIdx.x * kKvBlock + threadIdx.x; i < (uint64_t)(r.rows - r.len) * dim; i += gridDim.x * kKvBlock)
+        for (uint64_t i = blockIdx.x * threads + threadIdx.x; i < (uint64_t)(r.rows - r.len) * dim; i += gridDim.x * threads)
             out[(r.row0 + i / dim) * stride + i % dim] = 0.0f;
     PagePart p;
     for (uint32_t j = blockIdx.x; page_part(a.b, a.c, s, r, j, p); j += gridDim.x) {
         float* o = out + (uint64_t)p.row * stride;
         if (p.page < 0) {
             if (threadIdx.x == 0) set_status(a.status, kStatusKvBadIndex);
-            for (uint32_t i = threadIdx.x; i < p.n * dim; i += kKvBlock) o[i / dim * stride + i % dim] = __uint_as_float(0x7FC00000u);
+            for (uint32_t i = threadIdx.x; i < p.n * dim; i += threads) o[i / dim * stride + i % dim] = __uint_as_float(0x7FC00000u);
             continue;
         }
         const uint8_t* page = page_ptr(a.c, p.page);
         const uint8_t* codes = page + a.c.codes + (which * a.c.heads + head) * a.c.plane;
         const float scale = reinterpret_cast<const float*>(page + a.c.scales)[which * a.c.heads + head];
         if (which == 0) {
-            for (uint32_t i = threadIdx.x; i < p.n * dim / 4; i += kKvBlock) {
+            for (uint32_t i = threadIdx.x; i < p.n * dim / 4; i += threads) {
                 const uint32_t word = reinterpret_cast<const uint32_t*>(codes + p.off * dim)[i];
                 float* to = o + i / (dim / 4) * stride + i % (dim / 4) * 4;
 #pragma unroll
@@ -292,7 +296,7 @@ __global__ __launch_bounds__(kKvBlock) void k_kv_read(KvReadArgs a) {
             continue;
         }
         const uint32_t g0 = p.off / 16, g1 = (p.off + p.n + 15) / 16;
-        for (uint32_t i = threadIdx.x; i < (g1 - g0) * dim; i += kKvBlock) {
+        for (uint32_t i = threadIdx.x; i < (g1 - g0) * dim; i += threads) {
             const uint32_t d = i % dim, t0 = (g0 + i / dim) * 16;
             const uint4 w = *reinterpret_cast<const uint4*>(codes + d * a.c.block + t0);
             const uint32_t word[4] = {w.x, w.y, w.z, w.w};
@@ -316,10 +320,19 @@ int launch_write_typed(const KvWriteArgs& a, hipStream_t st) {
     bool wide = true;
     for (const HeadRows& r : a.x)
         wide = wide && reinterpret_cast<uintptr_t>(r.data) % (V * sizeof(T)) == 0 && r.stride % V == 0 && r.head_stride % V == 0 && r.stride <= 1u << 22;
-    // groups of 4 tokens of a page per thread
-    const uint32_t at_once = kKvBlock / (a.c.dim / V), each = (a.c.block / 4 + at_once - 1) / at_once;
-    auto* k = !wide ? k_kv_write<T, 1, 4> : each <= 1 ? k_kv_write<T, V, 1> : each <= 2 ? k_kv_write<T, V, 2> : each <= 4 ? k_kv_write<T, V, 4> : k_kv_write<T, V, 8>;
-    hipLaunchKernelGGL(k, page_grid(a.c, a.b), dim3(kKvBlock), 0, st, a);
+    // Up to two patches of a page per thread in small workgroups: 7 bf16 prompts of 200 to 2000 rows, 8 heads, pages of 16 tokens,
+    // written and read back at 64 / 128 / 256 dims in 24 / 32.7 / 56 us, against 32 / 39 / 62 with 256 threads (the reads
+    // alike). Larger pages are written faster by 256: pages of 64 tokens at 128 dims 35.9 against 37.4 with 128.
+    const uint32_t patches = a.c.block / 4 * (a.c.dim / V), at_once = kKvBlock / (a.c.dim / V);
+    const uint32_t each = (a.c.block / 4 + at_once - 1) / at_once;  // patches of a page per thread of 256
+    uint32_t threads = kKvBlock;
+    void (*k)(KvWriteArgs);
+    if (!wide) k = k_kv_write<T, 1, 4, kKvBlock>;
+    else if (patches <= 64) k = k_kv_write<T, V, 1, 64>, threads = 64;
+    else if (patches <= 128) k = k_kv_write<T, V, 2, 64>, threads = 64;
+    else if (patches <= 256) k = k_kv_write<T, V, 2, 128>, threads = 128;
+    else k = each <= 2 ? k_kv_write<T, V, 2, kKvBlock> : each <= 4 ? k_kv_write<T, V, 4, kKvBlock> : k_kv_write<T, V, 8, kKvBlock>;
+    hipLaunchKernelGGL(k, page_grid(a.c, a.b), dim3(threads), 0, st, a);
     return hip_status(hipGetLastError(), "KV_WRITE");
 }
 
@@ -334,7 +347,8 @@ int launch_kv_write(uint32_t type, const KvWriteArgs& a, hipStream_t st) {
 }
 
 int launch_kv_read(const KvReadArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(k_kv_read, page_grid(a.c, a.b), dim3(kKvBlock), 0, st, a);
+    const uint32_t threads = std::min(kKvBlock, (a.c.dim * a.c.block / 16 + 63) / 64 * 64);
+    hipLaunchKernelGGL(k_kv_read, page_grid(a.c, a.b), dim3(threads), 0, st, a);
     return hip_status(hipGetLastError(), "kv_read");
 }
 
