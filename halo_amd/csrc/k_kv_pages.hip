@@ -7,8 +7,8 @@
 // pages' bytes (hundreds of KB each with all layers) and long tables: a second kernel copies them with the whole GPU,
 // from lists that the first one leaves in scratch memory.
 //
-// Measured: 8 sequences forked 8 ways over 1300 pages, deciding 10.0 us (a chain of scans and reads) and copying 6.2; grown
-// 8.1 and 2.0; a pool of 1500 pages packed, 186 MB of pages read and written, 5.0 and 33.7 (5.5 TB/s).
+// Measured: 8 sequences forked 8 ways over 1300 pages, deciding 7.4 us (a chain of scans and reads) and copying 6.1; grown
+// 5.4 and 2.0; a pool of 1500 pages packed, 186 MB of pages read and written, 5.0 and 33.7 (5.5 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
