@@ -1241,7 +1241,9 @@ uint64_t plan_many(AttnArgs& a, uint64_t part_bytes) {
     uint64_t span = a.b.max_kv;
     if (a.window) span = std::min<uint64_t>(span, (uint64_t)a.window + rows / a.group + kStep);
     const uint64_t each = (uint64_t)a.b.n_rows * a.heads * (a.c.dim + 4) * sizeof(float);
-    a.splits = (uint32_t)std::max<uint64_t>(1, std::min({want / groups, (span + 4 * kStep - 1) / (4 * kStep), part_bytes / each}));
+    // a split has three steps at least: with two, 94 rows of 16 heads over 2500 tokens take 18.9 us against 18.0, with four 60 rows
+    // of 12 heads over 600 tokens 25.6 against 24.4
+    a.splits = (uint32_t)std::max<uint64_t>(1, std::min({want / groups, (span + 3 * kStep - 1) / (3 * kStep), part_bytes / each}));
     if ((uint64_t)a.b.n_rows * a.heads > 4 * kMaxGrid) a.splits = 1;  // the join's grid (rows behind the last sequence count)
     return a.splits > 1 ? a.splits * each : 0;
 }
