@@ -563,7 +563,7 @@ int halo_mi_kv_read(const halo_mi_kv_read_params* p, void* stream);
  * a multiple of n_kv_heads. A row of q that is not finite, and a row that sees a NaN block or a page out of
  * range, is NaN; tokens that a row does not see never reach it, whatever their bytes are.
  * Numerics: the codes are exact in the products; q and the softmax weights are rounded to 11 bits for 16-bit types (q
- * exactly, but for elements under 2^-28 of their row's largest), and carried in two pieces, to within 2^-22,
+ * exactly, but for elements under 2^-28 of their row's largest and for rows all under 2^-112), and carried in two pieces, to within 2^-22,
  * for fp32; sums and the softmax are in fp32.
  *   scale: 0 = 1 / sqrt(head_dim).
  *   workspace (optional, 16-byte aligned): workspace_bytes of device memory for the partial results of long
