@@ -101,6 +101,21 @@ def test_long(hl, dev, t, dim, rows, length, window):
     run(hl, dev, gpu, cache, tables, lens, np.array([rows, 1]), t, 3, q, window=window)
 
 
+@pytest.mark.parametrize("t", [F32, BF16], ids=lambda t: TYPE_NAMES[t])
+@pytest.mark.parametrize("seqs", [64, 65, 129, 300])
+def test_many_sequences(hl, dev, t, seqs):
+    """More sequences than a wave has lanes, empty ones among them, long ones split over several workgroups."""
+    print("[case] attention", TYPE_NAMES[t], seqs, "sequences", flush=True)
+    rng = np.random.default_rng(seqs)
+    rows, lens = rng.integers(0, 3, seqs), rng.integers(0, 40, seqs)
+    lens[rng.integers(0, seqs, 4)] = 1500
+    lens = np.maximum(lens, rows)
+    cache, tables, gpu = setup(hl, dev, rng, lens, 2, 64, 32)
+    q = rng.standard_normal((int(rows.sum()), 6, 64))
+    run(hl, dev, gpu, cache, tables, lens, rows, t, 6, q, max_rows=2, max_kv=1500)
+    run(hl, dev, gpu, cache, tables, lens, rows, t, 6, q)
+
+
 def test_launch_hints_are_only_hints(hl, dev):
     """max_rows and max_kv smaller than the truth: the same values."""
     rng = np.random.default_rng(2)
