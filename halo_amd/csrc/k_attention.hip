@@ -5,8 +5,9 @@
 // Products run on v_mfma_f32_16x16x32_f16. An int8 code is exact in f16, so K and V lose nothing; q, scaled per
 // row by a power of two to the top of f16's range, and the weights are one f16 piece (16-bit types) or two (fp32).
 // The scales stay out of the products: with x_t = s_t ks scale log2(e) + log2(vs), s_t = q . c_t, the weight of V's
-// codes is w_t = 2^(x_t - m), m a reference that follows the maximum of x_t, and the sum that divides is sum_t w_t / vs. One
-// multiply-add per score applies both scales, and w_t fits f16 whatever the blocks' scales are.
+// codes is w_t = 2^(x_t - m), m a reference that follows the maximum of x_t, and the sum that divides is sum_t w_t / vs (where
+// scales lie very far apart taken from the scores instead: sum_apart). One multiply-add per score applies both scales, and w_t fits f16
+// whatever the blocks' scales are.
 //
 // Layout of a step of 64 tokens (4 groups of 16, each inside one page since block_tokens is a multiple of 16). The
 // scores are computed transposed, S^T = K Q^T, 16 tokens a tile: tile a holds tokens 4 a .. 4 a + 3 of every
@@ -46,8 +47,15 @@ template <int NP>
 constexpr float kSlack = NP == 1 ? 7.5f : 1.5f;
 constexpr uint32_t kFewGrid = 768;      // workgroups of a call with few rows at most: three per CU
 constexpr float kTinyScale = 0x1p-80f;  // the scale that an all-zero block of V counts with
+// Once the largest weights are of blocks of V with a scale over 2^this, a wave takes its sums apart from its weights (sum_apart).
+constexpr float kFarLog2 = 10.0f;
 
 __device__ __forceinline__ float quiet_nan() { return __uint_as_float(0x7FC00000u); }
+
+// A value that the whole wave shares, as the scalar that the compiler cannot see it is; lane l's, l itself shared. Loop
+// bounds, pages' places and the mask's limits then stay out of the vector registers (36 bytes of scratch a lane, then none).
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ uint32_t of_lane(uint32_t v, uint32_t l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)l); }
 
 // max over the lanes of a column: lane, lane ^ 16, lane ^ 32, lane ^ 48
 __device__ __forceinline__ float column_max(float v) {
@@ -61,6 +69,12 @@ __device__ __forceinline__ float column_sum(float v) {
     v = __int_as_float(r[0]) + __int_as_float(r[1]);
     r = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
     return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+
+// l * 2^d, d <= 0 (NaN, of two references that are both -inf, counts as 0): the sums that divide span more powers of two
+// than one factor has.
+__device__ __forceinline__ float lowered(float l, float d) {
+    return l * __builtin_amdgcn_exp2f(fmaxf(d, -126.0f)) * __builtin_amdgcn_exp2f(fminf(d + 126.0f, 0.0f));
 }
 
 __device__ __forceinline__ void store_any(void* p, uint32_t type, uint64_t i, float v) {
@@ -197,21 +211,41 @@ __device__ __forceinline__ uint32_t seen_tokens(uint32_t tg, int32_t lo, int32_t
     return ((1u << to) - 1u) & ~((1u << from) - 1u);
 }
 
+// The sum that divides is of 2^(s k - m + shift): the weights' over V's scale, as long as no weight that it needs lies under fp32's
+// 2^-126. Scales are 2^-80 at least and the row's largest weight has 2^(shift - log2 vs) in the sum, so while its scale is under
+// 2^kFarLog2 what is lost is under 2^-44 of the sum a token. Else a lane sums its scores against their own largest and moves
+// the sum to the reference m (a block of V = 1.3e16 beside zeros, all scores alike: half of it, and not all). k is not negative.
+template <int NP, class Rows>
+__device__ __forceinline__ float sum_apart(const Rows& score, float k, float m, uint32_t seen) {
+    __asm__ volatile("" : "+v"(seen));  // masks are made where they are used: kept, they fill the scalar registers
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, seen >> i & 1 ? score(i) : -INFINITY);
+    const float base = top * k;
+    __asm__ volatile("" : "+v"(seen));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(seen >> i & 1 ? fmaf(score(i), k, -base) : -INFINITY);
+    const float half = __builtin_amdgcn_exp2f(0.5f * (base - m + kShift<NP>));
+    return seen ? sum * half * half : 0.0f;
+}
+
 // The running maximum and sum of a row, and its outputs: O^T as DT tiles of 16 dims.
 template <int DT>
 struct Running {
     float m, l;
+    bool far;  // of the wave: a scale over 2^kFarLog2 was met
     float4v o[DT];
     __device__ __forceinline__ void clear() {
         m = -INFINITY;
         l = 0.0f;
+        far = false;
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[t] = float4v{0, 0, 0, 0};
     }
 
     // A step's scores become weights w = 2^(s k + lv - m + kShift) as f16 fragments; m, l and o follow. The maximum is
     // taken over the scores (k is not negative), so a score costs half a max3, one multiply-add, one exp2, one add and
-    // half a conversion. Four parts, so that a caller can put products between them; in all: weigh().
+    // half a conversion. Four parts; in all: weigh().
 
     // The largest exponent of the lane's scores, of all 16 tokens of its group or of those that are `seen`.
     __device__ __forceinline__ static float peak(const float4v (&s)[4], const Scales& sc, float c) {
@@ -232,7 +266,7 @@ struct Running {
         top = column_max(top);
         if (__ballot(top > m + kSlack<NP>)) {
             const float m_new = fmaxf(m, top), f = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
-            l *= f;
+            l = lowered(l, m - m_new);
 #pragma unroll
             for (int t = 0; t < DT; ++t) o[t] *= f;
             m = m_new;
@@ -261,7 +295,7 @@ struct Running {
             sum += v;
             if constexpr (NP == 2) w[i / 8][1][i % 8] = (_Float16)(v - (float)w[i / 8][0][i % 8]);
         }
-        l += sum == 0.0f ? 0.0f : sum * sc.rv;
+        l += sum == 0.0f || far ? 0.0f : sum * sc.rv;
     }
     template <int NP>
     __device__ __forceinline__ void weigh(const float4v (&s)[4], const Scales& sc, float c, uint32_t tg, int32_t lo, int32_t hi, bool all,
@@ -274,6 +308,8 @@ struct Running {
             seen = seen_tokens(tg, lo, hi);
             raise<NP>(peak_seen(s, sc, c, seen));
         }
+        far = far || __ballot(sc.lv > kFarLog2);  // inside raise's branch the rest is compiled twice and spills
+        if (far) l += sum_apart<NP>([&](int i) { return s[i / 4][i % 4]; }, sc.k * c, m, seen);
         float x[16];
         exponents<NP>(s, sc, c, all, seen, x);
         weights<NP>(x, sc, w);
@@ -297,11 +333,6 @@ struct SeqUnits {
     uint32_t chunks, tiles;
     uint32_t units;
 };
-
-// A value that the whole wave shares, as the scalar that the compiler cannot see it is; lane l's, l itself shared. Loop
-// bounds, pages' places and the mask's limits then stay out of the vector registers (36 bytes of scratch a lane, then none).
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
-__device__ __forceinline__ uint32_t of_lane(uint32_t v, uint32_t l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)l); }
 
 template <int ROWS>
 __device__ __forceinline__ SeqUnits seq_units(const AttnArgs& a, const SeqRows& rows) {
@@ -567,7 +598,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attenti
             for (uint32_t w = 0; w < kAttnWaves; ++w) {
                 // a wave without a maximum has no weights, or only NaN
                 const float l = lds_l[w][16 * n + col];
-                sum += m[w] == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m[w] - peak);
+                sum += m[w] == -INFINITY ? l : lowered(l, m[w] - peak);
             }
             const float part_f = run[n].m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run[n].m - peak);
             const float f = !whole ? part_f : sum == 0.0f ? 0.0f : part_f / sum;
@@ -664,7 +695,7 @@ __global__ __launch_bounds__(256) void k_attention_few_join(AttnArgs a, uint32_t
             const uint32_t i = tid + k * 256;
             const float f = m[k] == -INFINITY ? (l[k] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m[k] - top);
             if (i < n) factor[i] = f;
-            sum += l[k] * f;
+            sum += m[k] == -INFINITY ? l[k] : lowered(l[k], m[k] - top);
         }
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
@@ -749,10 +780,12 @@ struct StepLds {
 template <int D>
 struct Running32 {
     float m, l;
+    bool far;
     float16v o[D / 32];
     __device__ __forceinline__ void clear() {
         m = -INFINITY;
         l = 0.0f;
+        far = false;
 #pragma unroll
         for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -785,12 +818,19 @@ struct Running32 {
         float peak = fmaxf(top[0], top[1]);
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(peak), __float_as_int(peak), false, false);
         peak = fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
-        if (__ballot(peak > m + kSlack<NP>)) {
+        if (__ballot(peak > m + kSlack<NP>) || far) {
             const float m_new = fmaxf(m, peak), f = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
-            l *= f;
+            l = lowered(l, m - m_new);
 #pragma unroll
             for (int t = 0; t < D / 32; ++t) o[t] *= f;
             m = m_new;
+            // the row's largest weight is of a step that raised m, so its scale is looked at here only (1 % of a call of prompts; 2 % with
+            // a look every step)
+            far = far || __ballot(fmaxf(sc[0].lv, sc[1].lv) > kFarLog2);
+            if (far) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) l += sum_apart<NP>([&](int i) { return s[u][i]; }, k[u], m, seen[u]);
+            }
         }
         const float base = m == -INFINITY ? 0.0f : m - kShift<NP>;
         float x[2][16];
@@ -815,7 +855,7 @@ struct Running32 {
                 w[u][i / 8][0][i % 8] = (_Float16)v;
                 if constexpr (NP == 2) w[u][i / 8][1][i % 8] = (_Float16)(v - (float)w[u][i / 8][0][i % 8]);
             }
-            l += sum == 0.0f ? 0.0f : sum * sc[u].rv;
+            l += sum == 0.0f || far ? 0.0f : sum * sc[u].rv;
         }
     }
 };
@@ -1182,14 +1222,14 @@ __global__ __launch_bounds__(256) void k_attention_many_join(AttnArgs a) {
 #pragma unroll
         for (uint32_t k = 0; k < kBatch; ++k) peak = fmaxf(peak, m[k]);
         const float moved = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - peak);
-        sum *= moved;
+        sum = top == -INFINITY ? sum : lowered(sum, top - peak);
         acc *= moved;
         top = peak;
 #pragma unroll
         for (uint32_t k = 0; k < kBatch; ++k) {
             if (s0 + k >= a.splits) continue;
             const float f = m[k] == -INFINITY ? (l[k] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m[k] - top);
-            sum += l[k] * f;
+            sum += m[k] == -INFINITY ? l[k] : lowered(l[k], m[k] - top);
             acc += o[k] * f;
         }
     }
