@@ -161,9 +161,12 @@ __global__ __launch_bounds__(kOwnerBlock) void k_kv_resize(KvPagesArgs a, const 
         if (want > len && len % a.block && have) {
             // tokens go behind others in a page: if it is held twice, into a copy
             const int32_t id = a.tables[(uint64_t)slot * a.table_stride + have - 1];
-            if ((uint32_t)id >= a.n_pages) set_status(status, kStatusKvBadIndex);
-            else if (a.refs[id] > 1) tail = id;
-            if (tail >= 0) {
+            if ((uint32_t)id >= a.n_pages) {  // the new tokens would share a page that is none: the slot stays as it is
+                ok = false;
+                take = 0;
+                set_status(status, kStatusKvBadIndex);
+            } else if (a.refs[id] > 1) {
+                tail = id;
                 ++take;
                 --column;
             }
@@ -201,7 +204,8 @@ __global__ __launch_bounds__(kOwnerBlock) void k_kv_fork(KvPagesArgs a, const in
             set_status(status, kStatusKvBadIndex);
         } else if (part) {
             tail = a.tables[(uint64_t)s * a.table_stride + full];
-            if ((uint32_t)tail >= a.n_pages) {
+            if ((uint32_t)tail >= a.n_pages) {  // a fresh page in its place would hold another sequence's tokens
+                ok = false;
                 tail = -1;
                 set_status(status, kStatusKvBadIndex);
             }

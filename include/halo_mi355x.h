@@ -600,8 +600,11 @@ uint64_t halo_mi_attention_workspace(const halo_mi_attention_params* p);
  * table_width; entries past ceil(len / block_tokens) are not read). A slot is a sequence or is empty (length 0).
  * The calls read and change this state in stream order, with no word from the host: a free page is one with refs
  * 0, and the lowest free ones are given first, in the order of the call's list. A listed slot outside [0,
- * n_slots), one that the list names before, and a page id out of range leave their entry's slot as it is and set
- * HALO_MI_STATUS_BAD_INDEX. Where the pages run out, that entry and every later one that needs pages are left as they
+ * n_slots), one that the list names before, and an id out of range in the place of a page that would be copied or written
+ * further (the last one, not full, of a fork's source or of a slot that grows) leave their entry's slot as it is and set
+ * HALO_MI_STATUS_BAD_INDEX. An id out of range among whole pages that a fork shares stays what it is in the new slot's table
+ * (what reads it gets NaN there, as from the source), one among pages given back becomes -1; both set the bit and are not
+ * counted. Where the pages run out, that entry and every later one that needs pages are left as they
  * are and HALO_MI_STATUS_KV_FULL is set; so is an entry whose length does not fit the table's columns.
  * At most HALO_MI_KV_LIST_MAX entries a call, and fewer than 2^32 columns of the entries' tables (or pages of the pool,
  * if it has fewer) together. The calls work in the stream's workspace: replays of graphs captured on one stream must not
