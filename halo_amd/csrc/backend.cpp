@@ -149,6 +149,7 @@ private:
     hipStream_t s_;
     std::uint32_t* status_;
     bool status_used_ = false;
+    std::uint32_t found_[2] = {};  // bits of the two words that no wait() has thrown for yet
 };
 
 // ---- operand resolution ---------------------------------------------------------------------
@@ -921,17 +922,21 @@ void HipStream::wait() {
         owner_->poison(false);
         throw Error(ErrorCode::Device, std::string("stream wait: ") + halo_mi_last_error());
     }
-    if (!status_used_) return;
-    status_used_ = false;
-    std::uint32_t words[2] = {};
-    if (hipMemcpy(words, status_, 8, hipMemcpyDeviceToHost) != hipSuccess ||
-        ((words[0] | words[1]) != 0 && hipMemsetAsync(status_, 0, 8, s_) != hipSuccess) || hipStreamSynchronize(s_) != hipSuccess) {
-        owner_->poison(false);
-        throw Error(ErrorCode::Device, "stream wait: cannot read the status word");
+    if (status_used_) {
+        status_used_ = false;
+        std::uint32_t words[2] = {};
+        if (hipMemcpy(words, status_, 8, hipMemcpyDeviceToHost) != hipSuccess ||
+            ((words[0] | words[1]) != 0 && hipMemsetAsync(status_, 0, 8, s_) != hipSuccess) || hipStreamSynchronize(s_) != hipSuccess) {
+            owner_->poison(false);
+            throw Error(ErrorCode::Device, "stream wait: cannot read the status word");
+        }
+        for (int i = 0; i < 2; ++i) found_[i] |= words[i];
     }
-    CHECK(!(words[0] & kStatusBadIndex), ErrorCode::Kernel, "GET_ROWS: an id lies outside the table (status 0x%x)", words[0]);
-    CHECK(!(words[1] & kStatusBadIndex), ErrorCode::Kernel, "paged cache: a page, slot or length is out of range (status 0x%x)", words[1]);
-    CHECK(!(words[1] & kStatusKvFull), ErrorCode::Memory, "paged cache: no free page, or no column in a table (status 0x%x)", words[1]);
+    // one kind a wait(): what is not thrown here is kept for the next one
+    const auto take = [&](int i, std::uint32_t bit) { return (found_[i] & bit) != 0 && (found_[i] &= ~bit, true); };
+    CHECK(!take(0, kStatusBadIndex), ErrorCode::Kernel, "GET_ROWS: an id lies outside the table");
+    CHECK(!take(1, kStatusBadIndex), ErrorCode::Kernel, "paged cache: a page, slot or length is out of range");
+    CHECK(!take(1, kStatusKvFull), ErrorCode::Memory, "paged cache: no free page, or no column in a table");
 }
 
 }  // namespace

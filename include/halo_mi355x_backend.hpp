@@ -475,8 +475,9 @@ struct GateUpArgs {
 // `type` is F32, F16 or BF16. Rows are TensorRef rows (row_stride in bytes, 0 = dense); a head stride
 // counts elements, 0 = head_dim. Lists are int32 on the device, read when the op runs. What an op finds wrong in
 // them is reported by the stream's next wait(): Error(Kernel) for an entry out of range, Error(Memory) where the
-// pages or a table's columns ran out; with `status` set (4 bytes, cleared by the op), the bits are left there instead
-// (kStatusBadIndex, kStatusKvFull) and wait() does not throw for them.
+// pages or a table's columns ran out, one kind a wait(): where ops found several, the wait()s after it throw for the
+// others. With `status` set (4 bytes, cleared by the op), the bits are left there instead (kStatusBadIndex,
+// kStatusKvFull) and wait() does not throw for them.
 
 inline constexpr std::uint32_t kStatusKvFull = 16u;
 
