@@ -353,14 +353,21 @@ __device__ __forceinline__ SeqUnits seq_units(const AttnArgs& a, uint32_t seq) {
     return seq_units<ROWS>(a, seq_rows(a.b, seq));
 }
 
-// Sums of lanes 0..lane, right for the lanes under n.
+// The call's units are under 2^31 where the row starts do not fall (plan_attention), and a sequence's always are; where starts fall,
+// rows count for several sequences. Sums stop at kMostUnits, so that they order as they should all the same, and units from there on
+// are nobody's: a wrapped sum would send the search for a unit's sequence past the last one, and the join past the workspace.
+constexpr uint32_t kMostUnits = 0x7FFFFFFFu;
+__device__ __forceinline__ uint32_t add_units(uint32_t a, uint32_t b) { return min(a + b, kMostUnits); }
+
+// Sums of lanes 0..lane, right for the lanes under n; and of the lanes below lane l.
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane, uint32_t n) {
     for (uint32_t off = 1; off < min(n, 64u); off <<= 1) {
         const uint32_t below = (uint32_t)__shfl_up((int)v, off);
-        if (lane >= off) v += below;
+        if (lane >= off) v = add_units(v, below);
     }
     return v;
 }
+__device__ __forceinline__ uint32_t below_lane(uint32_t sum, uint32_t l) { return l ? of_lane(sum, l - 1) : 0; }
 
 // The run of units of a workgroup (of `workgroups`), and the sequence that the run's first unit lies in, with the
 // units before that sequence. Every wave finds them for itself, 64 sequences at a time.
@@ -377,7 +384,7 @@ __device__ __forceinline__ Run find_run(const AttnArgs& a, uint32_t lane, uint32
     uint32_t v = lane < n ? seq_units<ROWS>(a, rows).units : 0, sum = wave_scan(v, lane, n), total = of_lane(sum, min(n, 64u) - 1);
     for (uint32_t s0 = 64; s0 < n; s0 += 64) {
         const uint32_t w = s0 + lane < n ? seq_units<ROWS>(a, s0 + lane).units : 0;
-        total += of_lane(wave_scan(w, lane, n - s0), min(n - s0, 64u) - 1);
+        total = add_units(total, of_lane(wave_scan(w, lane, n - s0), min(n - s0, 64u) - 1));
     }
     const uint32_t per = max(1u, (total + workgroups - 1) / workgroups);
     r.first = min(id * per, total);
@@ -391,7 +398,7 @@ __device__ __forceinline__ Run find_run(const AttnArgs& a, uint32_t lane, uint32
         const uint64_t hit = __ballot(s0 + lane < n && r.before + sum > r.first);
         if (hit) {
             const uint32_t l = (uint32_t)__ffsll((long long)hit) - 1;
-            r.before += of_lane(sum - v, l);
+            r.before += below_lane(sum, l);
             r.seq = s0 + l;
             r.rows = {of_lane(rows.row0, l), (int32_t)of_lane((uint32_t)rows.rows, l), (int32_t)of_lane((uint32_t)rows.len, l)};
             break;
@@ -652,8 +659,8 @@ __global__ __launch_bounds__(256) void k_attention_few_join(AttnArgs a, uint32_t
         uint32_t total = 0, before = 0;
         for (uint32_t s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
             const uint32_t n = min(a.b.n_seqs - s0, 64u), v = lane < n ? seq_units<ROWS>(a, s0 + lane).units : 0, sum = wave_scan(v, lane, n);
-            if (seq - s0 < 64) before = total + of_lane(sum - v, seq - s0);
-            total += of_lane(sum, n - 1);
+            if (seq - s0 < 64) before = add_units(total, below_lane(sum, seq - s0));
+            total = add_units(total, of_lane(sum, n - 1));
         }
         if (lane == 0) found[0] = max(1u, (total + workgroups - 1) / workgroups), found[1] = before;
     }
@@ -664,7 +671,7 @@ __global__ __launch_bounds__(256) void k_attention_few_join(AttnArgs a, uint32_t
     for (uint32_t tile = blockIdx.x % a.tiles, row = blockIdx.y; tile < su.tiles; row += gridDim.y) {
         const uint32_t u0 = before + (kvh * su.tiles + tile) * su.chunks, r = tile * ROWS + row;
         const uint32_t w0 = u0 / per, w1 = (u0 + su.chunks - 1) / per, n = w1 - w0 + 1;
-        if (n == 1 || row >= ROWS || r >= packed) {
+        if (n == 1 || w1 >= workgroups || row >= ROWS || r >= packed) {
             tile += a.tiles;
             row = blockIdx.y - gridDim.y;
             continue;

@@ -494,7 +494,8 @@ uint64_t halo_mi_kv_page_bytes(uint32_t n_layers, uint32_t n_kv_heads, uint32_t 
  * kv_lens[s] - n + i. Rows below row_starts[0] or from row_starts[n_seqs] on belong to no sequence:
  * they are neither read nor written. Token t of s lives in page tables[s * table_stride + t / block_tokens].
  *   tables: n_seqs rows of table_width int32, table_stride apart (0 = table_width).
- *   kv_lens: n_seqs int32. row_starts: n_seqs + 1 int32, not decreasing, at most n_rows.
+ *   kv_lens: n_seqs int32. row_starts: n_seqs + 1 int32, not decreasing, at most n_rows. They are cut to [0, n_rows];
+ *     where they fall, nothing outside the operands is touched, but rows are several sequences', and hold one's results.
  *   max_rows, max_kv: the most rows and tokens of a sequence, as the host knows them (0: n_rows, and
  *     table_width * block_tokens). They shape the launch; larger values than these on the device are still
  *     computed whole, only slower.
