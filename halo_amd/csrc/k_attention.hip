@@ -468,7 +468,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attenti
         // tokens that every row of the tile sees
         const int32_t pos0 = su.r.len - su.r.rows + (int32_t)(tile * ROWS / a.group);
         const int32_t pos1 = su.r.len - su.r.rows + (int32_t)((min(tile * ROWS + ROWS, packed) - 1) / a.group);
-        const uint32_t all_hi = (uint32_t)max(pos0 + 1, 0), all_lo = (uint32_t)first_seen(a, pos1, cap);
+        const uint32_t all_hi = (uint32_t)max(pos0 + 1, 0), all_lo = (uint32_t)first_seen(a, pos1, cap), any_lo = (uint32_t)first_seen(a, pos0, cap);
         const uint32_t end = (uint32_t)max(min(pos1 + 1, su.end), 0);
         const uint32_t t_first = (uint32_t)su.begin + (chunk << a.unit_log2) + wave * kStep;
         const uint32_t t_end = whole ? end : min((uint32_t)su.begin + ((chunk + n_chunks) << a.unit_log2), end);
@@ -533,7 +533,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attenti
             }
             __builtin_amdgcn_sched_barrier(0);
             const Scales sc = make_scales(ks, vs, ok || tg >= end);
-            if (!ok && tg < end) set_status(a.status, kStatusKvBadIndex);
+            if (!ok && tg < end && tg + 16 > any_lo) set_status(a.status, kStatusKvBadIndex);  // some row sees the group
             // dims outside, tiles inside: consecutive products have accumulators of their own
             float4v s[NQ][4];
 #pragma unroll
@@ -891,7 +891,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attention_many(AttnArgs a) {
         const uint32_t my0 = row0 + wave * 32, my_n = min(my0 + 32, row_n);  // this wave's rows: [my0, my_n)
         // tokens that the tile sees, and this split's share of them
         const int32_t tile_lo = first + (int32_t)(row0 / a.group), tile_hi = first + (int32_t)((row_n - 1) / a.group);
-        const uint32_t begin = (uint32_t)first_seen(a, tile_lo, cap) / kStep * kStep;
+        const uint32_t lo = (uint32_t)first_seen(a, tile_lo, cap), begin = lo / kStep * kStep;
         const uint32_t end = (uint32_t)max(min(tile_hi + 1, cap + 16), 0);
         const uint32_t steps = end > begin ? (end - begin + kStep - 1) / kStep : 0, share = (steps + a.splits - 1) / a.splits;
         const uint32_t t_first = begin + min(split * share, steps) * kStep, t_end = min(begin + min((split + 1) * share, steps) * kStep, end);
@@ -921,7 +921,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attention_many(AttnArgs a) {
             const uint32_t tg = t + 16 * (lane % 4);
             ok = (uint32_t)page_id < a.c.n_pages && (tg >> a.c.block_log2) < a.b.table_width;
             const int32_t number = ok ? page_id : 0;
-            ok = ok || tg >= end;
+            ok = ok || tg >= end || tg + 16 <= lo;  // no row sees the group
             const uint32_t kg = 2 * u0 + row / 4 % 2, vg = 2 * u0 + h;
             const uint8_t* k = page_ptr(a.c, __shfl(number, kg)) + head_codes + ((t + 16 * kg) % a.c.block + 4 * (row / 8) + row % 4) * D + 16 * h;
             const uint8_t* v = page_ptr(a.c, __shfl(number, vg)) + head_codes + a.c.heads * a.c.plane + row * a.c.block + (t + 16 * vg) % a.c.block;
@@ -1072,7 +1072,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attention_many16(AttnArgs a) 
         const uint32_t row0 = (tiles - 1 - back) * ROWS, row_n = min(row0 + ROWS, packed);
         const uint32_t my0 = row0 + wave * 16, my_n = min(my0 + 16, row_n);
         const int32_t tile_lo = first + (int32_t)(row0 / a.group), tile_hi = first + (int32_t)((row_n - 1) / a.group);
-        const uint32_t begin = (uint32_t)first_seen(a, tile_lo, cap) / kStep * kStep;
+        const uint32_t lo = (uint32_t)first_seen(a, tile_lo, cap), begin = lo / kStep * kStep;
         const uint32_t end = (uint32_t)max(min(tile_hi + 1, cap + 16), 0);
         const uint32_t steps = end > begin ? (end - begin + kStep - 1) / kStep : 0, share = (steps + a.splits - 1) / a.splits;
         const uint32_t t_first = begin + min(split * share, steps) * kStep, t_end = min(begin + min((split + 1) * share, steps) * kStep, end);
@@ -1098,7 +1098,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attention_many16(AttnArgs a) 
             const uint32_t tg = t + 16 * (lane % 4);
             ok = (uint32_t)page_id < a.c.n_pages && (tg >> a.c.block_log2) < a.b.table_width;
             const int32_t number = ok ? page_id : 0;
-            ok = ok || tg >= end;
+            ok = ok || tg >= end || tg + 16 <= lo;  // no row sees the group
             const uint32_t kg = col / 4;
             const uint8_t* k = page_ptr(a.c, __shfl(number, kg)) + head_codes + ((t + 16 * kg) % a.c.block + 4 * tile + col % 4) * D + 16 * g;
             const uint8_t* v = page_ptr(a.c, __shfl(number, g)) + head_codes + a.c.heads * a.c.plane + col * a.c.block + (t + 16 * g) % a.c.block;

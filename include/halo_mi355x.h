@@ -562,7 +562,8 @@ int halo_mi_kv_read(const halo_mi_kv_read_params* p, void* stream);
  * over the tokens t <= position (causal), and t > position - window where window is not 0. A row that sees
  * no token (a negative position) is zeros. q and out are n_rows rows of n_heads heads of head_dim; n_heads is
  * a multiple of n_kv_heads. A row of q that is not finite, and a row that sees a NaN block or a page out of
- * range, is NaN; tokens that a row does not see never reach it, whatever their bytes are.
+ * range, is NaN; tokens that a row does not see never reach it, whatever their bytes are. Pages that no row sees, as those behind
+ * a window, may be out of range.
  * Numerics: the codes are exact in the products; q and the softmax weights are rounded to 11 bits for 16-bit types (q
  * exactly, but for elements under 2^-28 of their row's largest and for rows all under 2^-112), and carried in two pieces, to within 2^-22,
  * for fp32; sums and the softmax are in fp32.
