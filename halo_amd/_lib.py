@@ -538,10 +538,17 @@ class KvState(typing.NamedTuple):
     table_stride: int = 0
 
 
-def _current_device() -> int:
-    """The current GPU, or -2 where nothing runs on one yet (no tensor is there then: a CPU tensor's is -1)."""
+@functools.lru_cache(None)
+def _torch():
+    """torch; an import statement costs a call 0.1 us each time."""
     import torch
 
+    return torch
+
+
+def _current_device() -> int:
+    """The current GPU, or -2 where nothing runs on one yet (no tensor is there then: a CPU tensor's is -1)."""
+    torch = _torch()
     return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
 
 
@@ -549,9 +556,15 @@ def _raw_stream(stream, dev: int) -> int:
     """The given stream, or torch's current one on device dev."""
     if stream is not None:
         return int(stream)
-    import torch
+    return _torch()._C._cuda_getCurrentRawStream(dev) if dev >= 0 else _stream(None)
 
-    return torch._C._cuda_getCurrentRawStream(dev) if dev >= 0 else _stream(None)
+
+@functools.lru_cache(None)
+def _kinds() -> tuple:
+    """The torch types that operands have: lists, status words (either), fp32 rows, frequencies, and rows by their element type."""
+    torch = _torch()
+    return (torch.int32, (torch.int32, torch.uint32), torch.float32, torch.float64,
+            {int(DType.F32): torch.float32, int(DType.F16): torch.float16, int(DType.BF16): torch.bfloat16})
 
 
 def _dev(t, dev: int) -> int:
@@ -565,18 +578,33 @@ def _dev(t, dev: int) -> int:
     return t.data_ptr()
 
 
+def _dev_of(t, dev: int, kind) -> int:
+    """... and of the type `kind` (several: one of them; None: a type that the call itself refuses)."""
+    if t is None:
+        return 0
+    if t.__class__ is int:
+        return t
+    if t.dtype is not kind:
+        kinds = kind if kind.__class__ is tuple else (kind,)
+        if kind is not None and t.dtype not in kinds:
+            raise HaloError(ErrorCode.Kernel, f"an operand is {t.dtype}, not {' or '.join(map(str, kinds))}")
+    if t.get_device() != dev:
+        raise HaloError(ErrorCode.Kernel, f"an operand is on {t.device}, not on the current GPU")
+    return t.data_ptr()
+
+
 def _cache(c: KvCache, dev: int) -> tuple:
     return (_dev(c[0], dev), *c[1:])
 
 
-def _batch(b: KvBatch, dev: int) -> tuple:
+def _batch(b: KvBatch, dev: int, ints) -> tuple:
     tables, width, kv_lens, row_starts, n_seqs, n_rows, max_rows, max_kv, stride = b
-    return _dev(tables, dev), stride, width, _dev(kv_lens, dev), _dev(row_starts, dev), n_seqs, n_rows, max_rows, max_kv
+    return _dev_of(tables, dev, ints), stride, width, _dev_of(kv_lens, dev, ints), _dev_of(row_starts, dev, ints), n_seqs, n_rows, max_rows, max_kv
 
 
-def _state(s: KvState, dev: int):
+def _state(s: KvState, dev: int, ints):
     refs, lens, tables, n_slots, width, stride = s
-    return _state_block(_dev(refs, dev), _dev(lens, dev), _dev(tables, dev), stride, width, n_slots)
+    return _state_block(_dev_of(refs, dev, ints), _dev_of(lens, dev, ints), _dev_of(tables, dev, ints), stride, width, n_slots)
 
 
 def rope_freqs(rot_dims: int, theta: float = 10000.0, *, scaling: int = RopeScaling.PLAIN, scale: float = 1.0,
@@ -599,9 +627,12 @@ def rope(t: int, positions, freqs, n_tokens: int, head_dim: int, rot_dims: int, 
     """PARTIAL_ROPE of q and, with k, of k in one launch (halo_mi_rope). q_out may be q, k_out may be k. positions:
     int32, freqs: float64 radians per position (rope_freqs), both on the device; strides in elements."""
     dev = _current_device()
-    p = _rope_params(_dev(q, dev), q_stride, q_head_stride, _dev(q_out, dev), q_out_stride, q_out_head_stride, n_heads,
-                     _dev(k, dev), k_stride, k_head_stride, _dev(k_out, dev), k_out_stride, k_out_head_stride, n_kv_heads,
-                     t, pairs, 0, 1 if k is None else 2, n_tokens, head_dim, rot_dims, _dev(positions, dev), _dev(freqs, dev), factor)
+    ints, _, _, doubles, values = _kinds()
+    x = values.get(t)
+    p = _rope_params(_dev_of(q, dev, x), q_stride, q_head_stride, _dev_of(q_out, dev, x), q_out_stride, q_out_head_stride, n_heads,
+                     _dev_of(k, dev, x), k_stride, k_head_stride, _dev_of(k_out, dev, x), k_out_stride, k_out_head_stride, n_kv_heads,
+                     t, pairs, 0, 1 if k is None else 2, n_tokens, head_dim, rot_dims, _dev_of(positions, dev, ints),
+                     _dev_of(freqs, dev, doubles), factor)
     at = ctypes.addressof(p)
     _POINTER.pack_into(p, _ROPE_PARAMS_AT + 8, at)  # halo_mi_rope_params.parts
     _check(lib().halo_mi_rope(at + _ROPE_PARAMS_AT, _raw_stream(stream, dev)))
@@ -616,8 +647,10 @@ def kv_write(t: int, cache: KvCache, layer: int, batch: KvBatch, k, v, *, k_stri
              v_stride: int = 0, v_head_stride: int = 0, status=None, status_keep: bool = False, stream=None) -> None:
     """KV_WRITE: the batch's rows of k and v into their sequences' pages (halo_mi_kv_write)."""
     dev = _current_device()
-    p = _kv_write_params(t, *_cache(cache, dev), layer, *_batch(batch, dev), _dev(k, dev), k_stride, k_head_stride, _dev(v, dev),
-                         v_stride, v_head_stride, _dev(status, dev), 1 if status_keep else 0)
+    ints, words, _, _, values = _kinds()
+    x = values.get(t)
+    p = _kv_write_params(t, *_cache(cache, dev), layer, *_batch(batch, dev, ints), _dev_of(k, dev, x), k_stride, k_head_stride,
+                         _dev_of(v, dev, x), v_stride, v_head_stride, _dev_of(status, dev, words), 1 if status_keep else 0)
     _check(lib().halo_mi_kv_write(p, _raw_stream(stream, dev)))
 
 
@@ -625,8 +658,9 @@ def kv_read(cache: KvCache, layer: int, batch: KvBatch, k_out=None, v_out=None, 
             v_stride: int = 0, v_head_stride: int = 0, status=None, status_keep: bool = False, stream=None) -> None:
     """The values that the cache holds for the batch's rows, in fp32 (halo_mi_kv_read)."""
     dev = _current_device()
-    p = _kv_read_params(*_cache(cache, dev), layer, *_batch(batch, dev), _dev(k_out, dev), k_stride, k_head_stride, _dev(v_out, dev),
-                        v_stride, v_head_stride, _dev(status, dev), 1 if status_keep else 0)
+    ints, words, singles, _, _ = _kinds()
+    p = _kv_read_params(*_cache(cache, dev), layer, *_batch(batch, dev, ints), _dev_of(k_out, dev, singles), k_stride, k_head_stride,
+                        _dev_of(v_out, dev, singles), v_stride, v_head_stride, _dev_of(status, dev, words), 1 if status_keep else 0)
     _check(lib().halo_mi_kv_read(p, _raw_stream(stream, dev)))
 
 
@@ -634,9 +668,11 @@ def _attention_params(t, cache, layer, batch, q, out, n_heads, scale, window, q_
                       workspace, workspace_bytes, status, status_keep, dev):
     if workspace is not None and not isinstance(workspace, int) and not workspace_bytes:
         workspace_bytes = workspace.numel() * workspace.element_size()
-    return _attention_block(t, *_cache(cache, dev), layer, *_batch(batch, dev), _dev(q, dev), q_stride, q_head_stride, _dev(out, dev),
-                            out_stride, out_head_stride, n_heads, scale, window, _dev(workspace, dev), workspace_bytes,
-                            _dev(status, dev), 1 if status_keep else 0)
+    ints, words, _, _, values = _kinds()
+    x = values.get(t)
+    return _attention_block(t, *_cache(cache, dev), layer, *_batch(batch, dev, ints), _dev_of(q, dev, x), q_stride, q_head_stride,
+                            _dev_of(out, dev, x), out_stride, out_head_stride, n_heads, scale, window, _dev(workspace, dev), workspace_bytes,
+                            _dev_of(status, dev, words), 1 if status_keep else 0)
 
 
 def attention(t: int, cache: KvCache, layer: int, batch: KvBatch, q, out, n_heads: int, *, scale: float = 0.0, window: int = 0,
@@ -662,31 +698,35 @@ def attention_workspace(t: int, cache: KvCache, layer: int, batch: KvBatch, q, o
 def kv_resize(cache: KvCache, state: KvState, slots, new_lens, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
     """Gives slots their new lengths, with pages taken and released (halo_mi_kv_resize); length 0 frees a slot."""
     dev = _current_device()
-    c, s = _cache_block(*_cache(cache, dev)), _state(state, dev)
-    _check(lib().halo_mi_kv_resize(c, s, _dev(slots, dev), _dev(new_lens, dev), n, _dev(status, dev),
+    ints, words = _kinds()[:2]
+    c, s = _cache_block(*_cache(cache, dev)), _state(state, dev, ints)
+    _check(lib().halo_mi_kv_resize(c, s, _dev_of(slots, dev, ints), _dev_of(new_lens, dev, ints), n, _dev_of(status, dev, words),
                                    1 if status_keep else 0, _raw_stream(stream, dev)))
 
 
 def kv_fork(cache: KvCache, state: KvState, src, dst, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
     """Empty slots dst become copies of src: whole pages shared, a last one that is not full copied (halo_mi_kv_fork)."""
     dev = _current_device()
-    c, s = _cache_block(*_cache(cache, dev)), _state(state, dev)
-    _check(lib().halo_mi_kv_fork(c, s, _dev(src, dev), _dev(dst, dev), n, _dev(status, dev),
+    ints, words = _kinds()[:2]
+    c, s = _cache_block(*_cache(cache, dev)), _state(state, dev, ints)
+    _check(lib().halo_mi_kv_fork(c, s, _dev_of(src, dev, ints), _dev_of(dst, dev, ints), n, _dev_of(status, dev, words),
                                  1 if status_keep else 0, _raw_stream(stream, dev)))
 
 
 def kv_compact(cache: KvCache, state: KvState, *, live=None, stream=None) -> None:
     """Moves the live pages to the front of the pool (halo_mi_kv_compact); live (uint32 or int32) receives their number."""
     dev = _current_device()
-    c, s = _cache_block(*_cache(cache, dev)), _state(state, dev)
-    _check(lib().halo_mi_kv_compact(c, s, _dev(live, dev), _raw_stream(stream, dev)))
+    ints, words = _kinds()[:2]
+    c, s = _cache_block(*_cache(cache, dev)), _state(state, dev, ints)
+    _check(lib().halo_mi_kv_compact(c, s, _dev_of(live, dev, words), _raw_stream(stream, dev)))
 
 
 def kv_copy_pages(cache: KvCache, src, dst, n: int, *, status=None, status_keep: bool = False, stream=None) -> None:
     """Copies whole pages (halo_mi_kv_copy_pages)."""
     dev = _current_device()
+    ints, words = _kinds()[:2]
     c = _cache_block(*_cache(cache, dev))
-    _check(lib().halo_mi_kv_copy_pages(c, _dev(src, dev), _dev(dst, dev), n, _dev(status, dev), 1 if status_keep else 0,
+    _check(lib().halo_mi_kv_copy_pages(c, _dev_of(src, dev, ints), _dev_of(dst, dev, ints), n, _dev_of(status, dev, words), 1 if status_keep else 0,
                                        _raw_stream(stream, dev)))
 
 
