@@ -127,13 +127,14 @@ Range tables_range(const KvBatch& b) { return {b.tables, extent(b.n_seqs, b.tabl
 Range lens_range(const KvBatch& b) { return {b.kv_lens, (uint64_t)b.n_seqs * 4, "kv_lens"}; }
 Range starts_range(const KvBatch& b) { return {b.row_starts, ((uint64_t)b.n_seqs + 1) * 4, "row_starts"}; }
 
-// Checks the optional status word (no operand of the call) and clears it unless the caller keeps it.
-int take_status(const char* op, uint32_t* status, uint32_t keep, hipStream_t st, std::initializer_list<Range> others) {
+// The optional status word is no operand of the call. It is cleared, unless the caller keeps it, once nothing else can refuse the
+// call.
+int check_status(const char* op, uint32_t* status, std::initializer_list<Range> others) {
     if (!status) return HALO_MI_OK;
     if (reinterpret_cast<uintptr_t>(status) % 4) return set_error(HALO_MI_E_KERNEL, "%s: status must be 4-byte aligned", op);
-    if (int rc = check_apart(op, {status, 4, "status"}, others)) return rc;
-    return keep ? HALO_MI_OK : launch_fill_u32(status, 1, 0u, st);
+    return check_apart(op, {status, 4, "status"}, others);
 }
+int clear_status(uint32_t* status, uint32_t keep, hipStream_t st) { return status && !keep ? launch_fill_u32(status, 1, 0u, st) : HALO_MI_OK; }
 
 // The checks of an attention call; *nothing: valid, but without rows.
 int check_attention(const halo_mi_attention_params* p, AttnArgs* a, std::initializer_list<Range*> ranges) {
@@ -347,7 +348,8 @@ int halo_mi_kv_write(const halo_mi_kv_write_params* p, void* stream) {
     if ((rc = check_apart(op, pool, {k, v, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
     a.status = p->status;
     auto st = static_cast<hipStream_t>(stream);
-    if ((rc = take_status(op, p->status, p->status_keep, st, {pool, k, v, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
+    if ((rc = check_status(op, p->status, {pool, k, v, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
+    if ((rc = clear_status(p->status, p->status_keep, st))) return rc;
     if (a.b.n_seqs == 0 || a.b.n_rows == 0) return HALO_MI_OK;
     return launch_kv_write(p->type, a, st);
 }
@@ -371,7 +373,8 @@ int halo_mi_kv_read(const halo_mi_kv_read_params* p, void* stream) {
     if ((rc = check_apart(op, out[0], {out[1]}))) return rc;
     a.status = p->status;
     auto st = static_cast<hipStream_t>(stream);
-    if ((rc = take_status(op, p->status, p->status_keep, st, {pool, out[0], out[1], tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
+    if ((rc = check_status(op, p->status, {pool, out[0], out[1], tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
+    if ((rc = clear_status(p->status, p->status_keep, st))) return rc;
     if (a.b.n_seqs == 0 || a.b.n_rows == 0 || (!p->k_out && !p->v_out)) return HALO_MI_OK;
     return launch_kv_read(a, st);
 }
@@ -387,15 +390,17 @@ int halo_mi_attention(const halo_mi_attention_params* p, void* stream) {
     if ((rc = check_apart(op, out, {q, pool, ws, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
     if ((rc = check_apart(op, ws, {q, pool, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
     auto st = static_cast<hipStream_t>(stream);
-    if ((rc = take_status(op, p->status, p->status_keep, st, {q, out, pool, ws, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
-    if (a.b.n_seqs == 0 || a.b.n_rows == 0) return HALO_MI_OK;
+    if ((rc = check_status(op, p->status, {q, out, pool, ws, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
+    const bool nothing = a.b.n_seqs == 0 || a.b.n_rows == 0;
     float* part = static_cast<float*>(p->workspace);
     uint64_t bytes = ws.bytes;
-    if (!part) {
+    if (!part && !nothing) {
         Workspace* w = nullptr;
         if ((rc = workspace_for(st, &w))) return rc;
         if (w) part = w->partials, bytes = kPartialFloats * sizeof(float);
     }
+    if ((rc = clear_status(p->status, p->status_keep, st))) return rc;
+    if (nothing) return HALO_MI_OK;
     if (plan_attention(a, bytes)) a.part = part;
     return launch_attention(a, st);
 }
@@ -417,8 +422,9 @@ int halo_mi_kv_resize(const halo_mi_kv_cache* cache, const halo_mi_kv_state* sta
     uint32_t* scratch = nullptr;
     auto st = static_cast<hipStream_t>(stream);
     if ((rc = check_state(op, cache, state, &a)) || (rc = check_lists(op, a, slots, new_lens, n))) return rc;
-    if ((rc = take_status(op, status, status_keep, st, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, tables_range(a), {slots, 4ull * n, "slots"}, {new_lens, 4ull * n, "new_lens"}, {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
-    if ((rc = scratch_for(op, st, 1 + 5ull * n + a.n_pages, &scratch))) return rc;
+    if ((rc = check_status(op, status, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, tables_range(a), {slots, 4ull * n, "slots"}, {new_lens, 4ull * n, "new_lens"}, {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
+    if (n && (rc = scratch_for(op, st, 1 + 5ull * n + a.n_pages, &scratch))) return rc;
+    if ((rc = clear_status(status, status_keep, st))) return rc;
     return n ? launch_kv_resize(a, slots, new_lens, n, scratch, status, st) : HALO_MI_OK;
 }
 
@@ -431,8 +437,9 @@ int halo_mi_kv_fork(const halo_mi_kv_cache* cache, const halo_mi_kv_state* state
     uint32_t* scratch = nullptr;
     auto st = static_cast<hipStream_t>(stream);
     if ((rc = check_state(op, cache, state, &a)) || (rc = check_lists(op, a, src, dst, n))) return rc;
-    if ((rc = take_status(op, status, status_keep, st, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, tables_range(a), {src, 4ull * n, "src"}, {dst, 4ull * n, "dst"}, {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
-    if ((rc = scratch_for(op, st, 1 + 5ull * n + a.n_pages, &scratch))) return rc;
+    if ((rc = check_status(op, status, {{a.refs, 4ull * a.n_pages, "refs"}, {a.lens, 4ull * a.n_slots, "lens"}, tables_range(a), {src, 4ull * n, "src"}, {dst, 4ull * n, "dst"}, {a.pool, a.n_pages * a.page_bytes, "the pool"}}))) return rc;
+    if (n && (rc = scratch_for(op, st, 1 + 5ull * n + a.n_pages, &scratch))) return rc;
+    if ((rc = clear_status(status, status_keep, st))) return rc;
     return n ? launch_kv_fork(a, src, dst, n, scratch, status, st) : HALO_MI_OK;
 }
 
@@ -468,7 +475,8 @@ int halo_mi_kv_copy_pages(const halo_mi_kv_cache* cache, const int32_t* src, con
         if ((rc = check_aligned(op, "src", src, 4)) || (rc = check_aligned(op, "dst", dst, 4))) return rc;
         if ((rc = check_apart(op, pool, {{src, 4ull * n, "src"}, {dst, 4ull * n, "dst"}}))) return rc;
     }
-    if ((rc = take_status(op, status, status_keep, st, {pool, {src, 4ull * n, "src"}, {dst, 4ull * n, "dst"}}))) return rc;
+    if ((rc = check_status(op, status, {pool, {src, 4ull * n, "src"}, {dst, 4ull * n, "dst"}}))) return rc;
+    if ((rc = clear_status(status, status_keep, st))) return rc;
     return n ? launch_kv_copy_pages(a, src, dst, n, status, st) : HALO_MI_OK;
 }
 

@@ -611,6 +611,8 @@ uint64_t halo_mi_attention_workspace(const halo_mi_attention_params* p);
  * At most HALO_MI_KV_LIST_MAX entries a call, and fewer than 2^32 columns of the entries' tables (or pages of the pool,
  * if it has fewer) together. The calls work in the stream's workspace: replays of graphs captured on one stream must not
  * overlap, and a capturing stream needs its workspace already (E_MEMORY; any earlier call that takes one makes it).
+ * It has room for lists and pools of 1 + 5 n + n_pages <= 2^23 (resize, fork) and 2 + 3 n_pages <= 2^23 (compact:
+ * 2 796 202 pages); larger ones are E_UNSUPPORTED. A refused call leaves the status word as it is.
  */
 #define HALO_MI_KV_LIST_MAX 1024u
 
