@@ -370,7 +370,8 @@ int halo_mi_kv_read(const halo_mi_kv_read_params* p, void* stream) {
             if ((rc = check_rows(op, out[i].name, a.out[i], a.b.n_rows, a.c.heads, a.c.dim, 4, &out[i].bytes))) return rc;
             if ((rc = check_apart(op, out[i], {pool, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
         }
-    if ((rc = check_apart(op, out[0], {out[1]}))) return rc;
+    if (!apart_in_rows(a.out[0], a.c.heads, a.out[1], a.c.heads, a.c.dim, 4, out[0], out[1]))
+        return set_error(HALO_MI_E_KERNEL, "%s: k_out overlaps v_out", op);
     a.status = p->status;
     auto st = static_cast<hipStream_t>(stream);
     if ((rc = check_status(op, p->status, {pool, out[0], out[1], tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
@@ -387,7 +388,8 @@ int halo_mi_attention(const halo_mi_attention_params* p, void* stream) {
     Range q, out;
     if ((rc = check_attention(p, &a, {&q, &out}))) return rc;
     const Range pool{a.c.pool, pool_bytes(a.c), "the pool"}, ws{p->workspace, p->workspace ? p->workspace_bytes : 0, "the workspace"};
-    if ((rc = check_apart(op, out, {q, pool, ws, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
+    if (!apart_in_rows(a.out, a.heads, a.q, a.heads, a.c.dim, elem_bytes(a.type), out, q)) return set_error(HALO_MI_E_KERNEL, "%s: out overlaps q", op);
+    if ((rc = check_apart(op, out, {pool, ws, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
     if ((rc = check_apart(op, ws, {q, pool, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;
     auto st = static_cast<hipStream_t>(stream);
     if ((rc = check_status(op, p->status, {q, out, pool, ws, tables_range(a.b), lens_range(a.b), starts_range(a.b)}))) return rc;

@@ -540,7 +540,7 @@ int halo_mi_kv_write(const halo_mi_kv_write_params* p, void* stream);
 /*
  * The values that the cache holds for the batch's rows: code * scale in fp32, k_out and v_out n_rows
  * rows of n_kv_heads heads of head_dim floats (either may be NULL). Rows at negative positions are zeros; rows in a
- * page out of range are NaN and set HALO_MI_STATUS_BAD_INDEX.
+ * page out of range are NaN and set HALO_MI_STATUS_BAD_INDEX. k_out and v_out may lie side by side in rows of one stride.
  */
 typedef struct halo_mi_kv_read_params {
     halo_mi_kv_cache cache;
@@ -572,7 +572,7 @@ int halo_mi_kv_read(const halo_mi_kv_read_params* p, void* stream);
  *     sequences, in place of the stream's own workspace. Graphs captured on one stream share that stream's
  *     workspace: give each its own if their replays may overlap. halo_mi_attention_workspace() says what a
  *     call makes use of; with less (or on a capturing stream that has none yet) sequences are split less.
- * out may not overlap q, the pool, the batch's lists or the workspace.
+ * out may not overlap q (they may lie side by side in rows of one stride), the pool, the batch's lists or the workspace.
  */
 typedef struct halo_mi_attention_params {
     uint32_t type;
