@@ -3,7 +3,8 @@
 //   out = sum_t p_t V_t / sum_t p_t, p_t = exp(scale q . K_t), K_t = ks c_t, V_t = vs c'_t with int8 codes c, c'.
 //
 // Products run on v_mfma_f32_16x16x32_f16. An int8 code is exact in f16, so K and V lose nothing; q, scaled per
-// row by a power of two to the top of f16's range, and the weights are one f16 piece (16-bit types) or two (fp32).
+// row by a power of two to the top of f16's range, is one f16 piece (16-bit types) or two (fp32); the weights are two for fp32, and
+// for F16 over few rows, else one.
 // The scales stay out of the products: with x_t = s_t ks scale log2(e) + log2(vs), s_t = q . c_t, the weight of V's
 // codes is w_t = 2^(x_t - m), m a reference that follows the maximum of x_t, and the sum that divides is sum_t w_t / vs (where
 // scales lie very far apart taken from the scores instead: sum_apart). One multiply-add per score applies both scales, and w_t fits f16
@@ -435,8 +436,10 @@ __device__ __forceinline__ uint4 stream16(const uint8_t* p) {
 template <int D, int NQ>
 constexpr int kFewPerCu = D == 64 && NQ == 1 ? 3 : D <= 128 && NQ == 1 ? 2 : 1;
 
-// D: head_dim. NP: f16 pieces of q and of the weights. NQ: row tiles of 16 that share K and V.
-template <int D, int NP, int NQ, bool ONCE>
+// D: head_dim. NP: f16 pieces of q. WP: of the weights: two for F16, whose outputs have as many bits as one piece has (8 verify steps
+// of 4 rows, 24 heads of 256: an rms error of 2.1e-4, the outputs' rounding, against 2.4e-4, for 25.6 us against 24.6); one for
+// BF16, 1/16 of whose rounding it is off by. NQ: row tiles of 16 that share K and V.
+template <int D, int NP, int WP, int NQ, bool ONCE>
 __global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attention_few(AttnArgs a) {
     constexpr int C = D / 64, TAIL = D % 64 / 32;  // 64-dim chunks of a K row, and a last one of 32
     constexpr int DT = D / 16;                     // tiles of 16 dims
@@ -571,16 +574,16 @@ __global__ __launch_bounds__(kAttnWaves * 64, (kFewPerCu<D, NQ>)) void k_attenti
             }
             __builtin_amdgcn_sched_barrier(0);
             const bool all = t0 >= all_lo && t0 + kStep <= all_hi;
-            half8v w[NQ][2][NP];
+            half8v w[NQ][2][WP];
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) run[n].template weigh<NP>(s[n], sc, q[n].c, tg, q[n].lo, q[n].hi, all, w[n]);
+            for (int n = 0; n < NQ; ++n) run[n].template weigh<WP>(s[n], sc, q[n].c, tg, q[n].lo, q[n].hi, all, w[n]);
 #pragma unroll
             for (int i = 0; i < DT; ++i) {
                 const half8v v0 = codes_f16(vb[i].x, vb[i].y), v1 = codes_f16(vb[i].z, vb[i].w);
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                    for (int p = 0; p < NP; ++p) {
+                    for (int p = 0; p < WP; ++p) {
                         run[n].o[i] = mfma(v0, w[n][0][p], run[n].o[i]);
                         run[n].o[i] = mfma(v1, w[n][1][p], run[n].o[i]);
                     }
@@ -738,7 +741,7 @@ __global__ __launch_bounds__(256) void k_attention_few_join(AttnArgs a, uint32_t
 // Rows of a tile: a wider one reads K and V once for twice the rows, where the registers hold its outputs.
 uint32_t few_rows(const AttnArgs& a) { return (uint64_t)a.b.max_rows * a.group <= 16 || a.c.dim > 128 ? 16 : 32; }
 
-template <int D, int NP>
+template <int D, int NP, int WP>
 void run_few(const AttnArgs& a, hipStream_t st) {
     const uint32_t rows = few_rows(a);
     const dim3 join(a.b.n_seqs * a.c.heads * a.tiles, std::min<uint32_t>(rows, std::max<uint64_t>(1, (uint64_t)a.b.max_rows * a.group)));
@@ -746,14 +749,19 @@ void run_few(const AttnArgs& a, hipStream_t st) {
     const bool once = a.tiles == 1 && 2ull * a.b.n_seqs * a.b.max_kv * a.c.heads * D > 32ull << 20;
     if constexpr (D <= 128) {
         if (rows == 32) {
-            hipLaunchKernelGGL((k_attention_few<D, NP, 2, false>), dim3(a.splits), dim3(kAttnWaves * 64), 0, st, a);
+            hipLaunchKernelGGL((k_attention_few<D, NP, WP, 2, false>), dim3(a.splits), dim3(kAttnWaves * 64), 0, st, a);
             if (a.part) hipLaunchKernelGGL(k_attention_few_join<32>, join, dim3(256), 0, st, a, a.splits);
             return;
         }
     }
-    auto* k = once ? k_attention_few<D, NP, 1, true> : k_attention_few<D, NP, 1, false>;
+    auto* k = once ? k_attention_few<D, NP, WP, 1, true> : k_attention_few<D, NP, WP, 1, false>;
     hipLaunchKernelGGL(k, dim3(a.splits), dim3(kAttnWaves * 64), 0, st, a);
     if (a.part) hipLaunchKernelGGL(k_attention_few_join<16>, join, dim3(256), 0, st, a, a.splits);
+}
+
+template <int D>
+void run_few_of(const AttnArgs& a, hipStream_t st) {
+    a.type == HALO_MI_F32 ? run_few<D, 2, 2>(a, st) : a.type == HALO_MI_F16 ? run_few<D, 1, 2>(a, st) : run_few<D, 1, 1>(a, st);
 }
 
 // ---- many rows: prompts and chunks ----------------------------------------------------------------------------
@@ -768,6 +776,9 @@ void run_few(const AttnArgs& a, hipStream_t st) {
 // (16 cycles of either form side by side with a v_exp_f32 stream: 1.01 against 1.13 times the stream alone). A
 // step is two tiles u of 32 tokens; lane (r, h) = (lane % 32, lane / 32) has the scores of row r with the 16 tokens of
 // group 2 u + h, as K's row r of tile u is token 4 (r / 8) + r % 4 of group 2 u + r / 4 % 2.
+//
+// The weights are one piece for both 16-bit types: V's products are half of the work here, and F16 prompts (16 heads of 256, up to
+// 3000 rows) in two pieces take 252 us against 204, for an rms error of 2.1e-4 against 2.6e-4; fp32 is for callers who need it.
 //
 // The tiles of the latest rows, which see most, start first. With fewer tiles than CUs the tokens of each are split, and
 // k_attention_many_join adds the parts.
@@ -1340,11 +1351,11 @@ int launch_attention(const AttnArgs& a, hipStream_t st) {
         return rc ? rc : hip_status(hipGetLastError(), "ATTENTION");
     }
     switch (a.c.dim) {
-        case 64: two ? run_few<64, 2>(a, st) : run_few<64, 1>(a, st); break;
-        case 96: two ? run_few<96, 2>(a, st) : run_few<96, 1>(a, st); break;
-        case 128: two ? run_few<128, 2>(a, st) : run_few<128, 1>(a, st); break;
-        case 192: two ? run_few<192, 2>(a, st) : run_few<192, 1>(a, st); break;
-        default: two ? run_few<256, 2>(a, st) : run_few<256, 1>(a, st); break;
+        case 64: run_few_of<64>(a, st); break;
+        case 96: run_few_of<96>(a, st); break;
+        case 128: run_few_of<128>(a, st); break;
+        case 192: run_few_of<192>(a, st); break;
+        default: run_few_of<256>(a, st); break;
     }
     return hip_status(hipGetLastError(), "ATTENTION");
 }

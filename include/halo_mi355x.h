@@ -564,9 +564,10 @@ int halo_mi_kv_read(const halo_mi_kv_read_params* p, void* stream);
  * a multiple of n_kv_heads. A row of q that is not finite, and a row that sees a NaN block or a page out of
  * range, is NaN; tokens that a row does not see never reach it, whatever their bytes are. Pages that no row sees, as those behind
  * a window, may be out of range.
- * Numerics: the codes are exact in the products; q and the softmax weights are rounded to 11 bits for 16-bit types (q
- * exactly, but for elements under 2^-28 of their row's largest and for rows all under 2^-112), and carried in two pieces, to within 2^-22,
- * for fp32; sums and the softmax are in fp32.
+ * Numerics: the codes are exact in the products. q is rounded to 11 bits for 16-bit types (exactly q, but for elements under
+ * 2^-28 of their row's largest and for rows all under 2^-112) and carried in two pieces, to within 2^-22, for fp32. The softmax
+ * weights are two pieces for fp32, and for F16 where rows are few (decode and verify steps: 16 and fewer rows of q a kv head, and up to
+ * four times as many for some shapes), else rounded to 11 bits. Sums and the softmax are in fp32.
  *   scale: 0 = 1 / sqrt(head_dim).
  *   workspace (optional, 16-byte aligned): workspace_bytes of device memory for the partial results of long
  *     sequences, in place of the stream's own workspace. Graphs captured on one stream share that stream's
