@@ -46,8 +46,7 @@ template <int NP>
 constexpr float kShift = NP == 1 ? 8.0f : 14.0f;
 template <int NP>
 constexpr float kSlack = NP == 1 ? 7.5f : 1.5f;
-constexpr uint32_t kFewGrid = 768;      // workgroups of a call with few rows at most: three per CU
-constexpr float kTinyScale = 0x1p-80f;  // the scale that an all-zero block of V counts with
+constexpr uint32_t kFewGrid = 768;  // workgroups of a call with few rows at most: three per CU
 // Once the largest weights are of blocks of V with a scale over 2^this, a wave takes its sums apart from its weights (sum_apart).
 constexpr float kFarLog2 = 10.0f;
 
@@ -202,7 +201,7 @@ struct Scales {
     float k, lv, rv;  // K's; log2 of V's and its reciprocal
 };
 __device__ __forceinline__ Scales make_scales(float ks, float vs, bool page) {
-    vs = vs == 0.0f ? kTinyScale : vs;
+    vs = vs == 0.0f ? kKvMinScale : vs;  // an all-zero block of V counts with the smallest scale
     return {page ? ks : quiet_nan(), __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
 }
 
@@ -1254,15 +1253,13 @@ __global__ __launch_bounds__(256) void k_attention_many_join(AttnArgs a) {
     store4(a.out, a.type, row * a.out.stride + head * a.out.head_stride + d, sum == 0.0f ? float4v{0, 0, 0, 0} : acc / sum);
 }
 
-// Waves of a workgroup: of 32 rows each, or of 16 where the outputs of 32 would leave one wave per SIMD.
-template <int D>
-constexpr int kManyWaves = 8;
+constexpr int kManyWaves = 8;  // of a workgroup: of 32 rows each, or of 16 where the outputs of 32 would leave one wave per SIMD
 template <int D>
 constexpr bool kHalfTiles = D > 128;
 
 template <int D, int NP>
 int run_many(const AttnArgs& a, hipStream_t st) {
-    constexpr int W = kManyWaves<D>;
+    constexpr int W = kManyWaves;
     void (*k)(AttnArgs);
     size_t lds;
     if constexpr (kHalfTiles<D>) {

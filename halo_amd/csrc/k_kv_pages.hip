@@ -3,7 +3,7 @@
 // serving loop needs no word from the host between steps and can be captured whole.
 //
 // Who gets which page is one order (the list's) over another (the free pages by number), so one workgroup of 1024
-// threads decides: prefix sums over the list and over the counts, 4096 counts a step. What costs time is the
+// threads decides: prefix sums over the list and over the counts, 4096 counts a step (1024 where pages move). What costs time is the
 // pages' bytes (hundreds of KB each with all layers) and long tables: a second kernel copies them with the whole GPU,
 // from lists that the first one leaves in scratch memory.
 //

@@ -98,7 +98,8 @@ struct KvPagesArgs {
 int launch_rope(uint32_t type, uint32_t pairs, const RopeArgs& a, hipStream_t st);
 int launch_kv_write(uint32_t type, const KvWriteArgs& a, hipStream_t st);
 int launch_kv_read(const KvReadArgs& a, hipStream_t st);
-// The split that fits part_bytes of partial results (0: unsplit); sets a.splits, a.chunk and a.tiles.
+// How the work is dealt out with part_bytes of partial results; returns the bytes made use of (0: nothing is split). Sets a.few,
+// a.splits and a.tiles, and where rows are few a.unit and a.unit_log2.
 uint64_t plan_attention(AttnArgs& a, uint64_t part_bytes);
 int launch_attention(const AttnArgs& a, hipStream_t st);
 // scratch: 1 + 5 n + n_pages words (resize, fork); 2 + 3 n_pages words (compact)
