@@ -17,9 +17,10 @@
 // [dim][token] in the page, so the A operand of 16 tokens is one 16-byte load per lane, as K's is per 16 dims.
 //
 // What bounds it, as measured: few rows are a stream of the cache (48 bf16 rows over 405 MB in 88 us, 200 rows over 1.6 GB in
-// 300: 4.7 and 5.5 TB/s; a 4 GiB copy runs at 4.7), or, when short, its chain of reads (one row over 777 tokens 15.7 us);
-// many rows are the products and the exponentials (three bf16 prompts of up to 5000 tokens, 321 GFLOP, in 375 to 393 us: 817 to 857 TFLOP/s
-// where a large f16 library product reaches 1140; 256 fp32 rows over 16300 tokens in 185 us, 1100 with the second pieces).
+// 300: 4.7 and 5.5 TB/s with the join; a plain read of 405 MB runs at 6.9), or, when short, its chain of reads (one row over 777 tokens 15.7 us);
+// many rows are the vector unit's work and the products, which overlap in part (three bf16 prompts of up to 5000 tokens, 321 GFLOP, in
+// 377 to 402 us: 799 to 852 TFLOP/s where a large bf16 library product reaches 1300; vector unit 51 % busy, matrix cores 35 %; 256 fp32 rows
+// over 16300 tokens in 185 to 196 us, 1040 to 1100 with the second pieces, 40 % and 44 %).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -498,7 +498,8 @@ uint64_t halo_mi_kv_page_bytes(uint32_t n_layers, uint32_t n_kv_heads, uint32_t 
  *     where they fall, nothing outside the operands is touched, but rows are several sequences', and hold one's results.
  *   max_rows, max_kv: the most rows and tokens of a sequence, as the host knows them (0: n_rows, and
  *     table_width * block_tokens). They shape the launch; larger values than these on the device are still
- *     computed whole, only slower.
+ *     computed whole, only slower. Attention of a decode batch needs max_rows to be fast: as the rows of one sequence, which 0 takes
+ *     them for, they go the way of prompts (48 sequences of one row: 276 us, with max_rows 1 86).
  */
 typedef struct halo_mi_kv_batch {
     const int32_t* tables;
