@@ -5,7 +5,8 @@ The compute path is hand-written HIP for gfx950 in ``libhalo_mi355x.so``, reache
 C ABI declared in ``include/halo_mi355x.h``. This package loads that library with ctypes and
 mirrors the reference's operator interface for the path (``Backend::gemv`` over
 ``GemvArgs``; include/halo/backend/backend.h:283-314, :562). Beside it stand rotary positions, an
-8-bit paged cache and the attention over it (``rope``, ``kv_*``, ``attention``). There is no CPU
+8-bit paged cache and the attention over it (``rope``, ``norm_rope``, ``kv_*``, ``attention``), products of 8-bit integers
+(``quantize_rows``, ``gemm_i8``) and linear attention with a state (``linear_attention``). There is no CPU
 fallback: if the library is missing every entry point raises.
 """
 from __future__ import annotations
@@ -18,6 +19,8 @@ from ._lib import (  # noqa: F401
     KvCache,
     KvState,
     Layout,
+    LinearBatch,
+    LinearState,
     RopePairs,
     RopeScaling,
     Variant,
@@ -38,6 +41,7 @@ from ._lib import (  # noqa: F401
     gate_up_swiglu,
     gemv,
     gemm_group,
+    gemm_i8,
     gemv_group,
     gemv_noalloc,
     get_rows,
@@ -49,8 +53,12 @@ from ._lib import (  # noqa: F401
     kv_resize,
     kv_write,
     lib,
+    linear_attention,
+    linear_attention_workspace,
     lm_head,
+    norm_rope,
     quantize,
+    quantize_rows,
     repack_slab,
     repack_slab_host,
     rms_norm,

@@ -224,6 +224,9 @@ _kv_write_params = _Layout("I4x", _CACHE, "I4x", _BATCH, _ROWS, _ROWS, _STATUS)
 _kv_read_params = _Layout(_CACHE, "I4x", _BATCH, _ROWS, _ROWS, _STATUS)
 _attention_block = _Layout("I4x", _CACHE, "I4x", _BATCH, _ROWS, _ROWS, "IfI4xPQ", _STATUS)
 _cache_block = _Layout(_CACHE)
+_norm_rope_params = _Layout(_ROPE_PART, _ROPE_PART, "IIPIIIIPPf4x", "PPf4x")  # the two parts, then halo_mi_norm_rope_params
+_gemm_i8_params = _Layout("I4xPQPPQPPQIII4x")
+_linear_attention_params = _Layout("5I4xPPI4xPPP3I4x", _ROWS, _ROWS, _ROWS, _ROWS, "PQIfPQ", _STATUS)
 _state_block = _Layout("PPPQII")
 
 
@@ -251,6 +254,7 @@ SIGNATURES = {
     "halo_mi_rms_norm": (_INT, [_VP, _U64, _VP, _VP, _U64, _U32, _U32, ctypes.c_float, _VP]),
     "halo_mi_rope_freqs": (_INT, [_U32, ctypes.c_double, ctypes.POINTER(_RopeScaling), _VP, ctypes.POINTER(ctypes.c_float)]),
     "halo_mi_rope": (_INT, [_VP, _VP]),
+    "halo_mi_norm_rope": (_INT, [_VP, _VP]),
     "halo_mi_kv_page_bytes": (_U64, [_U32, _U32, _U32, _U32]),
     "halo_mi_kv_write": (_INT, [_VP, _VP]),
     "halo_mi_kv_read": (_INT, [_VP, _VP]),
@@ -260,6 +264,10 @@ SIGNATURES = {
     "halo_mi_kv_fork": (_INT, [_VP, _VP, _VP, _VP, _U32, _VP, _U32, _VP]),
     "halo_mi_kv_compact": (_INT, [_VP, _VP, _VP, _VP]),
     "halo_mi_kv_copy_pages": (_INT, [_VP, _VP, _VP, _U32, _VP, _U32, _VP]),
+    "halo_mi_quantize_rows": (_INT, [_U32, _VP, _U64, _VP, _U64, _VP, _U32, _U32, _VP]),
+    "halo_mi_gemm_i8": (_INT, [_VP, _VP]),
+    "halo_mi_linear_attention": (_INT, [_VP, _VP]),
+    "halo_mi_linear_attention_workspace": (_U64, [_VP]),
     "halo_mi_stream_read": (_INT, [_VP, _U64, _U32, _U32, _VP, _VP]),
     "halo_mi_stream_check": (_INT, [_VP]),
     "halo_mi_stream_release": (_INT, [_VP]),
@@ -567,6 +575,27 @@ def _kinds() -> tuple:
             {int(DType.F32): torch.float32, int(DType.F16): torch.float16, int(DType.BF16): torch.bfloat16})
 
 
+@functools.lru_cache(None)
+def _int8():
+    return _torch().int8
+
+
+def _range(values, bits: int):
+    for v in values:
+        if not 0 <= int(v) < 1 << bits:
+            raise HaloError(ErrorCode.Kernel, f"an argument is out of range: {v}")
+    return values
+
+
+def _uints(*values):
+    """Arguments that are passed as uint32: ctypes would cut them to 32 bits without a word."""
+    return _range(values, 32)
+
+
+def _sizes(*values):
+    return _range(values, 64)
+
+
 def _dev(t, dev: int) -> int:
     """Device address of an operand; a tensor has to be on the current device."""
     if t is None:
@@ -636,6 +665,24 @@ def rope(t: int, positions, freqs, n_tokens: int, head_dim: int, rot_dims: int, 
     at = ctypes.addressof(p)
     _POINTER.pack_into(p, _ROPE_PARAMS_AT + 8, at)  # halo_mi_rope_params.parts
     _check(lib().halo_mi_rope(at + _ROPE_PARAMS_AT, _raw_stream(stream, dev)))
+
+
+def norm_rope(t: int, positions, freqs, n_tokens: int, head_dim: int, rot_dims: int, q, q_out, n_heads: int, *, q_norm=None, k=None,
+              k_out=None, n_kv_heads: int = 0, k_norm=None, eps: float = 1e-6, pairs: int = RopePairs.HALF, factor: float = 1.0,
+              q_stride: int = 0, q_head_stride: int = 0, q_out_stride: int = 0, q_out_head_stride: int = 0, k_stride: int = 0,
+              k_head_stride: int = 0, k_out_stride: int = 0, k_out_head_stride: int = 0, stream=None) -> None:
+    """rope with the RMS norm of each head before it, in one pass (halo_mi_norm_rope): q_norm and k_norm are head_dim fp32 weights, or
+    None where the heads are rotated only."""
+    dev = _current_device()
+    ints, _, singles, doubles, values = _kinds()
+    x = values.get(t)
+    p = _norm_rope_params(_dev_of(q, dev, x), q_stride, q_head_stride, _dev_of(q_out, dev, x), q_out_stride, q_out_head_stride, n_heads,
+                          _dev_of(k, dev, x), k_stride, k_head_stride, _dev_of(k_out, dev, x), k_out_stride, k_out_head_stride, n_kv_heads,
+                          t, pairs, 0, 1 if k is None else 2, n_tokens, head_dim, rot_dims, _dev_of(positions, dev, ints),
+                          _dev_of(freqs, dev, doubles), factor, _dev_of(q_norm, dev, singles), _dev_of(k_norm, dev, singles), eps)
+    at = ctypes.addressof(p)
+    _POINTER.pack_into(p, _ROPE_PARAMS_AT + 8, at)  # halo_mi_rope_params.parts
+    _check(lib().halo_mi_norm_rope(at + _ROPE_PARAMS_AT, _raw_stream(stream, dev)))
 
 
 def kv_page_bytes(n_layers: int, n_kv_heads: int, head_dim: int, block_tokens: int) -> int:
@@ -728,6 +775,97 @@ def kv_copy_pages(cache: KvCache, src, dst, n: int, *, status=None, status_keep:
     c = _cache_block(*_cache(cache, dev))
     _check(lib().halo_mi_kv_copy_pages(c, _dev_of(src, dev, ints), _dev_of(dst, dev, ints), n, _dev_of(status, dev, words), 1 if status_keep else 0,
                                        _raw_stream(stream, dev)))
+
+
+# ---- products of 8-bit integers ----------------------------------------------------------
+
+
+def quantize_rows(t: int, x, codes, scales, rows: int, cols: int, *, x_stride: int = 0, codes_stride: int = 0, stream=None) -> None:
+    """Rows of x as int8 codes and one fp32 scale each (halo_mi_quantize_rows). codes: int8 rows codes_stride bytes apart, a multiple of
+    16 (0: cols rounded up to 16), with zeros behind a row's codes."""
+    dev = _current_device()
+    _, _, singles, _, values = _kinds()
+    _check(lib().halo_mi_quantize_rows(*_uints(t), _dev_of(x, dev, values.get(t)), *_sizes(x_stride), _dev_of(codes, dev, _int8()), *_sizes(codes_stride),
+                                       _dev_of(scales, dev, singles), *_uints(rows, cols), _raw_stream(stream, dev)))
+
+
+def gemm_i8(t: int, w, w_scales, x, x_scales, y, rows: int, cols: int, n_vec: int, *, w_stride: int = 0, x_stride: int = 0, y_stride: int = 0,
+            stream=None) -> None:
+    """y[v][n] = x_scales[v] * w_scales[n] * sum_i x[v][i] w[n][i] over int8 codes as quantize_rows writes them, y of type t
+    (halo_mi_gemm_i8)."""
+    dev = _current_device()
+    _, _, singles, _, values = _kinds()
+    codes = _int8()
+    p = _gemm_i8_params(t, _dev_of(w, dev, codes), w_stride, _dev_of(w_scales, dev, singles), _dev_of(x, dev, codes), x_stride,
+                        _dev_of(x_scales, dev, singles), _dev_of(y, dev, values.get(t)), y_stride, rows, cols, n_vec)
+    _check(lib().halo_mi_gemm_i8(p, _raw_stream(stream, dev)))
+
+
+# ---- linear attention --------------------------------------------------------------------
+
+
+class LinearState(typing.NamedTuple):
+    """The states of linear attention's heads: n_slots slots of n_heads x k_dim x v_dim fp32, and where the new ones go (None: into the
+    same)."""
+
+    data: object
+    n_slots: int
+    n_heads: int
+    k_dim: int
+    v_dim: int
+    out: object = None
+
+
+class LinearBatch(typing.NamedTuple):
+    """The sequences of a call: rows row_starts[s] .. row_starts[s + 1] of the row operands are the next tokens of the sequence in slot
+    slots[s]; seq_lens (optional) its tokens with them. int32 on the device."""
+
+    slots: object
+    row_starts: object
+    n_seqs: int
+    n_rows: int
+    max_rows: int = 0
+    seq_lens: object = None
+
+
+def _linear_block(t, state, batch, q, k, v, out, decay, n_k_heads, decay_per_head, scale, decay_stride, q_stride, q_head_stride, k_stride,
+                  k_head_stride, v_stride, v_head_stride, out_stride, out_head_stride, workspace, workspace_bytes, status, status_keep, dev):
+    if workspace is not None and not isinstance(workspace, int) and not workspace_bytes:
+        workspace_bytes = workspace.numel() * workspace.element_size()
+    ints, words, singles, _, values = _kinds()
+    x = values.get(t)
+    data, n_slots, n_heads, k_dim, v_dim, new = state
+    slots, row_starts, n_seqs, n_rows, max_rows, seq_lens = batch
+    before = _dev_of(data, dev, singles)
+    return _linear_attention_params(
+        t, n_heads, n_k_heads, k_dim, v_dim, before, before if new is None else _dev_of(new, dev, singles), n_slots, _dev_of(slots, dev, ints),
+        _dev_of(row_starts, dev, ints), _dev_of(seq_lens, dev, ints), n_seqs, n_rows, max_rows, _dev_of(q, dev, x), q_stride, q_head_stride,
+        _dev_of(k, dev, x), k_stride, k_head_stride, _dev_of(v, dev, x), v_stride, v_head_stride, _dev_of(out, dev, x), out_stride,
+        out_head_stride, _dev_of(decay, dev, singles), decay_stride, 1 if decay_per_head else 0, scale, _dev(workspace, dev), workspace_bytes,
+        _dev_of(status, dev, words), 1 if status_keep else 0)
+
+
+def linear_attention(t: int, state: LinearState, batch: LinearBatch, q, k, v, out, decay, n_k_heads: int, *, decay_per_head: bool = False,
+                     scale: float = 0.0, decay_stride: int = 0, q_stride: int = 0, q_head_stride: int = 0, k_stride: int = 0,
+                     k_head_stride: int = 0, v_stride: int = 0, v_head_stride: int = 0, out_stride: int = 0, out_head_stride: int = 0,
+                     workspace=None, workspace_bytes: int = 0, status=None, status_keep: bool = False, stream=None) -> None:
+    """S <- exp(decay) S + k v^T, out = scale S^T q for each sequence's rows in order, S its heads' states (halo_mi_linear_attention).
+    decay: fp32 logarithms, [n_rows, n_heads], or [n_heads] with decay_per_head. scale 0: 1 / sqrt(k_dim)."""
+    dev = _current_device()
+    p = _linear_block(t, state, batch, q, k, v, out, decay, n_k_heads, decay_per_head, scale, decay_stride, q_stride, q_head_stride, k_stride,
+                      k_head_stride, v_stride, v_head_stride, out_stride, out_head_stride, workspace, workspace_bytes, status, status_keep, dev)
+    _check(lib().halo_mi_linear_attention(p, _raw_stream(stream, dev)))
+
+
+def linear_attention_workspace(t: int, state: LinearState, batch: LinearBatch, q, k, v, out, decay, n_k_heads: int, *,
+                               decay_per_head: bool = False, decay_stride: int = 0, q_stride: int = 0, q_head_stride: int = 0,
+                               k_stride: int = 0, k_head_stride: int = 0, v_stride: int = 0, v_head_stride: int = 0, out_stride: int = 0,
+                               out_head_stride: int = 0) -> int:
+    """Workspace bytes that the same linear_attention call makes use of (halo_mi_linear_attention_workspace)."""
+    dev = _current_device()
+    p = _linear_block(t, state, batch, q, k, v, out, decay, n_k_heads, decay_per_head, 0.0, decay_stride, q_stride, q_head_stride, k_stride,
+                      k_head_stride, v_stride, v_head_stride, out_stride, out_head_stride, None, 0, None, False, dev)
+    return int(lib().halo_mi_linear_attention_workspace(p))
 
 
 def stream_read(p, nbytes: int, workgroups: int, unroll: int, sink, stream=None) -> None:

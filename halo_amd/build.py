@@ -27,8 +27,8 @@ LIB = PKG / "libhalo_mi355x.so"
 CSRC = PKG / "csrc"
 # the kernel files first: they take longest and are compiled in parallel with the rest
 SOURCES = [CSRC / "k_attention.hip", CSRC / "k_gemv.hip", CSRC / "k_gemv_group.hip", CSRC / "k_gemv_gguf.hip", CSRC / "k_gemm.hip", CSRC / "k_gemm_sx.hip", CSRC / "k_dequant.hip", CSRC / "k_argmax.hip", CSRC / "k_norm.hip",
-           CSRC / "k_rope.hip", CSRC / "k_kv.hip", CSRC / "k_kv_pages.hip",
-           CSRC / "api.cpp", CSRC / "kv_api.cpp", CSRC / "upload.cpp", CSRC / "host_utils.cpp", CSRC / "backend.cpp"]
+           CSRC / "k_rope.hip", CSRC / "k_norm_rope.hip", CSRC / "k_quantize.hip", CSRC / "k_gemm_i8.hip", CSRC / "k_linear.hip", CSRC / "k_kv.hip", CSRC / "k_kv_pages.hip",
+           CSRC / "api.cpp", CSRC / "kv_api.cpp", CSRC / "layer_api.cpp", CSRC / "upload.cpp", CSRC / "host_utils.cpp", CSRC / "backend.cpp"]
 OBJ_DIR = PKG / "_build"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 

@@ -30,29 +30,6 @@ using namespace dev;
 
 constexpr uint32_t kKvBlock = 256;
 
-// The integer nearest to x / s (ties to even) as the low byte of the result's bits, for |x| <= 127 s (1 + 2^-23), s normal; inv =
-// 1 / s rounded. The multiply-add rounds x inv to an integer r, the quotient's or its neighbour (1.5 2^23 is where
-// fp32 has steps of 1), and e = x - r s decides: for r even and not 0, x >= 1.5 s is a multiple of s's last bit and e
-// fits 24 bits; for r = 0 e is x; for r = +-1 e is exact from x = s / 2 on, and below, where it may round to s / 2,
-// the tie moves an odd r the same way. Without EXACT only `unsure` is set where r may have to move.
-template <bool EXACT>
-__device__ __forceinline__ uint32_t nearest(float x, float s, float inv, bool& unsure) {
-    constexpr float kStepsOfOne = 12582912.0f;
-    const float t = fmaf(x, inv, kStepsOfOne), r = t - kStepsOfOne;
-    const float e = fmaf(-r, s, x), half = 0.5f * s;
-    if constexpr (EXACT) {
-        const bool move = fabsf(e) > half || (fabsf(e) == half && (__float_as_uint(t) & 1));
-        return __float_as_uint(move ? t + copysignf(1.0f, e) : t);
-    } else {
-        unsure = unsure || fabsf(e) >= half;
-        return __float_as_uint(t);
-    }
-}
-// The low bytes of four words.
-__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0400u), __builtin_amdgcn_perm(b, a, 0x0C0C0400u), 0x05040100u);
-}
-
 // The code c of a block of scale s0 in scale s1 > s0: the integer nearest to c * s0 / s1, exactly.
 __device__ __forceinline__ int32_t rescaled(int32_t c, float s0, float s1) {
     const double x2 = 2.0 * c * s0;

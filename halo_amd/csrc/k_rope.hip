@@ -17,6 +17,7 @@
 #include "kv.h"
 #include "kv_device.h"
 #include "launch.h"
+#include "rope_device.h"
 
 namespace halo_mi {
 namespace {
@@ -26,21 +27,6 @@ using namespace dev;
 constexpr uint32_t kRopeBlock = 256;
 constexpr uint32_t kRopeTokens = 1u << 23;  // of a launch: a grid has fewer than 2^32 threads along x
 constexpr uint32_t kRopePairs = HALO_MI_ROPE_INTERLEAVED;
-
-// cos and sin of `angle` radians: the nearest quarter turn comes off in 64 bits.
-__device__ __forceinline__ float2 turn(double angle) {
-    const double quarters = angle * 0.63661977236758134308;  // 2 / pi
-    const double n = rint(quarters);
-    float s, c;
-    sincospif((float)(quarters - n) * 0.5f, &s, &c);
-    const int32_t q = (int32_t)(int64_t)n & 3;
-    if (q & 1) {
-        const float t = s;
-        s = c;
-        c = -t;
-    }
-    return (q & 2) ? float2{-c, -s} : float2{c, s};
-}
 
 // One workgroup: token blockIdx.x, the heads from blockIdx.y * heads_per on. V elements per access.
 template <typename T, int V, bool INTERLEAVED>

@@ -1,4 +1,4 @@
-// The 8-bit paged cache between its C ABI (kv_api.cpp) and its kernels (k_rope.hip, k_kv.hip,
+// The 8-bit paged cache between its C ABI (kv_api.cpp) and its kernels (k_rope.hip, k_norm_rope.hip, k_kv.hip,
 // k_kv_pages.hip, k_attention.hip): geometry, argument blocks and launchers.
 #pragma once
 
@@ -55,6 +55,12 @@ struct RopeArgs {
     float factor;
 };
 
+struct NormRopeArgs {
+    RopeArgs rope;
+    const float* norm_w[2];  // of the parts; null: rotated only
+    float eps;
+};
+
 struct KvWriteArgs {
     KvLayer c;
     KvBatch b;
@@ -96,6 +102,7 @@ struct KvPagesArgs {
 };
 
 int launch_rope(uint32_t type, uint32_t pairs, const RopeArgs& a, hipStream_t st);
+int launch_norm_rope(uint32_t type, uint32_t pairs, const NormRopeArgs& a, hipStream_t st);
 int launch_kv_write(uint32_t type, const KvWriteArgs& a, hipStream_t st);
 int launch_kv_read(const KvReadArgs& a, hipStream_t st);
 // How the work is dealt out with part_bytes of partial results; returns the bytes made use of (0: nothing is split). Sets a.few,

@@ -1,75 +1,18 @@
 // The extern "C" entry points of attention over the 8-bit paged cache (include/halo_mi355x.h): argument
 // validation with the library's error mapping, geometry, the rotary frequencies, and the dispatch to
-// the launchers of k_rope.hip, k_kv.hip, k_kv_pages.hip and k_attention.hip.
+// the launchers of k_rope.hip, k_norm_rope.hip, k_kv.hip, k_kv_pages.hip and k_attention.hip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
 
+#include "checks.h"
 #include "kv.h"
 #include "launch.h"
 
 namespace halo_mi {
 namespace {
-
-// A range of an operand, for the overlap checks.
-struct Range {
-    const void* p;
-    uint64_t bytes;
-    const char* name;
-};
-
-int check_apart(const char* op, const Range& out, std::initializer_list<Range> others) {
-    for (const Range& r : others)
-        if (ranges_overlap(out.p, out.bytes, r.p, r.bytes)) return set_error(HALO_MI_E_KERNEL, "%s: %s overlaps %s", op, out.name, r.name);
-    return HALO_MI_OK;
-}
-
-uint32_t elem_bytes(uint32_t type) { return type == HALO_MI_F32 ? 4 : type == HALO_MI_F16 || type == HALO_MI_BF16 ? 2 : 0; }
-
-int check_type(const char* op, uint32_t type) {
-    if (elem_bytes(type) == 0) return set_error(HALO_MI_E_UNSUPPORTED, "%s: element type %u is not F32, F16 or BF16", op, type);
-    return HALO_MI_OK;
-}
-
-// Rows of heads: resolves the dense strides, checks alignment and that heads and rows do not overlap.
-// bytes receives the operand's extent.
-int check_rows(const char* op, const char* name, HeadRows& r, uint64_t rows, uint32_t heads, uint32_t dim, uint32_t size, uint64_t* bytes) {
-    if (r.head_stride == 0) r.head_stride = dim;
-    const uint64_t row = (uint64_t)(heads ? heads - 1 : 0) * r.head_stride + dim;
-    if (r.stride == 0) r.stride = (uint64_t)heads * r.head_stride;
-    *bytes = 0;
-    if (rows == 0 || heads == 0) return HALO_MI_OK;
-    if (!r.data) return set_error(HALO_MI_E_KERNEL, "%s: operand %s is empty", op, name);
-    if (r.head_stride > 1ull << 40 || r.stride > 1ull << 40 || (rows > 1 && r.stride > (1ull << 58) / rows)) return set_error(HALO_MI_E_KERNEL, "%s: a stride of %s is out of range", op, name);
-    if (heads > 1 && r.head_stride < dim) return set_error(HALO_MI_E_KERNEL, "%s: %s head stride < %u elements", op, name, dim);
-    // rows may lie inside the heads' stride (a layout [head][row][dim]) or around them
-    if (rows > 1 && r.stride < row && !(r.stride >= dim && (heads == 1 || r.head_stride >= (rows - 1) * r.stride + dim)))
-        return set_error(HALO_MI_E_KERNEL, "%s: %s row stride %llu lets rows overlap", op, name, (unsigned long long)r.stride);
-    if (reinterpret_cast<uintptr_t>(r.data) % size) return set_error(HALO_MI_E_KERNEL, "%s: %s must be %u-byte aligned", op, name, size);
-    *bytes = ((rows - 1) * r.stride + row) * size;
-    return HALO_MI_OK;
-}
-
-// Whether two operands share no element: their ranges are apart, or they lie side by side in rows of one
-// stride (q and k of a row-fused projection).
-bool apart_in_rows(const HeadRows& x, uint32_t x_heads, const HeadRows& y, uint32_t y_heads, uint32_t dim, uint32_t size, const Range& xr,
-                   const Range& yr) {
-    if (!ranges_overlap(xr.p, xr.bytes, yr.p, yr.bytes)) return true;
-    const uint64_t row = x.stride * size;
-    const uint64_t x_row = ((uint64_t)(x_heads - 1) * x.head_stride + dim) * size, y_row = ((uint64_t)(y_heads - 1) * y.head_stride + dim) * size;
-    if (x.stride != y.stride || x_row > row || y_row > row) return false;
-    const auto px = reinterpret_cast<uintptr_t>(x.data), py = reinterpret_cast<uintptr_t>(y.data);
-    const uint64_t off = py >= px ? (py - px) % row : (row - (px - py) % row) % row;  // of y's rows behind x's
-    return off >= x_row && off + y_row <= row;
-}
-
-int check_aligned(const char* op, const char* name, const void* p, uint32_t to) {
-    if (!p) return set_error(HALO_MI_E_KERNEL, "%s: operand %s is empty", op, name);
-    if (reinterpret_cast<uintptr_t>(p) % to) return set_error(HALO_MI_E_KERNEL, "%s: %s must be %u-byte aligned", op, name, to);
-    return HALO_MI_OK;
-}
 
 uint64_t page_bytes_of(uint32_t layers, uint32_t heads, uint32_t dim, uint32_t block) {
     if (dim != 64 && dim != 96 && dim != 128 && dim != 192 && dim != 256) return 0;
@@ -127,15 +70,6 @@ Range tables_range(const KvBatch& b) { return {b.tables, extent(b.n_seqs, b.tabl
 Range lens_range(const KvBatch& b) { return {b.kv_lens, (uint64_t)b.n_seqs * 4, "kv_lens"}; }
 Range starts_range(const KvBatch& b) { return {b.row_starts, ((uint64_t)b.n_seqs + 1) * 4, "row_starts"}; }
 
-// The optional status word is no operand of the call. It is cleared, unless the caller keeps it, once nothing else can refuse the
-// call.
-int check_status(const char* op, uint32_t* status, std::initializer_list<Range> others) {
-    if (!status) return HALO_MI_OK;
-    if (reinterpret_cast<uintptr_t>(status) % 4) return set_error(HALO_MI_E_KERNEL, "%s: status must be 4-byte aligned", op);
-    return check_apart(op, {status, 4, "status"}, others);
-}
-int clear_status(uint32_t* status, uint32_t keep, hipStream_t st) { return status && !keep ? launch_fill_u32(status, 1, 0u, st) : HALO_MI_OK; }
-
 // The checks of an attention call; *nothing: valid, but without rows.
 int check_attention(const halo_mi_attention_params* p, AttnArgs* a, std::initializer_list<Range*> ranges) {
     const char* op = "ATTENTION";
@@ -170,6 +104,56 @@ int check_attention(const halo_mi_attention_params* p, AttnArgs* a, std::initial
     const Range* found[] = {&q, &out};
     size_t i = 0;
     for (Range* r : ranges) *r = *found[i++];
+    return HALO_MI_OK;
+}
+
+// The checks of a rotation's operands. out receives the parts' outputs.
+int check_rope(const char* op, const halo_mi_rope_params* p, RopeArgs* args, Range* out) {
+    int rc;
+    if (!p || !p->parts) return set_error(HALO_MI_E_KERNEL, "%s: null params", op);
+    if ((rc = check_type(op, p->type))) return rc;
+    if (p->pairs > HALO_MI_ROPE_INTERLEAVED) return set_error(HALO_MI_E_CONFIG, "%s: unknown pairs %u", op, p->pairs);
+    if (p->n_parts == 0 || p->n_parts > 2) return set_error(HALO_MI_E_UNSUPPORTED, "%s: %u parts (1 or 2)", op, p->n_parts);
+    if (p->head_dim == 0 || p->head_dim > 65536) return set_error(HALO_MI_E_UNSUPPORTED, "%s: head_dim %u", op, p->head_dim);
+    if (p->rot_dims < 2 || p->rot_dims % 2 || p->rot_dims > 512 || p->rot_dims > p->head_dim)
+        return set_error(HALO_MI_E_KERNEL, "%s: rot_dims %u of %u is not even or not in 2..512", op, p->rot_dims, p->head_dim);
+    if (p->n_tokens > 0x7FFFFFFFu) return set_error(HALO_MI_E_KERNEL, "%s: n_tokens %u is out of range", op, p->n_tokens);
+    if (!std::isfinite(p->factor)) return set_error(HALO_MI_E_KERNEL, "%s: factor is not finite", op);
+    const uint32_t size = elem_bytes(p->type);
+    RopeArgs& a = *args;
+    Range in[2] = {};
+    out[0] = out[1] = {};
+    for (uint32_t i = 0; i < p->n_parts; ++i) {
+        const halo_mi_rope_part& s = p->parts[i];
+        RopePart& d = a.part[i];
+        d.heads = s.n_heads;
+        if (s.n_heads > 65535) return set_error(HALO_MI_E_UNSUPPORTED, "%s: %u heads", op, s.n_heads);
+        d.in = {s.in, s.in_stride, s.in_head_stride};
+        d.out = {s.out, s.out_stride, s.out_head_stride};
+        in[i] = {s.in, 0, "an input"};
+        out[i] = {s.out, 0, "an output"};
+        if ((rc = check_rows(op, "in", d.in, p->n_tokens, s.n_heads, p->head_dim, size, &in[i].bytes))) return rc;
+        if ((rc = check_rows(op, "out", d.out, p->n_tokens, s.n_heads, p->head_dim, size, &out[i].bytes))) return rc;
+        d.in_place = s.in == s.out && d.in.stride == d.out.stride && d.in.head_stride == d.out.head_stride;
+        if (!d.in_place && ranges_overlap(in[i].p, in[i].bytes, out[i].p, out[i].bytes))
+            return set_error(HALO_MI_E_KERNEL, "%s: out overlaps in", op);
+        a.heads += s.n_heads;
+    }
+    a.n_tokens = p->n_tokens;
+    a.dim = p->head_dim;
+    a.rot = p->rot_dims;
+    a.positions = p->positions;
+    a.freqs = p->freqs;
+    a.factor = p->factor;
+    if (a.n_tokens == 0 || a.heads == 0) return HALO_MI_OK;
+    if ((rc = check_aligned(op, "positions", p->positions, 4)) || (rc = check_aligned(op, "freqs", p->freqs, 8))) return rc;
+    for (int i = 0; i < 2; ++i) {
+        if ((rc = check_apart(op, out[i], {{p->positions, 4ull * a.n_tokens, "positions"}, {p->freqs, 4ull * a.rot, "freqs"}}))) return rc;
+        const RopePart &x = a.part[i], &y = a.part[1 - i];
+        if (!apart_in_rows(x.out, x.heads, y.in, y.heads, a.dim, size, out[i], in[1 - i]) ||
+            !apart_in_rows(x.out, x.heads, y.out, y.heads, a.dim, size, out[i], out[1 - i]))
+            return set_error(HALO_MI_E_KERNEL, "%s: an output overlaps the other part", op);
+    }
     return HALO_MI_OK;
 }
 
@@ -279,52 +263,32 @@ int halo_mi_rope_freqs(uint32_t rot_dims, double theta, const halo_mi_rope_scali
 
 int halo_mi_rope(const halo_mi_rope_params* p, void* stream) {
     clear_error();
-    const char* op = "PARTIAL_ROPE";
-    int rc;
-    if (!p || !p->parts) return set_error(HALO_MI_E_KERNEL, "%s: null params", op);
-    if ((rc = check_type(op, p->type))) return rc;
-    if (p->pairs > HALO_MI_ROPE_INTERLEAVED) return set_error(HALO_MI_E_CONFIG, "%s: unknown pairs %u", op, p->pairs);
-    if (p->n_parts == 0 || p->n_parts > 2) return set_error(HALO_MI_E_UNSUPPORTED, "%s: %u parts (1 or 2)", op, p->n_parts);
-    if (p->head_dim == 0 || p->head_dim > 65536) return set_error(HALO_MI_E_UNSUPPORTED, "%s: head_dim %u", op, p->head_dim);
-    if (p->rot_dims < 2 || p->rot_dims % 2 || p->rot_dims > 512 || p->rot_dims > p->head_dim)
-        return set_error(HALO_MI_E_KERNEL, "%s: rot_dims %u of %u is not even or not in 2..512", op, p->rot_dims, p->head_dim);
-    if (p->n_tokens > 0x7FFFFFFFu) return set_error(HALO_MI_E_KERNEL, "%s: n_tokens %u is out of range", op, p->n_tokens);
-    if (!std::isfinite(p->factor)) return set_error(HALO_MI_E_KERNEL, "%s: factor is not finite", op);
-    const uint32_t size = elem_bytes(p->type);
     RopeArgs a{};
-    Range in[2] = {}, out[2] = {};
-    for (uint32_t i = 0; i < p->n_parts; ++i) {
-        const halo_mi_rope_part& s = p->parts[i];
-        RopePart& d = a.part[i];
-        d.heads = s.n_heads;
-        if (s.n_heads > 65535) return set_error(HALO_MI_E_UNSUPPORTED, "%s: %u heads", op, s.n_heads);
-        d.in = {s.in, s.in_stride, s.in_head_stride};
-        d.out = {s.out, s.out_stride, s.out_head_stride};
-        in[i] = {s.in, 0, "an input"};
-        out[i] = {s.out, 0, "an output"};
-        if ((rc = check_rows(op, "in", d.in, p->n_tokens, s.n_heads, p->head_dim, size, &in[i].bytes))) return rc;
-        if ((rc = check_rows(op, "out", d.out, p->n_tokens, s.n_heads, p->head_dim, size, &out[i].bytes))) return rc;
-        d.in_place = s.in == s.out && d.in.stride == d.out.stride && d.in.head_stride == d.out.head_stride;
-        if (!d.in_place && ranges_overlap(in[i].p, in[i].bytes, out[i].p, out[i].bytes))
-            return set_error(HALO_MI_E_KERNEL, "%s: out overlaps in", op);
-        a.heads += s.n_heads;
-    }
-    a.n_tokens = p->n_tokens;
-    a.dim = p->head_dim;
-    a.rot = p->rot_dims;
-    a.positions = p->positions;
-    a.freqs = p->freqs;
-    a.factor = p->factor;
+    Range out[2];
+    if (int rc = check_rope("PARTIAL_ROPE", p, &a, out)) return rc;
     if (a.n_tokens == 0 || a.heads == 0) return HALO_MI_OK;
-    if ((rc = check_aligned(op, "positions", p->positions, 4)) || (rc = check_aligned(op, "freqs", p->freqs, 8))) return rc;
-    for (int i = 0; i < 2; ++i) {
-        if ((rc = check_apart(op, out[i], {{p->positions, 4ull * a.n_tokens, "positions"}, {p->freqs, 4ull * a.rot, "freqs"}}))) return rc;
-        const RopePart &x = a.part[i], &y = a.part[1 - i];
-        if (!apart_in_rows(x.out, x.heads, y.in, y.heads, a.dim, size, out[i], in[1 - i]) ||
-            !apart_in_rows(x.out, x.heads, y.out, y.heads, a.dim, size, out[i], out[1 - i]))
-            return set_error(HALO_MI_E_KERNEL, "%s: an output overlaps the other part", op);
-    }
     return launch_rope(p->type, p->pairs, a, static_cast<hipStream_t>(stream));
+}
+
+int halo_mi_norm_rope(const halo_mi_norm_rope_params* p, void* stream) {
+    clear_error();
+    const char* op = "norm_rope";
+    if (!p) return set_error(HALO_MI_E_KERNEL, "%s: null params", op);
+    NormRopeArgs a{};
+    Range out[2];
+    int rc;
+    if ((rc = check_rope(op, &p->rope, &a.rope, out))) return rc;
+    if (!(p->eps >= 0.0f) || !std::isfinite(p->eps)) return set_error(HALO_MI_E_KERNEL, "%s: eps must be finite and not negative", op);
+    if (a.rope.n_tokens == 0 || a.rope.heads == 0) return HALO_MI_OK;
+    a.eps = p->eps;
+    for (uint32_t i = 0; i < p->rope.n_parts; ++i) {
+        a.norm_w[i] = p->norm_w[i];
+        if (!a.norm_w[i]) continue;
+        if ((rc = check_aligned(op, "norm_w", a.norm_w[i], 4))) return rc;
+        for (const Range& r : out)
+            if ((rc = check_apart(op, r, {{a.norm_w[i], 4ull * a.rope.dim, "norm_w"}}))) return rc;
+    }
+    return launch_norm_rope(p->rope.type, p->rope.pairs, a, static_cast<hipStream_t>(stream));
 }
 
 uint64_t halo_mi_kv_page_bytes(uint32_t n_layers, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_tokens) {

@@ -1,4 +1,4 @@
-// Device helpers of the paged cache's kernels: element types, the pages of a sequence, the codes.
+// Device helpers of the paged cache's kernels and those beside them: element types, the pages of a sequence, the codes.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -30,6 +30,29 @@ __device__ __forceinline__ T from_f32(float v) {
 // |v| as a word that orders like it: infinities above every number, NaN above infinities.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 constexpr uint32_t kLargestFinite = 0x7F7FFFFFu;
+
+// The integer nearest to x / s (ties to even) as the low byte of the result's bits, for |x| <= 127 s (1 + 2^-23), s normal; inv =
+// 1 / s rounded. The multiply-add rounds x inv to an integer r, the quotient's or its neighbour (1.5 2^23 is where
+// fp32 has steps of 1), and e = x - r s decides: for r even and not 0, x >= 1.5 s is a multiple of s's last bit and e
+// fits 24 bits; for r = 0 e is x; for r = +-1 e is exact from x = s / 2 on, and below, where it may round to s / 2,
+// the tie moves an odd r the same way. Without EXACT only `unsure` is set where r may have to move.
+template <bool EXACT>
+__device__ __forceinline__ uint32_t nearest(float x, float s, float inv, bool& unsure) {
+    constexpr float kStepsOfOne = 12582912.0f;
+    const float t = fmaf(x, inv, kStepsOfOne), r = t - kStepsOfOne;
+    const float e = fmaf(-r, s, x), half = 0.5f * s;
+    if constexpr (EXACT) {
+        const bool move = fabsf(e) > half || (fabsf(e) == half && (__float_as_uint(t) & 1));
+        return __float_as_uint(move ? t + copysignf(1.0f, e) : t);
+    } else {
+        unsure = unsure || fabsf(e) >= half;
+        return __float_as_uint(t);
+    }
+}
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0400u), __builtin_amdgcn_perm(b, a, 0x0C0C0400u), 0x05040100u);
+}
 
 // A batch's rows of one sequence: its first row, row count and cached tokens. Row starts that fall or that
 // pass n_rows are cut to what the row operands hold.

@@ -472,6 +472,23 @@ typedef struct halo_mi_rope_params {
 int halo_mi_rope(const halo_mi_rope_params* p, void* stream);
 
 /*
+ * The norm of each head of q and k and the rotary positions in one pass over them: every head x becomes
+ *   (x_j / sqrt(sum_j x_j^2 / head_dim + eps)) * norm_w[i][j],
+ * which is then rotated as halo_mi_rope does; elements from rot_dims on are normed only. Sums and products are in 32 bits (a head
+ * whose squares sum past 2^128 becomes zeros), rounded once to `type` at the end.
+ *   rope: as halo_mi_rope takes it, with its checks.
+ *   norm_w[i]: head_dim fp32 of part i, or NULL (its heads are rotated only); no output may overlap it.
+ *   eps: finite, not negative.
+ */
+typedef struct halo_mi_norm_rope_params {
+    halo_mi_rope_params rope;
+    const float* norm_w[2];
+    float eps;
+} halo_mi_norm_rope_params;
+
+int halo_mi_norm_rope(const halo_mi_norm_rope_params* p, void* stream);
+
+/*
  * The cache: n_pages records of halo_mi_kv_page_bytes() bytes each (pool 16-byte aligned). A page holds
  * block_tokens tokens of every layer:
  *   int8 codes, for each layer: K [head][token][dim], then V [head][dim][token];
@@ -655,6 +672,114 @@ int halo_mi_kv_compact(const halo_mi_kv_cache* cache, const halo_mi_kv_state* st
  */
 int halo_mi_kv_copy_pages(const halo_mi_kv_cache* cache, const int32_t* src, const int32_t* dst, uint32_t n, uint32_t* status,
                           uint32_t status_keep, void* stream);
+
+/* ---- products of 8-bit integers --------------------------------------------------------------- */
+/*
+ * Rows held in 8 bits: codes (int8, a row of cols codes and zeros up to the next multiple of 16, rows codes_stride
+ * bytes apart, 16-byte aligned) and one fp32 scale each; a code c stands for c * scale. Both operands of halo_mi_gemm_i8 are
+ * such rows: x has a row for each token, w one for each output channel.
+ */
+
+/*
+ * Quantizes rows of x (rows x cols of `type` F32, F16 or BF16, x_stride elements apart, 0 = cols):
+ *   scale = max_i |x_i| / 127, rounded to fp32; one below 2^-80 counts as 0;
+ *   code  = x / scale rounded to the nearest integer, ties to even (0 where scale is 0).
+ * A row with a value that is not finite has scale NaN and codes 0. codes_stride: a multiple of 16, 0 = cols rounded
+ * up to 16; the zeros behind a row's codes are written too, what lies between them and the next row is not. codes and
+ * scales may not overlap x or each other. cols <= 131071, rows < 2^31.
+ */
+int halo_mi_quantize_rows(uint32_t type, const void* x, uint64_t x_stride, int8_t* codes, uint64_t codes_stride, float* scales,
+                          uint32_t rows, uint32_t cols, void* stream);
+
+/*
+ * y[t][n] = x_scales[t] * w_scales[n] * sum_i x[t][i] * w[n][i] for t < n_vec, n < rows, i < cols.
+ * The sum is exact (32-bit integers), so a row of y does not depend on the call's other rows; the scales are multiplied in fp32
+ * (x_scales[t] * w_scales[n] first, then with the sum rounded to fp32), and the result is rounded once to `type` (F32, F16, BF16).
+ *   w, x: int8 codes in rows of cols, as halo_mi_quantize_rows writes them (16-byte aligned; strides in bytes, multiples of 16,
+ *     0 = cols rounded up to 16, at most 2^20). The bytes from cols up to the next multiple of 16 are read, and are zeros in x or in
+ *     w. Codes of -128 are allowed.
+ *   w_scales: rows fp32, x_scales: n_vec fp32, any values.
+ *   y: n_vec rows of rows elements, y_stride elements apart (0 = rows); may not overlap the other operands.
+ *   cols <= 131071 (the sum fits 32 bits), rows and n_vec < 2^31.
+ */
+typedef struct halo_mi_gemm_i8_params {
+    uint32_t type;
+    const int8_t* w;
+    uint64_t w_stride;
+    const float* w_scales;
+    const int8_t* x;
+    uint64_t x_stride;
+    const float* x_scales;
+    void* y;
+    uint64_t y_stride;
+    uint32_t rows, cols, n_vec;
+} halo_mi_gemm_i8_params;
+
+int halo_mi_gemm_i8(const halo_mi_gemm_i8_params* p, void* stream);
+
+/* ---- linear attention ---------------------------------------------------------------------------- */
+/*
+ * Attention without a softmax over tokens that fade, for batches of sequences. Head h has a state S of k_dim x v_dim
+ * fp32 numbers, which holds all of a sequence's past; for a sequence's rows t in order
+ *   S <- exp(decay[t][h]) S + k[t][h'] v[t][h]^T,   out[t][h] = scale * S^T q[t][h'],   h' = h / (n_heads / n_k_heads).
+ * Prompts run in chunks on the matrix cores, few rows one after another; both follow the same formula.
+ *
+ * Rows [row_starts[s], row_starts[s + 1]) of the row operands are the next tokens of sequence s, whose state is slot slots[s]
+ * of the pool. A sequence without rows is left alone: its slot is not looked at. Rows below row_starts[0] or from row_starts[n_seqs] on are
+ * neither read nor written; row_starts that fall are cut as in halo_mi_kv_batch. The lists are read when the kernel runs, so a captured
+ * call follows their values at each replay. A slot outside [0, n_slots), or one that an earlier sequence with rows has, gives NaN rows, leaves the
+ * state alone and sets HALO_MI_STATUS_BAD_INDEX.
+ *   type: F32, F16 or BF16, of q, k, v and out. q, k: n_rows rows of n_k_heads heads of k_dim; v, out: of n_heads heads of v_dim; n_heads
+ *     is a multiple of n_k_heads. Strides in elements, 0 = dense.
+ *   decay: the logarithm of the factor on the state, fp32: n_rows rows of n_heads, decay_stride elements apart (0 = n_heads), or with
+ *     decay_per_head n_heads values that hold for every row. -infinity empties the state; values above 0 are taken as they are.
+ *   state: n_slots slots of n_heads x k_dim x v_dim fp32 (16-byte aligned, dense); state_out: where the new states go, of the same
+ *     shape; it is state itself, or does not overlap it (the states before the call are kept, as for a verify step that may be
+ *     taken back). Slots of state_out that no sequence with rows has keep their bytes.
+ *   seq_lens (optional): n_seqs int32, the tokens of each sequence with these rows. Where it is no more than the sequence's rows, the
+ *     sequence begins here, and its state is taken as zeros, whatever the slot holds.
+ *   k_dim, v_dim: 64, 96, 128, 192 or 256. scale: 0 = 1 / sqrt(k_dim).
+ *   max_rows: the most rows of a sequence, as the host knows it (0: n_rows). It chooses how the call runs; more rows on the device are
+ *     still computed whole, only slower.
+ *   workspace (optional, 16-byte aligned): device memory for the states inside long sequences, in place of the stream's own
+ *     workspace. Graphs captured on one stream share that stream's workspace: give each its own if their replays may overlap.
+ *     halo_mi_linear_attention_workspace() says what a call makes use of; with less (or on a capturing stream that has none
+ *     yet) sequences are split less.
+ * Numerics: the state, the sums and the decays are in 32 bits, the decays' running sums in 64. Where a value of v is not finite, its
+ * column of out is NaN from its row on, and that column of the state; one of k or a NaN decay: the head's rows from its own on.
+ * out may not overlap any other operand (it may lie beside q, k and v in rows of one stride), state_out none but state.
+ */
+typedef struct halo_mi_linear_attention_params {
+    uint32_t type;
+    uint32_t n_heads, n_k_heads, k_dim, v_dim;
+    const float* state;
+    float* state_out;
+    uint32_t n_slots;
+    const int32_t* slots;
+    const int32_t* row_starts;
+    const int32_t* seq_lens;
+    uint32_t n_seqs, n_rows, max_rows;
+    const void* q;
+    uint64_t q_stride, q_head_stride;
+    const void* k;
+    uint64_t k_stride, k_head_stride;
+    const void* v;
+    uint64_t v_stride, v_head_stride;
+    void* out;
+    uint64_t out_stride, out_head_stride;
+    const float* decay;
+    uint64_t decay_stride;
+    uint32_t decay_per_head;
+    float scale;
+    void* workspace;
+    uint64_t workspace_bytes;
+    uint32_t* status;
+    uint32_t status_keep;
+} halo_mi_linear_attention_params;
+
+int halo_mi_linear_attention(const halo_mi_linear_attention_params* p, void* stream);
+/* The workspace bytes that the call splits as it likes best with (0: none, or an argument out of range). */
+uint64_t halo_mi_linear_attention_workspace(const halo_mi_linear_attention_params* p);
 
 /* ---- stream state --------------------------------------------------------------------------- */
 /*
