@@ -110,6 +110,23 @@ def test_gemm_i8_strides(hl, dev, rows, cols, n_vec):
         product(hl, dev, t, rows, cols, n_vec, rng, w_pad=48, x_pad=16, y_pad=3, lo=-128)
 
 
+@pytest.mark.parametrize("rows,n_vec", [((1 << 21) + 40, 3), ((1 << 21) + 40, 17), (24, (1 << 16) + 100), (4500, 70)])
+def test_gemm_i8_past_a_launch(hl, dev, rows, n_vec):
+    """More channels or vectors than a launch takes: the ends of both, and the seams."""
+    import torch
+
+    print("[case] gemm_i8 past a launch", rows, n_vec, flush=True)
+    g = torch.Generator(device=dev).manual_seed(3)
+    cols = 24
+    w, x = (torch.randint(-127, 128, (n, 32), dtype=torch.int8, device=dev, generator=g) for n in (rows, n_vec))
+    x[:, cols:] = 0
+    ws, xs = (torch.rand(n, device=dev, generator=g) for n in (rows, n_vec))
+    y = torch.full((n_vec, rows), float("nan"), dtype=torch.bfloat16, device=dev)
+    hl.gemm_i8(BF16, w, ws, x, xs, y, rows, cols, n_vec)
+    want = torch.matmul(x.float(), w.float().t()).double() * (xs.double()[:, None] * ws.double())
+    assert bool(((y.double() - want).abs() <= want.abs() * (2.0 ** -8 * 1.01 + 2.0 ** -22)).all())
+
+
 def test_gemm_i8_largest_sums(hl, dev):
     """The longest rows of the largest codes: the sum takes all of 32 bits."""
     import torch
