@@ -141,6 +141,29 @@ struct Patch {
     Vec<T, 4> row[4];
 };
 
+// A row of a patch in its type's pieces.
+template <typename T>
+__device__ __forceinline__ void to_pieces(const Vec<T, 4>& x, uint2* w) {
+    if constexpr (kPieces<T> == 1) {
+        w[0] = __builtin_bit_cast(uint2, x);
+    } else {
+        const float f[4] = {to_f32(x.v[0]), to_f32(x.v[1]), to_f32(x.v[2]), to_f32(x.v[3])};
+        pieces_of<kPieces<T>>(f, w);
+    }
+}
+
+// The columns of a patch of 16-bit values.
+template <typename T>
+__device__ __forceinline__ void turned(const Patch<T>& p, uint2* w) {
+    uint2 r[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) r[t] = __builtin_bit_cast(uint2, p.row[t]);
+    w[0] = {__builtin_amdgcn_perm(r[1].x, r[0].x, 0x05040100u), __builtin_amdgcn_perm(r[3].x, r[2].x, 0x05040100u)};
+    w[1] = {__builtin_amdgcn_perm(r[1].x, r[0].x, 0x07060302u), __builtin_amdgcn_perm(r[3].x, r[2].x, 0x07060302u)};
+    w[2] = {__builtin_amdgcn_perm(r[1].y, r[0].y, 0x05040100u), __builtin_amdgcn_perm(r[3].y, r[2].y, 0x05040100u)};
+    w[3] = {__builtin_amdgcn_perm(r[1].y, r[0].y, 0x07060302u), __builtin_amdgcn_perm(r[3].y, r[2].y, 0x07060302u)};
+}
+
 // Whether one of a patch's elements is not a finite number.
 template <typename T>
 __device__ __forceinline__ bool not_finite(const Patch<T>& p) {
@@ -168,7 +191,7 @@ __device__ __forceinline__ bool not_finite(const Patch<T>& p) {
 // The chunked form. With b_i the sum of a chunk's decays up to its row i, S the state before the chunk and P_ij = e^(b_i - b_j) q_i . k_j for
 // j <= i:
 //   out_i = scale (e^(b_i) S^T q_i + sum_j P_ij v_j),     S <- e^(b_last) S + sum_j (e^(b_last - b_j) k_j) v_j^T.
-// One workgroup: 32 WAVES columns of a head's state, for a sequence or a segment of it. A wave keeps its 32 columns of S in its registers as
+// One workgroup: 16 UT WAVES columns of a head's state, for a sequence or a segment of it. A wave keeps its 16 UT columns of S in its registers as
 // the products leave them (rows 4 (lane / 16) + i, column lane % 16), which is also how the next product takes S^T: its order of k_dim is
 // that of the registers, and q and k lie in LDS in the same order. Products are of bf16 pieces, summed in 32 bits: q, k and v exactly (one
 // piece for BF16, two for F16, three for F32), the faded k in three, P and S in two where the output has 16 bits, else in three; of pairs of
@@ -182,12 +205,6 @@ struct Segments {
     float* states;          // what a segment but the last of its sequence adds, then the state before the next one; [boundary][head][k_dim][v_dim]
     float* fades;           // ... and its decays' sum (log2): [boundary][head]
 };
-
-// Which pieces of a row of q or k change places, so that 16 rows' pieces of one place lie in 16 different sixteenths of the banks.
-template <int KD>
-__device__ __forceinline__ uint32_t row_swap(uint32_t token) {
-    return KD % 128 == 0 ? token & 15 : KD == 96 ? token / 4 & 3 : token / 2 & 7;
-}
 
 // A sequence's boundaries between segments: their number, and how many lie before it. Where the room for their states ends (row starts that
 // fall count rows twice), a sequence is not cut. For all of a workgroup.
@@ -215,15 +232,50 @@ __device__ __forceinline__ bool look_up(const LinearArgs& a, const Segments& seg
     return good;
 }
 
-template <typename T, int KD, int WAVES, bool STATES>
-__global__ __launch_bounds__(WAVES * 64) void k_linear_chunks(LinearArgs a, Segments seg) {
+// LDS serves a 16-byte read of 64 lanes in four parts, each with lanes 4 .. 11 of one quarter of the wave and the others of its neighbour. With rows
+// an odd number of 16 bytes long, their pieces lie in different banks once rows 4 .. 11 of 16 have their pieces' pairs swapped.
+__device__ __forceinline__ uint32_t beside(uint32_t row) { return (row + 4) / 8 & 1; }
+
+// k^T and v^T: a row has a dim's 32 tokens, in 5 units of 16 bytes. Threads write four dims each, all lanes the same one of their four at a time, and
+// the products read 16 dims side by side: rows of equal row % 4 lie together, in planes that begin a quarter of the banks apart.
+constexpr int plane_of(int rows) { return rows / 4 * 5 + (20 - rows / 4 * 5 % 16) % 16; }
+template <int ROWS>
+__device__ __forceinline__ uint32_t turned_row(uint32_t row) { return row % 4 * plane_of(ROWS) + row / 4 * 5; }
+
+// LDS of a workgroup in units of 16 bytes: rows of q (which out passes through on its way), rows of k, k^T, v^T, and P by its rows.
+template <typename T, int KD>
+struct ChunkLds {
+    static constexpr int R = KD / 8 + 1;  // of a row of q or k
+    static constexpr int rows = kPieces<T> * kChunk * R, kt = 4 * plane_of(KD), p = kOutPieces<T> * kChunk * 5;
+    static constexpr int q(int columns) { return rows > kChunk * columns * (int)sizeof(T) / 16 ? rows : kChunk * columns * (int)sizeof(T) / 16; }
+    static constexpr int vt(int columns) { return 4 * plane_of(columns); }
+    static constexpr int bytes(int columns, bool k_rows) { return 16 * (q(columns) + (k_rows ? rows : 0) + 3 * kt + kPieces<T> * vt(columns) + p) + 2048; }
+};
+constexpr int kLds = 160 * 1024;
+// k's rows lie in LDS too, unless they keep a second workgroup from the CU, or do not fit; then they are read from memory again.
+template <typename T, int KD>
+constexpr bool k_in_lds(int columns) {
+    return ChunkLds<T, KD>::bytes(columns, true) <= (ChunkLds<T, KD>::bytes(columns, false) <= kLds / 2 ? kLds / 2 : kLds);
+}
+
+// The waves of a SIMD that a workgroup's registers leave room for: two, where LDS takes two workgroups or a workgroup is that many.
+template <typename T, int KD, int WAVES, int UT, bool STATES>
+constexpr int waves_at_least() {
+    typedef ChunkLds<T, KD> L;
+    constexpr int columns = 16 * UT * WAVES;
+    constexpr int bytes = STATES ? 16 * (3 * L::kt + kPieces<T> * L::vt(columns)) + 2048 : L::bytes(columns, k_in_lds<T, KD>(columns));
+    return bytes <= kLds / 2 && WAVES > 2 ? 2 : (WAVES + 3) / 4;
+}
+
+template <typename T, int KD, int WAVES, int UT, bool STATES>
+__global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATES>())) void k_linear_chunks(LinearArgs a, Segments seg) {
     constexpr int NP = kPieces<T>, NO = kOutPieces<T>, KT = KD / 16, KS = KD / 32, THREADS = WAVES * 64;
-    constexpr int QP = (KD / 4 * 8 + THREADS - 1) / THREADS;  // patches of q and k per thread
-    constexpr int kColumnsHere = 32 * WAVES;
-    constexpr bool K_ROWS = NP * KD < 768;  // k's rows lie in LDS too, where they fit
-    // Rows of q and k: KD codes of 2 bytes, 16-byte pieces swapped by the row; of k^T, v^T and P: 32 tokens, pieces swapped by a quarter of the row.
-    __shared__ uint4 q_lds[STATES ? 1 : NP * kChunk * KD / 8], k_lds[STATES || !K_ROWS ? 1 : NP * kChunk * KD / 8], kt_lds[3 * KD * 4], vt_lds[NP * kColumnsHere * 4],
-        p_lds[STATES ? 1 : NO * kChunk * 4];
+    constexpr int QP = (KD / 4 + THREADS / 8 - 1) / (THREADS / 8);  // patches of q and k per thread
+    constexpr int kColumnsHere = 16 * UT * WAVES;
+    constexpr bool K_ROWS = k_in_lds<T, KD>(kColumnsHere);
+    typedef ChunkLds<T, KD> L;
+    constexpr int R = L::R, KT_SIZE = L::kt, VT_SIZE = L::vt(kColumnsHere);
+    __shared__ uint4 q_lds[STATES ? 1 : L::q(kColumnsHere)], k_lds[STATES || !K_ROWS ? 1 : L::rows], kt_lds[3 * KT_SIZE], vt_lds[NP * VT_SIZE], p_lds[STATES ? 1 : L::p];
     __shared__ double sums_lds[kChunk];
     __shared__ int32_t bad_at[kColumnsHere];
     __shared__ int32_t bad_chunk;
@@ -231,15 +283,15 @@ __global__ __launch_bounds__(WAVES * 64) void k_linear_chunks(LinearArgs a, Segm
     const uint32_t v_blocks = a.v_dim / kColumnsHere, head = blockIdx.x / v_blocks, v0 = blockIdx.x % v_blocks * kColumnsHere;
     const uint32_t s = blockIdx.z, part = blockIdx.y;
     const LinearRows r = linear_rows(a, s);
-    // the segment's rows; the last segment has all that are left
-    const uint32_t first = part * seg.length;
-    if (first >= r.rows) return;
+    if (part > cuts_of(seg, r.rows) || r.rows == 0) return;
     const int32_t slot = a.slots[s];
     Cuts cuts;
     const bool bad = !look_up(a, seg, s, slot, r.rows, THREADS, cuts);
     if (part > cuts.parts || (STATES && part == cuts.parts)) return;
     const bool last_part = part == cuts.parts, begins = a.seq_lens && a.seq_lens[s] <= (int32_t)r.rows;
-    const uint32_t rows = last_part ? r.rows - first : seg.length, row0 = r.row0 + first, boundary = cuts.base + part;
+    // equal segments of whole chunks; the last one has what is left
+    const uint32_t each = (r.rows / (cuts.parts + 1) + kChunk) / kChunk * kChunk, first = part * each;
+    const uint32_t rows = last_part ? r.rows - min(first, r.rows) : min(each, r.rows - min(first, r.rows)), row0 = r.row0 + first, boundary = cuts.base + part;
     const uint32_t hk = head / a.group;
     T* out = const_cast<T*>(static_cast<const T*>(a.out.data)) + row0 * a.out.stride + head * a.out.head_stride + v0;
     if (bad) {
@@ -255,8 +307,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_linear_chunks(LinearArgs a, Segm
     const float* dg = a.decay + (uint64_t)row0 * a.decay_stride + head;
 
     // ---- the state: tile (t, u) has rows 16 t .. and columns 32 wave + 16 u ..
-    const uint64_t plane = (uint64_t)KD * a.v_dim, mine = v0 + wave * 32 + m + (uint64_t)(4 * g) * a.v_dim;
-    float4v S[KT][2] = {};
+    const uint64_t plane = (uint64_t)KD * a.v_dim, mine = v0 + wave * (16 * UT) + m + (uint64_t)(4 * g) * a.v_dim;
+    float4v S[KT][UT] = {};
     const float* before = nullptr;
     if (!STATES) {
         if (part > 0) before = seg.states + ((uint64_t)(boundary - 1) * a.heads + head) * plane;
@@ -266,86 +318,117 @@ __global__ __launch_bounds__(WAVES * 64) void k_linear_chunks(LinearArgs a, Segm
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < UT; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) S[t][u][i] = before[mine + (uint64_t)(16 * t + i) * a.v_dim + 16 * u];
 
-    // ---- a chunk's way into the registers, one chunk ahead
+    // ---- a chunk's way into the registers, one chunk ahead. This thread's patches: 4 tokens by 4 dims, lanes along
+    // the dims, so that a load covers whole lines. Rows behind the last are read as the last one, and put to zero on the way to LDS.
+    const uint32_t my_token = tid / (THREADS / 8) * 4, my_dim = tid % (THREADS / 8) * 4;
     Patch<T> qn[QP], kn[QP], vn;
-    float dn = 0.0f;
-    const auto patch = [&](const T* base, uint64_t stride, uint32_t row, uint32_t dim) {
-        Patch<T> p;
+    const T *q_from = qg, *k_from = kg, *v_from = vg;
+    const float* d_from = dg + lane % kChunk * a.decay_stride;
+    uint32_t q_off[4], k_off[4], v_off[4];
+    const auto place = [&](uint32_t left) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            p.row[t] = Vec<T, 4>{};
-            if (row + t < rows) p.row[t] = __builtin_bit_cast(Vec<T, 4>, *reinterpret_cast<const Loose<T, 4>*>(base + (row + t) * stride + dim));
+            const uint32_t token = min(my_token + t, left - 1);
+            q_off[t] = (token * (uint32_t)a.q.stride + my_dim) * sizeof(T);
+            k_off[t] = (token * (uint32_t)a.k.stride + my_dim) * sizeof(T);
+            v_off[t] = (token * (uint32_t)a.v.stride + my_dim) * sizeof(T);
         }
-        return p;
     };
-    const auto fetch = [&](uint32_t at) {
+    const auto fetch = [&](uint32_t left) {
+        if (left < kChunk) place(left);
+        const auto patch = [&](Patch<T>& p, const T* from, const uint32_t* off, int more) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                p.row[t] = __builtin_bit_cast(Vec<T, 4>, *reinterpret_cast<const Loose<T, 4>*>(reinterpret_cast<const uint8_t*>(from + more) + off[t]));
+        };
 #pragma unroll
         for (int j = 0; j < QP; ++j) {
-            const uint32_t i = tid + j * THREADS;
-            if (KD / 4 * 8 % THREADS != 0 && i >= KD / 4 * 8) continue;
-            const uint32_t dim = i % (KD / 4) * 4, row = at + i / (KD / 4) * 4;
-            if (!STATES) qn[j] = patch(qg, a.q.stride, row, dim);
-            kn[j] = patch(kg, a.k.stride, row, dim);
+            if (KD % (THREADS / 2) != 0 && my_dim + j * (THREADS / 2) >= KD) continue;
+            if (!STATES) patch(qn[j], q_from, q_off, j * (THREADS / 2));
+            patch(kn[j], k_from, k_off, j * (THREADS / 2));
         }
-        vn = patch(vg, a.v.stride, at + tid / (kColumnsHere / 4) * 4, tid % (kColumnsHere / 4) * 4);
-        // a decay of -infinity, or far under the smallest exponential, empties the state; NaN stays
-        const uint32_t t = at + lane % kChunk;
-        dn = t < rows ? dg[t * a.decay_stride] : 0.0f;
+        if (my_dim < kColumnsHere) patch(vn, v_from, v_off, 0);
+        q_from += kChunk * a.q.stride;
+        k_from += kChunk * a.k.stride;
+        v_from += kChunk * a.v.stride;
     };
     // q and k in the order of S's registers: dims 4 g .. + 3 and 16 + 4 g .. + 3 of 32 side by side
     const auto put_row = [](uint4* lds, int np, uint32_t token, uint32_t dim, uint2 v) {
-        reinterpret_cast<uint2*>(lds)[((np * kChunk + token) * (KD / 8) + ((dim / 32 * 4 + dim % 16 / 4) ^ row_swap<KD>(token))) * 2 + dim % 32 / 16] = v;
+        reinterpret_cast<uint2*>(lds)[((np * kChunk + token) * R + ((dim / 32 * 4 + dim % 16 / 4) ^ beside(token))) * 2 + dim % 32 / 16] = v;
     };
-    const auto row_at = [&](int np, uint32_t token, uint32_t ks) { return (np * kChunk + token) * (KD / 8) + ((ks * 4 + g) ^ row_swap<KD>(token)); };
-    const auto column_at = [](uint32_t row, uint32_t piece) { return row * 4 + (piece ^ (row / 4 & 3)); };
+    const auto row_at = [&](int np, uint32_t token, uint32_t ks) { return (np * kChunk + token) * R + ((ks * 4 + g) ^ beside(token)); };
+    // four tokens of a row that begins at `from`
+    const auto put_tokens = [](uint4* lds, uint32_t from, uint32_t row, uint32_t token, uint2 v) {
+        reinterpret_cast<uint2*>(lds)[(from + (token / 8 ^ beside(row))) * 2 + token / 4 % 2] = v;
+    };
+    const auto p_row = [](int x, uint32_t row) { return (x * kChunk + row) * 5; };
 
     for (uint32_t i = tid; i < kColumnsHere; i += THREADS) bad_at[i] = kChunk;
     if (tid == 0) bad_chunk = -1;
-    double total = 0.0;
-    fetch(0);
-    __syncthreads();
-    for (uint32_t at = 0; at < rows; at += kChunk) {
-        // ---- the decays' running sums, in 64 bits and turns of log2
-        double b = (double)(dn < -1e4f ? -1e4f : dn) * 1.4426950408889634;
+    // The decays' running sums of a chunk, in 64 bits and turns of log2: lane % 32 has its row's. A decay of -infinity, or far under the
+    // smallest exponential, empties the state; NaN stays.
+    const auto next_decay = [&](uint32_t at) {
+        const float d = at + lane % kChunk < rows ? *d_from : 0.0f;
+        d_from += kChunk * a.decay_stride;
+        return d;
+    };
+    const auto running = [&](float d) {
+        double b = (double)(d < -1e4f ? -1e4f : d) * 1.4426950408889634;
 #pragma unroll
         for (int i = 1; i < kChunk; i *= 2) {
             const double o = __shfl_up(b, i, kChunk);
             if ((int)(lane % kChunk) >= i) b += o;
         }
-        const double b_last = __shfl(b, kChunk - 1, kChunk);
+        return b;
+    };
+    // S is 2^held times what the registers hold: they take the decays only when those have grown large
+    double held = 0.0, total = 0.0;
+    if (rows) {
+        place(kChunk);
+        fetch(rows);
+    }
+    double b = running(next_decay(0));
+    float decay_ahead = next_decay(kChunk);
+    __syncthreads();
+    for (uint32_t at = 0; at < rows; at += kChunk) {
+        const double b_last = __shfl(b, kChunk - 1, kChunk), grown = held + b_last;
+        const bool settle = !(fabs(grown) < 40.0);
+        const float row_fade = __builtin_amdgcn_exp2f((float)(b + held)) * a.scale;                      // on S^T q of row lane % 32
+        const float k_fade = __builtin_amdgcn_exp2f((float)(settle ? b_last - b : b_last - b - grown));  // on k of token lane % 32
         if (STATES) total += b_last;
         if (tid < kChunk) sums_lds[tid] = b;
         // ---- to LDS, in pieces
+        if (rows - at < kChunk) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (my_token + t >= rows - at) {
+#pragma unroll
+                    for (int j = 0; j < QP; ++j) qn[j].row[t] = kn[j].row[t] = Vec<T, 4>{};
+                    vn.row[t] = Vec<T, 4>{};
+                }
+        }
+        float fade[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) fade[t] = __shfl(k_fade, my_token + t, kChunk);
 #pragma unroll
         for (int j = 0; j < QP; ++j) {
-            const uint32_t i = tid + j * THREADS;
-            const uint32_t dim = i % (KD / 4) * 4, token = i / (KD / 4) * 4;
-            // every lane takes part in the cross-lane reads
-            float fade[4];
+            const uint32_t dim = my_dim + j * (THREADS / 2);
+            if (KD % (THREADS / 2) != 0 && dim >= KD) continue;
+            if constexpr (!STATES) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) fade[t] = __builtin_amdgcn_exp2f((float)(b_last - __shfl(b, (token + t) % kChunk, kChunk)));
-            if (KD / 4 * 8 % THREADS != 0 && i >= KD / 4 * 8) continue;
-            float kf[4][4];
+                for (int t = 0; t < 4; ++t) {
+                    uint2 w[NP];
+                    to_pieces(qn[j].row[t], w);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                uint2 w[NP > 3 ? NP : 3];
-                float qf[4];
-#pragma unroll
-                for (int d = 0; d < 4; ++d) kf[t][d] = to_f32(kn[j].row[t].v[d]);
-                if constexpr (!STATES) {
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) qf[d] = to_f32(qn[j].row[t].v[d]);
-                    pieces_of<NP>(qf, w);
-#pragma unroll
-                    for (int p = 0; p < NP; ++p) put_row(q_lds, p, token + t, dim, w[p]);
+                    for (int p = 0; p < NP; ++p) put_row(q_lds, p, my_token + t, dim, w[p]);
                     if constexpr (K_ROWS) {
-                        pieces_of<NP>(kf[t], w);
+                        to_pieces(kn[j].row[t], w);
 #pragma unroll
-                        for (int p = 0; p < NP; ++p) put_row(k_lds, p, token + t, dim, w[p]);
+                        for (int p = 0; p < NP; ++p) put_row(k_lds, p, my_token + t, dim, w[p]);
                     }
                 }
             }
@@ -354,34 +437,43 @@ __global__ __launch_bounds__(WAVES * 64) void k_linear_chunks(LinearArgs a, Segm
                 uint2 w[3];
                 float f[4];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) f[t] = kf[t][d] * fade[t];
+                for (int t = 0; t < 4; ++t) f[t] = to_f32(kn[j].row[t].v[d]) * fade[t];
                 pieces_of<3>(f, w);
 #pragma unroll
-                for (int p = 0; p < 3; ++p) reinterpret_cast<uint2*>(kt_lds)[column_at(p * KD + dim + d, token / 8) * 2 + token / 4 % 2] = w[p];
+                for (int p = 0; p < 3; ++p) put_tokens(kt_lds, p * KT_SIZE + turned_row<KD>(dim + d), dim + d, my_token, w[p]);
             }
         }
-        {
-            const uint32_t col = tid % (kColumnsHere / 4) * 4, token = tid / (kColumnsHere / 4) * 4;
-            const bool odd = not_finite(vn);
-            if (odd) bad_chunk = (int32_t)(at / kChunk);
+        if (my_dim < kColumnsHere) {
+            if (not_finite(vn)) {
+                bad_chunk = (int32_t)(at / kChunk);
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                uint2 w[NP];
-                float f[4];
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    f[t] = to_f32(vn.row[t].v[d]);
-                    if (odd && abs_bits(f[t]) > kLargestFinite) {
-                        atomicMin(&bad_at[col + d], (int32_t)(token + t));
-                        f[t] = 0.0f;
-                    }
+                    for (int d = 0; d < 4; ++d)
+                        if (abs_bits(to_f32(vn.row[t].v[d])) > kLargestFinite) {
+                            atomicMin(&bad_at[my_dim + d], (int32_t)(my_token + t));
+                            vn.row[t].v[d] = from_f32<T>(0.0f);
+                        }
+            }
+            if constexpr (NP == 1) {
+                uint2 w[4];
+                turned(vn, w);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) put_tokens(vt_lds, turned_row<kColumnsHere>(my_dim + d), my_dim + d, my_token, w[d]);
+            } else {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    uint2 w[NP];
+                    const float f[4] = {to_f32(vn.row[0].v[d]), to_f32(vn.row[1].v[d]), to_f32(vn.row[2].v[d]), to_f32(vn.row[3].v[d])};
+                    pieces_of<NP>(f, w);
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) put_tokens(vt_lds, p * VT_SIZE + turned_row<kColumnsHere>(my_dim + d), my_dim + d, my_token, w[p]);
                 }
-                pieces_of<NP>(f, w);
-#pragma unroll
-                for (int p = 0; p < NP; ++p) reinterpret_cast<uint2*>(vt_lds)[column_at(p * kColumnsHere + col + d, token / 8) * 2 + token / 4 % 2] = w[p];
             }
         }
-        if (at + kChunk < rows) fetch(at + kChunk);
+        const float decays = decay_ahead;  // the next chunk's, asked for a chunk ago
+        if (at + kChunk < rows) fetch(rows - at - kChunk);
+        decay_ahead = next_decay(at + 2 * kChunk);
         __syncthreads();
         const bool some_bad = bad_chunk == (int32_t)(at / kChunk);
         // ---- P^T = K Q^T: tiles (tokens 16 jt .., rows 16 it ..) on and under the diagonal
@@ -420,19 +512,19 @@ __global__ __launch_bounds__(WAVES * 64) void k_linear_chunks(LinearArgs a, Segm
                 float f[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float w = p[i] * __builtin_amdgcn_exp2f((float)(bi - sums_lds[16 * jt + 4 * g + i]));
+                    const float w = p[i] * (__builtin_amdgcn_exp2f((float)(bi - sums_lds[16 * jt + 4 * g + i])) * a.scale);
                     f[i] = it > jt || m >= 4 * g + i ? w : 0.0f;
                 }
                 uint2 w[NO];
                 pieces_of<NO>(f, w);
 #pragma unroll
-                for (int x = 0; x < NO; ++x) reinterpret_cast<uint2*>(p_lds)[column_at(x * kChunk + 16 * it + m, 2 * jt + g / 2) * 2 + g % 2] = w[x];
+                for (int x = 0; x < NO; ++x) put_tokens(p_lds, p_row(x, 16 * it + m), m, 16 * jt + 4 * g, w[x]);
                 if (tile == 0)  // tokens 16 .. 31 of rows 0 .. 15
 #pragma unroll
-                    for (int x = 0; x < NO; ++x) reinterpret_cast<uint2*>(p_lds)[column_at(x * kChunk + m, 2 + g / 2) * 2 + g % 2] = uint2{0, 0};
+                    for (int x = 0; x < NO; ++x) put_tokens(p_lds, p_row(x, m), m, 16 + 4 * g, uint2{0, 0});
             }
             // ---- out^T = S^T q^T, faded
-            float4v o[2][2] = {};
+            float4v o[UT][2] = {};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 uint4 qf[NP][2];
@@ -441,7 +533,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_linear_chunks(LinearArgs a, Segm
 #pragma unroll
                     for (int it = 0; it < 2; ++it) qf[x][it] = q_lds[row_at(x, 16 * it + m, ks)];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < UT; ++u) {
                     uint2 lo[NO], hi[NO];
                     pieces_of<NO>(reinterpret_cast<const float*>(&S[2 * ks][u]), lo);
                     pieces_of<NO>(reinterpret_cast<const float*>(&S[2 * ks + 1][u]), hi);
@@ -455,80 +547,98 @@ __global__ __launch_bounds__(WAVES * 64) void k_linear_chunks(LinearArgs a, Segm
             }
 #pragma unroll
             for (int it = 0; it < 2; ++it) {
-                const float fade = __builtin_amdgcn_exp2f((float)sums_lds[16 * it + m]);
+                const float f = __shfl(row_fade, 16 * it + m, kChunk);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) o[u][it] *= fade;
+                for (int u = 0; u < UT; ++u) o[u][it] *= f;
             }
             __syncthreads();
             // ---- ... and V^T P^T
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < UT; ++u)
 #pragma unroll
                 for (int x = 0; x < NP; ++x) {
-                    const uint4 vf = vt_lds[column_at(x * kColumnsHere + wave * 32 + 16 * u + m, g)];
+                    const uint4 vf = vt_lds[x * VT_SIZE + turned_row<kColumnsHere>(wave * (16 * UT) + 16 * u + m) + (g ^ beside(m))];
 #pragma unroll
                     for (int y = 0; y < NO && x + y < NO; ++y)
 #pragma unroll
-                        for (int it = 0; it < 2; ++it) o[u][it] = mfma(vf, p_lds[column_at(y * kChunk + 16 * it + m, g)], o[u][it]);
+                        for (int it = 0; it < 2; ++it) o[u][it] = mfma(vf, p_lds[p_row(y, 16 * it + m) + (g ^ beside(m))], o[u][it]);
                 }
+            // ---- out, by way of this wave's part of LDS: lanes side by side in a row
+            constexpr int OP = 16 * UT * sizeof(T) / 16;  // pieces of a row
+            uint8_t* const o_lds = reinterpret_cast<uint8_t*>(q_lds) + wave * (kChunk * OP * 16);
+            const auto o_at = [](uint32_t row, uint32_t piece) { return (row * OP + (piece ^ (OP == 8 ? row / 2 & 7 : OP == 4 ? row / 4 & 3 : row / 8 & 1))) * 16; };
 #pragma unroll
-            for (int it = 0; it < 2; ++it) {
-                const uint32_t row = 16 * it + m;
-                if (at + row >= rows) continue;
+            for (int it = 0; it < 2; ++it)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint32_t col = wave * 32 + 16 * u + 4 * g;
-                    Loose<T, 4> y;
+                for (int u = 0; u < UT; ++u) {
+                    const uint32_t col = 16 * u + 4 * g, row = 16 * it + m;
+                    Vec<T, 4> y;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float v = o[u][it][i] * a.scale;
-                        if (some_bad && bad_at[col + i] <= (int32_t)row) v = __uint_as_float(0x7FC00000u);
+                        float v = o[u][it][i];
+                        if (some_bad && bad_at[wave * (16 * UT) + col + i] <= (int32_t)row) v = __uint_as_float(0x7FC00000u);
                         y.v[i] = from_f32<T>(v);
                     }
-                    *reinterpret_cast<Loose<T, 4>*>(out + (uint64_t)(at + row) * a.out.stride + col) = y;
+                    *reinterpret_cast<Vec<T, 4>*>(o_lds + o_at(row, col * sizeof(T) / 16) + col * sizeof(T) % 16) = y;
                 }
+            // the wave reads what its own lanes wrote: LDS serves a wave in order
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int j = 0; j < kChunk * OP / 64; ++j) {
+                const uint32_t row = (j * 64 + lane) / OP, piece = (j * 64 + lane) % OP;
+                typedef Loose<T, 16 / sizeof(T)> Piece;
+                const uint4 y = *reinterpret_cast<const uint4*>(o_lds + o_at(row, piece));
+                if (at + row < rows)
+                    *reinterpret_cast<Piece*>(out + (uint64_t)(at + row) * a.out.stride + wave * (16 * UT) + piece * (16 / sizeof(T))) = __builtin_bit_cast(Piece, y);
             }
         }
+        b = running(decays);
         // ---- S <- e^(b_last) S + k^T v
-        const float fade = __builtin_amdgcn_exp2f((float)b_last);
-        uint4 vf[NP][2];
+        held = settle ? 0.0 : grown;
+        if (settle) {
+            const float f = __builtin_amdgcn_exp2f((float)grown);
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int u = 0; u < UT; ++u) S[t][u] *= f;
+        }
+        uint4 vf[NP][UT];
 #pragma unroll
         for (int x = 0; x < NP; ++x)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) vf[x][u] = vt_lds[column_at(x * kColumnsHere + wave * 32 + 16 * u + m, g)];
+            for (int u = 0; u < UT; ++u) vf[x][u] = vt_lds[x * VT_SIZE + turned_row<kColumnsHere>(wave * (16 * UT) + 16 * u + m) + (g ^ beside(m))];
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) S[t][u] *= fade;
-#pragma unroll
             for (int x = 0; x < 3; ++x) {
-                const uint4 kf = kt_lds[column_at(x * KD + 16 * t + m, g)];
+                const uint4 kf = kt_lds[x * KT_SIZE + turned_row<KD>(16 * t + m) + (g ^ beside(m))];
 #pragma unroll
                 for (int y = 0; y < NP && x + y < 3; ++y)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) S[t][u] = mfma(kf, vf[y][u], S[t][u]);
+                    for (int u = 0; u < UT; ++u) S[t][u] = mfma(kf, vf[y][u], S[t][u]);
             }
         }
         if (some_bad) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-                if (bad_at[wave * 32 + 16 * u + m] < kChunk)
+            for (int u = 0; u < UT; ++u)
+                if (bad_at[wave * (16 * UT) + 16 * u + m] < kChunk)
 #pragma unroll
                     for (int t = 0; t < KT; ++t) S[t][u] = float4v{} + __uint_as_float(0x7FC00000u);
-            if (lane < 32) bad_at[wave * 32 + lane] = kChunk;  // these columns are this wave's alone
+            if (lane < 16 * UT) bad_at[wave * (16 * UT) + lane] = kChunk;  // these columns are this wave's alone
         }
         __syncthreads();
     }
     float* after = nullptr;
     if (STATES) after = seg.states + ((uint64_t)boundary * a.heads + head) * plane;
     else if (last_part) after = a.state_out + ((uint64_t)slot * a.heads + head) * plane;
+    const float settled = __builtin_amdgcn_exp2f((float)held);
     if (after)
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < UT; ++u)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) after[mine + (uint64_t)(16 * t + i) * a.v_dim + 16 * u] = S[t][u][i];
+                for (int i = 0; i < 4; ++i) after[mine + (uint64_t)(16 * t + i) * a.v_dim + 16 * u] = S[t][u][i] * settled;
     if (STATES && tid == 0 && v0 == 0) seg.fades[(uint64_t)boundary * a.heads + head] = (float)total;
 }
 
@@ -555,7 +665,7 @@ constexpr uint32_t kCus = 256;
 constexpr uint32_t kFewRows = 12;  // up to this many rows of a sequence go one after another
 
 // Columns of a workgroup: a whole head's where they are 64, 96 or 128.
-uint32_t waves_of(const LinearArgs& a) { return a.v_dim == 64 ? 2 : a.v_dim % 128 == 0 ? 4 : 3; }
+uint32_t columns_of(const LinearArgs& a) { return a.v_dim == 64 ? 64 : a.v_dim % 128 == 0 ? 128 : 96; }
 
 // How sequences are cut into segments with part_bytes of workspace, and the bytes made use of.
 Segments plan_segments(const LinearArgs& a, uint64_t part_bytes, uint64_t* bytes) {
@@ -563,9 +673,11 @@ Segments plan_segments(const LinearArgs& a, uint64_t part_bytes, uint64_t* bytes
     *bytes = 0;
     if (a.max_rows <= kFewRows) return seg;
     const uint64_t per = (uint64_t)a.heads * (a.k_dim * a.v_dim + 1) * 4;  // of a boundary
-    const uint64_t blocks = (uint64_t)a.heads * (a.v_dim / (32 * waves_of(a)));
-    // about three workgroups a CU, and no segment under 256 rows
-    uint64_t length = std::max<uint64_t>(256, (a.n_rows * blocks / (3 * kCus) + kChunk - 1) / kChunk * kChunk);
+    const uint64_t blocks = (uint64_t)a.heads * (a.v_dim / columns_of(a));
+    // two workgroups a CU, as many as run at once, where a sequence's last segment is half one; no segment under 256 rows
+    const uint64_t target = 2 * kCus, ends = a.n_seqs * blocks / 2;
+    uint64_t length = a.max_rows;
+    if (ends < target) length = std::max<uint64_t>(256, (a.n_rows * blocks / (target - ends) + kChunk - 1) / kChunk * kChunk);
     // boundaries: one behind every whole segment of a sequence but its last
     const auto boundaries = [&](uint64_t l) { return std::min<uint64_t>(a.n_rows / l, (uint64_t)a.n_seqs * ((a.max_rows + l - 1) / l - 1)); };
     while (length < a.max_rows && boundaries(length) * per > part_bytes) length += std::max<uint64_t>(kChunk, length / 16 / kChunk * kChunk);
@@ -579,11 +691,13 @@ Segments plan_segments(const LinearArgs& a, uint64_t part_bytes, uint64_t* bytes
 
 template <typename T, int KD>
 int launch_chunks(const LinearArgs& a, const Segments& seg, hipStream_t st) {
-    const uint32_t waves = waves_of(a), blocks = a.heads * (a.v_dim / (32 * waves));
+    const uint32_t columns = columns_of(a), blocks = a.heads * (a.v_dim / columns);
     const auto run = [&](auto states) {
         constexpr bool S = decltype(states)::value;
-        auto* k = waves == 2 ? k_linear_chunks<T, KD, 2, S> : waves == 3 ? k_linear_chunks<T, KD, 3, S> : k_linear_chunks<T, KD, 4, S>;
-        hipLaunchKernelGGL(k, dim3(blocks, S ? seg.most - 1 : seg.most, a.n_seqs), dim3(waves * 64), 0, st, a, seg);
+        // 16 columns a wave where q and k take most of the registers and one workgroup the CU (fp32, k_dim 256: 386 us against 441)
+        constexpr int UT = kPieces<T> * KD >= 768 ? 1 : 2;
+        auto* k = columns == 64 ? k_linear_chunks<T, KD, 4 / UT, UT, S> : columns == 96 ? k_linear_chunks<T, KD, 6 / UT, UT, S> : k_linear_chunks<T, KD, 8 / UT, UT, S>;
+        hipLaunchKernelGGL(k, dim3(blocks, S ? seg.most - 1 : seg.most, a.n_seqs), dim3(columns / 16 / UT * 64), 0, st, a, seg);
     };
     if (seg.most > 1) {
         run(std::true_type{});

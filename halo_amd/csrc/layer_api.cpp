@@ -51,6 +51,9 @@ int check_linear(const halo_mi_linear_attention_params* p, LinearArgs* a, bool* 
         (rc = check_rows(op, "v", a->v, p->n_rows, p->n_heads, p->v_dim, size, &v.bytes)) ||
         (rc = check_rows(op, "out", a->out, p->n_rows, p->n_heads, p->v_dim, size, &out.bytes)))
         return rc;
+    // the rows of a chunk are addressed with 32 bits
+    for (const HeadRows* r : {&a->q, &a->k, &a->v})
+        if (p->n_rows > 1 && r->stride > 1u << 24) return set_error(HALO_MI_E_UNSUPPORTED, "%s: a row stride over 2^24 elements", op);
     uint64_t decay_stride = p->decay_per_head ? 0 : p->decay_stride ? p->decay_stride : p->n_heads;
     if (p->decay_per_head && p->decay_stride) return set_error(HALO_MI_E_KERNEL, "%s: a decay stride with one decay per head", op);
     if (!p->decay_per_head && p->n_rows > 1 && (decay_stride < p->n_heads || decay_stride > 1ull << 40))
