@@ -101,6 +101,20 @@ struct __attribute__((packed, aligned(sizeof(T)))) Loose {
     T v[N];
 };
 
+// A value from the lanes before, 0 where there is none: CTRL 0x110 + n, from n lanes before in the same 16; 0x142 with rows 0xA, the last of the
+// 16 before to lanes 16 .. 31 of 32.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double lanes_before(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, CTRL, ROWS, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(bits >> 32), CTRL, ROWS, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, lane));
+}
+
 // What a type is in pieces of bf16, exactly: the first has its leading 8 bits, the next the 8 after them.
 template <typename T>
 constexpr int kPieces = sizeof(T) == 4 ? 3 : 2;
@@ -237,7 +251,8 @@ __device__ __forceinline__ bool look_up(const LinearArgs& a, const Segments& seg
 __device__ __forceinline__ uint32_t beside(uint32_t row) { return (row + 4) / 8 & 1; }
 
 // k^T and v^T: a row has a dim's 32 tokens, in 5 units of 16 bytes. Threads write four dims each, all lanes the same one of their four at a time, and
-// the products read 16 dims side by side: rows of equal row % 4 lie together, in planes that begin a quarter of the banks apart.
+// the products read 16 dims side by side: rows of equal row % 4 lie together, in planes that begin a quarter of the banks apart; of every other 64 rows the
+// halves of each 16 bytes have changed places, so that 32 lanes that write 8 bytes each meet all banks.
 constexpr int plane_of(int rows) { return rows / 4 * 5 + (20 - rows / 4 * 5 % 16) % 16; }
 template <int ROWS>
 __device__ __forceinline__ uint32_t turned_row(uint32_t row) { return row % 4 * plane_of(ROWS) + row / 4 * 5; }
@@ -277,6 +292,7 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
     constexpr int R = L::R, KT_SIZE = L::kt, VT_SIZE = L::vt(kColumnsHere);
     __shared__ uint4 q_lds[STATES ? 1 : L::q(kColumnsHere)], k_lds[STATES || !K_ROWS ? 1 : L::rows], kt_lds[3 * KT_SIZE], vt_lds[NP * VT_SIZE], p_lds[STATES ? 1 : L::p];
     __shared__ double sums_lds[kChunk];
+    __shared__ float fades_lds[kChunk];
     __shared__ int32_t bad_at[kColumnsHere];
     __shared__ int32_t bad_chunk;
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), m = lane % 16, g = lane / 16;
@@ -363,8 +379,9 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
     const auto row_at = [&](int np, uint32_t token, uint32_t ks) { return (np * kChunk + token) * R + ((ks * 4 + g) ^ beside(token)); };
     // four tokens of a row that begins at `from`
     const auto put_tokens = [](uint4* lds, uint32_t from, uint32_t row, uint32_t token, uint2 v) {
-        reinterpret_cast<uint2*>(lds)[(from + (token / 8 ^ beside(row))) * 2 + token / 4 % 2] = v;
+        reinterpret_cast<uint2*>(lds)[(from + (token / 8 ^ beside(row))) * 2 + (token / 4 + row / 64) % 2] = v;
     };
+    const auto halves = [](uint4 v, bool swapped) { return swapped ? uint4{v.z, v.w, v.x, v.y} : v; };
     const auto p_row = [](int x, uint32_t row) { return (x * kChunk + row) * 5; };
 
     for (uint32_t i = tid; i < kColumnsHere; i += THREADS) bad_at[i] = kChunk;
@@ -378,12 +395,11 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
     };
     const auto running = [&](float d) {
         double b = (double)(d < -1e4f ? -1e4f : d) * 1.4426950408889634;
-#pragma unroll
-        for (int i = 1; i < kChunk; i *= 2) {
-            const double o = __shfl_up(b, i, kChunk);
-            if ((int)(lane % kChunk) >= i) b += o;
-        }
-        return b;
+        b += lanes_before<0x111, 0xF>(b);
+        b += lanes_before<0x112, 0xF>(b);
+        b += lanes_before<0x114, 0xF>(b);
+        b += lanes_before<0x118, 0xF>(b);
+        return b + lanes_before<0x142, 0xA>(b);
     };
     // S is 2^held times what the registers hold: they take the decays only when those have grown large
     double held = 0.0, total = 0.0;
@@ -395,12 +411,12 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
     float decay_ahead = next_decay(kChunk);
     __syncthreads();
     for (uint32_t at = 0; at < rows; at += kChunk) {
-        const double b_last = __shfl(b, kChunk - 1, kChunk), grown = held + b_last;
+        const double b_last = lane_of(b, kChunk - 1), grown = held + b_last;
         const bool settle = !(fabs(grown) < 40.0);
         const float row_fade = __builtin_amdgcn_exp2f((float)(b + held)) * a.scale;                      // on S^T q of row lane % 32
         const float k_fade = __builtin_amdgcn_exp2f((float)(settle ? b_last - b : b_last - b - grown));  // on k of token lane % 32
         if (STATES) total += b_last;
-        if (tid < kChunk) sums_lds[tid] = b;
+        if (tid < kChunk) sums_lds[tid] = b, fades_lds[tid] = row_fade;
         // ---- to LDS, in pieces
         if (rows - at < kChunk) {
 #pragma unroll
@@ -547,7 +563,7 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
             }
 #pragma unroll
             for (int it = 0; it < 2; ++it) {
-                const float f = __shfl(row_fade, 16 * it + m, kChunk);
+                const float f = fades_lds[16 * it + m];
 #pragma unroll
                 for (int u = 0; u < UT; ++u) o[u][it] *= f;
             }
@@ -557,7 +573,7 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
             for (int u = 0; u < UT; ++u)
 #pragma unroll
                 for (int x = 0; x < NP; ++x) {
-                    const uint4 vf = vt_lds[x * VT_SIZE + turned_row<kColumnsHere>(wave * (16 * UT) + 16 * u + m) + (g ^ beside(m))];
+                    const uint4 vf = halves(vt_lds[x * VT_SIZE + turned_row<kColumnsHere>(wave * (16 * UT) + 16 * u + m) + (g ^ beside(m))], (wave * (16 * UT) + 16 * u) / 64 % 2);
 #pragma unroll
                     for (int y = 0; y < NO && x + y < NO; ++y)
 #pragma unroll
@@ -606,12 +622,12 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
 #pragma unroll
         for (int x = 0; x < NP; ++x)
 #pragma unroll
-            for (int u = 0; u < UT; ++u) vf[x][u] = vt_lds[x * VT_SIZE + turned_row<kColumnsHere>(wave * (16 * UT) + 16 * u + m) + (g ^ beside(m))];
+            for (int u = 0; u < UT; ++u) vf[x][u] = halves(vt_lds[x * VT_SIZE + turned_row<kColumnsHere>(wave * (16 * UT) + 16 * u + m) + (g ^ beside(m))], (wave * (16 * UT) + 16 * u) / 64 % 2);
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
 #pragma unroll
             for (int x = 0; x < 3; ++x) {
-                const uint4 kf = kt_lds[x * KT_SIZE + turned_row<KD>(16 * t + m) + (g ^ beside(m))];
+                const uint4 kf = halves(kt_lds[x * KT_SIZE + turned_row<KD>(16 * t + m) + (g ^ beside(m))], t / 4 % 2);
 #pragma unroll
                 for (int y = 0; y < NP && x + y < 3; ++y)
 #pragma unroll
