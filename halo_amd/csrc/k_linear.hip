@@ -409,6 +409,7 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
     }
     double b = running(next_decay(0));
     float decay_ahead = next_decay(kChunk);
+    asm volatile("" : "+v"(decay_ahead));  // waited for here, or the loop would wait for it, and for all that is in flight, every time
     __syncthreads();
     for (uint32_t at = 0; at < rows; at += kChunk) {
         const double b_last = lane_of(b, kChunk - 1), grown = held + b_last;
@@ -488,10 +489,10 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
             }
         }
         const float decays = decay_ahead;  // the next chunk's, asked for a chunk ago
-        if (at + kChunk < rows) fetch(rows - at - kChunk);
         decay_ahead = next_decay(at + 2 * kChunk);
+        if (at + kChunk < rows) fetch(rows - at - kChunk);
         __syncthreads();
-        const bool some_bad = bad_chunk == (int32_t)(at / kChunk);
+        const bool some_bad = __builtin_amdgcn_readfirstlane(bad_chunk) == (int32_t)(at / kChunk);
         // ---- P^T = K Q^T: tiles (tokens 16 jt .., rows 16 it ..) on and under the diagonal
         if constexpr (!STATES) {
             for (uint32_t tile = wave; tile < 3; tile += WAVES) {
@@ -583,6 +584,15 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
             constexpr int OP = 16 * UT * sizeof(T) / 16;  // pieces of a row
             uint8_t* const o_lds = reinterpret_cast<uint8_t*>(q_lds) + wave * (kChunk * OP * 16);
             const auto o_at = [](uint32_t row, uint32_t piece) { return (row * OP + (piece ^ (OP == 8 ? row / 2 & 7 : OP == 4 ? row / 4 & 3 : row / 8 & 1))) * 16; };
+            if (some_bad) {
+#pragma unroll
+                for (int it = 0; it < 2; ++it)
+#pragma unroll
+                    for (int u = 0; u < UT; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (bad_at[wave * (16 * UT) + 16 * u + 4 * g + i] <= (int32_t)(16 * it + m)) o[u][it][i] = __uint_as_float(0x7FC00000u);
+            }
 #pragma unroll
             for (int it = 0; it < 2; ++it)
 #pragma unroll
@@ -590,22 +600,18 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
                     const uint32_t col = 16 * u + 4 * g, row = 16 * it + m;
                     Vec<T, 4> y;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float v = o[u][it][i];
-                        if (some_bad && bad_at[wave * (16 * UT) + col + i] <= (int32_t)row) v = __uint_as_float(0x7FC00000u);
-                        y.v[i] = from_f32<T>(v);
-                    }
+                    for (int i = 0; i < 4; ++i) y.v[i] = from_f32<T>(o[u][it][i]);
                     *reinterpret_cast<Vec<T, 4>*>(o_lds + o_at(row, col * sizeof(T) / 16) + col * sizeof(T) % 16) = y;
                 }
             // the wave reads what its own lanes wrote: LDS serves a wave in order
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int j = 0; j < kChunk * OP / 64; ++j) {
-                const uint32_t row = (j * 64 + lane) / OP, piece = (j * 64 + lane) % OP;
+                // rows behind the last are the last one once more: stores that all lanes make are counted, and the loads in flight are not waited for
+                const uint32_t row = min((j * 64 + lane) / OP, rows - at - 1), piece = (j * 64 + lane) % OP;
                 typedef Loose<T, 16 / sizeof(T)> Piece;
                 const uint4 y = *reinterpret_cast<const uint4*>(o_lds + o_at(row, piece));
-                if (at + row < rows)
-                    *reinterpret_cast<Piece*>(out + (uint64_t)(at + row) * a.out.stride + wave * (16 * UT) + piece * (16 / sizeof(T))) = __builtin_bit_cast(Piece, y);
+                *reinterpret_cast<Piece*>(out + (uint64_t)(at + row) * a.out.stride + wave * (16 * UT) + piece * (16 / sizeof(T))) = __builtin_bit_cast(Piece, y);
             }
         }
         b = running(decays);
@@ -618,21 +624,27 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
 #pragma unroll
                 for (int u = 0; u < UT; ++u) S[t][u] *= f;
         }
-        uint4 vf[NP][UT];
+        uint4 vf[NP][UT], kf[2][3];  // k^T's tile and the next one's
+#pragma unroll
+        for (int x = 0; x < 3; ++x) kf[0][x] = kt_lds[x * KT_SIZE + turned_row<KD>(m) + (g ^ beside(m))];
 #pragma unroll
         for (int x = 0; x < NP; ++x)
 #pragma unroll
             for (int u = 0; u < UT; ++u) vf[x][u] = halves(vt_lds[x * VT_SIZE + turned_row<kColumnsHere>(wave * (16 * UT) + 16 * u + m) + (g ^ beside(m))], (wave * (16 * UT) + 16 * u) / 64 % 2);
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
+            if (t + 1 < KT)
+#pragma unroll
+                for (int x = 0; x < 3; ++x) kf[(t + 1) % 2][x] = kt_lds[x * KT_SIZE + turned_row<KD>(16 * (t + 1) + m) + (g ^ beside(m))];
 #pragma unroll
             for (int x = 0; x < 3; ++x) {
-                const uint4 kf = halves(kt_lds[x * KT_SIZE + turned_row<KD>(16 * t + m) + (g ^ beside(m))], t / 4 % 2);
+                const uint4 k = halves(kf[t % 2][x], t / 4 % 2);
 #pragma unroll
                 for (int y = 0; y < NP && x + y < 3; ++y)
 #pragma unroll
-                    for (int u = 0; u < UT; ++u) S[t][u] = mfma(kf, vf[y][u], S[t][u]);
+                    for (int u = 0; u < UT; ++u) S[t][u] = mfma(k, vf[y][u], S[t][u]);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (some_bad) {
 #pragma unroll
