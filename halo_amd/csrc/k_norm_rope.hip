@@ -1,8 +1,12 @@
 // gfx950 kernels of the heads' norms with the rotary positions: for a head x of head_dim elements
 //   y_j = x_j / sqrt(sum_j x_j^2 / head_dim + eps) * w_j,
 // then the rotation of k_rope.hip on y. The head is read once: the lanes that hold it add their squares with
-// cross-lane moves and turn what they have in their registers. The token's table of sines and cosines and both parts'
+// cross-lane moves and turn what they have in their registers. A token's table of sines and cosines and both parts'
 // weights are made once per workgroup, in LDS, while the first heads are on their way.
+//
+// Memory bounds it: 6133 tokens of 40 heads of 128 in bfloat16 take 31.5 us (4.0 TB/s read and written; adjacent pairs, 29.4 us in halves).
+// One token a workgroup took 35: 40 heads are two and a half rounds of its lanes, and every one waits for its table. A wave per token, with
+// its table and weights in registers, took 34 to 48, a head loaded ahead 32 to 37: fewer waves fit.
 //
 // Sums, products and the root are in 32 bits, one rounding to the type at the end: rounding the normed head to 16 bits before the
 // rotation, as two launches do, is left out.
@@ -22,46 +26,50 @@ namespace {
 using namespace dev;
 
 constexpr uint32_t kBlock = 256;
+constexpr uint32_t kTokensHere = 4;  // of a workgroup, at most
 constexpr uint32_t kTokens = 1u << 23;  // of a launch: a grid has fewer than 2^32 threads along x
 
 // The turned pair, rounded as k_rope.hip rounds it: a part without weights is bitwise what rope gives.
 __device__ __forceinline__ float first_of(float x, float y, float2 cs) { return fmaf(x, cs.x, -(y * cs.y)); }
 __device__ __forceinline__ float second_of(float x, float y, float2 cs) { return fmaf(x, cs.y, y * cs.x); }
 
-// One workgroup: token blockIdx.x, the heads from blockIdx.y * heads_per on. G lanes have a head between them, an item
-// each: V pairs (2 V elements), or V elements that are not turned.
+// One workgroup: tokens blockIdx.x * tokens .. + tokens - 1, of each the heads from blockIdx.y * heads_per on, side by side. G lanes have a head between
+// them, an item each: V pairs (2 V elements), or V elements that are not turned.
 template <typename T, int V, bool INTERLEAVED, int G>
-__global__ __launch_bounds__(kBlock) void k_norm_rope(NormRopeArgs n, uint32_t heads_per) {
+__global__ __launch_bounds__(kBlock) void k_norm_rope(NormRopeArgs n, uint32_t heads_per, uint32_t tokens) {
     const RopeArgs& a = n.rope;
-    __shared__ float2 table[256];
+    __shared__ alignas(16) float2 table[kTokensHere][V * G];
     __shared__ alignas(16) float weight[2][2 * V * G];
-    const uint32_t t = blockIdx.x, half = a.rot / 2, c = threadIdx.x % G, turned = half / V, items = turned + (a.dim - a.rot) / V;
-    const uint32_t h_end = min(a.heads, (blockIdx.y + 1) * heads_per);
+    const uint32_t t0 = blockIdx.x * tokens, here = min(tokens, a.n_tokens - t0), half = a.rot / 2, c = threadIdx.x % G, turned = half / V, items = turned + (a.dim - a.rot) / V;
+    const uint32_t h0 = blockIdx.y * heads_per, h_count = min(a.heads - h0, heads_per);
     // the item's elements: ex of the head and on, and for a turned one ey and on (adjacent pairs: the next V)
     const bool turns = c < turned, has = c < items;
     const uint32_t ex = turns ? c * V * (INTERLEAVED ? 2 : 1) : a.rot + (c - turned) * V;
     const uint32_t ey = INTERLEAVED ? ex + V : ex + half;
     Vec<T, V> x{}, y{};
-    const auto fetch = [&](uint32_t h) {
+    // head h0 + h of token t0 + t
+    const auto fetch = [&](uint32_t t, uint32_t h) {
+        h += h0;
         const bool second = h >= a.part[0].heads;
         const HeadRows& r = a.part[second].in;
-        const T* in = static_cast<const T*>(r.data) + t * r.stride + (second ? h - a.part[0].heads : h) * r.head_stride;
+        const T* in = static_cast<const T*>(r.data) + (t0 + t) * r.stride + (second ? h - a.part[0].heads : h) * r.head_stride;
         if (has) x = *reinterpret_cast<const Vec<T, V>*>(in + ex);
         if (turns) y = *reinterpret_cast<const Vec<T, V>*>(in + ey);
     };
-    uint32_t h = blockIdx.y * heads_per + threadIdx.x / G;
-    if (h < h_end) fetch(h);
+    uint32_t t = threadIdx.x / G / h_count, h = threadIdx.x / G % h_count;
+    const uint32_t t_step = kBlock / G / h_count, h_step = kBlock / G % h_count;
+    if (t < here) fetch(t, h);
     for (uint32_t i = threadIdx.x; i < a.dim; i += kBlock)
         for (int p = 0; p < 2; ++p) weight[p][i] = n.norm_w[p] ? n.norm_w[p][i] : 1.0f;
-    const double pos = (double)a.positions[t];
-    for (uint32_t i = threadIdx.x; i < half; i += kBlock) {
-        const float2 cs = turn(pos * a.freqs[i]);
-        table[i] = {cs.x * a.factor, cs.y * a.factor};
+    for (uint32_t i = threadIdx.x; i < half * here; i += kBlock) {
+        const float2 cs = turn((double)a.positions[t0 + i / half] * a.freqs[i % half]);
+        table[i / half][i % half] = {cs.x * a.factor, cs.y * a.factor};
     }
     __syncthreads();
     const float over_dim = 1.0f / (float)a.dim;
-    while (h < h_end) {
-        const bool second = h >= a.part[0].heads;
+    while (t < here) {
+        const uint32_t head = h0 + h;
+        const bool second = head >= a.part[0].heads;
         const HeadRows& r = a.part[second].out;
         float u[V], w[V], sum = 0.0f;
 #pragma unroll
@@ -77,7 +85,7 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope(NormRopeArgs n, uint32_t h
 #pragma unroll
         for (int i = 1; i < G; i *= 2) sum += __shfl_xor(sum, i, G);
         const float inv = n.norm_w[second] ? 1.0f / sqrtf(fmaf(sum, over_dim, n.eps)) : 1.0f;
-        T* out = const_cast<T*>(static_cast<const T*>(r.data)) + t * r.stride + (second ? h - a.part[0].heads : h) * r.head_stride;
+        T* out = const_cast<T*>(static_cast<const T*>(r.data)) + (t0 + t) * r.stride + (second ? head - a.part[0].heads : head) * r.head_stride;
         const float* wx = weight[second] + ex;
         if (turns) {
             const float* wy = weight[second] + ey;
@@ -86,7 +94,7 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope(NormRopeArgs n, uint32_t h
             for (int i = 0; i < V; ++i) u[i] = u[i] * inv * wx[i], w[i] = w[i] * inv * wy[i];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float2 cs = table[c * V + i];
+                const float2 cs = table[t][c * V + i];
                 if constexpr (INTERLEAVED) {
                     const float f = i < V / 2 ? u[2 * i] : w[2 * i - V], g = i < V / 2 ? u[2 * i + 1] : w[2 * i + 1 - V];
                     T* e = i < V / 2 ? &ox.v[2 * i] : &oy.v[2 * i - V];
@@ -105,14 +113,15 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope(NormRopeArgs n, uint32_t h
             for (int i = 0; i < V; ++i) ox.v[i] = from_f32<T>(u[i] * inv * wx[i]);
             *reinterpret_cast<Vec<T, V>*>(out + ex) = ox;
         }
-        h += kBlock / G;
-        if (h < h_end) fetch(h);
+        t += t_step, h += h_step;
+        if (h >= h_count) h -= h_count, ++t;
+        if (t < here) fetch(t, h);
     }
 }
 
 // Heads of any size and alignment: a wave has one, and reads it twice.
 template <typename T, bool INTERLEAVED>
-__global__ __launch_bounds__(kBlock) void k_norm_rope_any(NormRopeArgs n, uint32_t heads_per) {
+__global__ __launch_bounds__(kBlock) void k_norm_rope_any(NormRopeArgs n, uint32_t heads_per, uint32_t) {
     const RopeArgs& a = n.rope;
     __shared__ float2 table[256];
     const uint32_t t = blockIdx.x, half = a.rot / 2, lane = threadIdx.x % 64;
@@ -173,7 +182,7 @@ int launch_typed(uint32_t pairs, const NormRopeArgs& n, hipStream_t st) {
     };
     uint32_t v = 16 / sizeof(T);
     while (v > 1 && !fits(v)) v /= 2;
-    void (*k)(NormRopeArgs, uint32_t) = inter ? k_norm_rope_any<T, true> : k_norm_rope_any<T, false>;
+    void (*k)(NormRopeArgs, uint32_t, uint32_t) = inter ? k_norm_rope_any<T, true> : k_norm_rope_any<T, false>;
     uint32_t at_once = kBlock / 64;
     if (v > 1) {
         const uint32_t items = a.rot / 2 / v + (a.dim - a.rot) / v, g = items <= 8 ? 8 : items <= 16 ? 16 : items <= 32 ? 32 : 64;
@@ -185,7 +194,8 @@ int launch_typed(uint32_t pairs, const NormRopeArgs& n, hipStream_t st) {
         if constexpr (sizeof(T) == 2) k = v == 8 ? pick(std::integral_constant<int, 8>{}) : v == 4 ? pick(std::integral_constant<int, 4>{}) : pick(std::integral_constant<int, 2>{});
         else k = v == 4 ? pick(std::integral_constant<int, 4>{}) : pick(std::integral_constant<int, 2>{});
     }
-    // few tokens: their heads over several workgroups, one pass each
+    // many tokens: several a workgroup; few: their heads over several workgroups
+    const uint32_t tokens = v > 1 ? std::min(std::max(a.n_tokens / 1024, 1u), kTokensHere) : 1;
     const uint32_t passes = std::max<uint64_t>(1, std::min<uint64_t>(a.heads, (uint64_t)a.n_tokens * ((a.heads + at_once - 1) / at_once) / 2048));
     // at most 2^15 workgroups along y
     const uint32_t heads_per = std::min(a.heads, std::max(passes * at_once, a.heads / 32768 + 1));
@@ -195,7 +205,7 @@ int launch_typed(uint32_t pairs, const NormRopeArgs& n, hipStream_t st) {
         some.rope.positions += t;
         for (RopePart& p : some.rope.part)
             for (HeadRows* r : {&p.in, &p.out}) r->data = static_cast<const T*>(r->data) + t * r->stride;
-        hipLaunchKernelGGL(k, dim3(some.rope.n_tokens, (a.heads + heads_per - 1) / heads_per), dim3(kBlock), 0, st, some, heads_per);
+        hipLaunchKernelGGL(k, dim3((some.rope.n_tokens + tokens - 1) / tokens, (a.heads + heads_per - 1) / heads_per), dim3(kBlock), 0, st, some, heads_per, tokens);
     }
     return hip_status(hipGetLastError(), "norm_rope");
 }
