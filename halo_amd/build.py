@@ -80,7 +80,7 @@ def build_oracle() -> Path:
     return ROOT / "oracle" / "liboracle.so"
 
 
-CPP_TESTS = [ROOT / "tests" / "cpp" / name for name in ("backend_pair", "backend_kv", "backend_kv_status")]
+CPP_TESTS = [ROOT / "tests" / "cpp" / name for name in ("backend_pair", "backend_kv", "backend_kv_status", "backend_layer")]
 
 
 def build_cpp_tests() -> list[Path]:

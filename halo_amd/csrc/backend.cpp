@@ -243,7 +243,7 @@ private:
 
 // ---- variant registry (explicit, append-only ids; grouped by op) ----------------------------
 
-constexpr std::array<VariantInfo, 26> kVariants{{
+constexpr std::array<VariantInfo, 30> kVariants{{
     {kDequantRows, "dequant_rows_exact", OpId::GetRows, {}},
     {kRmsNorm, "rms_norm_cpu_order", OpId::RmsNorm, {}},
     {kGemvGgufRef, "gemv_gguf_ref_b256", OpId::Gemv, {}},
@@ -270,6 +270,10 @@ constexpr std::array<VariantInfo, 26> kVariants{{
     {kKv8Read, "kv8_read", OpId::Kv8Read, {}},
     {kKv8Attention, "kv8_attention_mfma", OpId::Kv8Attention, {}},
     {kKv8Pages, "kv8_pages", OpId::Kv8Pages, {}},
+    {kNormRope, "norm_rope", OpId::NormRope, {}},
+    {kQuantizeRows, "quantize_rows", OpId::QuantizeRows, {}},
+    {kGemmI8, "gemm_i8_mfma", OpId::GemmI8, {}},
+    {kLinearAttention, "linear_attention_mfma", OpId::LinearAttention, {}},
 }};
 
 bool has_variant(OpId op, std::uint32_t id) {
@@ -693,22 +697,9 @@ public:
     void rope(Stream& s, const RopeTableArgs& a) override {
         HipStream& st = stream(s, "ROPE");
         check_choice(a.kernel, OpId::Rope);
-        CHECK(a.n_parts == 1 || a.n_parts == 2, ErrorCode::Unsupported, "ROPE: %u parts (1 or 2)", a.n_parts);
         const Resolver r(this, "ROPE");
-        const std::uint32_t size = value_bytes(a.type, r.op());
         halo_mi_rope_part parts[2] = {};
-        for (std::uint32_t i = 0; i < a.n_parts; ++i) {
-            const RopePart& p = a.parts[i];
-            const Operand in = heads_of(r, p.in, a.n_tokens, p.n_heads, a.head_dim, p.in_head_stride, size, Access::Read, "in");
-            const Operand out = heads_of(r, p.out, a.n_tokens, p.n_heads, a.head_dim, p.out_head_stride, size, Access::Write, "out");
-            parts[i] = {in.base, in.stride / size, p.in_head_stride, out.base, out.stride / size, p.out_head_stride, p.n_heads};
-        }
-        const Operand pos = r.get(a.positions, 1, mul_u64(a.n_tokens, 4, r.op(), "positions"), 4, Access::Read, "positions");
-        const Operand freqs = r.get(a.freqs, 1, a.rot_dims / 2 * 8ull, 8, Access::Read, "freqs");
-        const halo_mi_rope_params p{static_cast<std::uint32_t>(a.type),
-                                    a.interleaved ? HALO_MI_ROPE_INTERLEAVED : HALO_MI_ROPE_HALF,
-                                    parts, a.n_parts, a.n_tokens, a.head_dim, a.rot_dims,
-                                    reinterpret_cast<const std::int32_t*>(pos.base), reinterpret_cast<const double*>(freqs.base), a.factor};
+        const halo_mi_rope_params p = rope_of(r, a, parts);
         check_abi(halo_mi_rope(&p, st.native()));
     }
 
@@ -780,6 +771,88 @@ public:
         check_abi(halo_mi_kv_compact(&c, &state, reinterpret_cast<std::uint32_t*>(live.base), st.native()));
     }
 
+    // ---- head norms with rotary positions, 8-bit products, linear attention: checked as the ops above
+
+    void norm_rope(Stream& s, const NormRopeArgs& a) override {
+        HipStream& st = stream(s, "NORM_ROPE");
+        check_choice(a.kernel, OpId::NormRope);
+        const Resolver r(this, "NORM_ROPE");
+        halo_mi_rope_part parts[2] = {};
+        halo_mi_norm_rope_params p{rope_of(r, a.rope, parts), {}, a.eps};
+        for (std::uint32_t i = 0; i < 2; ++i)
+            if (!a.norm_w[i].empty()) p.norm_w[i] = reinterpret_cast<const float*>(r.f32(a.norm_w[i], 1, a.rope.head_dim, Access::Read, "norm_w").base);
+        check_abi(halo_mi_norm_rope(&p, st.native()));
+    }
+
+    void quantize_rows(Stream& s, const QuantizeRowsArgs& a) override {
+        HipStream& st = stream(s, "QUANTIZE_ROWS");
+        check_choice(a.kernel, OpId::QuantizeRows);
+        const Resolver r(this, "QUANTIZE_ROWS");
+        const std::uint32_t size = value_bytes(a.type, r.op());
+        const Operand x = r.get(a.x, a.rows, mul_u64(a.cols, size, r.op(), "x"), size, Access::Read, "x");
+        const Operand codes = codes_of(r, a.codes, a.rows, a.cols, Access::Write, "codes");
+        const Operand scales = r.f32(a.scales, 1, a.rows, Access::Write, "scales");
+        check_abi(halo_mi_quantize_rows(static_cast<std::uint32_t>(a.type), x.base, x.stride / size, reinterpret_cast<std::int8_t*>(codes.base),
+                                        codes.stride, reinterpret_cast<float*>(scales.base), a.rows, a.cols, st.native()));
+    }
+
+    void gemm_i8(Stream& s, const GemmI8Args& a) override {
+        HipStream& st = stream(s, "GEMM_I8");
+        check_choice(a.kernel, OpId::GemmI8);
+        const Resolver r(this, "GEMM_I8");
+        const std::uint32_t size = value_bytes(a.type, r.op());
+        const Operand w = codes_of(r, a.w, a.rows, a.cols, Access::Read, "w"), x = codes_of(r, a.x, a.n_vec, a.cols, Access::Read, "x");
+        const Operand ws = r.f32(a.w_scales, 1, a.rows, Access::Read, "w_scales"), xs = r.f32(a.x_scales, 1, a.n_vec, Access::Read, "x_scales");
+        const Operand y = r.get(a.y, a.n_vec, mul_u64(a.rows, size, r.op(), "y"), size, Access::Write, "y");
+        const halo_mi_gemm_i8_params p{static_cast<std::uint32_t>(a.type),
+                                       reinterpret_cast<const std::int8_t*>(w.base), w.stride, reinterpret_cast<const float*>(ws.base),
+                                       reinterpret_cast<const std::int8_t*>(x.base), x.stride, reinterpret_cast<const float*>(xs.base),
+                                       y.base, y.stride / size, a.rows, a.cols, a.n_vec};
+        check_abi(halo_mi_gemm_i8(&p, st.native()));
+    }
+
+    void linear_attention(Stream& s, const LinearAttentionArgs& a) override {
+        HipStream& st = stream(s, "LINEAR_ATTENTION");
+        check_choice(a.kernel, OpId::LinearAttention);
+        const Resolver r(this, "LINEAR_ATTENTION");
+        const std::uint32_t size = value_bytes(a.type, r.op());
+        for (const std::uint32_t dim : {a.k_dim, a.v_dim})
+            CHECK(dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256, ErrorCode::Unsupported, "%s: k_dim %u, v_dim %u", r.op(),
+                  a.k_dim, a.v_dim);
+        const std::uint64_t slot = mul_u64(mul_u64(a.n_heads, a.k_dim, r.op(), "state"), mul_u64(a.v_dim, kF32, r.op(), "state"), r.op(), "state");
+        const bool in_place = a.state_out.empty();
+        const auto states = [&](const TensorRef& t, Access access, const char* name) {
+            CHECK(t.row_stride == 0 || t.row_stride == slot, ErrorCode::Kernel, "%s: states are dense", r.op());
+            return reinterpret_cast<float*>(r.get(t, a.n_slots, slot, 16, access, name).base);
+        };
+        halo_mi_linear_attention_params p{};
+        p.type = static_cast<std::uint32_t>(a.type);
+        p.n_heads = a.n_heads, p.n_k_heads = a.n_k_heads, p.k_dim = a.k_dim, p.v_dim = a.v_dim, p.n_slots = a.n_slots;
+        p.state = states(a.state, in_place ? Access::Write : Access::Read, "state");
+        p.state_out = states(in_place ? a.state : a.state_out, Access::Write, "state_out");
+        p.slots = list_of(r, a.slots, a.n_seqs, "slots");
+        p.row_starts = list_of(r, a.row_starts, a.n_seqs ? a.n_seqs + 1ull : 0, "row_starts");
+        if (!a.seq_lens.empty()) p.seq_lens = list_of(r, a.seq_lens, a.n_seqs, "seq_lens");
+        p.n_seqs = a.n_seqs, p.n_rows = a.n_rows, p.max_rows = a.max_rows;
+        const Operand q = heads_of(r, a.q, a.n_rows, a.n_k_heads, a.k_dim, a.q_head_stride, size, Access::Read, "q");
+        const Operand k = heads_of(r, a.k, a.n_rows, a.n_k_heads, a.k_dim, a.k_head_stride, size, Access::Read, "k");
+        const Operand v = heads_of(r, a.v, a.n_rows, a.n_heads, a.v_dim, a.v_head_stride, size, Access::Read, "v");
+        const Operand out = heads_of(r, a.out, a.n_rows, a.n_heads, a.v_dim, a.out_head_stride, size, Access::Write, "out");
+        p.q = q.base, p.q_stride = q.stride / size, p.q_head_stride = a.q_head_stride;
+        p.k = k.base, p.k_stride = k.stride / size, p.k_head_stride = a.k_head_stride;
+        p.v = v.base, p.v_stride = v.stride / size, p.v_head_stride = a.v_head_stride;
+        p.out = out.base, p.out_stride = out.stride / size, p.out_head_stride = a.out_head_stride;
+        const Operand decay = r.f32(a.decay, a.decay_per_head ? 1 : a.n_rows, a.n_heads, Access::Read, "decay");
+        p.decay = reinterpret_cast<const float*>(decay.base), p.decay_stride = a.decay_per_head ? 0 : decay.stride / kF32;
+        p.decay_per_head = a.decay_per_head, p.scale = a.scale;
+        if (!a.workspace.empty()) {
+            const Operand w = r.get(a.workspace, 1, a.workspace.view_bytes() / 16 * 16, 16, Access::Write, "workspace");
+            p.workspace = w.base, p.workspace_bytes = w.extent;
+        }
+        p.status = status_of(r, a.status, st, &p.status_keep);
+        check_abi(halo_mi_linear_attention(&p, st.native()));
+    }
+
     // The ops of the reference interface outside this path.
     void add_rms_norm(Stream&, const AddRmsNormArgs&) override { unsupported(OpId::AddRmsNorm); }
     void gdn_gates(Stream&, const GdnGateArgs&) override { unsupported(OpId::GdnGates); }
@@ -816,6 +889,33 @@ private:
         CHECK(head_stride <= 1ull << 40, ErrorCode::Kernel, "%s: the head stride of %s is out of range", r.op(), name);
         const std::uint64_t row = heads == 0 ? 0 : (heads - 1) * (head_stride ? head_stride : dim) + dim;
         return r.get(t, rows, mul_u64(row, size, r.op(), name), size, access, name);
+    }
+
+    // The rotary positions' operands; parts receives their rows.
+    static halo_mi_rope_params rope_of(const Resolver& r, const RopeTableArgs& a, halo_mi_rope_part* parts) {
+        CHECK(a.n_parts == 1 || a.n_parts == 2, ErrorCode::Unsupported, "%s: %u parts (1 or 2)", r.op(), a.n_parts);
+        const std::uint32_t size = value_bytes(a.type, r.op());
+        for (std::uint32_t i = 0; i < a.n_parts; ++i) {
+            const RopePart& p = a.parts[i];
+            const Operand in = heads_of(r, p.in, a.n_tokens, p.n_heads, a.head_dim, p.in_head_stride, size, Access::Read, "in");
+            const Operand out = heads_of(r, p.out, a.n_tokens, p.n_heads, a.head_dim, p.out_head_stride, size, Access::Write, "out");
+            parts[i] = {in.base, in.stride / size, p.in_head_stride, out.base, out.stride / size, p.out_head_stride, p.n_heads};
+        }
+        const Operand pos = r.get(a.positions, 1, mul_u64(a.n_tokens, 4, r.op(), "positions"), 4, Access::Read, "positions");
+        const Operand freqs = r.get(a.freqs, 1, a.rot_dims / 2 * 8ull, 8, Access::Read, "freqs");
+        return {static_cast<std::uint32_t>(a.type),
+                a.interleaved ? HALO_MI_ROPE_INTERLEAVED : HALO_MI_ROPE_HALF,
+                parts, a.n_parts, a.n_tokens, a.head_dim, a.rot_dims,
+                reinterpret_cast<const std::int32_t*>(pos.base), reinterpret_cast<const double*>(freqs.base), a.factor};
+    }
+
+    // Rows of cols 8-bit codes, padded to 16.
+    static Operand codes_of(const Resolver& r, const TensorRef& t, std::uint32_t rows, std::uint32_t cols, Access access, const char* name) {
+        return r.get(t, rows, (cols + 15ull) / 16 * 16, 16, access, name);
+    }
+
+    static const std::int32_t* list_of(const Resolver& r, const TensorRef& t, std::uint64_t n, const char* name) {
+        return reinterpret_cast<const std::int32_t*>(r.get(t, 1, 4 * n, 4, Access::Read, name).base);
     }
 
     static halo_mi_kv_cache cache_of(const Resolver& r, const Kv8Cache& c, Access access) {
@@ -997,6 +1097,10 @@ std::string_view op_name(OpId op) noexcept {
         case OpId::Kv8Read: return "KV8_READ";
         case OpId::Kv8Attention: return "KV8_ATTENTION";
         case OpId::Kv8Pages: return "KV8_PAGES";
+        case OpId::NormRope: return "NORM_ROPE";
+        case OpId::QuantizeRows: return "QUANTIZE_ROWS";
+        case OpId::GemmI8: return "GEMM_I8";
+        case OpId::LinearAttention: return "LINEAR_ATTENTION";
     }
     return "UNKNOWN";
 }
@@ -1042,7 +1146,8 @@ void Backend::run_op(Stream& s, const OpInvocation& inv) {
         case OpId::TopK: return top_k(s, args_of<TopKArgs>(inv));
         case OpId::Copy: return copy(s, args_of<CopyArgs>(inv));
         case OpId::GateUpSwiglu: case OpId::Rope: case OpId::Kv8Write: case OpId::Kv8Read: case OpId::Kv8Attention:
-        case OpId::Kv8Pages: break;  // additions with no args type in OpInvocation
+        case OpId::Kv8Pages: case OpId::NormRope: case OpId::QuantizeRows: case OpId::GemmI8: case OpId::LinearAttention:
+            break;  // additions with no args type in OpInvocation
     }
     fail(ErrorCode::Api, "run_op: unknown op id %u", static_cast<unsigned>(inv.op));
 }

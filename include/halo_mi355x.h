@@ -730,7 +730,7 @@ int halo_mi_gemm_i8(const halo_mi_gemm_i8_params* p, void* stream);
  * call follows their values at each replay. A slot outside [0, n_slots), or one that an earlier sequence with rows has, gives NaN rows, leaves the
  * state alone and sets HALO_MI_STATUS_BAD_INDEX.
  *   type: F32, F16 or BF16, of q, k, v and out. q, k: n_rows rows of n_k_heads heads of k_dim; v, out: of n_heads heads of v_dim; n_heads
- *     is a multiple of n_k_heads. Strides in elements, 0 = dense.
+ *     is a multiple of n_k_heads, 4096 at most. Strides in elements, 0 = dense; rows of q, k and v at most 2^24 apart. n_seqs <= 65535.
  *   decay: the logarithm of the factor on the state, fp32: n_rows rows of n_heads, decay_stride elements apart (0 = n_heads), or with
  *     decay_per_head n_heads values that hold for every row. -infinity empties the state; values above 0 are taken as they are.
  *   state: n_slots slots of n_heads x k_dim x v_dim fp32 (16-byte aligned, dense); state_out: where the new states go, of the same
@@ -744,9 +744,10 @@ int halo_mi_gemm_i8(const halo_mi_gemm_i8_params* p, void* stream);
  *   workspace (optional, 16-byte aligned): device memory for the states inside long sequences, in place of the stream's own
  *     workspace. Graphs captured on one stream share that stream's workspace: give each its own if their replays may overlap.
  *     halo_mi_linear_attention_workspace() says what a call makes use of; with less (or on a capturing stream that has none
- *     yet) sequences are split less.
- * Numerics: the state, the sums and the decays are in 32 bits, the decays' running sums in 64. Where a value of v is not finite, its
- * column of out is NaN from its row on, and that column of the state; one of k or a NaN decay: the head's rows from its own on.
+ *     yet) sequences are split less: the results are as right, and slower.
+ * Numerics: the state, the sums and the decays are in 32 bits, the decays' running sums in 64. A chunk's state is held with a factor of up to
+ * 2^40: k and k v^T are to stay below 2^80. Where a value of v is not finite, that column of out from its row on, and of the state, has no finite
+ * numbers (infinities or NaN); one of k, or a decay of NaN: all columns of the heads that read it, from its row on; one of q: its own row's.
  * out may not overlap any other operand (it may lie beside q, k and v in rows of one stride), state_out none but state.
  */
 typedef struct halo_mi_linear_attention_params {

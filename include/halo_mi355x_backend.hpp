@@ -26,8 +26,8 @@
 // layout (MiBackend::import_weights), GET_ROWS over a contiguous row range
 // (MiBackend::dequant_rows), the FFN's gate/up/SwiGLU composition (src/models/qwen35.cpp:789-805)
 // as one op (MiBackend::gate_up_swiglu), rotary positions and attention over a batch of sequences with
-// an 8-bit paged cache (MiBackend::rope, kv8_*), device addresses and layouts of buffers, and the hipStream_t
-// of a stream.
+// an 8-bit paged cache (MiBackend::rope, kv8_*), head norms, 8-bit products and linear attention (MiBackend::norm_rope,
+// quantize_rows, gemm_i8, linear_attention), device addresses and layouts of buffers, and the hipStream_t of a stream.
 #pragma once
 
 #include <cstddef>
@@ -146,6 +146,8 @@ enum class OpId : std::uint16_t {
     GateUpSwiglu = 18,  // addition: gemv(gate) + gemv(up) + swiglu in one launch (MiBackend::gate_up_swiglu)
     // additions: MiBackend's rotary positions from a table of frequencies and its 8-bit paged cache
     Rope = 19, Kv8Write = 20, Kv8Read = 21, Kv8Attention = 22, Kv8Pages = 23,
+    // additions: the heads' norms with those positions, rows held in 8 bits and their products, linear attention
+    NormRope = 24, QuantizeRows = 25, GemmI8 = 26, LinearAttention = 27,
 };
 inline constexpr std::size_t kOpCount = 18;  // the reference's ops
 
@@ -570,6 +572,52 @@ struct Kv8CompactArgs {
     KernelChoice kernel{};
 };
 
+// ---- head norms with rotary positions, 8-bit products, linear attention (halo_mi355x.h says what each computes) ------
+//
+// Types, rows, head strides, lists and status words are as above.
+
+/// rope with the RMS norm of each head before it; norm_w[i]: head_dim fp32 of part i, or empty (rotated only).
+struct NormRopeArgs {
+    RopeTableArgs rope{};
+    TensorRef norm_w[2]{};
+    float eps = 1e-6f;
+    KernelChoice kernel{};  ///< rope.kernel is not looked at
+};
+
+/// codes: rows of cols int8 and zeros up to the next multiple of 16; scales: rows fp32.
+struct QuantizeRowsArgs {
+    DType type = DType::F32;
+    TensorRef x{}, codes{}, scales{};
+    std::uint32_t rows = 0, cols = 0;
+    KernelChoice kernel{};
+};
+
+/// y[t][n] = x_scales[t] * w_scales[n] * sum_i x[t][i] * w[n][i], of two operands that quantize_rows wrote.
+struct GemmI8Args {
+    DType type = DType::F32;  ///< of y
+    TensorRef w{}, w_scales{}, x{}, x_scales{}, y{};
+    std::uint32_t rows = 0, cols = 0, n_vec = 0;
+    KernelChoice kernel{};
+};
+
+/// state_out: empty or state itself = the states are updated in place.
+struct LinearAttentionArgs {
+    DType type = DType::F32;
+    std::uint32_t n_heads = 0, n_k_heads = 0, k_dim = 0, v_dim = 0;
+    TensorRef state{}, state_out{};  ///< n_slots x n_heads x k_dim x v_dim fp32, dense
+    std::uint32_t n_slots = 0;
+    TensorRef slots{}, row_starts{}, seq_lens{};  ///< n_seqs; n_seqs + 1; n_seqs or empty
+    std::uint32_t n_seqs = 0, n_rows = 0, max_rows = 0;
+    TensorRef q{}, k{}, v{}, out{};
+    std::uint64_t q_head_stride = 0, k_head_stride = 0, v_head_stride = 0, out_head_stride = 0;
+    TensorRef decay{};            ///< n_rows rows of n_heads fp32, or n_heads
+    bool decay_per_head = false;
+    float scale = 0.0f;           ///< 0 = 1 / sqrt(k_dim)
+    TensorRef workspace{};        ///< empty = the stream's own
+    TensorRef status{};
+    KernelChoice kernel{};
+};
+
 /// The MI355X backend's own interface on top of the reference's.
 class MiBackend : public Backend {
 public:
@@ -588,6 +636,10 @@ public:
     virtual void kv8_fork(Stream&, const Kv8PagesArgs&) = 0;
     virtual void kv8_compact(Stream&, const Kv8CompactArgs&) = 0;
     virtual void kv8_copy_pages(Stream&, const Kv8PagesArgs&) = 0;
+    virtual void norm_rope(Stream&, const NormRopeArgs&) = 0;
+    virtual void quantize_rows(Stream&, const QuantizeRowsArgs&) = 0;
+    virtual void gemm_i8(Stream&, const GemmI8Args&) = 0;
+    virtual void linear_attention(Stream&, const LinearAttentionArgs&) = 0;
 };
 
 /// The kernel family a MATMUL or GATE_UP_SWIGLU call with `allow_gemm == false` and kernel
@@ -636,5 +688,9 @@ inline constexpr std::uint32_t kKv8Write = 52;          // kv8_write
 inline constexpr std::uint32_t kKv8Read = 53;           // kv8_read
 inline constexpr std::uint32_t kKv8Attention = 54;      // kv8_attention (the library picks the kernel by the rows)
 inline constexpr std::uint32_t kKv8Pages = 55;          // kv8_resize, kv8_fork, kv8_compact, kv8_copy_pages
+inline constexpr std::uint32_t kNormRope = 56;          // norm_rope
+inline constexpr std::uint32_t kQuantizeRows = 57;      // quantize_rows
+inline constexpr std::uint32_t kGemmI8 = 58;            // gemm_i8 (the library picks the kernel by the sizes)
+inline constexpr std::uint32_t kLinearAttention = 59;   // linear_attention (likewise)
 
 }  // namespace halo_mi::backend

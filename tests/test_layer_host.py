@@ -135,6 +135,8 @@ def test_linear_attention_refusals(hl):
     refused(hl, K, call, decay_stride=4, decay_per_head=True)
     refused(hl, K, call, q_stride=100)
     refused(hl, K, call, v_head_stride=64)
+    for name in ("q_stride", "k_stride", "v_stride"):  # a chunk's rows are addressed with 32 bits
+        refused(hl, U, call, **{name: (1 << 24) + 1})
     slot = 4 * 4 * 64 * 128
     refused(hl, K, call, out=A + 3 * slot - 4)  # over the states
     refused(hl, K, call, out=C)
