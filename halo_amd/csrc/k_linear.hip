@@ -74,9 +74,7 @@ __global__ __launch_bounds__(kBlock) void k_linear_rows(LinearArgs a) {
             o += qq * S[j];
         }
 #pragma unroll
-        for (int i = 8; i < 64; i *= 2)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[c] += __shfl_xor(o[c], i);
+        for (int c = 0; c < 4; ++c) o[c] = across32(across16(o[c] + lanes<0x128>(o[c])));
         if (tid % 64 < 8) *reinterpret_cast<float4v*>(&parts[t & 1][tid / 64][tid * 4 % kColumns]) = o;
         __syncthreads();
         if (tid < kColumns) {

@@ -4,9 +4,10 @@
 // cross-lane moves and turn what they have in their registers. A token's table of sines and cosines and both parts'
 // weights are made once per workgroup, in LDS, while the first heads are on their way.
 //
-// Memory bounds it: 6133 tokens of 40 heads of 128 in bfloat16 take 31.5 us (4.0 TB/s read and written; adjacent pairs, 29.4 us in halves).
-// One token a workgroup took 35: 40 heads are two and a half rounds of its lanes, and every one waits for its table. A wave per token, with
-// its table and weights in registers, took 34 to 48, a head loaded ahead 32 to 37: fewer waves fit.
+// Memory bounds it: 6133 tokens of 40 heads of 128 in bfloat16 take 27.6 us (4.5 TB/s read and written), of 256 with 64 turned 63.4 us (4.0). One
+// token a workgroup took 33.2: 40 heads are two and a half rounds of its lanes, and every one waits for its table. A wave per token, with its table and
+// weights in registers, took 34 to 48, a head loaded ahead 32 to 37: fewer waves fit. Sums by way of LDS took 28.2 and 80.7, adjacent
+// pairs loaded 32 bytes a lane 31.3.
 //
 // Sums, products and the root are in 32 bits, one rounding to the type at the end: rounding the normed head to 16 bits before the
 // rotation, as two launches do, is left out.
@@ -33,6 +34,36 @@ constexpr uint32_t kTokens = 1u << 23;  // of a launch: a grid has fewer than 2^
 __device__ __forceinline__ float first_of(float x, float y, float2 cs) { return fmaf(x, cs.x, -(y * cs.y)); }
 __device__ __forceinline__ float second_of(float x, float y, float2 cs) { return fmaf(x, cs.y, y * cs.x); }
 
+// The sum over G lanes, in all of them.
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+    v += lanes<0xB1>(v);   // the neighbour
+    v += lanes<0x4E>(v);   // the other pair of 4
+    v += lanes<0x141>(v);  // 8 lanes mirrored: the other 4
+    if (G >= 16) v += lanes<0x140>(v);
+    if (G >= 32) v = across16(v);
+    if (G == 64) v = across32(v);
+    return v;
+}
+
+// Both parts' rows, chosen lane by lane. They are kept in scalar registers by force: the compiler would choose the arguments' address instead, and
+// load them in front of every head.
+struct BothRows {
+    uint64_t data[2], stride[2], head_stride[2];
+    __device__ __forceinline__ BothRows(const HeadRows& a, const HeadRows& b, uint32_t heads, uint32_t size)
+        : data{reinterpret_cast<uint64_t>(a.data), reinterpret_cast<uint64_t>(b.data) - heads * b.head_stride * size},
+          stride{a.stride * size, b.stride * size},
+          head_stride{a.head_stride * size, b.head_stride * size} {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) asm volatile("" : "+s"(data[i]), "+s"(stride[i]), "+s"(head_stride[i]));
+    }
+    // head h of both parts' in a row, of token t
+    template <typename T>
+    __device__ __forceinline__ T* at(bool second, uint32_t t, uint32_t h) const {
+        return reinterpret_cast<T*>((second ? data[1] : data[0]) + t * (second ? stride[1] : stride[0]) + h * (second ? head_stride[1] : head_stride[0]));
+    }
+};
+
 // One workgroup: tokens blockIdx.x * tokens .. + tokens - 1, of each the heads from blockIdx.y * heads_per on, side by side. G lanes have a head between
 // them, an item each: V pairs (2 V elements), or V elements that are not turned.
 template <typename T, int V, bool INTERLEAVED, int G>
@@ -42,17 +73,16 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope(NormRopeArgs n, uint32_t h
     __shared__ alignas(16) float weight[2][2 * V * G];
     const uint32_t t0 = blockIdx.x * tokens, here = min(tokens, a.n_tokens - t0), half = a.rot / 2, c = threadIdx.x % G, turned = half / V, items = turned + (a.dim - a.rot) / V;
     const uint32_t h0 = blockIdx.y * heads_per, h_count = min(a.heads - h0, heads_per);
-    // the item's elements: ex of the head and on, and for a turned one ey and on (adjacent pairs: the next V)
+    // the item's elements: V of the head from ex on, and for a turned one V from ey on: its pairs' others, or other pairs
     const bool turns = c < turned, has = c < items;
-    const uint32_t ex = turns ? c * V * (INTERLEAVED ? 2 : 1) : a.rot + (c - turned) * V;
-    const uint32_t ey = INTERLEAVED ? ex + V : ex + half;
+    const uint32_t ex = turns ? c * V : a.rot + (c - turned) * V, ey = ex + half;
     Vec<T, V> x{}, y{};
+    const bool normed[2] = {n.norm_w[0] != nullptr, n.norm_w[1] != nullptr};
+    const BothRows in_rows(a.part[0].in, a.part[1].in, a.part[0].heads, sizeof(T)), out_rows(a.part[0].out, a.part[1].out, a.part[0].heads, sizeof(T));
     // head h0 + h of token t0 + t
     const auto fetch = [&](uint32_t t, uint32_t h) {
         h += h0;
-        const bool second = h >= a.part[0].heads;
-        const HeadRows& r = a.part[second].in;
-        const T* in = static_cast<const T*>(r.data) + (t0 + t) * r.stride + (second ? h - a.part[0].heads : h) * r.head_stride;
+        const T* in = in_rows.template at<const T>(h >= a.part[0].heads, t0 + t, h);
         if (has) x = *reinterpret_cast<const Vec<T, V>*>(in + ex);
         if (turns) y = *reinterpret_cast<const Vec<T, V>*>(in + ey);
     };
@@ -70,7 +100,6 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope(NormRopeArgs n, uint32_t h
     while (t < here) {
         const uint32_t head = h0 + h;
         const bool second = head >= a.part[0].heads;
-        const HeadRows& r = a.part[second].out;
         float u[V], w[V], sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -82,10 +111,9 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope(NormRopeArgs n, uint32_t h
             w[i] = to_f32(y.v[i]);
             sum = fmaf(w[i], w[i], sum);
         }
-#pragma unroll
-        for (int i = 1; i < G; i *= 2) sum += __shfl_xor(sum, i, G);
-        const float inv = n.norm_w[second] ? 1.0f / sqrtf(fmaf(sum, over_dim, n.eps)) : 1.0f;
-        T* out = const_cast<T*>(static_cast<const T*>(r.data)) + (t0 + t) * r.stride + (second ? head - a.part[0].heads : head) * r.head_stride;
+        sum = group_sum<G>(sum);
+        const float inv = (second ? normed[1] : normed[0]) ? 1.0f / sqrtf(fmaf(sum, over_dim, n.eps)) : 1.0f;
+        T* out = out_rows.template at<T>(second, t0 + t, head);
         const float* wx = weight[second] + ex;
         if (turns) {
             const float* wy = weight[second] + ey;
@@ -94,7 +122,7 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope(NormRopeArgs n, uint32_t h
             for (int i = 0; i < V; ++i) u[i] = u[i] * inv * wx[i], w[i] = w[i] * inv * wy[i];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float2 cs = table[t][c * V + i];
+                const float2 cs = table[t][INTERLEAVED ? (i < V / 2 ? ex : ey) / 2 + i % (V / 2) : ex + i];
                 if constexpr (INTERLEAVED) {
                     const float f = i < V / 2 ? u[2 * i] : w[2 * i - V], g = i < V / 2 ? u[2 * i + 1] : w[2 * i + 1 - V];
                     T* e = i < V / 2 ? &ox.v[2 * i] : &oy.v[2 * i - V];

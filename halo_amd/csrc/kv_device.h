@@ -54,6 +54,21 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
     return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0400u), __builtin_amdgcn_perm(b, a, 0x0C0C0400u), 0x05040100u);
 }
 
+// Sums across lanes by moves of the vector unit. lanes<CTRL>: another lane's value of the same 16, by the move's control.
+template <int CTRL>
+__device__ __forceinline__ float lanes(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+// v + the value 16, or 32, lanes away (lane ^ 16, lane ^ 32).
+__device__ __forceinline__ float across16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float across32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // A batch's rows of one sequence: its first row, row count and cached tokens. Row starts that fall or that
 // pass n_rows are cut to what the row operands hold.
 struct SeqRows {
