@@ -208,17 +208,23 @@ __device__ __forceinline__ bool not_finite(const Patch<T>& p) {
 // that of the registers, and q and k lie in LDS in the same order. Products are of bf16 pieces, summed in 32 bits: q, k and v exactly (one
 // piece for BF16, two for F16, three for F32), the faded k in three, P and S in two where the output has 16 bits, else in three; of pairs of
 // pieces those that matter in the result are multiplied.
-// Chunks of 32 tokens keep LDS at 52 KB for BF16 and k_dim 128, three workgroups a CU.
+//
+// What bounds it (BF16, 48 heads of 128, four prompts of 601 to 5000 rows, 329 us): two workgroups a CU, by their registers (220; LDS 55 KB),
+// whose waves issue vector instructions half of the time (735 a wave and chunk beside 92 matrix products, 192 of them S's pieces) and feed the
+// matrix cores a quarter of it; segments of unequal length leave a quarter of the places empty. Halved steps of it: stores that a branch may skip
+// made every chunk wait for all loads in flight (399 us against 380 for other prompts); k^T's pieces read one product ahead. What gave nothing: the
+// fade on v in place of k (405), loads a whole chunk ahead (386), the segments' pass with half the columns a workgroup (403).
 // STATES: only the state that a segment adds is made (from zeros), for the segments after it.
 // Sequences are cut into segments where there are too few for the GPU.
 struct Segments {
     uint32_t length, most;  // rows of a segment; segments of a sequence at most
     uint32_t room;          // boundaries that `states` holds
-    float* states;          // what a segment but the last of its sequence adds, then the state before the next one; [boundary][head][k_dim][v_dim]
+    float* states;          // what a segment but the last of its sequence adds, then the state before the next one; [boundary][head][k_dim][v_dim];
+                            // behind a sequence's boundaries the state before its first segment, where the last one writes over it
     float* fades;           // ... and its decays' sum (log2): [boundary][head]
 };
 
-// A sequence's boundaries between segments: their number, and how many lie before it. Where the room for their states ends (row starts that
+// A sequence's boundaries between segments: their number, and where they begin. Where the room for their states ends (row starts that
 // fall count rows twice), a sequence is not cut. For all of a workgroup.
 struct Cuts {
     uint32_t parts, base;
@@ -234,13 +240,14 @@ __device__ __forceinline__ bool look_up(const LinearArgs& a, const Segments& seg
     for (uint32_t i = threadIdx.x; i < s; i += threads) {
         const LinearRows other = linear_rows(a, i);
         good = good && !(other.rows > 0 && a.slots[i] == slot);
-        before += cuts_of(seg, other.rows);
+        const uint32_t parts = cuts_of(seg, other.rows);
+        before += parts + (parts > 0);
     }
     good = !__syncthreads_or(!good);
     if (before) atomicAdd(&count, before);
     __syncthreads();
     cuts = {cuts_of(seg, rows), count};
-    if (cuts.base > seg.room || seg.room - cuts.base < cuts.parts) cuts.parts = 0;
+    if (cuts.base > seg.room || seg.room - cuts.base <= cuts.parts) cuts.parts = 0;
     return good;
 }
 
@@ -326,7 +333,7 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
     const float* before = nullptr;
     if (!STATES) {
         if (part > 0) before = seg.states + ((uint64_t)(boundary - 1) * a.heads + head) * plane;
-        else if (!begins) before = a.state + ((uint64_t)slot * a.heads + head) * plane;
+        else if (!begins) before = !last_part && a.state == a.state_out ? seg.states + ((uint64_t)(cuts.base + cuts.parts) * a.heads + head) * plane : a.state + ((uint64_t)slot * a.heads + head) * plane;
     }
     if (before)
 #pragma unroll
@@ -679,6 +686,7 @@ __global__ __launch_bounds__(kBlock) void k_linear_join(LinearArgs a, Segments s
     if (at >= plane) return;
     const bool begins = a.seq_lens && a.seq_lens[s] <= (int32_t)r.rows;
     float4v S = begins ? float4v{} : *reinterpret_cast<const float4v*>(a.state + ((uint64_t)slot * a.heads + head) * plane + at);
+    if (!begins && cuts.parts > 0 && a.state == a.state_out) *reinterpret_cast<float4v*>(seg.states + ((uint64_t)(cuts.base + cuts.parts) * a.heads + head) * plane + at) = S;
     for (uint32_t p = 0; p < cuts.parts; ++p) {
         const uint64_t i = (uint64_t)(cuts.base + p) * a.heads + head;
         float4v* x = reinterpret_cast<float4v*>(seg.states + i * plane + at);
@@ -704,8 +712,10 @@ Segments plan_segments(const LinearArgs& a, uint64_t part_bytes, uint64_t* bytes
     const uint64_t target = 2 * kCus, ends = a.n_seqs * blocks / 2;
     uint64_t length = a.max_rows;
     if (ends < target) length = std::max<uint64_t>(256, (a.n_rows * blocks / (target - ends) + kChunk - 1) / kChunk * kChunk);
-    // boundaries: one behind every whole segment of a sequence but its last
-    const auto boundaries = [&](uint64_t l) { return std::min<uint64_t>(a.n_rows / l, (uint64_t)a.n_seqs * ((a.max_rows + l - 1) / l - 1)); };
+    // boundaries: one behind every whole segment of a sequence but its last, and one more for each sequence that is cut
+    const auto boundaries = [&](uint64_t l) {
+        return std::min<uint64_t>(a.n_rows / l, (uint64_t)a.n_seqs * ((a.max_rows + l - 1) / l - 1)) + std::min<uint64_t>(a.n_rows / l, a.n_seqs);
+    };
     while (length < a.max_rows && boundaries(length) * per > part_bytes) length += std::max<uint64_t>(kChunk, length / 16 / kChunk * kChunk);
     if (length >= a.max_rows) return seg;
     seg.length = (uint32_t)length;

@@ -357,3 +357,30 @@ def test_many_sequences_and_far_slots(hl, dev):
     batch = hl.LinearBatch(c.ints(c.slots + far), c.ints(c.starts), seqs, c.n, 1)
     hl.linear_attention(BF16, state, batch, c.q, c.k, c.v, c.out, c.d, 1)
     c.check((c.out.double().cpu().numpy(), s[far:].double().cpu().numpy()), in_place=True)
+
+
+@pytest.mark.parametrize("t, heads", [(F32, 64), (BF16, 40)], ids=["f32", "bf16"])
+def test_long_sequences_in_place(hl, dev, t, heads):
+    """The last segment of a sequence writes over the state that the first one begins with: in place is bitwise what it is beside it, with more
+    segments than the GPU holds at once and without any."""
+    import torch
+
+    kh, kd, vd, lens = heads // 8, 128, 128, [2600, 300, 3300]
+    rows, dt = sum(lens), torch.float32 if t == F32 else torch.bfloat16
+    g = torch.Generator(device=dev).manual_seed(5)
+    q, k, v = (torch.randn(rows, h, d, device=dev, generator=g).to(dt) for h, d in ((kh, kd), (kh, kd), (heads, vd)))
+    decay = -0.02 * torch.rand(rows, heads, device=dev, generator=g)
+    first = torch.randn(3, heads, kd, vd, device=dev, generator=g)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    batch = hl.LinearBatch(ints([2, 0, 1]), ints(np.concatenate([[0], np.cumsum(lens)]).tolist()), 3, rows, max(lens))
+    out, new = torch.empty_like(v), torch.empty_like(first)
+    beside = hl.LinearState(first, 3, heads, kd, vd, new)
+    # one workspace for both: the stream's own may be smaller, and sequences cut elsewhere round elsewhere
+    need = hl.linear_attention_workspace(t, beside, batch, q, k, v, out, decay, kh)
+    assert need > 0
+    space = torch.empty(need, dtype=torch.uint8, device=dev)
+    hl.linear_attention(t, beside, batch, q, k, v, out, decay, kh, workspace=space, workspace_bytes=need)
+    for _ in range(3):
+        state, again = first.clone(), torch.empty_like(out)
+        hl.linear_attention(t, hl.LinearState(state, 3, heads, kd, vd), batch, q, k, v, again, decay, kh, workspace=space, workspace_bytes=need)
+        assert torch.equal(again, out) and torch.equal(state, new)
