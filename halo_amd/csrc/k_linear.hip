@@ -219,12 +219,11 @@ __device__ __forceinline__ bool not_finite(const Patch<T>& p) {
 struct Segments {
     uint32_t length, most;  // rows of a segment; segments of a sequence at most
     uint32_t room;          // boundaries that `states` holds
-    float* states;          // what a segment but the last of its sequence adds, then the state before the next one; [boundary][head][k_dim][v_dim];
-                            // behind a sequence's boundaries the state before its first segment, where the last one writes over it
+    float* states;          // what a segment but the last of its sequence adds, then the state before the next one; [boundary][head][k_dim][v_dim]
     float* fades;           // ... and its decays' sum (log2): [boundary][head]
 };
 
-// A sequence's boundaries between segments: their number, and where they begin. Where the room for their states ends (row starts that
+// A sequence's boundaries between segments: their number, and how many lie before it. Where the room for their states ends (row starts that
 // fall count rows twice), a sequence is not cut. For all of a workgroup.
 struct Cuts {
     uint32_t parts, base;
@@ -240,14 +239,13 @@ __device__ __forceinline__ bool look_up(const LinearArgs& a, const Segments& seg
     for (uint32_t i = threadIdx.x; i < s; i += threads) {
         const LinearRows other = linear_rows(a, i);
         good = good && !(other.rows > 0 && a.slots[i] == slot);
-        const uint32_t parts = cuts_of(seg, other.rows);
-        before += parts + (parts > 0);
+        before += cuts_of(seg, other.rows);
     }
     good = !__syncthreads_or(!good);
     if (before) atomicAdd(&count, before);
     __syncthreads();
     cuts = {cuts_of(seg, rows), count};
-    if (cuts.base > seg.room || seg.room - cuts.base <= cuts.parts) cuts.parts = 0;
+    if (cuts.base > seg.room || seg.room - cuts.base < cuts.parts) cuts.parts = 0;
     return good;
 }
 
@@ -301,7 +299,9 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
     __shared__ int32_t bad_at[kColumnsHere];
     __shared__ int32_t bad_chunk;
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), m = lane % 16, g = lane / 16;
-    const uint32_t v_blocks = a.v_dim / kColumnsHere, head = blockIdx.x / v_blocks, v0 = blockIdx.x % v_blocks * kColumnsHere;
+    // workgroups go to the eight XCDs in turn: each takes heads side by side, whose q and k are the same
+    const uint32_t block = gridDim.x % 8 ? blockIdx.x : blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+    const uint32_t v_blocks = a.v_dim / kColumnsHere, head = block / v_blocks, v0 = block % v_blocks * kColumnsHere;
     const uint32_t s = blockIdx.z, part = blockIdx.y;
     const LinearRows r = linear_rows(a, s);
     if (part > cuts_of(seg, r.rows) || r.rows == 0) return;
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
     const float* before = nullptr;
     if (!STATES) {
         if (part > 0) before = seg.states + ((uint64_t)(boundary - 1) * a.heads + head) * plane;
-        else if (!begins) before = !last_part && a.state == a.state_out ? seg.states + ((uint64_t)(cuts.base + cuts.parts) * a.heads + head) * plane : a.state + ((uint64_t)slot * a.heads + head) * plane;
+        else if (!begins) before = a.state + ((uint64_t)slot * a.heads + head) * plane;
     }
     if (before)
 #pragma unroll
@@ -663,6 +663,7 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
     }
     float* after = nullptr;
     if (STATES) after = seg.states + ((uint64_t)boundary * a.heads + head) * plane;
+    else if (last_part && part > 0 && a.state == a.state_out) after = seg.states + ((uint64_t)(boundary - 1) * a.heads + head) * plane;  // for k_linear_settle
     else if (last_part) after = a.state_out + ((uint64_t)slot * a.heads + head) * plane;
     const float settled = __builtin_amdgcn_exp2f((float)held);
     if (after)
@@ -686,13 +687,25 @@ __global__ __launch_bounds__(kBlock) void k_linear_join(LinearArgs a, Segments s
     if (at >= plane) return;
     const bool begins = a.seq_lens && a.seq_lens[s] <= (int32_t)r.rows;
     float4v S = begins ? float4v{} : *reinterpret_cast<const float4v*>(a.state + ((uint64_t)slot * a.heads + head) * plane + at);
-    if (!begins && cuts.parts > 0 && a.state == a.state_out) *reinterpret_cast<float4v*>(seg.states + ((uint64_t)(cuts.base + cuts.parts) * a.heads + head) * plane + at) = S;
     for (uint32_t p = 0; p < cuts.parts; ++p) {
         const uint64_t i = (uint64_t)(cuts.base + p) * a.heads + head;
         float4v* x = reinterpret_cast<float4v*>(seg.states + i * plane + at);
         S = S * __builtin_amdgcn_exp2f(seg.fades[i]) + *x;
         *x = S;
     }
+}
+
+// In place, the last segment of a sequence leaves its state where the one before it was: the first segment may not have read the pool's yet. Then
+// it goes to the pool.
+__global__ __launch_bounds__(kBlock) void k_linear_settle(LinearArgs a, Segments seg) {
+    const uint32_t tid = threadIdx.x, head = blockIdx.y, s = blockIdx.z, at = (blockIdx.x * kBlock + tid) * 4, plane = a.k_dim * a.v_dim;
+    const LinearRows r = linear_rows(a, s);
+    if (cuts_of(seg, r.rows) == 0) return;
+    const int32_t slot = a.slots[s];
+    Cuts cuts;
+    if (!look_up(a, seg, s, slot, r.rows, kBlock, cuts) || cuts.parts == 0 || at >= plane) return;
+    *reinterpret_cast<float4v*>(a.state_out + ((uint64_t)slot * a.heads + head) * plane + at) =
+        *reinterpret_cast<const float4v*>(seg.states + ((uint64_t)(cuts.base + cuts.parts - 1) * a.heads + head) * plane + at);
 }
 
 constexpr uint32_t kCus = 256;
@@ -712,10 +725,8 @@ Segments plan_segments(const LinearArgs& a, uint64_t part_bytes, uint64_t* bytes
     const uint64_t target = 2 * kCus, ends = a.n_seqs * blocks / 2;
     uint64_t length = a.max_rows;
     if (ends < target) length = std::max<uint64_t>(256, (a.n_rows * blocks / (target - ends) + kChunk - 1) / kChunk * kChunk);
-    // boundaries: one behind every whole segment of a sequence but its last, and one more for each sequence that is cut
-    const auto boundaries = [&](uint64_t l) {
-        return std::min<uint64_t>(a.n_rows / l, (uint64_t)a.n_seqs * ((a.max_rows + l - 1) / l - 1)) + std::min<uint64_t>(a.n_rows / l, a.n_seqs);
-    };
+    // boundaries: one behind every whole segment of a sequence but its last
+    const auto boundaries = [&](uint64_t l) { return std::min<uint64_t>(a.n_rows / l, (uint64_t)a.n_seqs * ((a.max_rows + l - 1) / l - 1)); };
     while (length < a.max_rows && boundaries(length) * per > part_bytes) length += std::max<uint64_t>(kChunk, length / 16 / kChunk * kChunk);
     if (length >= a.max_rows) return seg;
     seg.length = (uint32_t)length;
@@ -738,11 +749,13 @@ int launch_chunks(const LinearArgs& a, const Segments& seg, hipStream_t st) {
         auto* k = columns == 64 ? k_linear_chunks<T, KD, 4, 1, S> : columns == 96 ? k_linear_chunks<T, KD, 6 / UT, UT, S> : k_linear_chunks<T, KD, 8 / UT, UT, S>;
         hipLaunchKernelGGL(k, dim3(blocks, S ? seg.most - 1 : seg.most, a.n_seqs), dim3(columns == 64 ? 256 : columns / 16 / UT * 64), 0, st, a, seg);
     };
+    const dim3 planes((a.k_dim * a.v_dim / 4 + kBlock - 1) / kBlock, a.heads, a.n_seqs);
     if (seg.most > 1) {
         run(std::true_type{});
-        hipLaunchKernelGGL(k_linear_join, dim3((a.k_dim * a.v_dim / 4 + kBlock - 1) / kBlock, a.heads, a.n_seqs), dim3(kBlock), 0, st, a, seg);
+        hipLaunchKernelGGL(k_linear_join, planes, dim3(kBlock), 0, st, a, seg);
     }
     run(std::false_type{});
+    if (seg.most > 1 && a.state == a.state_out) hipLaunchKernelGGL(k_linear_settle, planes, dim3(kBlock), 0, st, a, seg);
     return hip_status(hipGetLastError(), "linear_attention");
 }
 
