@@ -1,6 +1,11 @@
 // gfx950 kernels of the product of 8-bit integers with a scale for each token and each output channel,
 //   y[t][n] = sx[t] sw[n] sum_i x[t][i] w[n][i],
 // on the integer matrix cores: the sums are exact in 32 bits, whatever their order, so how K is split is free.
+//
+// Few vectors read w once, and its stream bounds them: 17408 channels of 5120 codes for one vector take 16.4 us (89 MB, 5.4 TB/s). Many are bound by
+// the products: 3990 vectors take 355 to 375 us (1.9 to 2.0 POP/s; a large library product of these sizes reaches 2.0), 44 % of the matrix cores'
+// cycles at the 2.1 GHz that the card then keeps; 4096 vectors of 8192 codes by 8192 channels 2.3 POP/s. In between, 61 vectors by 6144
+// channels take 12.7 us and 509 by 17408 62 (1.5 POP/s; 218 tiles on 256 CUs, whose loads take as long as their products).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
