@@ -221,3 +221,19 @@ def test_gemm_i8_captured(hl, dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, y2) and torch.equal(codes, c2)
+
+
+@TYPES
+@pytest.mark.parametrize("rows,cols,stride", [(700, 90, 91), (513, 1000, 1000), (900, 2040, 2051), (600, 2048, 2048), (515, 4111, 4111)])
+def test_quantize_rows_of_one_wave(hl, dev, t, rows, cols, stride):
+    """Many narrow rows, a wave each, and the first sizes past that; rows of zeros and of one NaN among them."""
+    import torch
+
+    rng = np.random.default_rng(cols)
+    x, xx = to_type(rng.standard_normal((rows, stride)) * np.exp(2 * rng.standard_normal((rows, 1))), t, dev)
+    x[5], xx[5] = 0, 0
+    x[rows - 2, cols - 1] = float("nan")
+    xx[rows - 2, cols - 1] = np.nan
+    codes, scales = torch.full((rows, padded(cols)), 77, dtype=torch.int8, device=dev), torch.full((rows,), 3.0, device=dev)
+    hl.quantize_rows(t, x, codes, scales, rows, cols, x_stride=stride)
+    check_rows(codes.cpu().numpy(), scales.cpu().numpy(), xx[:, :cols])

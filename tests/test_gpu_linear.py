@@ -384,3 +384,80 @@ def test_long_sequences_in_place(hl, dev, t, heads):
         state, again = first.clone(), torch.empty_like(out)
         hl.linear_attention(t, hl.LinearState(state, 3, heads, kd, vd), batch, q, k, v, again, decay, kh, workspace=space, workspace_bytes=need)
         assert torch.equal(again, out) and torch.equal(state, new)
+
+
+def test_replayed_in_place(hl, dev):
+    """A batch of prompts, cut into segments, captured in place and replayed: every replay goes on from the states of the one before, as eager
+    calls do."""
+    import torch
+
+    heads, kh, kd, vd, lens = 8, 4, 128, 128, [1500, 40, 2100]
+    rows = sum(lens)
+    g = torch.Generator(device=dev).manual_seed(6)
+    q, k, v = (torch.randn(rows, h, d, device=dev, generator=g).bfloat16() for h, d in ((kh, kd), (kh, kd), (heads, vd)))
+    decay = -0.05 * torch.rand(rows, heads, device=dev, generator=g)
+    first = torch.randn(4, heads, kd, vd, device=dev, generator=g)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    batch = hl.LinearBatch(ints([3, 0, 1]), ints(np.concatenate([[0], np.cumsum(lens)]).tolist()), 3, rows, max(lens))
+    state, out = first.clone(), torch.zeros_like(v)
+    pool = hl.LinearState(state, 4, heads, kd, vd)
+    need = hl.linear_attention_workspace(BF16, pool, batch, q, k, v, out, decay, kh)
+    assert need > 0
+    space = torch.empty(need, dtype=torch.uint8, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        hl.linear_attention(BF16, pool, batch, q, k, v, out, decay, kh, workspace=space, workspace_bytes=need)
+    eager, beside = first.clone(), torch.zeros_like(v)
+    for _ in range(4):
+        graph.replay()
+        hl.linear_attention(BF16, hl.LinearState(eager, 4, heads, kd, vd), batch, q, k, v, beside, decay, kh, workspace=space, workspace_bytes=need)
+        assert torch.equal(out, beside) and torch.equal(state, eager)
+    assert torch.equal(state[2], first[2])
+
+
+def test_two_streams_at_once(hl, dev):
+    """Calls on two streams, each with its stream's workspace, do not meet: bitwise what they give one after the other."""
+    import torch
+
+    heads, kh, kd, vd, rows = 8, 8, 128, 128, 3000
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    sides, calls = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for seed in (1, 2):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        q, k, v = (torch.randn(rows, heads, 128, device=dev, generator=g).bfloat16() for _ in range(3))
+        decay = -0.05 * torch.rand(rows, heads, device=dev, generator=g)
+        state = torch.randn(1, heads, kd, vd, device=dev, generator=g)
+        new, out = torch.empty_like(state), torch.empty_like(v)
+        args = (BF16, hl.LinearState(state, 1, heads, kd, vd, new), hl.LinearBatch(ints([0]), ints([0, rows]), 1, rows, rows), q, k, v, out, decay, kh)
+        calls.append((args, new, out))
+    want = []
+    for (args, new, out), side in zip(calls, sides):
+        torch.cuda.synchronize()
+        hl.linear_attention(*args, stream=side.cuda_stream)
+        torch.cuda.synchronize()
+        want.append((new.clone(), out.clone()))
+        new.zero_()
+        out.zero_()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (args, _, _), side in zip(calls, sides):
+            hl.linear_attention(*args, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    for (_, new, out), (n, o) in zip(calls, want):
+        assert torch.equal(new, n) and torch.equal(out, o)
+
+
+@pytest.mark.parametrize("rows", [8, 70], ids=["steps", "chunks"])
+def test_far_rows(hl, dev, rows):
+    """Rows as far apart as they may be, their offsets past 32 bits."""
+    import torch
+
+    stride, kd, vd = 1 << 24, 64, 64
+    far = [torch.empty(rows * stride, dtype=torch.float32, device=dev) for _ in range(2)]
+    c = Case(dev, F32, [rows], 2, 2, kd, vd, 91)
+    view = lambda b, at, x: b.view(rows, stride)[:, at:at + 128].copy_(x.reshape(rows, 128)) if x is not None else b.view(rows, stride)[:, at:at + 128]
+    view(far[0], 0, c.q), view(far[0], 200, c.k), view(far[0], 1000, c.v)
+    state = hl.LinearState(c.s, c.n_slots, 2, kd, vd, c.new)
+    batch = hl.LinearBatch(c.ints(c.slots), c.ints(c.starts), 1, rows, rows)
+    hl.linear_attention(F32, state, batch, far[0], far[0][200:], far[0][1000:], far[1], c.d, 2, q_stride=stride, k_stride=stride, v_stride=stride, out_stride=stride)
+    c.check((view(far[1], 0, None).double().cpu().numpy().reshape(rows, 2, vd), c.new.double().cpu().numpy()))

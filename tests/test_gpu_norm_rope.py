@@ -112,3 +112,44 @@ def test_norm_rope_past_a_grid(hl, dev, tokens, heads, kv):
     # every head was written
     for y in (qo, ko):
         assert not bool((y == 7).all(-1).any())
+
+
+@TYPES
+@pytest.mark.parametrize("pairs", [0, 1], ids=["half", "interleaved"])
+@pytest.mark.parametrize("tokens,heads,kv,dim,rot", [(2051, 5, 2, 128, 128), (4099, 3, 0, 64, 32), (1025, 9, 4, 256, 64)])
+def test_norm_rope_of_many_tokens(hl, dev, t, pairs, tokens, heads, kv, dim, rot):
+    """Several tokens a workgroup, the last one's not all there."""
+    import torch
+
+    rng = np.random.default_rng(tokens)
+    freqs, _ = hl.rope_freqs(rot, 1e4)
+    pos = rng.integers(0, 5000, tokens).astype(np.int32)
+    q, qx = to_type(rng.standard_normal((tokens, heads, dim)) * 2, t, dev)
+    k, kx = to_type(rng.standard_normal((tokens, max(kv, 1), dim)), t, dev)
+    qw, kw = ((1 + 0.2 * rng.standard_normal(dim)).astype(np.float32) for _ in range(2))
+    qwd, kwd, p, f = (torch.from_numpy(x).to(dev) for x in (qw, kw, pos, freqs))
+    qo, ko = torch.full_like(q, 7), torch.full_like(k, 7)
+    hl.norm_rope(t, p, f, tokens, dim, rot, q, qo, heads, q_norm=qwd, k=k if kv else None, k_out=ko if kv else None, n_kv_heads=kv, k_norm=kwd, pairs=pairs)
+    check(t, qo.double().cpu().numpy(), qx, qw.astype(np.float64), 1e-6, pos, freqs, rot, pairs, 1.0)
+    if kv:
+        check(t, ko.double().cpu().numpy(), kx, kw.astype(np.float64), 1e-6, pos, freqs, rot, pairs, 1.0)
+
+
+def test_norm_rope_of_far_rows(hl, dev):
+    """Rows whose offsets pass 32 bits of bytes and of elements, in place, on another stream than the current one."""
+    import torch
+
+    tokens, heads, dim, stride = 70, 2, 64, 1 << 26
+    big = torch.empty(tokens * stride, dtype=torch.bfloat16, device=dev)
+    rows = big.view(tokens, stride)[:, :heads * dim]
+    rng = np.random.default_rng(9)
+    x, xx = to_type(rng.standard_normal((tokens, heads * dim)), BF16, dev)
+    rows.copy_(x)
+    freqs, _ = hl.rope_freqs(dim, 1e4)
+    pos = np.arange(tokens, dtype=np.int32)
+    p, f, w = torch.from_numpy(pos).to(dev), torch.from_numpy(freqs).to(dev), torch.ones(dim, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    hl.norm_rope(BF16, p, f, tokens, dim, dim, big, big, heads, q_norm=w, q_stride=stride, q_out_stride=stride, stream=side.cuda_stream)
+    side.synchronize()
+    check(BF16, rows.double().cpu().numpy().reshape(tokens, heads, dim), xx.reshape(tokens, heads, dim), np.ones(dim), 1e-6, pos, freqs, dim, 0, 1.0)
