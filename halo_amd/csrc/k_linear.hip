@@ -36,10 +36,15 @@ __device__ __forceinline__ bool slot_taken(const LinearArgs& a, uint32_t s, int3
 }
 
 // Row after row. One workgroup: columns 32 blockIdx.x and on of head blockIdx.y's state in sequence blockIdx.z, in its registers: a
-// thread has 4 columns of rows tid / 8 + 32 j.
+// thread has 4 columns of rows tid / 8 + 32 j. Rows of q, k and v after the first come by way of LDS, one row ahead: loaded where they are used, each element
+// by eight lanes, rows of 61 sequences took 9 us each, and so 6.
+//
+// The states bound one row a sequence: 61 sequences of 48 heads of 128 x 128 in 78.5 us (4.9 TB/s read and written).
 template <typename T, int RK>
 __global__ __launch_bounds__(kBlock) void k_linear_rows(LinearArgs a) {
+    constexpr uint32_t KD = 32 * RK, kElements = (2 * KD + kColumns + kBlock - 1) / kBlock;  // of a row, per thread: q, k, then v
     __shared__ float parts[2][4][kColumns];
+    __shared__ alignas(16) float qk_lds[2][2][KD], v_lds[2][kColumns];  // q and k: the RK elements of a thread side by side
     const uint32_t tid = threadIdx.x, head = blockIdx.y, s = blockIdx.z;
     const uint32_t col = blockIdx.x * kColumns + tid % 8 * 4, row = tid / 8;
     const LinearRows r = linear_rows(a, s);
@@ -47,39 +52,69 @@ __global__ __launch_bounds__(kBlock) void k_linear_rows(LinearArgs a) {
     const int32_t slot = a.slots[s];
     const bool in_pool = (uint32_t)slot < a.n_slots, begins = a.seq_lens && a.seq_lens[s] <= (int32_t)r.rows;
     const uint64_t at = ((uint64_t)(in_pool ? slot : 0) * a.heads + head) * a.k_dim * a.v_dim + row * a.v_dim + col;
+    const uint32_t hk = head / a.group;
+    const T* q = static_cast<const T*>(a.q.data) + r.row0 * a.q.stride + hk * a.q.head_stride;
+    const T* k = static_cast<const T*>(a.k.data) + r.row0 * a.k.stride + hk * a.k.head_stride;
+    const T* v = static_cast<const T*>(a.v.data) + r.row0 * a.v.stride + head * a.v.head_stride + blockIdx.x * kColumns;
+    const float* g = a.decay + (uint64_t)r.row0 * a.decay_stride + head;
+    T* out = const_cast<T*>(static_cast<const T*>(a.out.data)) + r.row0 * a.out.stride + head * a.out.head_stride + blockIdx.x * kColumns;
+    T element[kElements];
+    const auto fetch = [&](uint32_t t) {
+#pragma unroll
+        for (uint32_t e = 0; e < kElements; ++e) {
+            const uint32_t i = tid + e * kBlock;
+            if (i < KD) element[e] = q[t * a.q.stride + i];
+            else if (i < 2 * KD) element[e] = k[t * a.k.stride + (i - KD)];
+            else if (i < 2 * KD + kColumns) element[e] = v[t * a.v.stride + (i - 2 * KD)];
+        }
+    };
+    const auto put = [&](uint32_t t) {
+#pragma unroll
+        for (uint32_t e = 0; e < kElements; ++e) {
+            const uint32_t i = tid + e * kBlock, d = i % KD;
+            if (i < 2 * KD) qk_lds[t & 1][i / KD][d % 32 * RK + d / 32] = to_f32(element[e]);
+            else if (i < 2 * KD + kColumns) v_lds[t & 1][i - 2 * KD] = to_f32(element[e]);
+        }
+    };
     float4v S[RK];
 #pragma unroll
     for (int j = 0; j < RK; ++j) S[j] = begins ? float4v{} : *reinterpret_cast<const float4v*>(a.state + at + j * 32 * a.v_dim);
+    // the first row as it is used: a single one is on its way with S
+    float kk[RK], qq[RK];
+    float4v vv;
+#pragma unroll
+    for (int j = 0; j < RK; ++j) kk[j] = to_f32(k[row + 32 * j]), qq[j] = to_f32(q[row + 32 * j]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vv[i] = to_f32(v[tid % 8 * 4 + i]);
     const bool bad = __syncthreads_or(!in_pool || slot_taken(a, s, slot, tid, kBlock));
-    const uint32_t hk = head / a.group;
-    const T* q = static_cast<const T*>(a.q.data) + r.row0 * a.q.stride + hk * a.q.head_stride + row;
-    const T* k = static_cast<const T*>(a.k.data) + r.row0 * a.k.stride + hk * a.k.head_stride + row;
-    const T* v = static_cast<const T*>(a.v.data) + r.row0 * a.v.stride + head * a.v.head_stride + col;
-    const float* g = a.decay + (uint64_t)r.row0 * a.decay_stride + head;
-    T* out = const_cast<T*>(static_cast<const T*>(a.out.data)) + r.row0 * a.out.stride + head * a.out.head_stride + blockIdx.x * kColumns;
     if (bad) {
         if (tid == 0 && blockIdx.x == 0 && head == 0) set_status(a.status, HALO_MI_STATUS_BAD_INDEX);
         for (uint32_t i = tid; i < r.rows * kColumns; i += kBlock) out[i / kColumns * a.out.stride + i % kColumns] = from_f32<T>(__uint_as_float(0x7FC00000u));
         return;
     }
     for (uint32_t t = 0; t < r.rows; ++t) {
+        if (t + 1 < r.rows) fetch(t + 1);
         const float fade = __expf(g[t * a.decay_stride]);
-        float4v vv, o{};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vv[i] = to_f32(v[t * a.v.stride + i]);
+        float4v o{};
 #pragma unroll
         for (int j = 0; j < RK; ++j) {
-            const float kk = to_f32(k[t * a.k.stride + j * 32]), qq = to_f32(q[t * a.q.stride + j * 32]);
-            S[j] = S[j] * fade + kk * vv;
-            o += qq * S[j];
+            S[j] = S[j] * fade + kk[j] * vv;
+            o += qq[j] * S[j];
         }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] = across32(across16(o[c] + lanes<0x128>(o[c])));
-        if (tid % 64 < 8) *reinterpret_cast<float4v*>(&parts[t & 1][tid / 64][tid * 4 % kColumns]) = o;
+        // the four columns' sums over the wave's rows: each step leaves a lane half of the columns
+        const float sum = both16(both32(o[0], o[1]), both32(o[2], o[3]));
+        const float all = sum + lanes<0x128>(sum);
+        if (tid % 16 < 8) parts[t & 1][tid / 64][tid % 8 * 4 + tid / 32 % 2 + tid / 16 % 2 * 2] = all;
+        if (t + 1 < r.rows) put(t + 1);
         __syncthreads();
         if (tid < kColumns) {
             const float sum = (parts[t & 1][0][tid] + parts[t & 1][1][tid]) + (parts[t & 1][2][tid] + parts[t & 1][3][tid]);
             out[t * a.out.stride + tid] = from_f32<T>(sum * a.scale);
+        }
+        if (t + 1 < r.rows) {
+#pragma unroll
+            for (int j = 0; j < RK; ++j) qq[j] = qk_lds[~t & 1][0][row * RK + j], kk[j] = qk_lds[~t & 1][1][row * RK + j];
+            vv = *reinterpret_cast<const float4v*>(&v_lds[~t & 1][tid % 8 * 4]);
         }
     }
 #pragma unroll
@@ -709,7 +744,11 @@ __global__ __launch_bounds__(kBlock) void k_linear_settle(LinearArgs a, Segments
 }
 
 constexpr uint32_t kCus = 256;
-constexpr uint32_t kFewRows = 12;  // up to this many rows of a sequence go one after another
+// Up to this many rows of a sequence go one after another: a chunk costs the same for one row as for 32, and more the more pieces its type has (48 heads
+// of 128; 8 and 61 sequences: rows of BF16 4 in 14.7 us, 6 in 84.6, 8 in 18.1, 12 in 117, a chunk 15.6 and 95 to 99; of F16 8 in 17.7, 12 in 117, a
+// chunk 17.5 and 106 to 110; of F32 16 in 25.3, 12 in 118, a chunk 25.5 and 154 to 160).
+template <typename T>
+constexpr uint32_t kFewRows = kPieces<T> == 1 ? 6 : kPieces<T> == 2 ? 8 : 16;
 
 // Columns of a workgroup: a whole head's where they are 64, 96 or 128.
 uint32_t columns_of(const LinearArgs& a) { return a.v_dim == 64 ? 64 : a.v_dim % 128 == 0 ? 128 : 96; }
@@ -718,10 +757,10 @@ uint32_t columns_of(const LinearArgs& a) { return a.v_dim == 64 ? 64 : a.v_dim %
 Segments plan_segments(const LinearArgs& a, uint64_t part_bytes, uint64_t* bytes) {
     Segments seg{std::max(a.max_rows, 1u), 1, 0, nullptr, nullptr};
     *bytes = 0;
-    if (a.max_rows <= kFewRows) return seg;
     const uint64_t per = (uint64_t)a.heads * (a.k_dim * a.v_dim + 1) * 4;  // of a boundary
     const uint64_t blocks = (uint64_t)a.heads * (a.v_dim / columns_of(a));
-    // two workgroups a CU, as many as run at once, where a sequence's last segment is half one; no segment under 256 rows
+    // two workgroups a CU, as many as run at once, where a sequence's last segment is half one (four prompts of 601 to 5000 rows, 48 heads: 380 us, with
+    // three 416; in fp32 767, with one 1038); no segment under 256 rows
     const uint64_t target = 2 * kCus, ends = a.n_seqs * blocks / 2;
     uint64_t length = a.max_rows;
     if (ends < target) length = std::max<uint64_t>(256, (a.n_rows * blocks / (target - ends) + kChunk - 1) / kChunk * kChunk);
@@ -744,7 +783,7 @@ int launch_chunks(const LinearArgs& a, const Segments& seg, hipStream_t st) {
     const uint32_t blocks = a.heads * (a.v_dim / columns);
     const auto run = [&](auto states) {
         constexpr bool S = decltype(states)::value;
-        // 16 columns a wave where q and k take most of the registers and one workgroup the CU (fp32, k_dim 256: 386 us against 441)
+        // 16 columns a wave where q and k take most of the registers and one workgroup the CU (fp32, k_dim 256: a seventh less time)
         constexpr int UT = kPieces<T> * KD >= 768 ? 1 : 2;
         auto* k = columns == 64 ? k_linear_chunks<T, KD, 4, 1, S> : columns == 96 ? k_linear_chunks<T, KD, 6 / UT, UT, S> : k_linear_chunks<T, KD, 8 / UT, UT, S>;
         hipLaunchKernelGGL(k, dim3(blocks, S ? seg.most - 1 : seg.most, a.n_seqs), dim3(columns == 64 ? 256 : columns / 16 / UT * 64), 0, st, a, seg);
@@ -761,7 +800,7 @@ int launch_chunks(const LinearArgs& a, const Segments& seg, hipStream_t st) {
 
 template <typename T>
 int launch_typed(const LinearArgs& a, float* part, uint64_t part_bytes, hipStream_t st) {
-    if (a.max_rows > kFewRows) {
+    if (a.max_rows > kFewRows<T>) {
         uint64_t bytes;
         Segments seg = plan_segments(a, part ? part_bytes : 0, &bytes);
         if (seg.most > 1) {

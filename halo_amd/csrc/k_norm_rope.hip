@@ -41,8 +41,8 @@ __device__ __forceinline__ float group_sum(float v) {
     v += lanes<0x4E>(v);   // the other pair of 4
     v += lanes<0x141>(v);  // 8 lanes mirrored: the other 4
     if (G >= 16) v += lanes<0x140>(v);
-    if (G >= 32) v = across16(v);
-    if (G == 64) v = across32(v);
+    if (G >= 32) v = both16(v, v);
+    if (G == 64) v = both32(v, v);
     return v;
 }
 

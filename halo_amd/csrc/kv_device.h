@@ -59,13 +59,13 @@ template <int CTRL>
 __device__ __forceinline__ float lanes(float v) {
     return __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, true));
 }
-// v + the value 16, or 32, lanes away (lane ^ 16, lane ^ 32).
-__device__ __forceinline__ float across16(float v) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+// The sum of a's two halves of 32 lanes in the lower half, of b's in the upper; both16: of a's two 16 in each even 16, of b's in the odd.
+__device__ __forceinline__ float both32(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-__device__ __forceinline__ float across32(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+__device__ __forceinline__ float both16(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 

@@ -461,3 +461,13 @@ def test_far_rows(hl, dev, rows):
     batch = hl.LinearBatch(c.ints(c.slots), c.ints(c.starts), 1, rows, rows)
     hl.linear_attention(F32, state, batch, far[0], far[0][200:], far[0][1000:], far[1], c.d, 2, q_stride=stride, k_stride=stride, v_stride=stride, out_stride=stride)
     c.check((view(far[1], 0, None).double().cpu().numpy().reshape(rows, 2, vd), c.new.double().cpu().numpy()))
+
+
+@TYPES
+@pytest.mark.parametrize("kd,vd", [(64, 96), (96, 64), (128, 128), (192, 192), (256, 64)])
+def test_rows_between_steps_and_chunks(hl, dev, t, kd, vd):
+    """The row counts where a call goes over from row after row to chunks, for each type and head size."""
+    for n in (2, 3, 6, 7, 8, 9, 15, 16, 17):
+        print("[case] linear between", TYPE_NAMES[t], kd, vd, n, flush=True)
+        c = Case(dev, t, [n, 1, n - 1, 0], 3, 1, kd, vd, 7 * n)
+        c.check(c.call(hl))
