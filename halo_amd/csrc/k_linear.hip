@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kBlock) void k_linear_rows(LinearArgs a) {
     const bool bad = __syncthreads_or(!in_pool || slot_taken(a, s, slot, tid, kBlock));
     if (bad) {
         if (tid == 0 && blockIdx.x == 0 && head == 0) set_status(a.status, HALO_MI_STATUS_BAD_INDEX);
-        for (uint32_t i = tid; i < r.rows * kColumns; i += kBlock) out[i / kColumns * a.out.stride + i % kColumns] = from_f32<T>(__uint_as_float(0x7FC00000u));
+        for (uint64_t i = tid; i < (uint64_t)r.rows * kColumns; i += kBlock) out[i / kColumns * a.out.stride + i % kColumns] = from_f32<T>(__uint_as_float(0x7FC00000u));
         return;
     }
     for (uint32_t t = 0; t < r.rows; ++t) {
