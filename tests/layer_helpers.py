@@ -83,3 +83,33 @@ def linear_ref(t, q, k, v, decay, state, scale):
         far += HALF_STEP[t] * np.abs(out) * 1.01 + HALF_LEAST[t] + 1e-37
         # the chunked form adds a chunk's terms to the state at once, 64 roundings
         return out, far, state, off + 64 * U * reach + 1e-37
+
+
+def tile_plan(shapes, rows, cols, n_vec):
+    """The shape of tiles that gemm_i8 takes for many vectors, as k_gemm_i8.hip's plan_tiles chooses among `shapes` (fragments along the channels and
+    the vectors, stages), with the tiles in both directions and what each has: (shape, tiles_n, tiles_t, each_n, each_t)."""
+    cus, up = 256, lambda a, b: -(-a // b)
+    best, least = None, 1e300
+    for fn, ft, stages in shapes:
+        tiles_t = up(n_vec, 64 * ft)
+        each_t = up(n_vec, tiles_t)
+        tiles_t = up(n_vec, each_t)
+        few = up(rows, 32 * fn)
+        stage = (up(32 * fn, 64) * 64 + 64 * ft) * 128
+        beside = min(max(1, 160 * 1024 // (stages * stage)), up(few * tiles_t, cus))
+        slots, products = cus * beside, 0.056 * fn * ft
+        rounds = up(few * tiles_t, slots)
+
+        def share(n):
+            return up(up(rows, n), 8) * 8
+
+        def loads(each_n):
+            return 0.015 / 8 * (each_n + each_t) + 0.04 * (fn + ft) - 0.05
+
+        each_n = share(few)
+        if loads(each_n) > products:
+            each_n = share(max(few, min(slots * rounds // tiles_t, up(rows, 8))))
+        time = rounds * (2.0 + up(cols, 128) * beside * max(products, loads(each_n)))
+        if time < least:
+            least, best = time, ((fn, ft, stages), up(rows, each_n), tiles_t, each_n, each_t)
+    return best
