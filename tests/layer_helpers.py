@@ -85,6 +85,30 @@ def linear_ref(t, q, k, v, decay, state, scale):
         return out, far, state, off + 64 * U * reach + 1e-37
 
 
+def linear_ref_on(t, q, k, v, decay, state, scale):
+    """linear_ref in torch, for states of many heads: tensors of 64 bits on one device. Multiplies and sums elements, no library product."""
+    import torch
+
+    rows, heads, kd = q.shape
+    state, reach = state.clone(), state.abs()
+    off = torch.zeros_like(state)
+    out, far = torch.zeros_like(v), torch.zeros_like(v)
+    c = (kd + 192) * U + (0.0 if t == F32 else 2.0 ** -15)
+    g = decay.clamp(min=-1e4)  # NaN stays
+    fades, grown = g.exp(), (6 + g.abs()) * U
+    for r in range(rows):
+        fade = fades[r, :, None, None]
+        new = k[r, :, :, None] * v[r, :, None, :]
+        off = fade * (off + grown[r, :, None, None] * reach) + 2.0 ** -120 * reach
+        state = fade * state + new
+        reach = fade * reach + new.abs()
+        off += 4 * U * reach
+        out[r] = scale * (q[r, :, :, None] * state).sum(1)
+        far[r] = abs(scale) * (q[r, :, :, None].abs() * (off + c * reach)).sum(1)
+    far += HALF_STEP[t] * out.abs() * 1.01 + HALF_LEAST[t] + 1e-37
+    return out, far, state, off + 64 * U * reach + 1e-37
+
+
 def tile_plan(shapes, rows, cols, n_vec):
     """The shape of tiles that gemm_i8 takes for many vectors, as k_gemm_i8.hip's plan_tiles chooses among `shapes` (fragments along the channels and
     the vectors, stages), with the tiles in both directions and what each has: (shape, tiles_n, tiles_t, each_n, each_t)."""

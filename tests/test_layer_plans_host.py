@@ -1,9 +1,13 @@
 """What the tests of the layers' kernels on the GPU rest on, without one: the sizes of test_gpu_gemm_i8_tiles.py make the product take every
-shape of tiles that it has."""
+shape of tiles that it has, and the recurrence in torch is the one in numpy."""
 import re
 from pathlib import Path
 
-from layer_helpers import tile_plan
+import numpy as np
+import pytest
+
+from kv_helpers import BF16, F16, F32
+from layer_helpers import linear_ref, linear_ref_on, tile_plan
 from test_gpu_gemm_i8_tiles import BATCHES, BESIDE, SHAPES
 
 
@@ -29,3 +33,18 @@ def test_every_shape_of_tiles_is_tested():
     # the rows that are compared between calls meet many shapes
     rows, cols = BESIDE
     assert len({tile_plan(shapes(), rows, cols, n)[0] for n in BATCHES if n > 16}) >= 6
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+def test_recurrence_in_torch_is_the_one_in_numpy(t):
+    import torch
+
+    rng = np.random.default_rng(t)
+    q, k, v = rng.standard_normal((9, 3, 5)), rng.standard_normal((9, 3, 5)), rng.standard_normal((9, 3, 4))
+    decay = (-3 * rng.uniform(0, 1, (9, 3))).astype(np.float32)
+    decay[4, 1], decay[6, 2], v[7, 0, 1] = -np.inf, 0.25, np.nan
+    state = rng.standard_normal((3, 5, 4)).astype(np.float32)
+    want = linear_ref(t, q, k, v, decay, state, 0.5)
+    got = linear_ref_on(t, *(torch.from_numpy(x).double() for x in (q, k, v, decay, state)), 0.5)
+    for w, g in zip(want, got):
+        assert np.allclose(w, g.numpy(), rtol=1e-13, atol=1e-300, equal_nan=True)
