@@ -153,9 +153,9 @@ template <typename T>
 constexpr int kPieces = sizeof(T) == 4 ? 3 : 2;
 template <>
 constexpr int kPieces<__bf16> = 1;
-// Pieces that a 32-bit weight or state is cut to on its way to an output of type T.
-template <typename T>
-constexpr int kOutPieces = sizeof(T) == 4 ? 3 : 2;
+// Pieces that a 32-bit weight or state is cut to on its way to an output: all of its 24 bits, so that the output's rounding is the only one to fewer. With
+// two, 16 bits, outputs of 16 bits were up to a tenth of a step further off.
+constexpr int kOutPieces = 3;
 
 __device__ __forceinline__ uint32_t high_halves(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
 __device__ __forceinline__ float without_high(float a) { return a - __uint_as_float(__float_as_uint(a) & 0xFFFF0000u); }
@@ -241,8 +241,7 @@ __device__ __forceinline__ bool not_finite(const Patch<T>& p) {
 // One workgroup: 16 UT WAVES columns of a head's state, for a sequence or a segment of it. A wave keeps its 16 UT columns of S in its registers as
 // the products leave them (rows 4 (lane / 16) + i, column lane % 16), which is also how the next product takes S^T: its order of k_dim is
 // that of the registers, and q and k lie in LDS in the same order. Products are of bf16 pieces, summed in 32 bits: q, k and v exactly (one
-// piece for BF16, two for F16, three for F32), the faded k in three, P and S in two where the output has 16 bits, else in three; of pairs of
-// pieces those that matter in the result are multiplied.
+// piece for BF16, two for F16, three for F32), the faded k, P and S in three; of pairs of pieces those that matter in 24 bits are multiplied.
 //
 // What bounds it (BF16, 48 heads of 128, four prompts of 601 to 5000 rows, 329 us): two workgroups a CU, by their registers (220; LDS 55 KB),
 // whose waves issue vector instructions half of the time (735 a wave and chunk beside 92 matrix products, 192 of them S's pieces) and feed the
@@ -299,7 +298,7 @@ __device__ __forceinline__ uint32_t turned_row(uint32_t row) { return row % 4 * 
 template <typename T, int KD>
 struct ChunkLds {
     static constexpr int R = KD / 8 + 1;  // of a row of q or k
-    static constexpr int rows = kPieces<T> * kChunk * R, kt = 4 * plane_of(KD), p = kOutPieces<T> * kChunk * 5;
+    static constexpr int rows = kPieces<T> * kChunk * R, kt = 4 * plane_of(KD), p = kOutPieces * kChunk * 5;
     static constexpr int q(int columns) { return rows > kChunk * columns * (int)sizeof(T) / 16 ? rows : kChunk * columns * (int)sizeof(T) / 16; }
     static constexpr int vt(int columns) { return 4 * plane_of(columns); }
     static constexpr int bytes(int columns, bool k_rows) { return 16 * (q(columns) + (k_rows ? rows : 0) + 3 * kt + kPieces<T> * vt(columns) + p) + 2048; }
@@ -322,7 +321,7 @@ constexpr int waves_at_least() {
 
 template <typename T, int KD, int WAVES, int UT, bool STATES>
 __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATES>())) void k_linear_chunks(LinearArgs a, Segments seg) {
-    constexpr int NP = kPieces<T>, NO = kOutPieces<T>, KT = KD / 16, KS = KD / 32, THREADS = WAVES * 64;
+    constexpr int NP = kPieces<T>, NO = kOutPieces, KT = KD / 16, KS = KD / 32, THREADS = WAVES * 64;
     constexpr int QP = (KD / 4 + THREADS / 8 - 1) / (THREADS / 8);  // patches of q and k per thread
     constexpr int kColumnsHere = 16 * UT * WAVES;
     constexpr bool K_ROWS = k_in_lds<T, KD>(kColumnsHere);
@@ -745,8 +744,8 @@ __global__ __launch_bounds__(kBlock) void k_linear_settle(LinearArgs a, Segments
 
 constexpr uint32_t kCus = 256;
 // Up to this many rows of a sequence go one after another: a chunk costs the same for one row as for 32, and more the more pieces its type has (48 heads
-// of 128; 8 and 61 sequences: rows of BF16 4 in 14.7 us, 6 in 84.6, 8 in 18.1, 12 in 117, a chunk 15.6 and 95 to 99; of F16 8 in 17.7, 12 in 117, a
-// chunk 17.5 and 106 to 110; of F32 16 in 25.3, 12 in 118, a chunk 25.5 and 154 to 160).
+// of 128; 8 and 61 sequences: 6 rows of BF16 in 16.3 and 86.0 us, a chunk in 17.0 and 97 to 100; 8 of F16 in 18.8 and 93.6, a chunk in 19.2 and 111 to 115; 16
+// of F32 in 25.5 and 142, a chunk in 26.2 and 163).
 template <typename T>
 constexpr uint32_t kFewRows = kPieces<T> == 1 ? 6 : kPieces<T> == 2 ? 8 : 16;
 
