@@ -243,11 +243,12 @@ __device__ __forceinline__ bool not_finite(const Patch<T>& p) {
 // that of the registers, and q and k lie in LDS in the same order. Products are of bf16 pieces, summed in 32 bits: q, k and v exactly (one
 // piece for BF16, two for F16, three for F32), the faded k, P and S in three; of pairs of pieces those that matter in 24 bits are multiplied.
 //
-// What bounds it (BF16, 48 heads of 128, four prompts of 601 to 5000 rows, 329 us): two workgroups a CU, by their registers (220; LDS 55 KB),
-// whose waves issue vector instructions half of the time (735 a wave and chunk beside 92 matrix products, 192 of them S's pieces) and feed the
-// matrix cores a quarter of it; segments of unequal length leave a quarter of the places empty. Halved steps of it: stores that a branch may skip
-// made every chunk wait for all loads in flight (399 us against 380 for other prompts); k^T's pieces read one product ahead. What gave nothing: the
-// fade on v in place of k (405), loads a whole chunk ahead (386), the segments' pass with half the columns a workgroup (403).
+// What bounds it (BF16, 48 heads of 128, four prompts of 1639 to 5000 rows, 351 to 356 us): two workgroups a CU, by their registers (236; LDS 67 KB),
+// whose waves issue vector instructions half of the time (835 a wave and chunk, 112 matrix products and 352 for S's pieces among them) and feed the
+// matrix cores a quarter of it; segments of unequal length leave a quarter of the places empty. An earlier state of it, which cut S to two pieces for 16-bit
+// types, took 399 us: its stores, which a branch could skip, made every chunk wait for all loads in flight. With stores that every lane makes, and k^T's
+// pieces read one product ahead, it took 380. Tried on that state, and slower: the fade on v in place of k (405), loads a whole chunk ahead (386), the
+// segments' pass with half the columns a workgroup (403).
 // STATES: only the state that a segment adds is made (from zeros), for the segments after it.
 // Sequences are cut into segments where there are too few for the GPU.
 struct Segments {
@@ -289,7 +290,8 @@ __device__ __forceinline__ uint32_t beside(uint32_t row) { return (row + 4) / 8 
 
 // k^T and v^T: a row has a dim's 32 tokens, in 5 units of 16 bytes. Threads write four dims each, all lanes the same one of their four at a time, and
 // the products read 16 dims side by side: rows of equal row % 4 lie together, in planes that begin a quarter of the banks apart; of every other 64 rows the
-// halves of each 16 bytes have changed places, so that 32 lanes that write 8 bytes each meet all banks.
+// halves of each 16 bytes have changed places. By these alone 32 lanes that write 8 bytes each would meet all banks; with the swap of the 16-byte reads
+// (`beside`) they share them two by two, and a write takes twice its cycles.
 constexpr int plane_of(int rows) { return rows / 4 * 5 + (20 - rows / 4 * 5 % 16) % 16; }
 template <int ROWS>
 __device__ __forceinline__ uint32_t turned_row(uint32_t row) { return row % 4 * plane_of(ROWS) + row / 4 * 5; }
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(WAVES * 64, (waves_at_least<T, KD, WAVES, UT, STATE
     const bool bad = !look_up(a, seg, s, slot, r.rows, THREADS, cuts);
     if (part > cuts.parts || (STATES && part == cuts.parts)) return;
     const bool last_part = part == cuts.parts, begins = a.seq_lens && a.seq_lens[s] <= (int32_t)r.rows;
-    // equal segments of whole chunks; the last one has what is left
+    // segments of whole chunks, one more than the mean length has (512 rows in two: 288 and 224); the last one has what is left, which may be nothing
     const uint32_t each = (r.rows / (cuts.parts + 1) + kChunk) / kChunk * kChunk, first = part * each;
     const uint32_t rows = last_part ? r.rows - min(first, r.rows) : min(each, r.rows - min(first, r.rows)), row0 = r.row0 + first, boundary = cuts.base + part;
     const uint32_t hk = head / a.group;
@@ -758,8 +760,9 @@ Segments plan_segments(const LinearArgs& a, uint64_t part_bytes, uint64_t* bytes
     *bytes = 0;
     const uint64_t per = (uint64_t)a.heads * (a.k_dim * a.v_dim + 1) * 4;  // of a boundary
     const uint64_t blocks = (uint64_t)a.heads * (a.v_dim / columns_of(a));
-    // two workgroups a CU, as many as run at once, where a sequence's last segment is half one (four prompts of 601 to 5000 rows, 48 heads: 380 us, with
-    // three 416; in fp32 767, with one 1038); no segment under 256 rows
+    // two workgroups a CU, as many as run at once, where a sequence's last segment is half one (four prompts of 1639 to 5000 rows, 48 heads: BF16 351 us, with
+    // three 405; F32 746, with three 796); no segment under 256 rows. Every sequence counts here, those of one row too: a prompt of 5000 rows beside 16 of one
+    // row is cut into three, beside 20 not at all (134, 267 and 501 us)
     const uint64_t target = 2 * kCus, ends = a.n_seqs * blocks / 2;
     uint64_t length = a.max_rows;
     if (ends < target) length = std::max<uint64_t>(256, (a.n_rows * blocks / (target - ends) + kChunk - 1) / kChunk * kChunk);

@@ -745,9 +745,11 @@ int halo_mi_gemm_i8(const halo_mi_gemm_i8_params* p, void* stream);
  *     workspace. Graphs captured on one stream share that stream's workspace: give each its own if their replays may overlap.
  *     halo_mi_linear_attention_workspace() says what a call makes use of; with less (or on a capturing stream that has none
  *     yet) sequences are split less: the results are as right, and slower.
- * Numerics: the state, the sums and the decays are in 32 bits, the decays' running sums in 64. A chunk's state is held with a factor of up to
- * 2^40: k and k v^T are to stay below 2^80. Where a value of v is not finite, that column of out from its row on, and of the state, has no finite
- * numbers (infinities or NaN); one of k, or a decay of NaN: all columns of the heads that read it, from its row on; one of q: its own row's.
+ * Attention of models whose state only fades and adds; the gated delta rule, whose state takes k times (v - S^T k), is another recurrence.
+ * Numerics: the state, the sums and the decays are in 32 bits, the decays' running sums in 64; an output is rounded to its type once. A chunk's state
+ * is held with a factor of up to 2^40 either way: k, the state and its products with q are to stay below 2^80, and what lies under
+ * 2^-80 may be lost. Where a value of v is not finite, that column of out from its row on, and of the state, has no finite numbers (infinities
+ * or NaN); one of k, or a decay of NaN: all columns of the heads that read it, from its row on; one of q: its own row's.
  * out may not overlap any other operand (it may lie beside q, k and v in rows of one stride), state_out none but state.
  */
 typedef struct halo_mi_linear_attention_params {
