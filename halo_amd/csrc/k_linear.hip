@@ -243,7 +243,7 @@ __device__ __forceinline__ bool not_finite(const Patch<T>& p) {
 // that of the registers, and q and k lie in LDS in the same order. Products are of bf16 pieces, summed in 32 bits: q, k and v exactly (one
 // piece for BF16, two for F16, three for F32), the faded k, P and S in three; of pairs of pieces those that matter in 24 bits are multiplied.
 //
-// What bounds it (BF16, 48 heads of 128, four prompts of 1639 to 5000 rows, 351 to 356 us): two workgroups a CU, by their registers (236; LDS 67 KB),
+// What bounds it (BF16, 48 heads of 128, four prompts of 1639 to 5000 rows, 351 to 357 us): two workgroups a CU, by their registers (236; LDS 67 KB),
 // whose waves issue vector instructions half of the time (835 a wave and chunk, 112 matrix products and 352 for S's pieces among them) and feed the
 // matrix cores a quarter of it; segments of unequal length leave a quarter of the places empty. An earlier state of it, which cut S to two pieces for 16-bit
 // types, took 399 us: its stores, which a branch could skip, made every chunk wait for all loads in flight. With stores that every lane makes, and k^T's
